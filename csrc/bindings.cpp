@@ -73,6 +73,22 @@ void gemm_bf16(const at::Tensor& a, const at::Tensor& b, c10::optional<at::Tenso
 void gemm_bf16_ex(const at::Tensor& a, const at::Tensor& b, c10::optional<at::Tensor> a2, c10::optional<at::Tensor> b2,
                   c10::optional<at::Tensor> bias, c10::optional<at::Tensor> d, c10::optional<at::Tensor> d32,
                   double alpha, int64_t act, bool a_mn, bool b_mn, int64_t split);
+void fp4_quantize(const at::Tensor& x, at::Tensor& data, at::Tensor& scales, c10::optional<at::Tensor> row_scale,
+                  bool nv);
+void fp4_dequantize(const at::Tensor& data, const at::Tensor& scales, c10::optional<at::Tensor> row_scale,
+                    at::Tensor& out, bool nv);
+void fp4_gemm(const at::Tensor& a, const at::Tensor& sa, c10::optional<at::Tensor> ra, const at::Tensor& b,
+              const at::Tensor& sb, c10::optional<at::Tensor> rb, c10::optional<at::Tensor> bias, at::Tensor& d,
+              int64_t K, bool nv);
+void head_norm_rope_fwd(const at::Tensor& q, const at::Tensor& k, c10::optional<at::Tensor> wq,
+                        c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cosT, c10::optional<at::Tensor> sinT,
+                        c10::optional<at::Tensor> positions, at::Tensor& qo, at::Tensor& ko, double eps,
+                        bool interleaved);
+void head_norm_rope_bwd(const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q, const at::Tensor& k,
+                        c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cosT,
+                        c10::optional<at::Tensor> sinT, c10::optional<at::Tensor> positions, at::Tensor& dq,
+                        at::Tensor& dk, c10::optional<at::Tensor> dwq, c10::optional<at::Tensor> dwk, double eps,
+                        bool interleaved);
 void fsdp_gather(std::vector<int64_t> shard_ptrs, at::Tensor& dst, int64_t len, int64_t numel);
 void flash_fwd_accumulate(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor& o,
                           at::Tensor& lse, at::Tensor& acc_o, at::Tensor& acc_lse, bool read, bool final_,
@@ -121,6 +137,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cp_head_to_seq", &dmad::cp_head_to_seq);
   m.def("gemm_bf16", &dmad::gemm_bf16);
   m.def("gemm_bf16_ex", &dmad::gemm_bf16_ex);
+  m.def("fp4_quantize", &dmad::fp4_quantize);
+  m.def("fp4_dequantize", &dmad::fp4_dequantize);
+  m.def("fp4_gemm", &dmad::fp4_gemm);
+  m.def("head_norm_rope_fwd", &dmad::head_norm_rope_fwd);
+  m.def("head_norm_rope_bwd", &dmad::head_norm_rope_bwd);
   m.def("fsdp_gather", &dmad::fsdp_gather);
   m.def("fsdp_reduce_scatter", &dmad::fsdp_reduce_scatter);
   m.def("flash_fwd_accumulate", &dmad::flash_fwd_accumulate);

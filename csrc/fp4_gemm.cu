@@ -1,0 +1,338 @@
+// Persistent tcgen05 GEMM of block-scaled 4-bit operands for sm_100a.
+//
+//   D[M, N] = ra[m] rb[n] * sum_k A[m, k] B[n, k] + bias[n]          (bf16 or fp16 out, fp32 accumulation)
+//
+// A and B are e2m1 codes with one scale per 32 (mxfp4) or 16 (nvfp4) columns of K, multiplied on the tensor core
+// (kind::mxf4 / kind::mxf4nvf4), ra / rb the nvfp4 row scales applied to the accumulator in the epilogue.
+// The storage layout is described in fp4.cuh.
+//
+// Structure (one CTA per SM, persistent over 128 x 256 output tiles):
+//   warp 0      producer: a ring of stages of 256 columns of K: A 128 x 128 bytes and B 256 x 128 bytes by TMA
+//               (128-byte swizzle), and their scale tiles by plain bulk copies
+//   warp 1      TMEM owner; one thread copies a stage's scale tiles to tensor memory (tcgen05.cp) and issues its
+//               four K = 64 MMAs
+//   warps 2..5  epilogue: tcgen05.ld (thread = output row), row scales, bias, stores
+// Tensor memory: scales of a stage take up to 48 columns, double-buffered in the last 96 columns; the two 256-column
+// accumulators overlap in columns [160, 256).  The epilogue drains the shared columns first and then releases the
+// accumulator, so the next tile's MMAs start while five eighths of the tile are still being stored.
+// Every mbarrier wait is bounded (2 s), records a status code and makes all roles leave.
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include "common.cuh"
+#include "fp4.cuh"
+#include "sm100.cuh"
+#include "tma_host.h"
+
+namespace dmad {
+
+int* device_status_ptr(int device);
+void check_fp4(const at::Tensor& data, const at::Tensor& scales, const c10::optional<at::Tensor>& row_scale, bool nv,
+               int64_t R, int64_t K, const at::Device& device, const char* name);
+
+namespace {
+
+constexpr int kBM = 128, kBN = 256, kStages = 4;
+constexpr int kBK = 256;                 // columns of K of a stage: 128 bytes of codes
+constexpr int kABytes = kBM * 128;       // 16 KB
+constexpr int kBBytes = kBN * 128;       // 32 KB
+constexpr int kMaxTiles = 4;             // scale tiles along K of a stage (nvfp4; mxfp4 has two)
+constexpr int kSaBytes = kMaxTiles * kFp4TileBytes;      // 2 KB
+constexpr int kSbBytes = 2 * kMaxTiles * kFp4TileBytes;  // 4 KB
+constexpr int kAcc1 = 160;               // first column of the second accumulator
+constexpr int kSfCol = 416;              // first column of the scales
+constexpr int kSfCols = 48;              // columns of one scale buffer
+
+struct Smem {
+  uint8_t a[kStages][kABytes];
+  uint8_t b[kStages][kBBytes];
+  uint8_t sa[kStages][kSaBytes];
+  uint8_t sb[kStages][kSbBytes];
+  uint64_t full[kStages], empty[kStages];
+  uint64_t acc_full[2], acc_free;
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct Params {
+  void* d;
+  int64_t ldd;
+  const uint8_t* sa;
+  const uint8_t* sb;
+  const float* ra;
+  const float* rb;
+  const void* bias;
+  int bias_type;  // 0 fp32, 1 bf16, 2 fp16
+  int out_fp16;
+  int M, N, K;
+  int ktiles;     // scale tiles along K
+  int ksteps;     // stages along K
+  int tiles_m, tiles_n, num_tiles;
+  int* status;
+};
+
+__device__ __forceinline__ float load_bias(const Params& p, int n) {
+  if (p.bias_type == 0) return __ldg(static_cast<const float*>(p.bias) + n);
+  if (p.bias_type == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[n]);
+  return __half2float(static_cast<const __half*>(p.bias)[n]);
+}
+
+__device__ __forceinline__ uint32_t pack_out(const Params& p, float lo, float hi) {
+  if (p.out_fp16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return pack_bf16x2(lo, hi);
+}
+
+__device__ __forceinline__ void tile_coords(const Params& p, int t, int& tm, int& tn) {
+  // column-major raster within groups of 8 M-tiles: neighbouring CTAs share B tiles in L2
+  constexpr int kGroup = 8;
+  const int group = t / (kGroup * p.tiles_n);
+  const int first_m = group * kGroup;
+  const int gm = min(kGroup, p.tiles_m - first_m);
+  const int in = t % (kGroup * p.tiles_n);
+  tm = first_m + in % gm;
+  tn = in / gm;
+}
+
+template <bool NV>
+__global__ void __launch_bounds__(192, 1)
+fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, Params p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  volatile int* abort_flag = &sm.abort_flag;
+  const int warp = warp_id(), lane = lane_id();
+  constexpr int kStageTiles = NV ? 4 : 2;  // scale tiles along K of a whole stage
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    mbar_init(&sm.acc_full[0], 1);
+    mbar_init(&sm.acc_full[1], 1);
+    mbar_init(&sm.acc_free, 128);
+    mbar_init(&sm.drain, 1);
+    sm.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_base, 512);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (elect_one()) {
+      int it = 0;  // global stage counter (ring position)
+      bool ok = true;
+      const int sb_rows = (p.N + kFp4TileRows - 1) / kFp4TileRows;
+      for (int t = blockIdx.x; ok && t < p.num_tiles; t += gridDim.x) {
+        int tm, tn;
+        tile_coords(p, t, tm, tn);
+        const bool second = tn * 2 + 1 < sb_rows;  // whether B's tile has rows in a second scale tile
+        for (int k = 0; k < p.ksteps; ++k, ++it) {
+          const int s = it % kStages;
+          const uint32_t ph = (it / kStages) & 1;
+          if (!(ok = mbar_wait(&sm.empty[s], ph ^ 1, kStatusTimeoutEmpty, abort_flag, p.status))) break;
+          const int kt = k * kStageTiles;
+          const uint32_t bytes = (uint32_t)min(kStageTiles, p.ktiles - kt) * kFp4TileBytes;
+          mbar_arrive_expect_tx(&sm.full[s], kABytes + kBBytes + bytes * (second ? 3 : 2));
+          tma_load_2d(sm.a[s], &tm_a, &sm.full[s], k * 128, tm * kBM);
+          tma_load_2d(sm.b[s], &tm_b, &sm.full[s], k * 128, tn * kBN);
+          bulk_load(sm.sa[s], p.sa + ((int64_t)tm * p.ktiles + kt) * kFp4TileBytes, bytes, &sm.full[s]);
+          const uint8_t* sb = p.sb + ((int64_t)(2 * tn) * p.ktiles + kt) * kFp4TileBytes;
+          bulk_load(sm.sb[s], sb, bytes, &sm.full[s]);
+          if (second) bulk_load(sm.sb[s] + kSaBytes, sb + (int64_t)p.ktiles * kFp4TileBytes, bytes, &sm.full[s]);
+        }
+      }
+      // all issued copies land before the CTA's shared memory goes away
+      for (int j = max(0, it - kStages); j < it; ++j)
+        mbar_wait(&sm.full[j % kStages], (j / kStages) & 1, kStatusTimeoutTmaFull, nullptr, p.status);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (elect_one()) {
+      int it = 0, tl = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < p.num_tiles; t += gridDim.x, ++tl) {
+        // the columns shared with the previous tile's accumulator have been drained
+        if (tl > 0 && !(ok = mbar_wait(&sm.acc_free, (tl - 1) & 1, kStatusTimeoutSoftmax, abort_flag, p.status))) break;
+        tc_fence_after();
+        const uint32_t d = tmem + ((tl & 1) ? kAcc1 : 0);
+        for (int k = 0; k < p.ksteps; ++k, ++it) {
+          const int s = it % kStages;
+          if (!(ok = mbar_wait(&sm.full[s], (it / kStages) & 1, kStatusTimeoutTmaFull, abort_flag, p.status))) break;
+          // this stage's scale buffer was last read by the MMAs of two stages ago
+          if (it >= 2 && !(ok = mbar_wait(&sm.empty[(it - 2) % kStages], ((it - 2) / kStages) & 1, kStatusTimeoutMma,
+                                          abort_flag, p.status)))
+            break;
+          tc_fence_after();
+          const uint32_t sfa = tmem + kSfCol + (it & 1) * kSfCols, sfb = sfa + 16;
+          const int nt = min(kStageTiles, p.ktiles - k * kStageTiles);
+          const uint32_t aa = smem_u32(sm.a[s]), bb = smem_u32(sm.b[s]);
+          const uint32_t ssa = smem_u32(sm.sa[s]), ssb = smem_u32(sm.sb[s]);
+          for (int j = 0; j < nt; ++j) {
+            tmem_cp_scales(sfa + 4 * j, smem_desc_scales(ssa + j * kFp4TileBytes));
+            tmem_cp_scales(sfb + 8 * j, smem_desc_scales(ssb + j * kFp4TileBytes));
+            tmem_cp_scales(sfb + 8 * j + 4, smem_desc_scales(ssb + kSaBytes + j * kFp4TileBytes));
+          }
+          const int nk = min(4, (p.K - k * kBK + 63) / 64);
+          for (int kk = 0; kk < nk; ++kk) {
+            const int j = NV ? kk : kk >> 1;
+            const uint32_t idesc = idesc_fp4(NV, kBM, kBN, NV ? 0 : (kk & 1) * 2);
+            mma_fp4_ss<NV>(d, smem_desc_sw128(aa + kk * 32, 16, 1024), smem_desc_sw128(bb + kk * 32, 16, 1024), idesc,
+                           sfa + 4 * j, sfb + 8 * j, (k > 0 || kk > 0) ? 1u : 0u);
+          }
+          mma_commit(&sm.empty[s]);
+        }
+        if (!ok) break;
+        mma_commit(&sm.acc_full[tl & 1]);
+      }
+      if (!ok) *abort_flag = 1;
+      mma_commit(&sm.drain);
+      mbar_wait(&sm.drain, 0, kStatusTimeoutMma, nullptr, p.status);
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue (warps 2..5)
+    const int wq = warp & 3;  // TMEM lane quarter this warp may access
+    const int row = wq * 32 + lane;
+    const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
+    const bool vec = p.N % 8 == 0;  // 16-byte stores: rows of D are multiples of 16 bytes
+    int tl = 0;
+    for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x, ++tl) {
+      if (!__all_sync(0xffffffffu,
+                      mbar_wait(&sm.acc_full[tl & 1], (tl >> 1) & 1, kStatusTimeoutMma, abort_flag, p.status)))
+        break;
+      tc_fence_after();
+      int tm, tn;
+      tile_coords(p, t, tm, tn);
+      const int m = tm * kBM + row;
+      const float ra = (NV && m < p.M) ? p.ra[m] : 1.f;
+      uint16_t* drow = static_cast<uint16_t*>(p.d) + (int64_t)m * p.ldd;
+      const uint32_t acc = tmem + lane_base + ((tl & 1) ? kAcc1 : 0);
+      // chunks of 32 columns, the ones shared with the other accumulator first: the last three of the
+      // first accumulator, the first three of the second
+#pragma unroll 1
+      for (int i = 0; i < kBN / 32; ++i) {
+        const int c = (tl & 1) ? i : (i < 3 ? 5 + i : i - 3);
+        uint32_t r[32];
+        tmem_ld32(acc + c * 32, r);
+        tmem_wait_ld();
+        if (i == 2) {
+          tc_fence_before();
+          mbar_arrive(&sm.acc_free);
+        }
+        const int nc = tn * kBN + c * 32;
+        if (m < p.M && nc < p.N) {
+          float v[32];
+#pragma unroll
+          for (int q = 0; q < 32; ++q) {
+            float x = __uint_as_float(r[q]);
+            const int n = min(nc + q, p.N - 1);
+            if (NV) x *= ra * __ldg(p.rb + n);
+            if (p.bias != nullptr) x += load_bias(p, n);
+            v[q] = x;
+          }
+          if (vec) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (nc + q * 8 < p.N)
+                *reinterpret_cast<uint4*>(drow + nc + q * 8) =
+                    make_uint4(pack_out(p, v[8 * q], v[8 * q + 1]), pack_out(p, v[8 * q + 2], v[8 * q + 3]),
+                               pack_out(p, v[8 * q + 4], v[8 * q + 5]), pack_out(p, v[8 * q + 6], v[8 * q + 7]));
+          } else {
+#pragma unroll
+            for (int q = 0; q < 32; ++q)
+              if (nc + q < p.N) drow[nc + q] = (uint16_t)pack_out(p, v[q], 0.f);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+CUtensorMap code_map(const at::Tensor& x, uint32_t box_rows) {
+  const uint64_t dims[2] = {(uint64_t)x.size(1), (uint64_t)x.size(0)};
+  const uint64_t strides[1] = {(uint64_t)x.size(1)};
+  const uint32_t box[2] = {128u, box_rows};
+  return make_tmap_u8(x.data_ptr(), 2, dims, strides, box);
+}
+
+template <bool NV>
+void launch(const CUtensorMap& ma, const CUtensorMap& mb, const Params& p, int sms, cudaStream_t stream) {
+  const int smem = (int)sizeof(Smem) + 1024;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(fp4_gemm_kernel<NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  fp4_gemm_kernel<NV><<<std::min(p.num_tiles, sms), 192, smem, stream>>>(ma, mb, p);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+}  // namespace
+
+// d [M, N] (bf16 or fp16, contiguous) = A B^T with A [M, K], B [N, K] stored as fp4.cuh says, + bias [N].
+void fp4_gemm(const at::Tensor& a, const at::Tensor& sa, c10::optional<at::Tensor> ra, const at::Tensor& b,
+              const at::Tensor& sb, c10::optional<at::Tensor> rb, c10::optional<at::Tensor> bias, at::Tensor& d,
+              int64_t K, bool nv) {
+  TORCH_CHECK(d.is_cuda() && d.dim() == 2 && d.is_contiguous() &&
+                  (d.scalar_type() == at::kBFloat16 || d.scalar_type() == at::kHalf),
+              "fp4_gemm: d must be a contiguous CUDA bf16 or fp16 matrix");
+  const int64_t M = d.size(0), N = d.size(1);
+  check_fp4(a, sa, ra, nv, M, K, d.device(), "fp4_gemm: a");
+  check_fp4(b, sb, rb, nv, N, K, d.device(), "fp4_gemm: b");
+  Params p;
+  p.bias = nullptr;
+  p.bias_type = 0;
+  if (bias.has_value() && bias->defined()) {
+    TORCH_CHECK(bias->device() == d.device() && bias->dim() == 1 && bias->size(0) == N && bias->is_contiguous() &&
+                    (bias->scalar_type() == at::kFloat || bias->scalar_type() == at::kBFloat16 ||
+                     bias->scalar_type() == at::kHalf),
+                "fp4_gemm: bias must be contiguous fp32, bf16 or fp16 [", N, "] on d's device");
+    p.bias = bias->data_ptr();
+    p.bias_type = bias->scalar_type() == at::kFloat ? 0 : bias->scalar_type() == at::kBFloat16 ? 1 : 2;
+  }
+  if (M == 0 || N == 0) return;
+  c10::cuda::CUDAGuard guard(d.device());
+  p.d = d.data_ptr();
+  p.ldd = N;
+  p.sa = sa.data_ptr<uint8_t>();
+  p.sb = sb.data_ptr<uint8_t>();
+  p.ra = nv ? ra->data_ptr<float>() : nullptr;
+  p.rb = nv ? rb->data_ptr<float>() : nullptr;
+  p.out_fp16 = d.scalar_type() == at::kHalf ? 1 : 0;
+  p.M = (int)M;
+  p.N = (int)N;
+  p.K = (int)K;
+  p.ktiles = (int)sa.size(1);
+  p.ksteps = (int)((K + kBK - 1) / kBK);
+  p.tiles_m = (int)((M + kBM - 1) / kBM);
+  p.tiles_n = (int)((N + kBN - 1) / kBN);
+  TORCH_CHECK((int64_t)p.tiles_m * p.tiles_n <= INT32_MAX, "fp4_gemm: too many output tiles");
+  p.num_tiles = p.tiles_m * p.tiles_n;
+  p.status = device_status_ptr(d.get_device());
+  int sms = 148;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d.get_device());
+  const CUtensorMap ma = code_map(a, kBM), mb = code_map(b, kBN);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  nv ? launch<true>(ma, mb, p, sms, stream) : launch<false>(ma, mb, p, sms, stream);
+}
+
+}  // namespace dmad

@@ -1,0 +1,423 @@
+// Quantisation of rows to block-scaled 4-bit floating point (e2m1) and back.
+//
+//   mxfp4:  s_b = 2^(floor(log2 max_b |x|) - 2),                       code = e2m1(x / s_b)
+//   nvfp4:  g_r = the smallest 2^p with max_r |x| <= 6 * 448 * 2^p,
+//           s_b = e4m3(max_b |x| / (6 g_r)),                           code = e2m1(x / (s_b g_r))
+//
+// (e2m1 and e4m3 round to nearest with halves to the even code; e2m1 saturates at 6.)  A block that holds an
+// infinity or a NaN gets the scale code NaN, so all its values read back as NaN; such blocks do not count
+// in g_r.  Scales are exact powers of two or quotients rounded once, so a code depends on nothing but the
+// numbers: the CPU restatement gives the same bytes.
+//
+// The kernel reads each element once and is bound by HBM.  A thread takes units of 16 columns (one 32-byte
+// load of 16-bit elements, one 8-byte store of codes); a row is held by one block in registers between the
+// row maximum and the encoding, so nvfp4's two levels cost no second read while the row fits (32768 columns;
+// longer rows are read twice).
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include "common.cuh"
+#include "fp4.cuh"
+
+namespace dmad {
+namespace {
+
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+template <typename T>
+struct Unit {  // 16 elements
+  uint32_t w[4 * sizeof(T)];
+};
+
+__device__ __forceinline__ void ld256(const void* p, uint32_t* w) {
+  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void st256(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ Unit<T> load_unit(const T* __restrict__ row, int c0, int K) {
+  Unit<T> u;
+  if constexpr (ALIGNED) {  // K is a multiple of 16: a unit is inside the row or past it
+    if (c0 < K) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) ld256(row + c0 + i * 32 / (int)sizeof(T), u.w + 8 * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4 * (int)sizeof(T); ++i) u.w[i] = 0u;
+    }
+  } else if constexpr (sizeof(T) == 4) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(row);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) u.w[i] = c0 + i < K ? __ldg(p + c0 + i) : 0u;
+  } else {
+    const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t lo = c0 + 2 * i < K ? __ldg(p + c0 + 2 * i) : 0u;
+      const uint32_t hi = c0 + 2 * i + 1 < K ? __ldg(p + c0 + 2 * i + 1) : 0u;
+      u.w[i] = lo | (hi << 16);
+    }
+  }
+  return u;
+}
+
+// max |x| of a unit as the bits of an fp32 number.  Non-negative numbers order as their bits do, with infinity
+// and NaN above all finite ones.
+template <typename T>
+__device__ __forceinline__ uint32_t absmax_bits(const Unit<T>& u) {
+  uint32_t m = 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, u.w[i] & 0x7fffffffu);
+    return m;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, u.w[i] & 0x7fff7fffu);
+    m = max(m & 0xffffu, m >> 16);
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) return m << 16;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void unit_to_float(const Unit<T>& u, float (&f)[16]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(u.w[i]);
+  } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[2 * i] = __uint_as_float(u.w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(u.w[i] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&u.w[i]));
+      f[2 * i] = h.x;
+      f[2 * i + 1] = h.y;
+    }
+  }
+}
+
+// The smallest power of two g with amax <= 6 * 448 * g (6 * 448 = 1.3125 * 2^11), 1 for amax = 0.
+__device__ __forceinline__ float row_scale_of(uint32_t amax_bits) {
+  if (amax_bits == 0u) return 1.f;
+  int e = (int)(amax_bits >> 23) - 127 - 11 + ((amax_bits & 0x7fffffu) > 0x280000u ? 1 : 0);
+  e = max(e, -126);
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+// Codes of one unit for nvfp4; returns the block's scale code.
+template <typename T>
+__device__ __forceinline__ uint32_t encode_nv(const Unit<T>& u, uint32_t amax, float ginv, uint32_t (&out)[2]) {
+  if (amax >= kInfBits) {
+    out[0] = out[1] = 0u;
+    return 0x7fu;
+  }
+  const uint32_t code = float_to_e4m3(__fdiv_rn(__uint_as_float(amax) * ginv, 6.f));
+  const float s = e4m3_to_float(code);
+  float f[16], y[8];
+  unit_to_float(u, f);
+  // 16-bit elements: x / s differs from a border b of two codes by 2^-11 b or more unless it is b, and then the
+  // product with the rounded 1 / s is off by 2^-23 of it; the addition and subtraction of 384 rounds to steps of
+  // 2^-15, which moves such a product onto b and no other onto it.  fp32 elements are divided.
+  const float r = s > 0.f ? __frcp_rn(s) : 0.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = f[8 * h + i], t = x * ginv;
+      if constexpr (sizeof(T) == 4) {
+        y[i] = s > 0.f ? __fdiv_rn(t, s) : t * 0.f;
+      } else {
+        y[i] = copysignf(fmaf(t, r, 384.f) - 384.f, x);
+      }
+    }
+    out[h] = float8_to_e2m1x8(y);
+  }
+  return code;
+}
+
+// Codes of one unit for mxfp4 with the block's (two units') maximum; returns the scale code.
+template <typename T>
+__device__ __forceinline__ uint32_t encode_mx(const Unit<T>& u, uint32_t amax, uint32_t (&out)[2]) {
+  if (amax >= kInfBits) {
+    out[0] = out[1] = 0u;
+    return 0xffu;
+  }
+  const uint32_t code = (uint32_t)max((int)(amax >> 23) - 2, 0);
+  const float m = __uint_as_float((254u - code) << 23);  // 2^(127 - code)
+  float f[16], y[8];
+  unit_to_float(u, f);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = f[8 * h + i] * m;
+    out[h] = float8_to_e2m1x8(y);
+  }
+  return code;
+}
+
+struct QuantParams {
+  const void* x;
+  int64_t ld;
+  int R, K;
+  uint8_t* data;
+  uint8_t* scales;
+  float* row_scale;
+  int row_bytes, ktiles;
+};
+
+// blockDim = (threads of a row, rows); more than one warp a row means one row a block.
+template <typename T, bool NV, bool ALIGNED, int UPT>
+__global__ void __launch_bounds__(512) quant_kernel(QuantParams p) {
+  __shared__ uint32_t red[16];
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  const int TX = blockDim.x;
+  const int units = p.ktiles * kFp4TileBlocks * (fp4_block(NV) / 16);
+  const bool live = row < p.R;
+  const T* xr = static_cast<const T*>(p.x) + row * p.ld;
+  const int chunks = (units + TX * UPT - 1) / (TX * UPT);
+  Unit<T> v[UPT];
+  auto load = [&](int c) {
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) {
+      const int u = threadIdx.x + (c * UPT + i) * TX;
+      v[i] = load_unit<T, ALIGNED>(xr, u * 16, live ? p.K : 0);
+    }
+  };
+  float ginv = 1.f;
+  if constexpr (NV) {
+    uint32_t m = 0;
+    for (int c = 0; c < chunks; ++c) {
+      load(c);
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        const uint32_t a = absmax_bits(v[i]);
+        m = max(m, a < kInfBits ? a : 0u);
+      }
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (TX > 32) {
+      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+      __syncthreads();
+      const int nw = TX >> 5;
+      m = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < nw ? red[threadIdx.x & 31] : 0u);
+    }
+    const float g = row_scale_of(m);
+    ginv = __uint_as_float((254u << 23) - __float_as_uint(g));  // 1 / g of a power of two
+    if (threadIdx.x == 0 && live) p.row_scale[row] = g;
+  }
+  // rows past R up to the scale tile's end have zero scales and no data
+  const bool tile_row = row < ((int64_t)p.R + kFp4TileRows - 1) / kFp4TileRows * kFp4TileRows;
+  for (int c = 0; c < chunks; ++c) {
+    if (!NV || chunks > 1) load(c);
+#pragma unroll
+    for (int i = 0; i < UPT; ++i) {
+      const int u = threadIdx.x + (c * UPT + i) * TX;
+      uint32_t amax = absmax_bits(v[i]);
+      uint32_t codes[2], sc;
+      if constexpr (NV) {
+        sc = encode_nv(v[i], amax, ginv, codes);
+      } else {
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        sc = encode_mx(v[i], amax, codes);
+      }
+      if (live && u * 8 < p.row_bytes)
+        *reinterpret_cast<uint2*>(p.data + row * p.row_bytes + (int64_t)u * 8) = make_uint2(codes[0], codes[1]);
+      // the four scales of a tile's row are one word, stored by the first of their lanes
+      constexpr int STEP = fp4_block(NV) / 16;
+      uint32_t word = sc;
+      word |= __shfl_down_sync(0xffffffffu, sc, STEP) << 8;
+      word |= __shfl_down_sync(0xffffffffu, sc, 2 * STEP) << 16;
+      word |= __shfl_down_sync(0xffffffffu, sc, 3 * STEP) << 24;
+      if (u % (4 * STEP) == 0 && u < units && tile_row)
+        *reinterpret_cast<uint32_t*>(p.scales + fp4_scale_offset(row, u / STEP, p.ktiles)) = word;
+    }
+  }
+}
+
+template <typename T, bool NV, bool ALIGNED>
+void launch_quant(const QuantParams& p, cudaStream_t stream) {
+  const int units = p.ktiles * kFp4TileBlocks * (fp4_block(NV) / 16);
+  const int64_t rows = ((int64_t)p.R + kFp4TileRows - 1) / kFp4TileRows * kFp4TileRows;
+  constexpr int UPT = sizeof(T) == 4 ? 2 : 4;
+  auto go = [&](auto upt) {
+    constexpr int U = decltype(upt)::value;
+    int tx = (units + U - 1) / U;
+    tx = std::min(512, (tx + 31) / 32 * 32);
+    const int ty = tx == 32 ? 4 : 1;
+    quant_kernel<T, NV, ALIGNED, U><<<(unsigned)((rows + ty - 1) / ty), dim3(tx, ty), 0, stream>>>(p);
+  };
+  // two units a thread keep the rows of up to 16384 columns in one block of 512 threads
+  if (units <= 1024) go(std::integral_constant<int, 2>{});
+  else go(std::integral_constant<int, UPT>{});
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+template <typename T>
+void quant_typed(const QuantParams& p, bool nv, cudaStream_t stream) {
+  const bool aligned = p.K % 16 == 0 && (p.ld * sizeof(T)) % 32 == 0 && reinterpret_cast<uintptr_t>(p.x) % 32 == 0;
+  if (nv) aligned ? launch_quant<T, true, true>(p, stream) : launch_quant<T, true, false>(p, stream);
+  else aligned ? launch_quant<T, false, true>(p, stream) : launch_quant<T, false, false>(p, stream);
+}
+
+// ---------------------------------------------------------------- dequantisation
+template <typename O, bool NV, bool ALIGNED>
+__global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict__ data, int row_bytes,
+                                                      const uint8_t* __restrict__ scales, int ktiles,
+                                                      const float* __restrict__ row_scale, O* __restrict__ out, int R,
+                                                      int K) {
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= R) return;
+  const float g = NV ? row_scale[row] : 1.f;
+  O* orow = out + row * K;
+  for (int u = threadIdx.x; u * 16 < K; u += blockDim.x) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(data + row * row_bytes + (int64_t)u * 8));
+    const uint32_t sc = __ldg(scales + fp4_scale_offset(row, NV ? u : u >> 1, ktiles));
+    const float s = NV ? e4m3_to_float(sc) * g : ue8m0_to_float(sc);
+    float f[16];
+    {
+      float a[8], b[8];
+      e2m1x8_to_float8(w.x, a);
+      e2m1x8_to_float8(w.y, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f[i] = a[i] * s;
+        f[8 + i] = b[i] * s;
+      }
+    }
+    if constexpr (ALIGNED) {
+      if constexpr (sizeof(O) == 4) {
+        st256(orow + u * 16, reinterpret_cast<const uint32_t*>(f));
+        st256(orow + u * 16 + 8, reinterpret_cast<const uint32_t*>(f) + 8);
+      } else {
+        uint32_t o[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if constexpr (std::is_same_v<O, __nv_bfloat16>) {
+            o[i] = f2_to_bf16x2(f[2 * i], f[2 * i + 1]);
+          } else {
+            const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+            o[i] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        }
+        st256(orow + u * 16, o);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (u * 16 + i < K) {
+          if constexpr (sizeof(O) == 4) orow[u * 16 + i] = f[i];
+          else if constexpr (std::is_same_v<O, __nv_bfloat16>) orow[u * 16 + i] = __float2bfloat16_rn(f[i]);
+          else orow[u * 16 + i] = __float2half_rn(f[i]);
+        }
+    }
+  }
+}
+
+template <typename O, bool NV>
+void launch_dequant(const at::Tensor& data, const at::Tensor& scales, const float* rs, at::Tensor& out,
+                    cudaStream_t stream) {
+  const int R = (int)out.size(0), K = (int)out.size(1);
+  const int units = (K + 15) / 16;
+  const int tx = std::min(256, (units + 31) / 32 * 32), ty = 256 / tx;
+  const unsigned grid = (unsigned)((R + ty - 1) / ty);
+  const bool aligned = K % 16 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 32 == 0;
+  auto* d = data.data_ptr<uint8_t>();
+  auto* s = scales.data_ptr<uint8_t>();
+  O* o = reinterpret_cast<O*>(out.data_ptr());
+  if (aligned)
+    dequant_kernel<O, NV, true><<<grid, dim3(tx, ty), 0, stream>>>(d, (int)data.size(1), s, (int)scales.size(1), rs, o, R, K);
+  else
+    dequant_kernel<O, NV, false><<<grid, dim3(tx, ty), 0, stream>>>(d, (int)data.size(1), s, (int)scales.size(1), rs, o, R, K);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+}  // namespace
+
+// Shapes, types and placement of a stored 4-bit matrix [R, K].
+void check_fp4(const at::Tensor& data, const at::Tensor& scales, const c10::optional<at::Tensor>& row_scale, bool nv,
+               int64_t R, int64_t K, const at::Device& device, const char* name) {
+  const int64_t block = fp4_block(nv);
+  const int64_t ktiles = ((K + block - 1) / block + kFp4TileBlocks - 1) / kFp4TileBlocks;
+  TORCH_CHECK(K >= 1 && K <= (1 << 24) && R >= 0 && R <= INT32_MAX - 256, name, ": sizes out of range");
+  TORCH_CHECK(data.device() == device && data.scalar_type() == at::kByte && data.dim() == 2 && data.size(0) == R &&
+                  data.size(1) == (K + 31) / 32 * 16 && data.is_contiguous(),
+              name, ".data must be contiguous uint8 [", R, ", ", (K + 31) / 32 * 16, "] on ", device);
+  TORCH_CHECK(scales.device() == device && scales.scalar_type() == at::kByte && scales.dim() == 3 &&
+                  scales.size(0) == (R + kFp4TileRows - 1) / kFp4TileRows && scales.size(1) == ktiles &&
+                  scales.size(2) == kFp4TileBytes && scales.is_contiguous(),
+              name, ".scales must be contiguous uint8 [", (R + kFp4TileRows - 1) / kFp4TileRows, ", ", ktiles,
+              ", 512] on ", device);
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
+              name, ": data and scales must be 16-byte aligned");
+  if (nv) {
+    TORCH_CHECK(row_scale.has_value() && row_scale->defined() && row_scale->device() == device &&
+                    row_scale->scalar_type() == at::kFloat && row_scale->dim() == 1 && row_scale->size(0) == R &&
+                    row_scale->is_contiguous(),
+                name, ".row_scale must be contiguous fp32 [", R, "] on ", device);
+  }
+}
+
+// x [R, K] (bf16, fp16 or fp32, contiguous columns, any row stride) -> data, scales, row_scale (nvfp4).
+void fp4_quantize(const at::Tensor& x, at::Tensor& data, at::Tensor& scales, c10::optional<at::Tensor> row_scale,
+                  bool nv) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1),
+              "fp4_quantize: x must be a CUDA matrix with contiguous columns");
+  const int64_t R = x.size(0), K = x.size(1);
+  check_fp4(data, scales, row_scale, nv, R, K, x.device(), "fp4_quantize");
+  if (R == 0) return;
+  c10::cuda::CUDAGuard guard(x.device());
+  QuantParams p;
+  p.x = x.data_ptr();
+  p.ld = x.stride(0);
+  p.R = (int)R;
+  p.K = (int)K;
+  p.data = data.data_ptr<uint8_t>();
+  p.scales = scales.data_ptr<uint8_t>();
+  p.row_scale = nv ? row_scale->data_ptr<float>() : nullptr;
+  p.row_bytes = (int)data.size(1);
+  p.ktiles = (int)scales.size(1);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  switch (x.scalar_type()) {
+    case at::kBFloat16: quant_typed<__nv_bfloat16>(p, nv, stream); break;
+    case at::kHalf: quant_typed<__half>(p, nv, stream); break;
+    case at::kFloat: quant_typed<float>(p, nv, stream); break;
+    default: TORCH_CHECK(false, "fp4_quantize: x must be bf16, fp16 or fp32");
+  }
+}
+
+// out [R, K] (bf16, fp16 or fp32, contiguous) = the values that the codes stand for, rounded to out's type.
+void fp4_dequantize(const at::Tensor& data, const at::Tensor& scales, c10::optional<at::Tensor> row_scale,
+                    at::Tensor& out, bool nv) {
+  TORCH_CHECK(out.is_cuda() && out.dim() == 2 && out.is_contiguous(), "fp4_dequantize: out must be a contiguous CUDA matrix");
+  check_fp4(data, scales, row_scale, nv, out.size(0), out.size(1), out.device(), "fp4_dequantize");
+  if (out.size(0) == 0) return;
+  c10::cuda::CUDAGuard guard(out.device());
+  const float* rs = nv ? row_scale->data_ptr<float>() : nullptr;
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  auto go = [&](auto tag) {
+    using O = decltype(tag);
+    nv ? launch_dequant<O, true>(data, scales, rs, out, stream) : launch_dequant<O, false>(data, scales, rs, out, stream);
+  };
+  switch (out.scalar_type()) {
+    case at::kBFloat16: go(__nv_bfloat16{}); break;
+    case at::kHalf: go(__half{}); break;
+    case at::kFloat: go(float{}); break;
+    default: TORCH_CHECK(false, "fp4_dequantize: out must be bf16, fp16 or fp32");
+  }
+}
+
+}  // namespace dmad

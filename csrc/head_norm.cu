@@ -1,0 +1,577 @@
+// Per-head RMSNorm of queries and keys with the position rotation in the same pass, and its backward.
+//
+//   n = x / sqrt(mean(x^2) + eps),   y = n * w,   out = Rot(y)              (per row and head of hd elements)
+//   gy = Rot^-1(g),   dw = sum gy * n,   dx = (gy w - n mean(gy w n)) / sqrt(mean(x^2) + eps)
+//
+// Rot turns the first `rot` elements of a head: pairs (2i, 2i + 1) (interleaved) or (i, i + rot / 2) (halves) by the
+// angle whose cosine and sine stand in row t, column i of the tables; t is the row's entry of `positions`, or
+// r % T.  Everything is fp32 between the load and the one rounding at the store.
+//
+// Bound by HBM: the forward reads and writes q and k once, the backward reads g and x and writes dx; the
+// statistics are taken again from x, which is in registers anyway, so nothing is kept between the passes.  A
+// head is held by a group of G lanes, eight elements a lane (16-byte accesses of 16-bit types), and a group
+// takes U heads of one row at a time: U loads in flight, one read of the row's angles.  gridDim.y separates q
+// from k, so a thread has one weight slice and one gradient accumulator.  dw: per-thread sums over the tasks
+// of a persistent grid, one partial row a block, and a second kernel that adds the partials in a fixed order.
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include "common.cuh"
+
+namespace dmad {
+
+int* device_status_ptr(int device);
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// How the angles are applied.  The vectorised forms need table rows of whole 16-byte pieces and, for halves,
+// partners that are whole lanes apart; kAny takes every other size one element at a time.
+enum RotMode { kNone = 0, kPairs = 1, kHalves = 2, kAny = 3 };
+
+struct Side {  // the queries or the keys
+  const void* x;
+  const void* g;
+  void* out;      // forward: the result; backward: dx
+  int64_t xr, xh, gr, gh, orow, oh;  // row and head strides
+  const void* w;  // nullptr: ones
+  int wtype;      // 0 fp32, 1 bf16, 2 fp16
+  int H, chunks;
+  float* partial;  // backward: [gridDim.x, hd] sums of gy * n, or nullptr
+};
+
+struct Params {
+  Side side[2];
+  const float* cosT;
+  const float* sinT;
+  const void* positions;
+  int pos64;
+  int64_t T;
+  int64_t R;
+  int hd, rot, interleaved;
+  float eps;
+  int* status;
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        f[2 * i] = __uint_as_float(w[i] << 16);
+        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        f[2 * i] = h.x;
+        f[2 * i + 1] = h.y;
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        w[i] = f2_to_bf16x2(f[2 * i], f[2 * i + 1]);
+      } else {
+        const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+__device__ __forceinline__ float load_any(const void* p, int type, int i) {
+  if (type == 0) return static_cast<const float*>(p)[i];
+  if (type == 1) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __bfloat162float(v);
+  else return __half2float(v);
+}
+
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The angles that a lane needs of table row t.  kPairs: c[0..3] for its four pairs; kHalves: c[0..7] for its
+// eight elements.  Elements past `rot` keep (1, 0).
+template <int MODE>
+struct Angles {
+  float c[MODE == kPairs ? 4 : 8], s[MODE == kPairs ? 4 : 8];
+  int64_t off;  // kAny: offset of the row, -1 if there is none
+
+  __device__ __forceinline__ void load(const Params& p, int64_t row, int e0, bool valid) {
+    if constexpr (MODE == kNone) return;
+    constexpr int N = MODE == kPairs ? 4 : 8;
+    int64_t t = 0;
+    if (valid) {
+      t = p.positions == nullptr ? (row < p.T ? row : row % p.T)
+          : p.pos64              ? static_cast<const int64_t*>(p.positions)[row]
+                                 : static_cast<const int*>(p.positions)[row];
+    }
+    const bool bad = t < 0 || t >= p.T;
+    if (bad) atomicCAS(p.status, 0, 6);  // bounds: the rotated elements become NaN
+    const int half = p.rot >> 1;
+    if constexpr (MODE == kAny) {
+      off = bad ? -1 : t * half;
+    } else {
+      const int col = MODE == kPairs ? e0 >> 1 : (e0 < half ? e0 : e0 - half);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        c[i] = bad ? __int_as_float(0x7fffffff) : 1.f;
+        s[i] = bad ? __int_as_float(0x7fffffff) : 0.f;
+      }
+      if (e0 < p.rot && !bad) {
+        const float4* pc = reinterpret_cast<const float4*>(p.cosT + t * half + col);
+        const float4* ps = reinterpret_cast<const float4*>(p.sinT + t * half + col);
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+          const float4 a = __ldg(pc + i), b = __ldg(ps + i);
+          c[4 * i] = a.x; c[4 * i + 1] = a.y; c[4 * i + 2] = a.z; c[4 * i + 3] = a.w;
+          s[4 * i] = b.x; s[4 * i + 1] = b.y; s[4 * i + 2] = b.z; s[4 * i + 3] = b.w;
+        }
+      }
+    }
+  }
+
+  // y <- the rotated y (forward) or the back-rotated y (INV).  other(i): element i of the head, for kAny.
+  template <bool INV, typename F>
+  __device__ __forceinline__ void apply(const Params& p, int e0, float (&y)[8], F other) const {
+    if constexpr (MODE == kPairs) {
+      if (e0 >= p.rot) return;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = y[2 * j], b = y[2 * j + 1], sn = INV ? -s[j] : s[j];
+        y[2 * j] = a * c[j] - b * sn;
+        y[2 * j + 1] = b * c[j] + a * sn;
+      }
+    } else if constexpr (MODE == kHalves) {
+      const int half = p.rot >> 1;
+      const int from = e0 < half ? half >> 3 : e0 < p.rot ? -(half >> 3) : 0;
+      const float sign = (e0 < half) == INV ? 1.f : -1.f;  // first half: a c - b s; second half: b c + a s
+      const int lane = threadIdx.x & 31;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float o = __shfl_sync(0xffffffffu, y[j], lane + from);
+        if (e0 < p.rot) y[j] = y[j] * c[j] + sign * s[j] * o;
+      }
+    } else if constexpr (MODE == kAny) {
+      const int half = p.rot >> 1;
+      float z[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = e0 + j;
+        z[j] = y[j];
+        if (i < p.rot) {
+          const bool first = p.interleaved ? (j & 1) == 0 : i < half;
+          const int col = p.interleaved ? i >> 1 : first ? i : i - half;
+          const float o = p.interleaved ? y[j ^ 1] : other(first ? i + half : i - half);
+          const float cc = off < 0 ? __int_as_float(0x7fffffff) : __ldg(p.cosT + off + col);
+          const float ss = off < 0 ? __int_as_float(0x7fffffff) : __ldg(p.sinT + off + col);
+          z[j] = y[j] * cc + (first == INV ? ss : -ss) * o;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = z[j];
+    }
+  }
+};
+
+__device__ __forceinline__ void split_task(int64_t task, int64_t tasks, int chunks, int64_t& row, int& chunk) {
+  if (tasks <= 0x7fffffff) {
+    row = (uint32_t)task / (uint32_t)chunks;
+    chunk = (int)((uint32_t)task - (uint32_t)row * (uint32_t)chunks);
+  } else {
+    row = task / chunks;
+    chunk = (int)(task - row * chunks);
+  }
+}
+
+template <typename T, int G, int MODE, int U>
+__global__ void __launch_bounds__(kThreads) head_norm_fwd_kernel(const __grid_constant__ Params p) {
+  const Side& sd = p.side[blockIdx.y];
+  const int lane = threadIdx.x & (G - 1), e0 = lane * 8;
+  const bool in = e0 < p.hd;
+  const int64_t tasks = p.R * sd.chunks;
+  const int64_t stride = (int64_t)gridDim.x * (kThreads / G);
+  float w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = in && sd.w != nullptr ? load_any(sd.w, sd.wtype, e0 + j) : 1.f;
+  const float inv_hd = 1.f / (float)p.hd;
+  const int group = threadIdx.x / G;
+  // all lanes of a warp stay in the loop together: the sums below are warp-wide shuffles
+  for (int64_t first = (int64_t)blockIdx.x * (kThreads / G) + (group & ~(32 / G - 1)); first < tasks; first += stride) {
+    const int64_t task = first + (group & (32 / G - 1));
+    const bool valid = task < tasks;
+    int64_t row = 0;
+    int chunk = 0;
+    if (valid) split_task(task, tasks, sd.chunks, row, chunk);
+    const T* x = static_cast<const T*>(sd.x) + row * sd.xr + (int64_t)chunk * U * sd.xh;
+    T* o = static_cast<T*>(sd.out) + row * sd.orow + (int64_t)chunk * U * sd.oh;
+    const int nh = valid ? min(U, sd.H - chunk * U) : 0;
+    float f[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (in && u < nh) {
+        load8(x + u * sd.xh + e0, f[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[u][j] = 0.f;
+      }
+    }
+    Angles<MODE> ang;
+    ang.load(p, row, e0, valid);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(f[u][j], f[u][j], ss);
+      const float r = rsqrtf(group_sum<G>(ss) * inv_hd + p.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[u][j] = f[u][j] * r * w[j];
+      ang.template apply<false>(p, e0, f[u], [&](int i) {
+        return u < nh ? to_float(x[u * sd.xh + i]) * r * (sd.w != nullptr ? load_any(sd.w, sd.wtype, i) : 1.f) : 0.f;
+      });
+      if (in && u < nh) store8(o + u * sd.oh + e0, f[u]);
+    }
+  }
+}
+
+template <typename T, int G, int MODE, int U>
+__global__ void __launch_bounds__(kThreads) head_norm_bwd_kernel(const __grid_constant__ Params p) {
+  __shared__ float red[kThreads * 8];
+  const Side& sd = p.side[blockIdx.y];
+  const int lane = threadIdx.x & (G - 1), e0 = lane * 8;
+  const bool in = e0 < p.hd;
+  const int64_t tasks = p.R * sd.chunks;
+  const int64_t stride = (int64_t)gridDim.x * (kThreads / G);
+  float w[8], acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    w[j] = in && sd.w != nullptr ? load_any(sd.w, sd.wtype, e0 + j) : 1.f;
+    acc[j] = 0.f;
+  }
+  const float inv_hd = 1.f / (float)p.hd;
+  const int group = threadIdx.x / G;
+  for (int64_t first = (int64_t)blockIdx.x * (kThreads / G) + (group & ~(32 / G - 1)); first < tasks; first += stride) {
+    const int64_t task = first + (group & (32 / G - 1));
+    const bool valid = task < tasks;
+    int64_t row = 0;
+    int chunk = 0;
+    if (valid) split_task(task, tasks, sd.chunks, row, chunk);
+    const T* x = static_cast<const T*>(sd.x) + row * sd.xr + (int64_t)chunk * U * sd.xh;
+    const T* g = static_cast<const T*>(sd.g) + row * sd.gr + (int64_t)chunk * U * sd.gh;
+    T* o = static_cast<T*>(sd.out) + row * sd.orow + (int64_t)chunk * U * sd.oh;
+    const int nh = valid ? min(U, sd.H - chunk * U) : 0;
+    float f[U][8], d[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (in && u < nh) {
+        load8(x + u * sd.xh + e0, f[u]);
+        load8(g + u * sd.gh + e0, d[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[u][j] = d[u][j] = 0.f;
+      }
+    }
+    Angles<MODE> ang;
+    ang.load(p, row, e0, valid);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      ang.template apply<true>(p, e0, d[u], [&](int i) { return u < nh ? to_float(g[u * sd.gh + i]) : 0.f; });
+      float ss = 0.f, dot = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        ss = fmaf(f[u][j], f[u][j], ss);
+        dot = fmaf(d[u][j] * w[j], f[u][j], dot);
+      }
+      const float r = rsqrtf(group_sum<G>(ss) * inv_hd + p.eps);
+      const float c = group_sum<G>(dot) * r * inv_hd;  // mean(gy w n)
+      float dx[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float n = f[u][j] * r;
+        if (u < nh) acc[j] = fmaf(d[u][j], n, acc[j]);
+        dx[j] = (d[u][j] * w[j] - n * c) * r;
+      }
+      if (in && u < nh) store8(o + u * sd.oh + e0, dx);
+    }
+  }
+  if (sd.partial == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) red[threadIdx.x * 8 + j] = acc[j];
+  __syncthreads();
+  // red[group][lane * 8 + j]: add the block's groups in order
+  for (int i = threadIdx.x; i < p.hd; i += kThreads) {
+    float t = 0.f;
+    for (int q = 0; q < kThreads / G; ++q) t += red[q * G * 8 + i];
+    sd.partial[(int64_t)blockIdx.x * p.hd + i] = t;
+  }
+}
+
+// dw[i] = sum over the blocks of partial[block][i], in a fixed order.
+__global__ void __launch_bounds__(1024)
+head_norm_dw_kernel(const float* __restrict__ pq, const float* __restrict__ pk, int blocks, int hd, void* dwq, int tq,
+                    void* dwk, int tk) {
+  __shared__ float red[32][33];
+  const float* part = blockIdx.y == 0 ? pq : pk;
+  void* dw = blockIdx.y == 0 ? dwq : dwk;
+  const int type = blockIdx.y == 0 ? tq : tk;
+  if (dw == nullptr) return;
+  const int i = blockIdx.x * 32 + threadIdx.x;
+  float t = 0.f;
+  if (i < hd)
+    for (int b = threadIdx.y; b < blocks; b += 32) t += part[(int64_t)b * hd + i];
+  red[threadIdx.y][threadIdx.x] = t;
+  __syncthreads();
+  if (threadIdx.y == 0 && i < hd) {
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < 32; ++b) sum += red[b][threadIdx.x];
+    if (type == 0) static_cast<float*>(dw)[i] = sum;
+    else if (type == 1) static_cast<__nv_bfloat16*>(dw)[i] = __float2bfloat16_rn(sum);
+    else static_cast<__half*>(dw)[i] = __float2half_rn(sum);
+  }
+}
+
+int float_type(const at::Tensor& t, const char* name) {
+  if (t.scalar_type() == at::kFloat) return 0;
+  if (t.scalar_type() == at::kBFloat16) return 1;
+  TORCH_CHECK(t.scalar_type() == at::kHalf, name, " must be fp32, bf16 or fp16");
+  return 2;
+}
+
+// Checks one [R, H, hd] operand and returns its row and head strides.
+std::pair<int64_t, int64_t> check_heads(const at::Tensor& t, const at::Tensor& like, int64_t R, int64_t H, int64_t hd,
+                                        const char* name) {
+  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == like.scalar_type() && t.dim() == 3 && t.size(0) == R &&
+                  t.size(1) == H && t.size(2) == hd,
+              name, " must be [", R, ", ", H, ", ", hd, "] of the type and on the device of the queries");
+  const int64_t per16 = 16 / (int64_t)t.element_size();
+  TORCH_CHECK(t.numel() == 0 || (t.stride(2) == 1 && (H == 1 || t.stride(1) % per16 == 0) &&
+                                 (R == 1 || t.stride(0) % per16 == 0) &&
+                                 reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0),
+              name, ": heads must be contiguous, row and head strides and the start multiples of 16 bytes");
+  return {t.stride(0), t.stride(1)};
+}
+
+RotMode fill_common(Params& p, const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& wq,
+                    const c10::optional<at::Tensor>& wk, const c10::optional<at::Tensor>& cosT,
+                    const c10::optional<at::Tensor>& sinT, const c10::optional<at::Tensor>& positions, double eps,
+                    bool interleaved) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 3, "head_norm_rope: q and k must be CUDA [R, H, hd] tensors");
+  const int64_t R = q.size(0), hd = q.size(2);
+  TORCH_CHECK(hd >= 8 && hd <= 256 && hd % 8 == 0, "head_norm_rope: the head size must be a multiple of 8 up to 256");
+  TORCH_CHECK(q.size(1) >= 1 && k.size(1) >= 1 && q.size(1) <= 65536 && k.size(1) <= 65536,
+              "head_norm_rope: q and k need 1 to 65536 heads");
+  const at::Tensor* xs[2] = {&q, &k};
+  const c10::optional<at::Tensor>* ws[2] = {&wq, &wk};
+  for (int i = 0; i < 2; ++i) {
+    Side& s = p.side[i];
+    std::tie(s.xr, s.xh) = check_heads(*xs[i], q, R, xs[i]->size(1), hd, i ? "k" : "q");
+    s.x = xs[i]->data_ptr();
+    s.H = (int)xs[i]->size(1);
+    s.g = nullptr;
+    s.gr = s.gh = 0;
+    s.partial = nullptr;
+    s.w = nullptr;
+    s.wtype = 0;
+    if (ws[i]->has_value() && (*ws[i])->defined()) {
+      const at::Tensor& w = **ws[i];
+      TORCH_CHECK(w.device() == q.device() && w.dim() == 1 && w.size(0) == hd && w.is_contiguous(),
+                  "head_norm_rope: a weight must be contiguous [", hd, "] on the device of the queries");
+      s.w = w.data_ptr();
+      s.wtype = float_type(w, "head_norm_rope: a weight");
+    }
+  }
+  p.R = R;
+  p.hd = (int)hd;
+  p.rot = 0;
+  p.T = 1;
+  p.cosT = p.sinT = nullptr;
+  p.positions = nullptr;
+  p.pos64 = 0;
+  p.interleaved = interleaved ? 1 : 0;
+  p.eps = (float)eps;
+  p.status = device_status_ptr(q.get_device());
+  if (!(cosT.has_value() && cosT->defined())) return kNone;
+  TORCH_CHECK(sinT.has_value() && sinT->defined(), "head_norm_rope: cos needs sin");
+  for (const at::Tensor* t : {&*cosT, &*sinT})
+    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kFloat && t->dim() == 2 && t->is_contiguous() &&
+                    t->sizes() == cosT->sizes() && t->size(0) >= 1,
+                "head_norm_rope: cos and sin must be contiguous fp32 [T, rot / 2] on the device of the queries, T >= 1");
+  p.rot = (int)cosT->size(1) * 2;
+  TORCH_CHECK(cosT->size(1) * 2 <= hd, "head_norm_rope: the tables turn ", cosT->size(1) * 2, " of ", hd, " elements");
+  if (p.rot == 0) return kNone;
+  p.T = cosT->size(0);
+  p.cosT = cosT->data_ptr<float>();
+  p.sinT = sinT->data_ptr<float>();
+  if (positions.has_value() && positions->defined()) {
+    TORCH_CHECK(positions->device() == q.device() && positions->dim() == 1 && positions->size(0) == R &&
+                    positions->is_contiguous() &&
+                    (positions->scalar_type() == at::kLong || positions->scalar_type() == at::kInt),
+                "head_norm_rope: positions must be contiguous int32 or int64 [", R, "] on the device of the queries");
+    p.positions = positions->data_ptr();
+    p.pos64 = positions->scalar_type() == at::kLong ? 1 : 0;
+  }
+  const bool tables16 = reinterpret_cast<uintptr_t>(p.cosT) % 16 == 0 && reinterpret_cast<uintptr_t>(p.sinT) % 16 == 0;
+  if (interleaved) return tables16 && p.rot % 8 == 0 ? kPairs : kAny;
+  return tables16 && p.rot % 16 == 0 ? kHalves : kAny;
+}
+
+template <typename F>
+void dispatch_mode(RotMode m, F f) {
+  if (m == kNone) f(std::integral_constant<int, kNone>{});
+  else if (m == kPairs) f(std::integral_constant<int, kPairs>{});
+  else if (m == kHalves) f(std::integral_constant<int, kHalves>{});
+  else f(std::integral_constant<int, kAny>{});
+}
+template <typename F>
+void dispatch_group(int hd, F f) {
+  if (hd <= 32) f(std::integral_constant<int, 4>{});
+  else if (hd <= 64) f(std::integral_constant<int, 8>{});
+  else if (hd <= 128) f(std::integral_constant<int, 16>{});
+  else f(std::integral_constant<int, 32>{});
+}
+template <typename F>
+void dispatch_type(at::ScalarType t, F f) {
+  if (t == at::kBFloat16) f(__nv_bfloat16{});
+  else if (t == at::kHalf) f(__half{});
+  else if (t == at::kFloat) f(float{});
+  else TORCH_CHECK(false, "head_norm_rope: q and k must be bf16, fp16 or fp32");
+}
+
+int64_t blocks_for(const Params& p, int G, int64_t most) {
+  const int per = kThreads / G;
+  int64_t b = 1;
+  for (const Side& s : p.side) b = std::max(b, (p.R * s.chunks + per - 1) / per);
+  return std::min(b, most);
+}
+
+int sm_count(int device) {
+  int sms = 148;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  return sms;
+}
+
+}  // namespace
+
+// qo, ko = Rot(norm(q) * wq), Rot(norm(k) * wk) per head; [R, H, hd] each, any row and head strides.
+void head_norm_rope_fwd(const at::Tensor& q, const at::Tensor& k, c10::optional<at::Tensor> wq,
+                        c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cosT, c10::optional<at::Tensor> sinT,
+                        c10::optional<at::Tensor> positions, at::Tensor& qo, at::Tensor& ko, double eps,
+                        bool interleaved) {
+  Params p;
+  const RotMode mode = fill_common(p, q, k, wq, wk, cosT, sinT, positions, eps, interleaved);
+  at::Tensor* outs[2] = {&qo, &ko};
+  for (int i = 0; i < 2; ++i) {
+    Side& s = p.side[i];
+    std::tie(s.orow, s.oh) = check_heads(*outs[i], q, p.R, s.H, p.hd, i ? "ko" : "qo");
+    s.out = outs[i]->data_ptr();
+  }
+  if (p.R == 0) return;
+  c10::cuda::CUDAGuard guard(q.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int sms = sm_count(q.get_device());
+  dispatch_type(q.scalar_type(), [&](auto tag) {
+    using T = decltype(tag);
+    dispatch_group(p.hd, [&](auto g) {
+      dispatch_mode(mode, [&](auto m) {
+        constexpr int U = 4;
+        for (Side& s : p.side) s.chunks = (s.H + U - 1) / U;
+        const dim3 grid((unsigned)blocks_for(p, g, (int64_t)sms * 16), 2);
+        head_norm_fwd_kernel<T, decltype(g)::value, decltype(m)::value, U><<<grid, kThreads, 0, stream>>>(p);
+      });
+    });
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// dq, dk of the forward given gq, gk (gradients of its results) and its inputs; dwq, dwk [hd] where wanted.
+void head_norm_rope_bwd(const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q, const at::Tensor& k,
+                        c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cosT,
+                        c10::optional<at::Tensor> sinT, c10::optional<at::Tensor> positions, at::Tensor& dq,
+                        at::Tensor& dk, c10::optional<at::Tensor> dwq, c10::optional<at::Tensor> dwk, double eps,
+                        bool interleaved) {
+  Params p;
+  const RotMode mode = fill_common(p, q, k, wq, wk, cosT, sinT, positions, eps, interleaved);
+  const at::Tensor* gs[2] = {&gq, &gk};
+  at::Tensor* outs[2] = {&dq, &dk};
+  const c10::optional<at::Tensor>* dws[2] = {&dwq, &dwk};
+  void* dwp[2] = {nullptr, nullptr};
+  int dwt[2] = {0, 0};
+  for (int i = 0; i < 2; ++i) {
+    Side& s = p.side[i];
+    std::tie(s.gr, s.gh) = check_heads(*gs[i], q, p.R, s.H, p.hd, i ? "gk" : "gq");
+    std::tie(s.orow, s.oh) = check_heads(*outs[i], q, p.R, s.H, p.hd, i ? "dk" : "dq");
+    s.g = gs[i]->data_ptr();
+    s.out = outs[i]->data_ptr();
+    if (dws[i]->has_value() && (*dws[i])->defined()) {
+      const at::Tensor& dw = **dws[i];
+      TORCH_CHECK(dw.device() == q.device() && dw.dim() == 1 && dw.size(0) == p.hd && dw.is_contiguous(),
+                  "head_norm_rope: a weight gradient must be contiguous [", p.hd, "]");
+      dwp[i] = dw.data_ptr();
+      dwt[i] = float_type(dw, "head_norm_rope: a weight gradient");
+    }
+  }
+  c10::cuda::CUDAGuard guard(q.device());
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const int sms = sm_count(q.get_device());
+  const bool want_dw = dwp[0] != nullptr || dwp[1] != nullptr;
+  at::Tensor partial;
+  int blocks = 0;
+  if (p.R > 0) {
+    dispatch_type(q.scalar_type(), [&](auto tag) {
+      using T = decltype(tag);
+      dispatch_group(p.hd, [&](auto g) {
+        dispatch_mode(mode, [&](auto m) {
+          constexpr int U = 2;
+          for (Side& s : p.side) s.chunks = (s.H + U - 1) / U;
+          blocks = (int)blocks_for(p, g, (int64_t)sms * 4);
+          if (want_dw) {
+            partial = at::empty({2, blocks, p.hd}, q.options().dtype(at::kFloat));
+            for (int i = 0; i < 2; ++i)
+              p.side[i].partial = dwp[i] != nullptr ? partial.data_ptr<float>() + (int64_t)i * blocks * p.hd : nullptr;
+          }
+          head_norm_bwd_kernel<T, decltype(g)::value, decltype(m)::value, U>
+              <<<dim3((unsigned)blocks, 2), kThreads, 0, stream>>>(p);
+        });
+      });
+    });
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  if (want_dw) {
+    head_norm_dw_kernel<<<dim3((p.hd + 31) / 32, 2), dim3(32, 32), 0, stream>>>(p.side[0].partial, p.side[1].partial,
+                                                                              blocks, p.hd, dwp[0], dwt[0], dwp[1], dwt[1]);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+}
+
+}  // namespace dmad

@@ -40,11 +40,11 @@ inline void ensure_context() {
   }
 }
 
-// bf16 tensor map with a 128-byte swizzle.  dims/strides are innermost-first;
+// Tensor map with a 128-byte swizzle.  dims/strides are innermost-first;
 // strides are in bytes for dims 1..rank-1 (dim 0 is contiguous).  Every
 // stride must be a multiple of 16 bytes and the base 16-byte aligned.
-inline CUtensorMap make_tmap_bf16(const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
-                                  const uint32_t* box, CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B) {
+inline CUtensorMap make_tmap(CUtensorMapDataType type, const void* base, int rank, const uint64_t* dims,
+                             const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swz) {
   CUtensorMap m;
   if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) throw std::runtime_error("dmad: TMA base not 16B aligned");
   ensure_context();
@@ -61,11 +61,21 @@ inline CUtensorMap make_tmap_bf16(const void* base, int rank, const uint64_t* di
     s[i] = strides_bytes[i];
     if (s[i] % 16 != 0) throw std::runtime_error("dmad: TMA stride not a multiple of 16 bytes");
   }
-  CUresult r = get_encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d, s, b, es,
+  CUresult r = get_encode_tiled()(&m, type, rank, const_cast<void*>(base), d, s, b, es,
                                   CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw std::runtime_error("dmad: cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
   return m;
+}
+
+inline CUtensorMap make_tmap_bf16(const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                                  const uint32_t* box, CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B) {
+  return make_tmap(CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, rank, dims, strides_bytes, box, swz);
+}
+
+inline CUtensorMap make_tmap_u8(const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                                const uint32_t* box, CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B) {
+  return make_tmap(CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rank, dims, strides_bytes, box, swz);
 }
 
 }  // namespace dmad

@@ -62,6 +62,8 @@ def check_device_status(device: int | None = None) -> None:
 from .attention import flash_attention, attention_reference, flash_attention_jvp, attention_jvp_reference  # noqa: E402
 from .norm import ln_mod, gate_residual, qk_norm_rope, rope, rope_apply, rms_norm, layer_norm_affine  # noqa: E402
 from .activation import gelu_tanh  # noqa: E402
+from .fp4 import Fp4Tensor, quantize_fp4, dequantize_fp4, fp4_linear  # noqa: E402
+from .head_norm import qk_head_norm_rope  # noqa: E402
 from .temb import sinusoidal_embedding, small_linear  # noqa: E402
 
 __all__ = [
@@ -81,6 +83,11 @@ __all__ = [
     "rms_norm",
     "layer_norm_affine",
     "gelu_tanh",
+    "Fp4Tensor",
+    "quantize_fp4",
+    "dequantize_fp4",
+    "fp4_linear",
+    "qk_head_norm_rope",
     "sinusoidal_embedding",
     "small_linear",
 ]
