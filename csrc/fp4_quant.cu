@@ -346,7 +346,8 @@ void launch_dequant(const at::Tensor& data, const at::Tensor& scales, const floa
 
 }  // namespace
 
-// Shapes, types and placement of a stored 4-bit matrix [R, K].
+// Shapes, types and placement of a stored 4-bit matrix [R, K].  (The messages hold numbers and texts only: a
+// libstdc++ linked into this module statically cannot hand its streams to the printers in libc10.)
 void check_fp4(const at::Tensor& data, const at::Tensor& scales, const c10::optional<at::Tensor>& row_scale, bool nv,
                int64_t R, int64_t K, const at::Device& device, const char* name) {
   const int64_t block = fp4_block(nv);
@@ -354,12 +355,12 @@ void check_fp4(const at::Tensor& data, const at::Tensor& scales, const c10::opti
   TORCH_CHECK(K >= 1 && K <= (1 << 24) && R >= 0 && R <= INT32_MAX - 256, name, ": sizes out of range");
   TORCH_CHECK(data.device() == device && data.scalar_type() == at::kByte && data.dim() == 2 && data.size(0) == R &&
                   data.size(1) == (K + 31) / 32 * 16 && data.is_contiguous(),
-              name, ".data must be contiguous uint8 [", R, ", ", (K + 31) / 32 * 16, "] on ", device);
+              name, ".data must be contiguous uint8 [", R, ", ", (K + 31) / 32 * 16, "] on the device of the output");
   TORCH_CHECK(scales.device() == device && scales.scalar_type() == at::kByte && scales.dim() == 3 &&
                   scales.size(0) == (R + kFp4TileRows - 1) / kFp4TileRows && scales.size(1) == ktiles &&
                   scales.size(2) == kFp4TileBytes && scales.is_contiguous(),
               name, ".scales must be contiguous uint8 [", (R + kFp4TileRows - 1) / kFp4TileRows, ", ", ktiles,
-              ", 512] on ", device);
+              ", 512] on the device of the output");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
               name, ": data and scales must be 16-byte aligned");
@@ -367,7 +368,7 @@ void check_fp4(const at::Tensor& data, const at::Tensor& scales, const c10::opti
     TORCH_CHECK(row_scale.has_value() && row_scale->defined() && row_scale->device() == device &&
                     row_scale->scalar_type() == at::kFloat && row_scale->dim() == 1 && row_scale->size(0) == R &&
                     row_scale->is_contiguous(),
-                name, ".row_scale must be contiguous fp32 [", R, "] on ", device);
+                name, ".row_scale must be contiguous fp32 [", R, "] on the device of the output");
   }
 }
 
