@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cstdint>
+#include <string>
 
 // Row kernels: vector count per row -> (vectors per thread VEC, threads per block TH).
 #define DMAD_ROW_DISPATCH(nvec, ...)                                        \
@@ -26,6 +27,10 @@
 #endif
 
 namespace dmad {
+
+// A number as text for an error message.  The compiler links libstdc++ into this module statically while torch
+// brings its own; formatting a number on a stream then finds the other library's locale tables and crashes.
+inline std::string num(int64_t v) { return std::to_string(v); }
 
 struct alignas(16) bf16x8 {
   uint32_t w[4];

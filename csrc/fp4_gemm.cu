@@ -305,7 +305,7 @@ void fp4_gemm(const at::Tensor& a, const at::Tensor& sa, c10::optional<at::Tenso
     TORCH_CHECK(bias->device() == d.device() && bias->dim() == 1 && bias->size(0) == N && bias->is_contiguous() &&
                     (bias->scalar_type() == at::kFloat || bias->scalar_type() == at::kBFloat16 ||
                      bias->scalar_type() == at::kHalf),
-                "fp4_gemm: bias must be contiguous fp32, bf16 or fp16 [", N, "] on d's device");
+                "fp4_gemm: bias must be contiguous fp32, bf16 or fp16 [", num(N), "] on d's device");
     p.bias = bias->data_ptr();
     p.bias_type = bias->scalar_type() == at::kFloat ? 0 : bias->scalar_type() == at::kBFloat16 ? 1 : 2;
   }

@@ -346,8 +346,8 @@ void launch_dequant(const at::Tensor& data, const at::Tensor& scales, const floa
 
 }  // namespace
 
-// Shapes, types and placement of a stored 4-bit matrix [R, K].  (The messages hold numbers and texts only: a
-// libstdc++ linked into this module statically cannot hand its streams to the printers in libc10.)
+// Shapes, types and placement of a stored 4-bit matrix [R, K].  Numbers in the messages
+// go through num(): see common.cuh.
 void check_fp4(const at::Tensor& data, const at::Tensor& scales, const c10::optional<at::Tensor>& row_scale, bool nv,
                int64_t R, int64_t K, const at::Device& device, const char* name) {
   const int64_t block = fp4_block(nv);
@@ -355,11 +355,11 @@ void check_fp4(const at::Tensor& data, const at::Tensor& scales, const c10::opti
   TORCH_CHECK(K >= 1 && K <= (1 << 24) && R >= 0 && R <= INT32_MAX - 256, name, ": sizes out of range");
   TORCH_CHECK(data.device() == device && data.scalar_type() == at::kByte && data.dim() == 2 && data.size(0) == R &&
                   data.size(1) == (K + 31) / 32 * 16 && data.is_contiguous(),
-              name, ".data must be contiguous uint8 [", R, ", ", (K + 31) / 32 * 16, "] on the device of the output");
+              name, ".data must be contiguous uint8 [", num(R), ", ", num((K + 31) / 32 * 16), "] on the device of the output");
   TORCH_CHECK(scales.device() == device && scales.scalar_type() == at::kByte && scales.dim() == 3 &&
                   scales.size(0) == (R + kFp4TileRows - 1) / kFp4TileRows && scales.size(1) == ktiles &&
                   scales.size(2) == kFp4TileBytes && scales.is_contiguous(),
-              name, ".scales must be contiguous uint8 [", (R + kFp4TileRows - 1) / kFp4TileRows, ", ", ktiles,
+              name, ".scales must be contiguous uint8 [", num((R + kFp4TileRows - 1) / kFp4TileRows), ", ", num(ktiles),
               ", 512] on the device of the output");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0 &&
                   reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
@@ -368,17 +368,18 @@ void check_fp4(const at::Tensor& data, const at::Tensor& scales, const c10::opti
     TORCH_CHECK(row_scale.has_value() && row_scale->defined() && row_scale->device() == device &&
                     row_scale->scalar_type() == at::kFloat && row_scale->dim() == 1 && row_scale->size(0) == R &&
                     row_scale->is_contiguous(),
-                name, ".row_scale must be contiguous fp32 [", R, "] on the device of the output");
+                name, ".row_scale must be contiguous fp32 [", num(R), "] on the device of the output");
   }
 }
 
 // x [R, K] (bf16, fp16 or fp32, contiguous columns, any row stride) -> data, scales, row_scale (nvfp4).
 void fp4_quantize(const at::Tensor& x, at::Tensor& data, at::Tensor& scales, c10::optional<at::Tensor> row_scale,
                   bool nv) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1),
-              "fp4_quantize: x must be a CUDA matrix with contiguous columns");
+  TORCH_CHECK(x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1),
+              "fp4_quantize: x must be a matrix with contiguous columns");
   const int64_t R = x.size(0), K = x.size(1);
   check_fp4(data, scales, row_scale, nv, R, K, x.device(), "fp4_quantize");
+  TORCH_CHECK(x.is_cuda(), "fp4_quantize: x must be a CUDA tensor");
   if (R == 0) return;
   c10::cuda::CUDAGuard guard(x.device());
   QuantParams p;

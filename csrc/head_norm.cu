@@ -373,7 +373,7 @@ std::pair<int64_t, int64_t> check_heads(const at::Tensor& t, const at::Tensor& l
                                         const char* name) {
   TORCH_CHECK(t.device() == like.device() && t.scalar_type() == like.scalar_type() && t.dim() == 3 && t.size(0) == R &&
                   t.size(1) == H && t.size(2) == hd,
-              name, " must be [", R, ", ", H, ", ", hd, "] of the type and on the device of the queries");
+              name, " must be [", num(R), ", ", num(H), ", ", num(hd), "] of the type and on the device of the queries");
   const int64_t per16 = 16 / (int64_t)t.element_size();
   TORCH_CHECK(t.numel() == 0 || (t.stride(2) == 1 && (H == 1 || t.stride(1) % per16 == 0) &&
                                  (R == 1 || t.stride(0) % per16 == 0) &&
@@ -406,7 +406,7 @@ RotMode fill_common(Params& p, const at::Tensor& q, const at::Tensor& k, const c
     if (ws[i]->has_value() && (*ws[i])->defined()) {
       const at::Tensor& w = **ws[i];
       TORCH_CHECK(w.device() == q.device() && w.dim() == 1 && w.size(0) == hd && w.is_contiguous(),
-                  "head_norm_rope: a weight must be contiguous [", hd, "] on the device of the queries");
+                  "head_norm_rope: a weight must be contiguous [", num(hd), "] on the device of the queries");
       s.w = w.data_ptr();
       s.wtype = float_type(w, "head_norm_rope: a weight");
     }
@@ -428,7 +428,7 @@ RotMode fill_common(Params& p, const at::Tensor& q, const at::Tensor& k, const c
                     t->sizes() == cosT->sizes() && t->size(0) >= 1,
                 "head_norm_rope: cos and sin must be contiguous fp32 [T, rot / 2] on the device of the queries, T >= 1");
   p.rot = (int)cosT->size(1) * 2;
-  TORCH_CHECK(cosT->size(1) * 2 <= hd, "head_norm_rope: the tables turn ", cosT->size(1) * 2, " of ", hd, " elements");
+  TORCH_CHECK(cosT->size(1) * 2 <= hd, "head_norm_rope: the tables turn ", num(cosT->size(1) * 2), " of ", num(hd), " elements");
   if (p.rot == 0) return kNone;
   p.T = cosT->size(0);
   p.cosT = cosT->data_ptr<float>();
@@ -437,7 +437,7 @@ RotMode fill_common(Params& p, const at::Tensor& q, const at::Tensor& k, const c
     TORCH_CHECK(positions->device() == q.device() && positions->dim() == 1 && positions->size(0) == R &&
                     positions->is_contiguous() &&
                     (positions->scalar_type() == at::kLong || positions->scalar_type() == at::kInt),
-                "head_norm_rope: positions must be contiguous int32 or int64 [", R, "] on the device of the queries");
+                "head_norm_rope: positions must be contiguous int32 or int64 [", num(R), "] on the device of the queries");
     p.positions = positions->data_ptr();
     p.pos64 = positions->scalar_type() == at::kLong ? 1 : 0;
   }
@@ -536,7 +536,7 @@ void head_norm_rope_bwd(const at::Tensor& gq, const at::Tensor& gk, const at::Te
     if (dws[i]->has_value() && (*dws[i])->defined()) {
       const at::Tensor& dw = **dws[i];
       TORCH_CHECK(dw.device() == q.device() && dw.dim() == 1 && dw.size(0) == p.hd && dw.is_contiguous(),
-                  "head_norm_rope: a weight gradient must be contiguous [", p.hd, "]");
+                  "head_norm_rope: a weight gradient must be contiguous [", num(p.hd), "]");
       dwp[i] = dw.data_ptr();
       dwt[i] = float_type(dw, "head_norm_rope: a weight gradient");
     }

@@ -102,3 +102,21 @@ def test_refusals():
             f()
     with torch.no_grad():
         assert ops.fp4_linear(g, w).shape == (4, 8)
+
+
+def test_native_checks_raise():
+    """The extension's own checks end in a Python error, numbers in their messages included."""
+    if not ops.native_available():
+        pytest.skip("extension not built")
+    e = ops.ext()
+    x = torch.randn(4, 64)
+    q = ops.quantize_fp4(torch.randn(8, 64))
+    for f in (lambda: e.fp4_quantize(x, q.data, q.scales, q.row_scale, True),
+              lambda: e.fp4_quantize(x[:, :63], q.data[:4], q.scales, q.row_scale, True),
+              lambda: e.fp4_quantize(x, q.data[:4], q.scales, q.row_scale, True),
+              lambda: e.fp4_quantize(x, q.data[:4], q.scales, q.row_scale[:4], True),
+              lambda: e.fp4_dequantize(q.data, q.scales, q.row_scale, x, True),
+              lambda: e.fp4_gemm(q.data, q.scales, q.row_scale, q.data, q.scales, q.row_scale, None, x, 64, True),
+              lambda: e.head_norm_rope_fwd(x, x, None, None, None, None, None, x, x, 1e-6, True)):
+        with pytest.raises(RuntimeError):
+            f()
