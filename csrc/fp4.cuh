@@ -28,6 +28,18 @@ __host__ __device__ __forceinline__ int64_t fp4_scale_offset(int64_t row, int64_
   return ((row >> 7) * ktiles + (block >> 2)) * kFp4TileBytes + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
 }
 
+// 32-byte accesses (whole sectors; 32-byte aligned addresses).
+__device__ __forceinline__ void ld256(const void* p, uint32_t* w) {
+  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void st256(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 // ---------------------------------------------------------------- conversions
 // Eight floats -> eight e2m1 codes (v[0] in the low four bits): nearest, halves to the even code, 6 at most.
 __device__ __forceinline__ uint32_t float8_to_e2m1x8(const float (&v)[8]) {

@@ -51,6 +51,8 @@ struct Smem {
   uint8_t b[kStages][kBBytes];
   uint8_t sa[kStages][kSaBytes];
   uint8_t sb[kStages][kSbBytes];
+  float2 col[2][kBN];                  // row factor of B and bias of a tile's columns, by tile parity
+  uint16_t stage[4][32][18];           // a warp's 32 rows x 16 columns on their way to unaligned rows of D
   uint64_t full[kStages], empty[kStages];
   uint64_t acc_full[2], acc_free;
   uint64_t drain;
@@ -68,6 +70,7 @@ struct Params {
   const void* bias;
   int bias_type;  // 0 fp32, 1 bf16, 2 fp16
   int out_fp16;
+  int vec;        // bytes of a store: 32, 16 or 2, by the alignment of D's rows
   int M, N, K;
   int ktiles;     // scale tiles along K
   int ksteps;     // stages along K
@@ -98,6 +101,39 @@ __device__ __forceinline__ void tile_coords(const Params& p, int t, int& tm, int
   const int in = t % (kGroup * p.tiles_n);
   tm = first_m + in % gm;
   tn = in / gm;
+}
+
+// Stores 32 columns from nc of this lane's row (a warp holds rows m0 .. m0 + 31).  Whole 32-byte sectors where the
+// rows of D allow it; other rows go through shared memory, so that a warp still writes runs of 32 bytes.
+__device__ __forceinline__ void store_chunk(const Params& p, uint16_t (*stage)[18], uint16_t* drow, int m0, int nc,
+                                            const uint32_t (&o)[16]) {
+  const int lane = lane_id();
+  if (p.vec == 32) {  // N % 16 == 0: a group of 16 columns is inside the row or past it
+    if (m0 + lane < p.M) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        if (nc + 16 * q < p.N) st256(drow + nc + 16 * q, o + 8 * q);
+    }
+  } else if (p.vec == 16) {
+    if (m0 + lane < p.M) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (nc + 8 * q < p.N)
+          *reinterpret_cast<uint4*>(drow + nc + 8 * q) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+    }
+  } else {
+    uint16_t* d0 = static_cast<uint16_t*>(p.d) + (int64_t)m0 * p.ldd + nc;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      __syncwarp();
+#pragma unroll
+      for (int q = 0; q < 8; ++q) *reinterpret_cast<uint32_t*>(&stage[lane][2 * q]) = o[8 * h + q];
+      __syncwarp();
+      const int cc = lane & 15, n = 16 * h + cc;
+      for (int r = lane >> 4; r < 32; r += 2)
+        if (m0 + r < p.M && nc + n < p.N) d0[(int64_t)r * p.ldd + n] = stage[r][cc];
+    }
+  }
 }
 
 template <bool NV>
@@ -211,17 +247,25 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
     const int wq = warp & 3;  // TMEM lane quarter this warp may access
     const int row = wq * 32 + lane;
     const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
-    const bool vec = p.N % 8 == 0;  // 16-byte stores: rows of D are multiples of 16 bytes
+    const int et = threadIdx.x - 64;
     int tl = 0;
     for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x, ++tl) {
-      if (!__all_sync(0xffffffffu,
-                      mbar_wait(&sm.acc_full[tl & 1], (tl >> 1) & 1, kStatusTimeoutMma, abort_flag, p.status)))
-        break;
-      tc_fence_after();
       int tm, tn;
       tile_coords(p, t, tm, tn);
       const int m = tm * kBM + row;
-      const float ra = (NV && m < p.M) ? p.ra[m] : 1.f;
+      // the tile's column factors and biases, read while its MMAs run (a buffer is written again only after
+      // the barrier of the tile in between)
+      float2* col = sm.col[tl & 1];
+#pragma unroll
+      for (int i = et; i < kBN; i += 128) {
+        const int n = min(tn * kBN + i, p.N - 1);
+        col[i] = make_float2(NV ? __ldg(p.rb + n) : 1.f, p.bias != nullptr ? load_bias(p, n) : 0.f);
+      }
+      const float ra = (NV && m < p.M) ? __ldg(p.ra + m) : 1.f;
+      const bool ok = mbar_wait(&sm.acc_full[tl & 1], (tl >> 1) & 1, kStatusTimeoutMma, abort_flag, p.status);
+      // also the barrier of the column factors; all four warps leave together, since it counts them
+      if (named_bar_any(1, 128, !ok)) break;
+      tc_fence_after();
       uint16_t* drow = static_cast<uint16_t*>(p.d) + (int64_t)m * p.ldd;
       const uint32_t acc = tmem + lane_base + ((tl & 1) ? kAcc1 : 0);
       // chunks of 32 columns, the ones shared with the other accumulator first: the last three of the
@@ -237,29 +281,16 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
           mbar_arrive(&sm.acc_free);
         }
         const int nc = tn * kBN + c * 32;
-        if (m < p.M && nc < p.N) {
-          float v[32];
+        if (nc >= p.N) continue;
+        uint32_t o[16];
+        const float4* cf = reinterpret_cast<const float4*>(col + c * 32);
 #pragma unroll
-          for (int q = 0; q < 32; ++q) {
-            float x = __uint_as_float(r[q]);
-            const int n = min(nc + q, p.N - 1);
-            if (NV) x *= ra * __ldg(p.rb + n);
-            if (p.bias != nullptr) x += load_bias(p, n);
-            v[q] = x;
-          }
-          if (vec) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (nc + q * 8 < p.N)
-                *reinterpret_cast<uint4*>(drow + nc + q * 8) =
-                    make_uint4(pack_out(p, v[8 * q], v[8 * q + 1]), pack_out(p, v[8 * q + 2], v[8 * q + 3]),
-                               pack_out(p, v[8 * q + 4], v[8 * q + 5]), pack_out(p, v[8 * q + 6], v[8 * q + 7]));
-          } else {
-#pragma unroll
-            for (int q = 0; q < 32; ++q)
-              if (nc + q < p.N) drow[nc + q] = (uint16_t)pack_out(p, v[q], 0.f);
-          }
+        for (int q = 0; q < 16; ++q) {
+          const float4 f = cf[q];
+          o[q] = pack_out(p, fmaf(__uint_as_float(r[2 * q]) * ra, f.x, f.y),
+                          fmaf(__uint_as_float(r[2 * q + 1]) * ra, f.z, f.w));
         }
+        store_chunk(p, sm.stage[wq], drow, m - lane, nc, o);
       }
     }
   }
@@ -318,6 +349,8 @@ void fp4_gemm(const at::Tensor& a, const at::Tensor& sa, c10::optional<at::Tenso
   p.ra = nv ? ra->data_ptr<float>() : nullptr;
   p.rb = nv ? rb->data_ptr<float>() : nullptr;
   p.out_fp16 = d.scalar_type() == at::kHalf ? 1 : 0;
+  const uintptr_t align = reinterpret_cast<uintptr_t>(p.d) | (uintptr_t)(2 * N);
+  p.vec = align % 32 == 0 ? 32 : align % 16 == 0 ? 16 : 2;
   p.M = (int)M;
   p.N = (int)N;
   p.K = (int)K;

@@ -32,17 +32,6 @@ struct Unit {  // 16 elements
   uint32_t w[4 * sizeof(T)];
 };
 
-__device__ __forceinline__ void ld256(const void* p, uint32_t* w) {
-  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4]), "=r"(w[5]), "=r"(w[6]), "=r"(w[7])
-               : "l"(p));
-}
-__device__ __forceinline__ void st256(void* p, const uint32_t* w) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-               : "memory");
-}
-
 template <typename T, bool ALIGNED>
 __device__ __forceinline__ Unit<T> load_unit(const T* __restrict__ row, int c0, int K) {
   Unit<T> u;
