@@ -73,17 +73,20 @@ void gemm_bf16(const at::Tensor& a, const at::Tensor& b, c10::optional<at::Tenso
 void gemm_bf16_ex(const at::Tensor& a, const at::Tensor& b, c10::optional<at::Tensor> a2, c10::optional<at::Tensor> b2,
                   c10::optional<at::Tensor> bias, c10::optional<at::Tensor> d, c10::optional<at::Tensor> d32,
                   double alpha, int64_t act, bool a_mn, bool b_mn, int64_t split);
-void fp4_quantize(const at::Tensor& x, at::Tensor& data, at::Tensor& scales, c10::optional<at::Tensor> row_scale,
-                  bool nv);
-void fp4_dequantize(const at::Tensor& data, const at::Tensor& scales, c10::optional<at::Tensor> row_scale,
-                    at::Tensor& out, bool nv);
-void fp4_gemm(const at::Tensor& a, const at::Tensor& sa, c10::optional<at::Tensor> ra, const at::Tensor& b,
-              const at::Tensor& sb, c10::optional<at::Tensor> rb, c10::optional<at::Tensor> bias, at::Tensor& d,
-              int64_t K, bool nv);
-void head_norm_rope_fwd(const at::Tensor& q, const at::Tensor& k, c10::optional<at::Tensor> wq,
-                        c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cosT, c10::optional<at::Tensor> sinT,
-                        c10::optional<at::Tensor> positions, at::Tensor& qo, at::Tensor& ko, double eps,
-                        bool interleaved);
+std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> fp4_quantize(const at::Tensor& x, bool nv);
+at::Tensor fp4_dequantize(const at::Tensor& data, const at::Tensor& scales, c10::optional<at::Tensor> row_scale,
+                          int64_t R, int64_t K, bool nv, int64_t type);
+at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& data, const at::Tensor& scales,
+                      c10::optional<at::Tensor> row_scale, c10::optional<at::Tensor> bias, int64_t N, int64_t K, bool nv,
+                      int64_t out_type);
+at::Tensor fp4_matmul(const at::Tensor& xdata, const at::Tensor& xscales, c10::optional<at::Tensor> xrow_scale,
+                      int64_t M, const at::Tensor& data, const at::Tensor& scales, c10::optional<at::Tensor> row_scale,
+                      c10::optional<at::Tensor> bias, int64_t N, int64_t K, bool nv, int64_t out_type);
+std::tuple<at::Tensor, at::Tensor> head_norm_rope_fwd(const at::Tensor& q, const at::Tensor& k,
+                                                      c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk,
+                                                      c10::optional<at::Tensor> cosT, c10::optional<at::Tensor> sinT,
+                                                      c10::optional<at::Tensor> positions, double eps,
+                                                      bool interleaved);
 void head_norm_rope_bwd(const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q, const at::Tensor& k,
                         c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cosT,
                         c10::optional<at::Tensor> sinT, c10::optional<at::Tensor> positions, at::Tensor& dq,
@@ -139,7 +142,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_bf16_ex", &dmad::gemm_bf16_ex);
   m.def("fp4_quantize", &dmad::fp4_quantize);
   m.def("fp4_dequantize", &dmad::fp4_dequantize);
-  m.def("fp4_gemm", &dmad::fp4_gemm);
+  m.def("fp4_linear", &dmad::fp4_linear);
+  m.def("fp4_matmul", &dmad::fp4_matmul);
   m.def("head_norm_rope_fwd", &dmad::head_norm_rope_fwd);
   m.def("head_norm_rope_bwd", &dmad::head_norm_rope_bwd);
   m.def("fsdp_gather", &dmad::fsdp_gather);

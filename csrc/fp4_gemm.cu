@@ -23,15 +23,14 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include "common.cuh"
-#include "fp4.cuh"
+#include "fp4_host.h"
 #include "sm100.cuh"
 #include "tma_host.h"
 
 namespace dmad {
 
 int* device_status_ptr(int device);
-void check_fp4(const at::Tensor& data, const at::Tensor& scales, const c10::optional<at::Tensor>& row_scale, bool nv,
-               int64_t R, int64_t K, const at::Device& device, const char* name);
+at::Tensor fp4_rows(const at::Tensor& x, const char* name);
 
 namespace {
 
@@ -302,70 +301,113 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
   }
 }
 
-CUtensorMap code_map(const at::Tensor& x, uint32_t box_rows) {
-  const uint64_t dims[2] = {(uint64_t)x.size(1), (uint64_t)x.size(0)};
-  const uint64_t strides[1] = {(uint64_t)x.size(1)};
+CUtensorMap code_map(const Fp4Matrix& x, uint32_t box_rows) {
+  const uint64_t dims[2] = {(uint64_t)x.row_bytes(), (uint64_t)x.rows};
+  const uint64_t strides[1] = {(uint64_t)x.row_bytes()};
   const uint32_t box[2] = {128u, box_rows};
-  return make_tmap_u8(x.data_ptr(), 2, dims, strides, box);
+  return make_tmap_u8(x.data, 2, dims, strides, box);
 }
 
 template <bool NV>
-void launch(const CUtensorMap& ma, const CUtensorMap& mb, const Params& p, int sms, cudaStream_t stream) {
+void launch(const CUtensorMap& ma, const CUtensorMap& mb, const Params& p, int device, cudaStream_t stream) {
   const int smem = (int)sizeof(Smem) + 1024;
-  C10_CUDA_CHECK(cudaFuncSetAttribute(fp4_gemm_kernel<NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  fp4_gemm_kernel<NV><<<std::min(p.num_tiles, sms), 192, smem, stream>>>(ma, mb, p);
+  static std::array<std::atomic<bool>, 64> configured{};
+  if (device >= 64 || !configured[device].load(std::memory_order_acquire)) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(fp4_gemm_kernel<NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (device < 64) configured[device].store(true, std::memory_order_release);
+  }
+  fp4_gemm_kernel<NV><<<std::min(p.num_tiles, sm_count(device)), 192, smem, stream>>>(ma, mb, p);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-}  // namespace
-
-// d [M, N] (bf16 or fp16, contiguous) = A B^T with A [M, K], B [N, K] stored as fp4.cuh says, + bias [N].
-void fp4_gemm(const at::Tensor& a, const at::Tensor& sa, c10::optional<at::Tensor> ra, const at::Tensor& b,
-              const at::Tensor& sb, c10::optional<at::Tensor> rb, c10::optional<at::Tensor> bias, at::Tensor& d,
-              int64_t K, bool nv) {
-  TORCH_CHECK(d.is_cuda() && d.dim() == 2 && d.is_contiguous() &&
-                  (d.scalar_type() == at::kBFloat16 || d.scalar_type() == at::kHalf),
-              "fp4_gemm: d must be a contiguous CUDA bf16 or fp16 matrix");
-  const int64_t M = d.size(0), N = d.size(1);
-  check_fp4(a, sa, ra, nv, M, K, d.device(), "fp4_gemm: a");
-  check_fp4(b, sb, rb, nv, N, K, d.device(), "fp4_gemm: b");
+// d [a.rows, b.rows] (bf16 or fp16, contiguous) = a b^T + bias, on the current device and stream.
+void gemm(const Fp4Matrix& a, const Fp4Matrix& b, const c10::optional<at::Tensor>& bias, at::Tensor& d,
+          cudaStream_t stream) {
+  const int64_t M = a.rows, N = b.rows, K = a.cols;
+  if (M == 0 || N == 0) return;
   Params p;
   p.bias = nullptr;
   p.bias_type = 0;
   if (bias.has_value() && bias->defined()) {
-    TORCH_CHECK(bias->device() == d.device() && bias->dim() == 1 && bias->size(0) == N && bias->is_contiguous() &&
-                    (bias->scalar_type() == at::kFloat || bias->scalar_type() == at::kBFloat16 ||
-                     bias->scalar_type() == at::kHalf),
-                "fp4_gemm: bias must be contiguous fp32, bf16 or fp16 [", num(N), "] on d's device");
     p.bias = bias->data_ptr();
     p.bias_type = bias->scalar_type() == at::kFloat ? 0 : bias->scalar_type() == at::kBFloat16 ? 1 : 2;
   }
-  if (M == 0 || N == 0) return;
-  c10::cuda::CUDAGuard guard(d.device());
   p.d = d.data_ptr();
   p.ldd = N;
-  p.sa = sa.data_ptr<uint8_t>();
-  p.sb = sb.data_ptr<uint8_t>();
-  p.ra = nv ? ra->data_ptr<float>() : nullptr;
-  p.rb = nv ? rb->data_ptr<float>() : nullptr;
+  p.sa = a.scales;
+  p.sb = b.scales;
+  p.ra = a.row_scale;
+  p.rb = b.row_scale;
   p.out_fp16 = d.scalar_type() == at::kHalf ? 1 : 0;
   const uintptr_t align = reinterpret_cast<uintptr_t>(p.d) | (uintptr_t)(2 * N);
   p.vec = align % 32 == 0 ? 32 : align % 16 == 0 ? 16 : 2;
   p.M = (int)M;
   p.N = (int)N;
   p.K = (int)K;
-  p.ktiles = (int)sa.size(1);
+  p.ktiles = (int)a.ktiles();
   p.ksteps = (int)((K + kBK - 1) / kBK);
   p.tiles_m = (int)((M + kBM - 1) / kBM);
   p.tiles_n = (int)((N + kBN - 1) / kBN);
-  TORCH_CHECK((int64_t)p.tiles_m * p.tiles_n <= INT32_MAX, "fp4_gemm: too many output tiles");
+  DMAD_VALUE_CHECK((int64_t)p.tiles_m * p.tiles_n <= INT32_MAX, "fp4_linear: too many output tiles");
   p.num_tiles = p.tiles_m * p.tiles_n;
-  p.status = device_status_ptr(d.get_device());
-  int sms = 148;
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, d.get_device());
+  const int device = d.get_device();
+  p.status = device_status_ptr(device);
   const CUtensorMap ma = code_map(a, kBM), mb = code_map(b, kBN);
+  a.nv ? launch<true>(ma, mb, p, device, stream) : launch<false>(ma, mb, p, device, stream);
+}
+
+c10::optional<at::Tensor> checked_bias(const c10::optional<at::Tensor>& bias, int64_t N, const at::Device& device) {
+  if (!(bias.has_value() && bias->defined())) return c10::nullopt;
+  DMAD_VALUE_CHECK(bias->device() == device && bias->dim() == 1 && bias->size(0) == N && is_float_type(bias->scalar_type()),
+                   "fp4_linear: bias must be bf16, fp16 or fp32 (" + num(N) + ",) on the device of w, got " +
+                       dtype_name(bias->scalar_type()) + " " + shape_text(*bias));
+  return bias->contiguous();
+}
+
+}  // namespace
+
+// x W^T + bias for x [..., K] (bf16 or fp16), quantised here, and W [N, K] stored in 4 bits; the result in bf16 (0),
+// fp16 (1) or x's type (-1).
+at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& data, const at::Tensor& scales,
+                      c10::optional<at::Tensor> row_scale, c10::optional<at::Tensor> bias, int64_t N, int64_t K, bool nv,
+                      int64_t out_type) {
+  const auto dt = x.scalar_type();
+  DMAD_VALUE_CHECK(x.is_cuda() && (dt == at::kBFloat16 || dt == at::kHalf), "fp4_linear: x must be bf16 or fp16 on CUDA");
+  DMAD_VALUE_CHECK(x.dim() >= 1 && x.size(-1) == K, "fp4_linear: x " + shape_text(x) + " must have " + num(K) + " columns");
+  const Fp4Matrix w = fp4_matrix(data, scales, row_scale, N, K, nv, x.device(), "fp4_linear: w");
+  const auto b = checked_bias(bias, N, x.device());
+  const at::Tensor x2 = fp4_rows(x, "fp4_linear");
+  Fp4Matrix q{nullptr, nullptr, nullptr, x2.size(0), K, nv};
+  DMAD_VALUE_CHECK(q.rows <= INT32_MAX - 256, "fp4_linear: sizes out of range");
+  c10::cuda::CUDAGuard guard(x.device());
+  // codes, scales and row factors of x in one piece, freed to the stream's pool when the call returns
+  const int64_t at_scales = (q.data_bytes() + 511) / 512 * 512, at_rows = at_scales + q.scale_bytes();
+  const auto plain = x.options().requires_grad(false);
+  at::Tensor work = at::empty({at_rows + (nv ? 4 * q.rows : 0)}, plain.dtype(at::kByte));
+  q.data = work.data_ptr<uint8_t>();
+  q.scales = q.data + at_scales;
+  q.row_scale = nv ? reinterpret_cast<float*>(q.data + at_rows) : nullptr;
+  c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  at::Tensor y = at::empty(shape, plain.dtype(out_type == 0 ? at::kBFloat16 : out_type == 1 ? at::kHalf : dt));
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  nv ? launch<true>(ma, mb, p, sms, stream) : launch<false>(ma, mb, p, sms, stream);
+  fp4_quantize_launch(x2, q, stream);
+  gemm(q, w, b, y, stream);
+  return y;
+}
+
+// The same for an x [M, K] that is stored in 4 bits; the result [M, N] in bf16 (0) or fp16 (1).
+at::Tensor fp4_matmul(const at::Tensor& xdata, const at::Tensor& xscales, c10::optional<at::Tensor> xrow_scale,
+                      int64_t M, const at::Tensor& data, const at::Tensor& scales, c10::optional<at::Tensor> row_scale,
+                      c10::optional<at::Tensor> bias, int64_t N, int64_t K, bool nv, int64_t out_type) {
+  DMAD_VALUE_CHECK(data.is_cuda(), "fp4_linear: the native kernel takes CUDA tensors");
+  const Fp4Matrix w = fp4_matrix(data, scales, row_scale, N, K, nv, data.device(), "fp4_linear: w");
+  const Fp4Matrix q = fp4_matrix(xdata, xscales, xrow_scale, M, K, nv, data.device(), "fp4_linear: x");
+  const auto b = checked_bias(bias, N, data.device());
+  c10::cuda::CUDAGuard guard(data.device());
+  at::Tensor y = at::empty({M, N}, data.options().dtype(out_type == 1 ? at::kHalf : at::kBFloat16));
+  gemm(q, w, b, y, at::cuda::getCurrentCUDAStream());
+  return y;
 }
 
 }  // namespace dmad

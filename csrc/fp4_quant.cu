@@ -20,7 +20,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include "common.cuh"
-#include "fp4.cuh"
+#include "fp4_host.h"
 
 namespace dmad {
 namespace {
@@ -316,99 +316,112 @@ __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict_
 }
 
 template <typename O, bool NV>
-void launch_dequant(const at::Tensor& data, const at::Tensor& scales, const float* rs, at::Tensor& out,
-                    cudaStream_t stream) {
-  const int R = (int)out.size(0), K = (int)out.size(1);
+void launch_dequant(const Fp4Matrix& q, at::Tensor& out, cudaStream_t stream) {
+  const int R = (int)q.rows, K = (int)q.cols, row_bytes = (int)q.row_bytes(), ktiles = (int)q.ktiles();
   const int units = (K + 15) / 16;
   const int tx = std::min(256, (units + 31) / 32 * 32), ty = 256 / tx;
   const unsigned grid = (unsigned)((R + ty - 1) / ty);
   const bool aligned = K % 16 == 0 && reinterpret_cast<uintptr_t>(out.data_ptr()) % 32 == 0;
-  auto* d = data.data_ptr<uint8_t>();
-  auto* s = scales.data_ptr<uint8_t>();
   O* o = reinterpret_cast<O*>(out.data_ptr());
   if (aligned)
-    dequant_kernel<O, NV, true><<<grid, dim3(tx, ty), 0, stream>>>(d, (int)data.size(1), s, (int)scales.size(1), rs, o, R, K);
+    dequant_kernel<O, NV, true><<<grid, dim3(tx, ty), 0, stream>>>(q.data, row_bytes, q.scales, ktiles, q.row_scale, o, R, K);
   else
-    dequant_kernel<O, NV, false><<<grid, dim3(tx, ty), 0, stream>>>(d, (int)data.size(1), s, (int)scales.size(1), rs, o, R, K);
+    dequant_kernel<O, NV, false><<<grid, dim3(tx, ty), 0, stream>>>(q.data, row_bytes, q.scales, ktiles, q.row_scale, o, R, K);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 }  // namespace
 
-// Shapes, types and placement of a stored 4-bit matrix [R, K].  Numbers in the messages
-// go through num(): see common.cuh.
-void check_fp4(const at::Tensor& data, const at::Tensor& scales, const c10::optional<at::Tensor>& row_scale, bool nv,
-               int64_t R, int64_t K, const at::Device& device, const char* name) {
-  const int64_t block = fp4_block(nv);
-  const int64_t ktiles = ((K + block - 1) / block + kFp4TileBlocks - 1) / kFp4TileBlocks;
-  TORCH_CHECK(K >= 1 && K <= (1 << 24) && R >= 0 && R <= INT32_MAX - 256, name, ": sizes out of range");
-  TORCH_CHECK(data.device() == device && data.scalar_type() == at::kByte && data.dim() == 2 && data.size(0) == R &&
-                  data.size(1) == (K + 31) / 32 * 16 && data.is_contiguous(),
-              name, ".data must be contiguous uint8 [", num(R), ", ", num((K + 31) / 32 * 16), "] on the device of the output");
-  TORCH_CHECK(scales.device() == device && scales.scalar_type() == at::kByte && scales.dim() == 3 &&
-                  scales.size(0) == (R + kFp4TileRows - 1) / kFp4TileRows && scales.size(1) == ktiles &&
-                  scales.size(2) == kFp4TileBytes && scales.is_contiguous(),
-              name, ".scales must be contiguous uint8 [", num((R + kFp4TileRows - 1) / kFp4TileRows), ", ", num(ktiles),
-              ", 512] on the device of the output");
-  TORCH_CHECK(reinterpret_cast<uintptr_t>(data.data_ptr()) % 16 == 0 &&
-                  reinterpret_cast<uintptr_t>(scales.data_ptr()) % 16 == 0,
-              name, ": data and scales must be 16-byte aligned");
-  if (nv) {
-    TORCH_CHECK(row_scale.has_value() && row_scale->defined() && row_scale->device() == device &&
-                    row_scale->scalar_type() == at::kFloat && row_scale->dim() == 1 && row_scale->size(0) == R &&
-                    row_scale->is_contiguous(),
-                name, ".row_scale must be contiguous fp32 [", num(R), "] on the device of the output");
-  }
+Fp4Matrix fp4_matrix(const at::Tensor& data, const at::Tensor& scales, const c10::optional<at::Tensor>& row_scale,
+                     int64_t rows, int64_t cols, bool nv, const at::Device& device, const char* name) {
+  Fp4Matrix m{nullptr, nullptr, nullptr, rows, cols, nv};
+  const std::string who(name);
+  DMAD_VALUE_CHECK(cols >= 1 && cols <= (1 << 24) && rows >= 0 && rows <= INT32_MAX - 256, who + ": sizes out of range");
+  DMAD_VALUE_CHECK(data.scalar_type() == at::kByte && data.dim() == 2 && data.size(0) == rows &&
+                       data.size(1) == m.row_bytes() && data.is_contiguous(),
+                   who + ".data must be contiguous uint8 (" + num(rows) + ", " + num(m.row_bytes()) + "), got " +
+                       shape_text(data));
+  DMAD_VALUE_CHECK(scales.scalar_type() == at::kByte && scales.dim() == 3 && scales.size(0) == m.row_tiles() &&
+                       scales.size(1) == m.ktiles() && scales.size(2) == kFp4TileBytes && scales.is_contiguous(),
+                   who + ".scales must be contiguous uint8 (" + num(m.row_tiles()) + ", " + num(m.ktiles()) +
+                       ", 512), got " + shape_text(scales));
+  const bool has_rs = row_scale.has_value() && row_scale->defined();
+  DMAD_VALUE_CHECK(nv == has_rs, who + ": nvfp4 has a row_scale and mxfp4 has none");
+  DMAD_VALUE_CHECK(!nv || (row_scale->scalar_type() == at::kFloat && row_scale->dim() == 1 &&
+                           row_scale->size(0) == rows && row_scale->is_contiguous()),
+                   who + ".row_scale must be contiguous fp32 (" + num(rows) + ",)");
+  DMAD_VALUE_CHECK(data.device() == device && scales.device() == device && (!nv || row_scale->device() == device),
+                   who + ": all tensors must be on one device");
+  m.data = data.data_ptr<uint8_t>();
+  m.scales = scales.data_ptr<uint8_t>();
+  m.row_scale = nv ? row_scale->data_ptr<float>() : nullptr;
+  DMAD_VALUE_CHECK(reinterpret_cast<uintptr_t>(m.data) % 16 == 0 && reinterpret_cast<uintptr_t>(m.scales) % 16 == 0,
+                   who + ": data and scales must start on 16 bytes");
+  return m;
 }
 
-// x [R, K] (bf16, fp16 or fp32, contiguous columns, any row stride) -> data, scales, row_scale (nvfp4).
-void fp4_quantize(const at::Tensor& x, at::Tensor& data, at::Tensor& scales, c10::optional<at::Tensor> row_scale,
-                  bool nv) {
-  TORCH_CHECK(x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1),
-              "fp4_quantize: x must be a matrix with contiguous columns");
-  const int64_t R = x.size(0), K = x.size(1);
-  check_fp4(data, scales, row_scale, nv, R, K, x.device(), "fp4_quantize");
-  TORCH_CHECK(x.is_cuda(), "fp4_quantize: x must be a CUDA tensor");
-  if (R == 0) return;
-  c10::cuda::CUDAGuard guard(x.device());
+void fp4_quantize_launch(const at::Tensor& x, const Fp4Matrix& q, cudaStream_t stream) {
+  if (q.rows == 0) return;
   QuantParams p;
   p.x = x.data_ptr();
   p.ld = x.stride(0);
-  p.R = (int)R;
-  p.K = (int)K;
-  p.data = data.data_ptr<uint8_t>();
-  p.scales = scales.data_ptr<uint8_t>();
-  p.row_scale = nv ? row_scale->data_ptr<float>() : nullptr;
-  p.row_bytes = (int)data.size(1);
-  p.ktiles = (int)scales.size(1);
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  switch (x.scalar_type()) {
-    case at::kBFloat16: quant_typed<__nv_bfloat16>(p, nv, stream); break;
-    case at::kHalf: quant_typed<__half>(p, nv, stream); break;
-    case at::kFloat: quant_typed<float>(p, nv, stream); break;
-    default: TORCH_CHECK(false, "fp4_quantize: x must be bf16, fp16 or fp32");
-  }
+  p.R = (int)q.rows;
+  p.K = (int)q.cols;
+  p.data = q.data;
+  p.scales = q.scales;
+  p.row_scale = q.row_scale;
+  p.row_bytes = (int)q.row_bytes();
+  p.ktiles = (int)q.ktiles();
+  if (x.scalar_type() == at::kBFloat16) quant_typed<__nv_bfloat16>(p, q.nv, stream);
+  else if (x.scalar_type() == at::kHalf) quant_typed<__half>(p, q.nv, stream);
+  else quant_typed<float>(p, q.nv, stream);
 }
 
-// out [R, K] (bf16, fp16 or fp32, contiguous) = the values that the codes stand for, rounded to out's type.
-void fp4_dequantize(const at::Tensor& data, const at::Tensor& scales, c10::optional<at::Tensor> row_scale,
-                    at::Tensor& out, bool nv) {
-  TORCH_CHECK(out.is_cuda() && out.dim() == 2 && out.is_contiguous(), "fp4_dequantize: out must be a contiguous CUDA matrix");
-  check_fp4(data, scales, row_scale, nv, out.size(0), out.size(1), out.device(), "fp4_dequantize");
-  if (out.size(0) == 0) return;
-  c10::cuda::CUDAGuard guard(out.device());
-  const float* rs = nv ? row_scale->data_ptr<float>() : nullptr;
+// x [..., K] as a matrix [R, K] with contiguous columns.
+at::Tensor fp4_rows(const at::Tensor& x, const char* name) {
+  DMAD_VALUE_CHECK(x.dim() >= 1 && x.size(-1) >= 1, std::string(name) + ": the last dimension must hold at least one "
+                                                                        "column, got " + shape_text(x));
+  const int64_t K = x.size(-1);
+  at::Tensor r = x.dim() == 2 ? x : x.reshape({x.numel() / K, K});
+  return r.stride(1) == 1 || K == 1 ? r : r.contiguous();
+}
+
+// (data, scales, row_scale) of x [..., K] (bf16, fp16 or fp32 on CUDA).
+std::tuple<at::Tensor, at::Tensor, c10::optional<at::Tensor>> fp4_quantize(const at::Tensor& x, bool nv) {
+  DMAD_VALUE_CHECK(x.is_cuda() && is_float_type(x.scalar_type()), "quantize_fp4: x must be bf16, fp16 or fp32 on CUDA");
+  const at::Tensor x2 = fp4_rows(x, "quantize_fp4");
+  Fp4Matrix q{nullptr, nullptr, nullptr, x2.size(0), x2.size(1), nv};
+  DMAD_VALUE_CHECK(q.cols <= (1 << 24) && q.rows <= INT32_MAX - 256, "quantize_fp4: sizes out of range");
+  c10::cuda::CUDAGuard guard(x.device());
+  const auto bytes = x.options().dtype(at::kByte).requires_grad(false);
+  at::Tensor data = at::empty({q.rows, q.row_bytes()}, bytes);
+  at::Tensor scales = at::empty({q.row_tiles(), q.ktiles(), kFp4TileBytes}, bytes);
+  c10::optional<at::Tensor> rs;
+  if (nv) rs = at::empty({q.rows}, bytes.dtype(at::kFloat));
+  q.data = data.data_ptr<uint8_t>();
+  q.scales = scales.data_ptr<uint8_t>();
+  q.row_scale = nv ? rs->data_ptr<float>() : nullptr;
+  fp4_quantize_launch(x2, q, at::cuda::getCurrentCUDAStream());
+  return {data, scales, rs};
+}
+
+// The values [R, K] that the codes stand for, rounded to bf16 (0), fp16 (1) or fp32 (2).
+at::Tensor fp4_dequantize(const at::Tensor& data, const at::Tensor& scales, c10::optional<at::Tensor> row_scale,
+                          int64_t R, int64_t K, bool nv, int64_t type) {
+  const Fp4Matrix q = fp4_matrix(data, scales, row_scale, R, K, nv, data.device(), "dequantize_fp4");
+  DMAD_VALUE_CHECK(data.is_cuda(), "dequantize_fp4: the native kernel takes CUDA tensors");
+  c10::cuda::CUDAGuard guard(data.device());
+  at::Tensor out = at::empty({R, K}, data.options().dtype(type == 0 ? at::kBFloat16 : type == 1 ? at::kHalf : at::kFloat));
+  if (R == 0) return out;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   auto go = [&](auto tag) {
     using O = decltype(tag);
-    nv ? launch_dequant<O, true>(data, scales, rs, out, stream) : launch_dequant<O, false>(data, scales, rs, out, stream);
+    nv ? launch_dequant<O, true>(q, out, stream) : launch_dequant<O, false>(q, out, stream);
   };
-  switch (out.scalar_type()) {
-    case at::kBFloat16: go(__nv_bfloat16{}); break;
-    case at::kHalf: go(__half{}); break;
-    case at::kFloat: go(float{}); break;
-    default: TORCH_CHECK(false, "fp4_dequantize: out must be bf16, fp16 or fp32");
-  }
+  if (type == 0) go(__nv_bfloat16{});
+  else if (type == 1) go(__half{});
+  else go(float{});
+  return out;
 }
 
 }  // namespace dmad

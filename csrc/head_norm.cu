@@ -19,6 +19,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include "checks.h"
 #include "common.cuh"
 
 namespace dmad {
@@ -361,42 +362,57 @@ head_norm_dw_kernel(const float* __restrict__ pq, const float* __restrict__ pk, 
   }
 }
 
-int float_type(const at::Tensor& t, const char* name) {
-  if (t.scalar_type() == at::kFloat) return 0;
-  if (t.scalar_type() == at::kBFloat16) return 1;
-  TORCH_CHECK(t.scalar_type() == at::kHalf, name, " must be fp32, bf16 or fp16");
-  return 2;
-}
+int float_type(const at::Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : 2; }
 
-// Checks one [R, H, hd] operand and returns its row and head strides.
-std::pair<int64_t, int64_t> check_heads(const at::Tensor& t, const at::Tensor& like, int64_t R, int64_t H, int64_t hd,
-                                        const char* name) {
-  TORCH_CHECK(t.device() == like.device() && t.scalar_type() == like.scalar_type() && t.dim() == 3 && t.size(0) == R &&
-                  t.size(1) == H && t.size(2) == hd,
-              name, " must be [", num(R), ", ", num(H), ", ", num(hd), "] of the type and on the device of the queries");
+const char* const kOp = "qk_head_norm_rope: ";
+
+bool rows_ok(const at::Tensor& t) {
   const int64_t per16 = 16 / (int64_t)t.element_size();
-  TORCH_CHECK(t.numel() == 0 || (t.stride(2) == 1 && (H == 1 || t.stride(1) % per16 == 0) &&
-                                 (R == 1 || t.stride(0) % per16 == 0) &&
-                                 reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0),
-              name, ": heads must be contiguous, row and head strides and the start multiples of 16 bytes");
-  return {t.stride(0), t.stride(1)};
+  return t.numel() == 0 || (t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) % per16 == 0) &&
+                            (t.size(0) == 1 || t.stride(0) % per16 == 0) &&
+                            reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0);
 }
 
-RotMode fill_common(Params& p, const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& wq,
-                    const c10::optional<at::Tensor>& wk, const c10::optional<at::Tensor>& cosT,
-                    const c10::optional<at::Tensor>& sinT, const c10::optional<at::Tensor>& positions, double eps,
-                    bool interleaved) {
-  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && k.dim() == 3, "head_norm_rope: q and k must be CUDA [R, H, hd] tensors");
+// A [R, H, hd] operand that the kernels can read: the tensor itself or a contiguous copy.
+at::Tensor readable(const at::Tensor& t) { return rows_ok(t) ? t : t.contiguous(); }
+
+void check_heads(const at::Tensor& t, const at::Tensor& q, int64_t H, const char* name, bool in_place) {
+  DMAD_VALUE_CHECK(t.device() == q.device() && t.scalar_type() == q.scalar_type() && t.dim() == 3 &&
+                       t.size(0) == q.size(0) && t.size(1) == H && t.size(2) == q.size(2),
+                   std::string(kOp) + name + " must be (" + num(q.size(0)) + ", " + num(H) + ", " + num(q.size(2)) +
+                       ") of the type and on the device of q, got " + shape_text(t));
+  DMAD_VALUE_CHECK(!in_place || rows_ok(t), std::string(kOp) + name +
+                                                ": heads must be contiguous, strides and the start multiples of 16 bytes");
+}
+
+struct Prepared {  // what the kernels' parameters point into
+  at::Tensor x[2], w[2], cosT, sinT, positions;
+  RotMode mode = kNone;
+};
+
+Prepared fill_common(Params& p, const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& wq,
+                     const c10::optional<at::Tensor>& wk, const c10::optional<at::Tensor>& cosT,
+                     const c10::optional<at::Tensor>& sinT, const c10::optional<at::Tensor>& positions, double eps,
+                     bool interleaved) {
+  Prepared keep;
+  const std::string op(kOp);
+  DMAD_VALUE_CHECK(q.dim() == 3 && k.dim() == 3 && is_float_type(q.scalar_type()),
+                   op + "q and k must be [R, heads, hd] in bf16, fp16 or fp32, got " + shape_text(q) + " and " + shape_text(k));
   const int64_t R = q.size(0), hd = q.size(2);
-  TORCH_CHECK(hd >= 8 && hd <= 256 && hd % 8 == 0, "head_norm_rope: the head size must be a multiple of 8 up to 256");
-  TORCH_CHECK(q.size(1) >= 1 && k.size(1) >= 1 && q.size(1) <= 65536 && k.size(1) <= 65536,
-              "head_norm_rope: q and k need 1 to 65536 heads");
+  DMAD_VALUE_CHECK(hd >= 8 && hd <= 256 && hd % 8 == 0 && q.size(1) >= 1 && k.size(1) >= 1 && q.size(1) <= 65536 &&
+                       k.size(1) <= 65536,
+                   op + "the head size must be a multiple of 8 up to 256 and q and k have heads, got " + shape_text(q) +
+                       " and " + shape_text(k));
+  check_heads(k, q, k.size(1), "k", false);
+  DMAD_VALUE_CHECK(q.is_cuda(), op + "the native kernel takes CUDA tensors");
   const at::Tensor* xs[2] = {&q, &k};
   const c10::optional<at::Tensor>* ws[2] = {&wq, &wk};
   for (int i = 0; i < 2; ++i) {
     Side& s = p.side[i];
-    std::tie(s.xr, s.xh) = check_heads(*xs[i], q, R, xs[i]->size(1), hd, i ? "k" : "q");
-    s.x = xs[i]->data_ptr();
+    keep.x[i] = readable(*xs[i]);
+    s.x = keep.x[i].data_ptr();
+    s.xr = keep.x[i].stride(0);
+    s.xh = keep.x[i].stride(1);
     s.H = (int)xs[i]->size(1);
     s.g = nullptr;
     s.gr = s.gh = 0;
@@ -405,10 +421,12 @@ RotMode fill_common(Params& p, const at::Tensor& q, const at::Tensor& k, const c
     s.wtype = 0;
     if (ws[i]->has_value() && (*ws[i])->defined()) {
       const at::Tensor& w = **ws[i];
-      TORCH_CHECK(w.device() == q.device() && w.dim() == 1 && w.size(0) == hd && w.is_contiguous(),
-                  "head_norm_rope: a weight must be contiguous [", num(hd), "] on the device of the queries");
-      s.w = w.data_ptr();
-      s.wtype = float_type(w, "head_norm_rope: a weight");
+      DMAD_VALUE_CHECK(w.device() == q.device() && w.dim() == 1 && w.size(0) == hd && is_float_type(w.scalar_type()),
+                       op + (i ? "wk" : "wq") + " must be bf16, fp16 or fp32 (" + num(hd) + ",) on the device of q, got " +
+                           dtype_name(w.scalar_type()) + " " + shape_text(w));
+      keep.w[i] = w.contiguous();
+      s.w = keep.w[i].data_ptr();
+      s.wtype = float_type(w);
     }
   }
   p.R = R;
@@ -421,29 +439,38 @@ RotMode fill_common(Params& p, const at::Tensor& q, const at::Tensor& k, const c
   p.interleaved = interleaved ? 1 : 0;
   p.eps = (float)eps;
   p.status = device_status_ptr(q.get_device());
-  if (!(cosT.has_value() && cosT->defined())) return kNone;
-  TORCH_CHECK(sinT.has_value() && sinT->defined(), "head_norm_rope: cos needs sin");
-  for (const at::Tensor* t : {&*cosT, &*sinT})
-    TORCH_CHECK(t->device() == q.device() && t->scalar_type() == at::kFloat && t->dim() == 2 && t->is_contiguous() &&
-                    t->sizes() == cosT->sizes() && t->size(0) >= 1,
-                "head_norm_rope: cos and sin must be contiguous fp32 [T, rot / 2] on the device of the queries, T >= 1");
+  const bool has_cos = cosT.has_value() && cosT->defined(), has_sin = sinT.has_value() && sinT->defined();
+  const bool has_pos = positions.has_value() && positions->defined();
+  DMAD_VALUE_CHECK(has_cos == has_sin && (has_cos || !has_pos), op + "cos and sin come together, and positions with them");
+  if (!has_cos) return keep;
+  DMAD_VALUE_CHECK(cosT->dim() == 2 && cosT->sizes() == sinT->sizes() && cosT->size(0) >= 1 && 2 * cosT->size(1) <= hd,
+                   op + "cos and sin must be [T, rot / 2] with T >= 1 and rot <= " + num(hd) + ", got " +
+                       shape_text(*cosT) + " and " + shape_text(*sinT));
+  DMAD_VALUE_CHECK(cosT->device() == q.device() && sinT->device() == q.device() && at::isFloatingType(cosT->scalar_type()) &&
+                       at::isFloatingType(sinT->scalar_type()) && !cosT->requires_grad() && !sinT->requires_grad(),
+                   op + "cos and sin are constant floating-point tables on the device of q (no gradient)");
+  keep.cosT = cosT->to(at::kFloat).contiguous();
+  keep.sinT = sinT->to(at::kFloat).contiguous();
+  if (has_pos) {
+    DMAD_VALUE_CHECK(positions->device() == q.device() && positions->dim() == 1 && positions->size(0) == R &&
+                         (positions->scalar_type() == at::kLong || positions->scalar_type() == at::kInt),
+                     op + "positions must be int32 or int64 (" + num(R) + ",) on the device of q, got " +
+                         shape_text(*positions));
+  }
   p.rot = (int)cosT->size(1) * 2;
-  TORCH_CHECK(cosT->size(1) * 2 <= hd, "head_norm_rope: the tables turn ", num(cosT->size(1) * 2), " of ", num(hd), " elements");
-  if (p.rot == 0) return kNone;
+  if (p.rot == 0) return keep;
   p.T = cosT->size(0);
-  p.cosT = cosT->data_ptr<float>();
-  p.sinT = sinT->data_ptr<float>();
-  if (positions.has_value() && positions->defined()) {
-    TORCH_CHECK(positions->device() == q.device() && positions->dim() == 1 && positions->size(0) == R &&
-                    positions->is_contiguous() &&
-                    (positions->scalar_type() == at::kLong || positions->scalar_type() == at::kInt),
-                "head_norm_rope: positions must be contiguous int32 or int64 [", num(R), "] on the device of the queries");
-    p.positions = positions->data_ptr();
+  p.cosT = keep.cosT.data_ptr<float>();
+  p.sinT = keep.sinT.data_ptr<float>();
+  if (has_pos) {
+    keep.positions = positions->contiguous();
+    p.positions = keep.positions.data_ptr();
     p.pos64 = positions->scalar_type() == at::kLong ? 1 : 0;
   }
   const bool tables16 = reinterpret_cast<uintptr_t>(p.cosT) % 16 == 0 && reinterpret_cast<uintptr_t>(p.sinT) % 16 == 0;
-  if (interleaved) return tables16 && p.rot % 8 == 0 ? kPairs : kAny;
-  return tables16 && p.rot % 16 == 0 ? kHalves : kAny;
+  if (interleaved) keep.mode = tables16 && p.rot % 8 == 0 ? kPairs : kAny;
+  else keep.mode = tables16 && p.rot % 16 == 0 ? kHalves : kAny;
+  return keep;
 }
 
 template <typename F>
@@ -464,8 +491,7 @@ template <typename F>
 void dispatch_type(at::ScalarType t, F f) {
   if (t == at::kBFloat16) f(__nv_bfloat16{});
   else if (t == at::kHalf) f(__half{});
-  else if (t == at::kFloat) f(float{});
-  else TORCH_CHECK(false, "head_norm_rope: q and k must be bf16, fp16 or fp32");
+  else f(float{});
 }
 
 int64_t blocks_for(const Params& p, int G, int64_t most) {
@@ -475,29 +501,28 @@ int64_t blocks_for(const Params& p, int G, int64_t most) {
   return std::min(b, most);
 }
 
-int sm_count(int device) {
-  int sms = 148;
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-  return sms;
-}
-
 }  // namespace
 
-// qo, ko = Rot(norm(q) * wq), Rot(norm(k) * wk) per head; [R, H, hd] each, any row and head strides.
-void head_norm_rope_fwd(const at::Tensor& q, const at::Tensor& k, c10::optional<at::Tensor> wq,
-                        c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cosT, c10::optional<at::Tensor> sinT,
-                        c10::optional<at::Tensor> positions, at::Tensor& qo, at::Tensor& ko, double eps,
-                        bool interleaved) {
+// Rot(norm(q) * wq), Rot(norm(k) * wk) per head, contiguous.
+std::tuple<at::Tensor, at::Tensor> head_norm_rope_fwd(const at::Tensor& q, const at::Tensor& k,
+                                                      c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk,
+                                                      c10::optional<at::Tensor> cosT, c10::optional<at::Tensor> sinT,
+                                                      c10::optional<at::Tensor> positions, double eps,
+                                                      bool interleaved) {
+  c10::cuda::OptionalCUDAGuard guard;
+  if (q.is_cuda()) guard.set_device(q.device());
   Params p;
-  const RotMode mode = fill_common(p, q, k, wq, wk, cosT, sinT, positions, eps, interleaved);
-  at::Tensor* outs[2] = {&qo, &ko};
+  const Prepared keep = fill_common(p, q, k, wq, wk, cosT, sinT, positions, eps, interleaved);
+  const auto plain = q.options().requires_grad(false);
+  at::Tensor outs[2] = {at::empty(q.sizes(), plain), at::empty(k.sizes(), plain)};
   for (int i = 0; i < 2; ++i) {
     Side& s = p.side[i];
-    std::tie(s.orow, s.oh) = check_heads(*outs[i], q, p.R, s.H, p.hd, i ? "ko" : "qo");
-    s.out = outs[i]->data_ptr();
+    s.orow = outs[i].stride(0);
+    s.oh = outs[i].stride(1);
+    s.out = outs[i].data_ptr();
   }
-  if (p.R == 0) return;
-  c10::cuda::CUDAGuard guard(q.device());
+  if (p.R == 0) return {outs[0], outs[1]};
+  const RotMode mode = keep.mode;
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const int sms = sm_count(q.get_device());
   dispatch_type(q.scalar_type(), [&](auto tag) {
@@ -512,6 +537,7 @@ void head_norm_rope_fwd(const at::Tensor& q, const at::Tensor& k, c10::optional<
     });
   });
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {outs[0], outs[1]};
 }
 
 // dq, dk of the forward given gq, gk (gradients of its results) and its inputs; dwq, dwk [hd] where wanted.
@@ -520,28 +546,37 @@ void head_norm_rope_bwd(const at::Tensor& gq, const at::Tensor& gk, const at::Te
                         c10::optional<at::Tensor> sinT, c10::optional<at::Tensor> positions, at::Tensor& dq,
                         at::Tensor& dk, c10::optional<at::Tensor> dwq, c10::optional<at::Tensor> dwk, double eps,
                         bool interleaved) {
+  c10::cuda::OptionalCUDAGuard guard;
+  if (q.is_cuda()) guard.set_device(q.device());
   Params p;
-  const RotMode mode = fill_common(p, q, k, wq, wk, cosT, sinT, positions, eps, interleaved);
+  const Prepared keep = fill_common(p, q, k, wq, wk, cosT, sinT, positions, eps, interleaved);
+  const RotMode mode = keep.mode;
   const at::Tensor* gs[2] = {&gq, &gk};
   at::Tensor* outs[2] = {&dq, &dk};
   const c10::optional<at::Tensor>* dws[2] = {&dwq, &dwk};
+  at::Tensor g[2];
   void* dwp[2] = {nullptr, nullptr};
   int dwt[2] = {0, 0};
   for (int i = 0; i < 2; ++i) {
     Side& s = p.side[i];
-    std::tie(s.gr, s.gh) = check_heads(*gs[i], q, p.R, s.H, p.hd, i ? "gk" : "gq");
-    std::tie(s.orow, s.oh) = check_heads(*outs[i], q, p.R, s.H, p.hd, i ? "dk" : "dq");
-    s.g = gs[i]->data_ptr();
+    check_heads(*gs[i], q, s.H, i ? "gk" : "gq", false);
+    check_heads(*outs[i], q, s.H, i ? "dk" : "dq", true);
+    g[i] = readable(*gs[i]);
+    s.g = g[i].data_ptr();
+    s.gr = g[i].stride(0);
+    s.gh = g[i].stride(1);
     s.out = outs[i]->data_ptr();
+    s.orow = outs[i]->stride(0);
+    s.oh = outs[i]->stride(1);
     if (dws[i]->has_value() && (*dws[i])->defined()) {
       const at::Tensor& dw = **dws[i];
-      TORCH_CHECK(dw.device() == q.device() && dw.dim() == 1 && dw.size(0) == p.hd && dw.is_contiguous(),
-                  "head_norm_rope: a weight gradient must be contiguous [", num(p.hd), "]");
+      DMAD_VALUE_CHECK(dw.device() == q.device() && dw.dim() == 1 && dw.size(0) == p.hd && dw.is_contiguous() &&
+                           is_float_type(dw.scalar_type()),
+                       std::string(kOp) + "a weight gradient must be contiguous bf16, fp16 or fp32 (" + num(p.hd) + ",)");
       dwp[i] = dw.data_ptr();
-      dwt[i] = float_type(dw, "head_norm_rope: a weight gradient");
+      dwt[i] = float_type(dw);
     }
   }
-  c10::cuda::CUDAGuard guard(q.device());
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   const int sms = sm_count(q.get_device());
   const bool want_dw = dwp[0] != nullptr || dwp[1] != nullptr;

@@ -18,6 +18,7 @@ take 4.25 (mxfp4) or 4.5 (nvfp4) bits an element and the product runs on the ten
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -176,25 +177,17 @@ def dequantize_fp4_reference(q: Fp4Tensor) -> torch.Tensor:
 
 def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4") -> Fp4Tensor:
     """The 4-bit form of ``x`` [..., K] (bf16, fp16 or fp32), quantised along the last dimension."""
-    blk = _block(fmt)
+    nv = _block(fmt) == 16
+    if x.requires_grad:
+        _no_grad("quantize_fp4", x)
+    if x.is_cuda:  # the same checks are the extension's
+        return Fp4Tensor(*ext().fp4_quantize(x, nv), fmt, tuple(x.shape))
     if x.dtype not in _DTYPES:
         raise ValueError(f"quantize_fp4: x must be bf16, fp16 or fp32, got {x.dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"quantize_fp4: the last dimension must hold at least one column, got {tuple(x.shape)}")
-    _no_grad("quantize_fp4", x)
     K = x.shape[-1]
-    x2 = x.reshape(x.numel() // K, K)
-    if not x.is_cuda:
-        return Fp4Tensor(*quantize_fp4_reference(x2, fmt), fmt, tuple(x.shape))
-    if x2.stride(-1) != 1 and K > 1:
-        x2 = x2.contiguous()
-    R = x2.shape[0]
-    ds, ss = fp4_storage_shapes(R, K, fmt)
-    data = torch.empty(ds, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(ss, dtype=torch.uint8, device=x.device)
-    row_scale = torch.empty(R, dtype=torch.float32, device=x.device) if blk == 16 else None
-    ext().fp4_quantize(x2, data, scales, row_scale, blk == 16)
-    return Fp4Tensor(data, scales, row_scale, fmt, tuple(x.shape))
+    return Fp4Tensor(*quantize_fp4_reference(x.detach().reshape(x.numel() // K, K), fmt), fmt, tuple(x.shape))
 
 
 def dequantize_fp4(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
@@ -202,12 +195,11 @@ def dequantize_fp4(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.T
     significant bits of a scale by two of a code) above bf16's subnormals; fp16 rounds and can overflow."""
     if dtype not in _DTYPES:
         raise ValueError(f"dequantize_fp4: dtype must be bf16, fp16 or fp32, got {dtype}")
-    R, K = _check(q, "q")
     if not q.data.is_cuda:
         return dequantize_fp4_reference(q).to(dtype).reshape(q.shape)
-    out = torch.empty((R, K), dtype=dtype, device=q.device)
-    ext().fp4_dequantize(q.data, q.scales, q.row_scale, out, q.fmt == "nvfp4")
-    return out.view(q.shape)
+    out = ext().fp4_dequantize(q.data, q.scales, q.row_scale, math.prod(q.shape[:-1]), q.shape[-1], _block(q.fmt) == 16,
+                               _DTYPES.index(dtype))
+    return out if len(q.shape) == 2 else out.view(q.shape)
 
 
 def fp4_linear(x: torch.Tensor | Fp4Tensor, w: Fp4Tensor, bias: torch.Tensor | None = None,
@@ -217,36 +209,35 @@ def fp4_linear(x: torch.Tensor | Fp4Tensor, w: Fp4Tensor, bias: torch.Tensor | N
 
     fp32 accumulation, one rounding to ``out_dtype`` (bf16 or fp16; x's type, bf16 for a quantised x).
     """
-    N, K = _check(w, "w")
     if len(w.shape) != 2:
         raise ValueError(f"fp4_linear: w must be a matrix, got shape {tuple(w.shape)}")
-    if isinstance(x, Fp4Tensor):
-        if x.fmt != w.fmt:
-            raise ValueError(f"fp4_linear: x is {x.fmt}, w is {w.fmt}")
-        xq = x
-        _check(xq, "x")
-    else:
-        if x.dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError(f"fp4_linear: x must be bf16 or fp16, got {x.dtype}")
-        xq = None
+    if out_dtype not in (None, torch.bfloat16, torch.float16):
+        raise ValueError(f"fp4_linear: out_dtype must be bf16 or fp16, got {out_dtype}")
+    N, K = w.shape
+    nv = _block(w.fmt) == 16
+    coded = isinstance(x, Fp4Tensor)
+    if coded and x.fmt != w.fmt:
+        raise ValueError(f"fp4_linear: x is {x.fmt}, w is {w.fmt}")
+    if torch.is_grad_enabled():
+        _no_grad("fp4_linear", None if coded else x, bias)
+    if w.data.is_cuda:  # the same checks are the extension's
+        out = -1 if out_dtype is None else _DTYPES.index(out_dtype)
+        if not coded:
+            return ext().fp4_linear(x, w.data, w.scales, w.row_scale, bias, N, K, nv, out)
+        if x.shape[-1] != K:
+            raise ValueError(f"fp4_linear: x has {x.shape[-1]} columns, w has {K}")
+        y = ext().fp4_matmul(x.data, x.scales, x.row_scale, math.prod(x.shape[:-1]), w.data, w.scales, w.row_scale, bias,
+                             N, K, nv, out)
+        return y if len(x.shape) == 2 else y.view(*x.shape[:-1], N)
+    if not coded and x.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"fp4_linear: x must be bf16 or fp16, got {x.dtype}")
     if x.shape[-1] != K:
         raise ValueError(f"fp4_linear: x has {x.shape[-1]} columns, w has {K}")
     if x.device != w.device or (bias is not None and bias.device != w.device):
         raise ValueError("fp4_linear: x, w and bias must be on one device")
     if bias is not None and (tuple(bias.shape) != (N,) or bias.dtype not in _DTYPES):
         raise ValueError(f"fp4_linear: bias must be bf16, fp16 or fp32 ({N},), got {bias.dtype} {tuple(bias.shape)}")
-    if out_dtype is None:
-        out_dtype = torch.bfloat16 if xq is not None else x.dtype
-    if out_dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"fp4_linear: out_dtype must be bf16 or fp16, got {out_dtype}")
-    _no_grad("fp4_linear", None if xq is not None else x, bias)
-    if xq is None:
-        xq = quantize_fp4(x.detach(), w.fmt)
-    if not w.data.is_cuda:
-        y = dequantize_fp4_reference(xq) @ dequantize_fp4_reference(w).t()
-        y = y if bias is None else y + bias.float()
-        return y.to(out_dtype).reshape(*xq.shape[:-1], N)
-    y = torch.empty((xq.rows, N), dtype=out_dtype, device=w.device)
-    ext().fp4_gemm(xq.data, xq.scales, xq.row_scale, w.data, w.scales, w.row_scale,
-                   bias.detach().contiguous() if bias is not None else None, y, K, w.fmt == "nvfp4")
-    return y.view(*xq.shape[:-1], N)
+    xq = x if coded else quantize_fp4(x.detach(), w.fmt)
+    y = dequantize_fp4_reference(xq) @ dequantize_fp4_reference(w).t()
+    y = y if bias is None else y + bias.detach().float()
+    return y.to(out_dtype or (torch.bfloat16 if coded else x.dtype)).reshape(*xq.shape[:-1], N)

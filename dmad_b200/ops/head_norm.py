@@ -50,25 +50,12 @@ def qk_head_norm_rope_reference(q, k, wq=None, wk=None, cos=None, sin=None, posi
     return tuple(outs)
 
 
-def _heads_ok(t):
-    per16 = 16 // t.element_size()
-    return (t.stride(-1) == 1 and t.stride(0) % per16 == 0 and t.stride(1) % per16 == 0 and t.data_ptr() % 16 == 0)
-
-
-def _heads(t):
-    return t if t.numel() == 0 or _heads_ok(t) else t.contiguous()
-
-
 class _HeadNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, interleaved):
-        qs, ks = _heads(q), _heads(k)
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        ext().head_norm_rope_fwd(qs, ks, wq, wk, cos, sin, positions, qo, ko, eps, interleaved)
         ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
         ctx.cfg = (eps, interleaved)
-        return qo, ko
+        return ext().head_norm_rope_fwd(q, k, wq, wk, cos, sin, positions, eps, interleaved)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -76,14 +63,13 @@ class _HeadNormRope(torch.autograd.Function):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dwq = torch.empty_like(wq) if ctx.needs_input_grad[2] else None
-        dwk = torch.empty_like(wk) if ctx.needs_input_grad[3] else None
-        ext().head_norm_rope_bwd(_heads(gq), _heads(gk), _heads(q), _heads(k), wq, wk, cos, sin, positions, dq, dk,
-                                 dwq, dwk, *ctx.cfg)
+        dwq = torch.empty(wq.shape, dtype=wq.dtype, device=wq.device) if ctx.needs_input_grad[2] else None
+        dwk = torch.empty(wk.shape, dtype=wk.dtype, device=wk.device) if ctx.needs_input_grad[3] else None
+        ext().head_norm_rope_bwd(gq, gk, q, k, wq, wk, cos, sin, positions, dq, dk, dwq, dwk, *ctx.cfg)
         return dq, dk, dwq, dwk, None, None, None, None, None
 
 
-def check_head_norm_rope(q, k, wq, wk, cos, sin, positions):
+def _check(q, k, wq, wk, cos, sin, positions):
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"qk_head_norm_rope: q and k must be [R, heads, hd] with one R and hd, got {tuple(q.shape)} "
                          f"and {tuple(k.shape)}")
@@ -123,12 +109,10 @@ def qk_head_norm_rope(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor | None 
     position outside [0, T) turns its row's rotated elements to NaN and, on CUDA, records status 6 for
     ``check_device_status``.
     """
-    check_head_norm_rope(q, k, wq, wk, cos, sin, positions)
     if not q.is_cuda:
+        _check(q, k, wq, wk, cos, sin, positions)
         return qk_head_norm_rope_reference(q, k, wq, wk, cos, sin, positions, eps, interleaved)
-    if cos is not None:
-        cos, sin = cos.float().contiguous(), sin.float().contiguous()
-    wq = wq if wq is None else wq.contiguous()
-    wk = wk if wk is None else wk.contiguous()
-    positions = positions if positions is None else positions.contiguous()
-    return _HeadNormRope.apply(q, k, wq, wk, cos, sin, positions, float(eps), bool(interleaved))
+    # on CUDA the same checks are the extension's
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, wq, wk)):
+        return _HeadNormRope.apply(q, k, wq, wk, cos, sin, positions, eps, interleaved)
+    return ext().head_norm_rope_fwd(q, k, wq, wk, cos, sin, positions, eps, interleaved)

@@ -111,12 +111,17 @@ def test_native_checks_raise():
     e = ops.ext()
     x = torch.randn(4, 64)
     q = ops.quantize_fp4(torch.randn(8, 64))
-    for f in (lambda: e.fp4_quantize(x, q.data, q.scales, q.row_scale, True),
-              lambda: e.fp4_quantize(x[:, :63], q.data[:4], q.scales, q.row_scale, True),
-              lambda: e.fp4_quantize(x, q.data[:4], q.scales, q.row_scale, True),
-              lambda: e.fp4_quantize(x, q.data[:4], q.scales, q.row_scale[:4], True),
-              lambda: e.fp4_dequantize(q.data, q.scales, q.row_scale, x, True),
-              lambda: e.fp4_gemm(q.data, q.scales, q.row_scale, q.data, q.scales, q.row_scale, None, x, 64, True),
-              lambda: e.head_norm_rope_fwd(x, x, None, None, None, None, None, x, x, 1e-6, True)):
-        with pytest.raises(RuntimeError):
+    z = torch.randn(4, 2, 16)
+    for f in (lambda: e.fp4_quantize(x, True),
+              lambda: e.fp4_dequantize(q.data[:4], q.scales, q.row_scale, 8, 64, True, 0),
+              lambda: e.fp4_dequantize(q.data, q.scales[:, :0], q.row_scale, 8, 64, True, 0),
+              lambda: e.fp4_dequantize(q.data, q.scales, q.row_scale[:4], 8, 64, True, 0),
+              lambda: e.fp4_dequantize(q.data, q.scales, None, 8, 64, True, 0),
+              lambda: e.fp4_dequantize(q.data, q.scales, q.row_scale, 8, 64, True, 0),
+              lambda: e.fp4_linear(x.bfloat16(), q.data, q.scales, q.row_scale, None, 8, 64, True, -1),
+              lambda: e.fp4_matmul(q.data, q.scales, q.row_scale, 8, q.data, q.scales, q.row_scale, None, 8, 64, True, 0),
+              lambda: e.head_norm_rope_fwd(x, x, None, None, None, None, None, 1e-6, True),
+              lambda: e.head_norm_rope_fwd(z, z[:3], None, None, None, None, None, 1e-6, True),
+              lambda: e.head_norm_rope_fwd(z, z, None, None, None, None, None, 1e-6, True)):
+        with pytest.raises(ValueError):
             f()

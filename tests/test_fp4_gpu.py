@@ -158,8 +158,13 @@ def test_refusals_on_the_gpu():
         ops.fp4_linear(x, w, torch.zeros(8))
     with pytest.raises(ValueError):
         ops.dequantize_fp4(ops.Fp4Tensor(w.data, w.scales.cpu(), w.row_scale, "nvfp4", (8, 64)))
-    with pytest.raises(RuntimeError):  # a start that TMA cannot read
+    with pytest.raises(ValueError):  # a start that TMA cannot read
         ops.fp4_linear(x, ops.Fp4Tensor(torch.zeros(8 * 32 + 8, dtype=torch.uint8, device=dev)[8:].view(8, 32), w.scales,
                                         w.row_scale, "nvfp4", (8, 64)))
-    with pytest.raises(RuntimeError):
-        ops.ext().fp4_quantize(x, w.data, w.scales, w.row_scale, True)
+    for f in (lambda: ops.fp4_linear(x[:, :32], w), lambda: ops.fp4_linear(x.float(), w),
+              lambda: ops.fp4_linear(ops.quantize_fp4(x[:, :32], "nvfp4"), w), lambda: ops.quantize_fp4(x.double()),
+              lambda: ops.quantize_fp4(x[:, :0]), lambda: ops.fp4_linear(x, w, torch.zeros(7, device=dev)),
+              lambda: ops.fp4_linear(x, w, torch.zeros(8, device=dev, dtype=torch.double)),
+              lambda: ops.dequantize_fp4(ops.Fp4Tensor(w.data, w.scales, None, "nvfp4", (8, 64)))):
+        with pytest.raises(ValueError):
+            f()

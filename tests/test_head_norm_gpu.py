@@ -166,3 +166,18 @@ def test_empty_positions_status_streams_and_graphs():
     torch.cuda.synchronize()
     want = ops.qk_head_norm_rope(q, k, *ws, c, s, pos)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_refusals_on_the_gpu():
+    ops = _ops()
+    q, k, w, c, s = _case(3, 2, 1, 16, 8, 4, torch.bfloat16, torch.float32)
+    p = torch.zeros(3, dtype=torch.long, device=dev)
+    f = ops.qk_head_norm_rope
+    for g in (lambda: f(q[0], k), lambda: f(q, k[:2]), lambda: f(q, k.half()), lambda: f(q.double(), k.double()),
+              lambda: f(q[..., :12], k[..., :12]), lambda: f(q, k.cpu()), lambda: f(q, k, w[0][:8]),
+              lambda: f(q, k, w[0].cpu(), w[1]), lambda: f(q, k, *w, c), lambda: f(q, k, *w, positions=p),
+              lambda: f(q, k, *w, c[:0], s[:0]), lambda: f(q, k, *w, torch.ones(4, 9, device=dev), torch.ones(4, 9, device=dev)),
+              lambda: f(q, k, *w, c.clone().requires_grad_(True), s), lambda: f(q, k, *w, c, s, p[:2]),
+              lambda: f(q, k, *w, c, s, p.float()), lambda: f(q, k, *w, c.cpu(), s.cpu())):
+        with pytest.raises(ValueError):
+            g()
