@@ -58,28 +58,40 @@ struct Params {
   int* status;
 };
 
+// Eight elements as they lie in memory: they stay packed until their head is worked on, which halves the registers
+// that the loads in flight occupy.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&f)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-        f[2 * i] = __uint_as_float(w[i] << 16);
-        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      } else {
-        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        f[2 * i] = h.x;
-        f[2 * i + 1] = h.y;
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void unpack(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 4) {
+          f[4 * i + j] = __uint_as_float(w[j]);
+        } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+          f[2 * j] = __uint_as_float(w[j] << 16);
+          f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        } else {
+          const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+          f[2 * j] = h.x;
+          f[2 * j + 1] = h.y;
+        }
       }
     }
   }
-}
+};
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
@@ -216,7 +228,7 @@ __device__ __forceinline__ void split_task(int64_t task, int64_t tasks, int chun
 }
 
 template <typename T, int G, int MODE, int U>
-__global__ void __launch_bounds__(kThreads) head_norm_fwd_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 4) head_norm_fwd_kernel(const __grid_constant__ Params p) {
   const Side& sd = p.side[blockIdx.y];
   const int lane = threadIdx.x & (G - 1), e0 = lane * 8;
   const bool in = e0 < p.hd;
@@ -237,36 +249,34 @@ __global__ void __launch_bounds__(kThreads) head_norm_fwd_kernel(const __grid_co
     const T* x = static_cast<const T*>(sd.x) + row * sd.xr + (int64_t)chunk * U * sd.xh;
     T* o = static_cast<T*>(sd.out) + row * sd.orow + (int64_t)chunk * U * sd.oh;
     const int nh = valid ? min(U, sd.H - chunk * U) : 0;
-    float f[U][8];
+    Raw8<T> raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (in && u < nh) {
-        load8(x + u * sd.xh + e0, f[u]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[u][j] = 0.f;
-      }
+      if (in && u < nh) raw[u].load(x + u * sd.xh + e0);
+      else raw[u].zero();
     }
     Angles<MODE> ang;
     ang.load(p, row, e0, valid);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      float f[8];
+      raw[u].unpack(f);
       float ss = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(f[u][j], f[u][j], ss);
+      for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
       const float r = rsqrtf(group_sum<G>(ss) * inv_hd + p.eps);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[u][j] = f[u][j] * r * w[j];
-      ang.template apply<false>(p, e0, f[u], [&](int i) {
+      for (int j = 0; j < 8; ++j) f[j] = f[j] * r * w[j];
+      ang.template apply<false>(p, e0, f, [&](int i) {
         return u < nh ? to_float(x[u * sd.xh + i]) * r * (sd.w != nullptr ? load_any(sd.w, sd.wtype, i) : 1.f) : 0.f;
       });
-      if (in && u < nh) store8(o + u * sd.oh + e0, f[u]);
+      if (in && u < nh) store8(o + u * sd.oh + e0, f);
     }
   }
 }
 
 template <typename T, int G, int MODE, int U>
-__global__ void __launch_bounds__(kThreads) head_norm_bwd_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 2) head_norm_bwd_kernel(const __grid_constant__ Params p) {
   __shared__ float red[kThreads * 8];
   const Side& sd = p.side[blockIdx.y];
   const int lane = threadIdx.x & (G - 1), e0 = lane * 8;
@@ -291,36 +301,39 @@ __global__ void __launch_bounds__(kThreads) head_norm_bwd_kernel(const __grid_co
     const T* g = static_cast<const T*>(sd.g) + row * sd.gr + (int64_t)chunk * U * sd.gh;
     T* o = static_cast<T*>(sd.out) + row * sd.orow + (int64_t)chunk * U * sd.oh;
     const int nh = valid ? min(U, sd.H - chunk * U) : 0;
-    float f[U][8], d[U][8];
+    Raw8<T> rawx[U], rawg[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (in && u < nh) {
-        load8(x + u * sd.xh + e0, f[u]);
-        load8(g + u * sd.gh + e0, d[u]);
+        rawx[u].load(x + u * sd.xh + e0);
+        rawg[u].load(g + u * sd.gh + e0);
       } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[u][j] = d[u][j] = 0.f;
+        rawx[u].zero();
+        rawg[u].zero();
       }
     }
     Angles<MODE> ang;
     ang.load(p, row, e0, valid);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      ang.template apply<true>(p, e0, d[u], [&](int i) { return u < nh ? to_float(g[u * sd.gh + i]) : 0.f; });
+      float f[8], d[8];
+      rawx[u].unpack(f);
+      rawg[u].unpack(d);
+      ang.template apply<true>(p, e0, d, [&](int i) { return u < nh ? to_float(g[u * sd.gh + i]) : 0.f; });
       float ss = 0.f, dot = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        ss = fmaf(f[u][j], f[u][j], ss);
-        dot = fmaf(d[u][j] * w[j], f[u][j], dot);
+        ss = fmaf(f[j], f[j], ss);
+        dot = fmaf(d[j] * w[j], f[j], dot);
       }
       const float r = rsqrtf(group_sum<G>(ss) * inv_hd + p.eps);
       const float c = group_sum<G>(dot) * r * inv_hd;  // mean(gy w n)
       float dx[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float n = f[u][j] * r;
-        if (u < nh) acc[j] = fmaf(d[u][j], n, acc[j]);
-        dx[j] = (d[u][j] * w[j] - n * c) * r;
+        const float n = f[j] * r;
+        if (u < nh) acc[j] = fmaf(d[j], n, acc[j]);
+        dx[j] = (d[j] * w[j] - n * c) * r;
       }
       if (in && u < nh) store8(o + u * sd.oh + e0, dx);
     }
@@ -587,7 +600,7 @@ void head_norm_rope_bwd(const at::Tensor& gq, const at::Tensor& gk, const at::Te
       using T = decltype(tag);
       dispatch_group(p.hd, [&](auto g) {
         dispatch_mode(mode, [&](auto m) {
-          constexpr int U = 2;
+          constexpr int U = 4;
           for (Side& s : p.side) s.chunks = (s.H + U - 1) / U;
           blocks = (int)blocks_for(p, g, (int64_t)sms * 4);
           if (want_dw) {
