@@ -101,27 +101,23 @@ __host__ __device__ constexpr uint32_t idesc_fp4(bool nv, int M, int N, int scal
          ((uint32_t)(M >> 7) << 27) | ((uint32_t)scale_id << 29);
 }
 
-// D[tmem] (+)= (A * scale_a)[smem] (B * scale_b)[smem]^T over 64 columns of K.
-template <bool NV>
+// D[tmem] (+)= (A * scale_a)[smem] (B * scale_b)[smem]^T over 64 columns of K.  CG = 2: issued by one thread of a CTA
+// pair for both, A's and D's rows split over the two CTAs and B's rows loaded half by each; every address is the
+// same in both.
+template <bool NV, int CG>
 __device__ __forceinline__ void mma_fp4_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                            uint32_t sfa_tmem, uint32_t sfb_tmem, uint32_t accumulate) {
-  if constexpr (NV) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-            d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
-        : "memory");
-  } else {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
-            d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
-        : "memory");
-  }
+#define DMAD_FP4_MMA(GROUP, KIND)                                                                                     \
+  asm volatile("{\n\t.reg .pred p;\n\t"                                                                              \
+               "setp.ne.b32 p, %6, 0;\n\t"                                                                           \
+               "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem), \
+               "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)                   \
+               : "memory")
+  if constexpr (NV && CG == 1) DMAD_FP4_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+  else if constexpr (NV) DMAD_FP4_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+  else if constexpr (CG == 1) DMAD_FP4_MMA("1", "mxf4.block_scale.scale_vec::2X");
+  else DMAD_FP4_MMA("2", "mxf4.block_scale.scale_vec::2X");
+#undef DMAD_FP4_MMA
 }
 
 // Descriptor of an unswizzled scale tile: 32 rows of 16 bytes, eight-row groups 128 bytes apart.
@@ -129,9 +125,14 @@ __device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
   return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
 }
 
-// One scale tile (512 bytes) -> four columns of tensor memory, in each of the four lane quarters.
+// One scale tile (512 bytes) -> four columns of tensor memory, in each of the four lane quarters.  CG = 2: in both
+// CTAs of the pair, each from its own shared memory.
+template <int CG>
 __device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
 
 }  // namespace dmad

@@ -221,15 +221,15 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
           const uint32_t aa = smem_u32(sm.a[s]), bb = smem_u32(sm.b[s]);
           const uint32_t ssa = smem_u32(sm.sa[s]), ssb = smem_u32(sm.sb[s]);
           for (int j = 0; j < nt; ++j) {
-            tmem_cp_scales(sfa + 4 * j, smem_desc_scales(ssa + j * kFp4TileBytes));
-            tmem_cp_scales(sfb + 8 * j, smem_desc_scales(ssb + j * kFp4TileBytes));
-            tmem_cp_scales(sfb + 8 * j + 4, smem_desc_scales(ssb + kSaBytes + j * kFp4TileBytes));
+            tmem_cp_scales<1>(sfa + 4 * j, smem_desc_scales(ssa + j * kFp4TileBytes));
+            tmem_cp_scales<1>(sfb + 8 * j, smem_desc_scales(ssb + j * kFp4TileBytes));
+            tmem_cp_scales<1>(sfb + 8 * j + 4, smem_desc_scales(ssb + kSaBytes + j * kFp4TileBytes));
           }
           const int nk = min(4, (p.K - k * kBK + 63) / 64);
           for (int kk = 0; kk < nk; ++kk) {
             const int j = NV ? kk : kk >> 1;
             const uint32_t idesc = idesc_fp4(NV, kBM, kBN, NV ? 0 : (kk & 1) * 2);
-            mma_fp4_ss<NV>(d, smem_desc_sw128(aa + kk * 32, 16, 1024), smem_desc_sw128(bb + kk * 32, 16, 1024), idesc,
+            mma_fp4_ss<NV, 1>(d, smem_desc_sw128(aa + kk * 32, 16, 1024), smem_desc_sw128(bb + kk * 32, 16, 1024), idesc,
                            sfa + 4 * j, sfb + 8 * j, (k > 0 || kk > 0) ? 1u : 0u);
           }
           mma_commit(&sm.empty[s]);
@@ -301,6 +301,224 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
   }
 }
 
+// ---------------------------------------------------------------- CTA pairs
+// The same product with a pair of CTAs on each 256 x 256 tile (cta_group::2): each CTA holds 128 rows of A and of D and
+// loads 128 of B's 256 rows, so a stage moves 38 KB into an SM instead of 54 KB and the L2 is read a third less.
+//   warp 0      producer of its own CTA's operands and scales (all of B's scales: each CTA multiplies all of B), which
+//               all complete on the leader's barriers
+//   warp 1      leader CTA: the MMA thread, which also copies the scales of both CTAs to tensor memory
+//   warps 2..9  epilogue of the CTA's 128 rows: two warps a lane quarter, every other 32 columns each
+// Tensor memory: scale buffers in the last 144 columns (three of 48 for nvfp4, six of 24 for mxfp4, so that scales can
+// be copied while the MMAs of the stages before run), accumulators at 0 and 112.  The epilogue reads the 144 shared
+// columns into registers at once and then releases the accumulator.
+constexpr int kPairBM = 256, kPairStages = 5;
+constexpr int kPairAcc1 = 112, kPairSfCol = 368;
+constexpr int kEpiWarps = 8, kPairThreads = 64 + 32 * kEpiWarps;
+
+struct PairSmem {
+  uint8_t a[kPairStages][kABytes];
+  uint8_t b[kPairStages][kABytes];
+  uint8_t sa[kPairStages][kSaBytes];
+  uint8_t sb[kPairStages][kSbBytes];
+  float2 col[2][kBN];
+  uint16_t stage[kEpiWarps][32][18];
+  uint64_t full[kPairStages], empty[kPairStages];
+  uint64_t acc_full[2], acc_free;
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+template <bool NV>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                     const __grid_constant__ CUtensorMap tm_sa, const __grid_constant__ CUtensorMap tm_sb, Params p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  PairSmem& sm = *reinterpret_cast<PairSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  volatile int* abort_flag = &sm.abort_flag;
+  const int warp = warp_id(), lane = lane_id();
+  const uint32_t rank = cluster_rank();
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  constexpr int kStageTiles = NV ? 4 : 2;          // scale tiles along K of a whole stage
+  constexpr int kSfBufCols = 12 * kStageTiles;     // A: 4 columns a tile, B: 8
+  constexpr int kSfBufs = 144 / kSfBufCols;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&sm.full[s], 1);  // the leader's counts both CTAs' bytes; the other CTA's is not used
+      mbar_init(&sm.empty[s], 1);
+    }
+    mbar_init(&sm.acc_full[0], 1);
+    mbar_init(&sm.acc_full[1], 1);
+    mbar_init(&sm.acc_free, 2 * kEpiWarps);
+    mbar_init(&sm.drain, 1);
+    sm.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(&sm.tmem_base, 512);
+    tmem_relinquish_pair();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (elect_one()) {
+      int it = 0;
+      bool ok = true;
+      const int sa_rows = (p.M + kFp4TileRows - 1) / kFp4TileRows, sb_rows = (p.N + kFp4TileRows - 1) / kFp4TileRows;
+      for (int t = cluster; ok && t < p.num_tiles; t += clusters) {
+        int tm, tn;
+        tile_coords(p, t, tm, tn);
+        // scale tiles past the matrix do not exist; their rows are zeros in A and B and are not stored from D
+        const int ra = tm * 2 + (int)rank;
+        const bool second = tn * 2 + 1 < sb_rows;
+        const uint32_t scale_boxes = (tm * 2 + 1 < sa_rows ? 2 : 1) + (second ? 4 : 2);  // of both CTAs
+        for (int k = 0; k < p.ksteps; ++k, ++it) {
+          const int s = it % kPairStages;
+          const uint32_t ph = (it / kPairStages) & 1;
+          if (!(ok = mbar_wait(&sm.empty[s], ph ^ 1, kStatusTimeoutEmpty, abort_flag, p.status))) break;
+          // a box is written, and counted, whole: columns past K and scale tiles past the last are zeros
+          constexpr uint32_t box = kStageTiles * kFp4TileBytes;
+          if (rank == 0) mbar_arrive_expect_tx(&sm.full[s], 4 * kABytes + box * scale_boxes);
+          const uint32_t full = cluster_map(&sm.full[s], 0);
+          const int kt = k * kStageTiles * (kFp4TileBytes / 8);
+          tma_load_2d_pair(sm.a[s], &tm_a, full, k * 128, ra * kBM);
+          tma_load_2d_pair(sm.b[s], &tm_b, full, k * 128, (tn * 2 + (int)rank) * kBM);
+          if (ra < sa_rows) tma_load_2d_pair(sm.sa[s], &tm_sa, full, kt, ra);
+          tma_load_2d_pair(sm.sb[s], &tm_sb, full, kt, 2 * tn);
+          if (second) tma_load_2d_pair(sm.sb[s] + kSaBytes, &tm_sb, full, kt, 2 * tn + 1);
+        }
+      }
+      // all issued copies land before a CTA's shared memory goes away
+      if (rank == 0)
+        for (int j = max(0, it - kPairStages); j < it; ++j)
+          mbar_wait_cluster(&sm.full[j % kPairStages], (j / kPairStages) & 1, kStatusTimeoutTmaFull, nullptr, p.status);
+    }
+  } else if (warp == 1 && rank != 0) {
+    // the leader issues the pair's MMAs
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader)
+    if (elect_one()) {
+      int it = 0, tl = 0;
+      bool ok = true;
+      for (int t = cluster; ok && t < p.num_tiles; t += clusters, ++tl) {
+        // both CTAs have read the columns shared with the previous tile's accumulator
+        if (tl > 0 &&
+            !(ok = mbar_wait_cluster(&sm.acc_free, (tl - 1) & 1, kStatusTimeoutSoftmax, abort_flag, p.status)))
+          break;
+        tc_fence_after();
+        const uint32_t d = tmem + ((tl & 1) ? kPairAcc1 : 0);
+        for (int k = 0; k < p.ksteps; ++k, ++it) {
+          const int s = it % kPairStages;
+          if (!(ok = mbar_wait_cluster(&sm.full[s], (it / kPairStages) & 1, kStatusTimeoutTmaFull, abort_flag, p.status)))
+            break;
+          // this stage's scale buffer was last read by the MMAs of kSfBufs stages ago (with as many buffers as
+          // stages the ring itself has waited for them)
+          if (kSfBufs < kPairStages && it >= kSfBufs &&
+              !(ok = mbar_wait(&sm.empty[(it - kSfBufs) % kPairStages], ((it - kSfBufs) / kPairStages) & 1,
+                               kStatusTimeoutMma, abort_flag, p.status)))
+            break;
+          tc_fence_after();
+          const uint32_t sfa = tmem + kPairSfCol + (it % kSfBufs) * kSfBufCols, sfb = sfa + 4 * kStageTiles;
+          const int nt = min(kStageTiles, p.ktiles - k * kStageTiles);
+          const uint32_t aa = smem_u32(sm.a[s]), bb = smem_u32(sm.b[s]);
+          const uint32_t ssa = smem_u32(sm.sa[s]), ssb = smem_u32(sm.sb[s]);
+          for (int j = 0; j < nt; ++j) {
+            tmem_cp_scales<2>(sfa + 4 * j, smem_desc_scales(ssa + j * kFp4TileBytes));
+            tmem_cp_scales<2>(sfb + 8 * j, smem_desc_scales(ssb + j * kFp4TileBytes));
+            tmem_cp_scales<2>(sfb + 8 * j + 4, smem_desc_scales(ssb + kSaBytes + j * kFp4TileBytes));
+          }
+          const int nk = min(4, (p.K - k * kBK + 63) / 64);
+          for (int kk = 0; kk < nk; ++kk) {
+            const int j = NV ? kk : kk >> 1;
+            const uint32_t idesc = idesc_fp4(NV, kPairBM, kBN, NV ? 0 : (kk & 1) * 2);
+            mma_fp4_ss<NV, 2>(d, smem_desc_sw128(aa + kk * 32, 16, 1024), smem_desc_sw128(bb + kk * 32, 16, 1024),
+                              idesc, sfa + 4 * j, sfb + 8 * j, (k > 0 || kk > 0) ? 1u : 0u);
+          }
+          mma_commit_pair(&sm.empty[s]);
+        }
+        if (!ok) break;
+        mma_commit_pair(&sm.acc_full[tl & 1]);
+      }
+      if (!ok) *abort_flag = 1;
+      mma_commit_pair(&sm.drain);
+      mbar_wait(&sm.drain, 0, kStatusTimeoutMma, nullptr, p.status);
+    }
+  } else {
+    // ------------------------------------------------------------ epilogue (warps 2..9)
+    const int ew = warp - 2, wq = warp & 3, half = ew >> 2;
+    const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
+    const int et = threadIdx.x - 64;
+    const uint32_t acc_free = cluster_map(&sm.acc_free, 0);
+    int tl = 0;
+    for (int t = cluster; t < p.num_tiles; t += clusters, ++tl) {
+      int tm, tn;
+      tile_coords(p, t, tm, tn);
+      const int m0 = tm * kPairBM + (int)rank * kBM + wq * 32, m = m0 + lane;
+      // the tile's column factors and biases, read while its MMAs run (a buffer is written again only after the
+      // barrier of the tile in between)
+      float2* col = sm.col[tl & 1];
+      {
+        const int n = min(tn * kBN + et, p.N - 1);
+        col[et] = make_float2(NV ? __ldg(p.rb + n) : 1.f, p.bias != nullptr ? load_bias(p, n) : 0.f);
+      }
+      const float ra = (NV && m < p.M) ? __ldg(p.ra + m) : 1.f;
+      const bool ok = mbar_wait(&sm.acc_full[tl & 1], (tl >> 1) & 1, kStatusTimeoutMma, abort_flag, p.status);
+      // also the barrier of the column factors; all warps leave together, since it counts them
+      if (named_bar_any(1, 32 * kEpiWarps, !ok)) break;
+      tc_fence_after();
+      uint16_t* drow = static_cast<uint16_t*>(p.d) + (int64_t)m * p.ldd;
+      const uint32_t acc = tmem + lane_base + ((tl & 1) ? kPairAcc1 : 0);
+      // order of the 32-column chunks: the five that share columns with the other accumulator first (3..7 of the
+      // first, 0..4 of the second); this warp takes every other one
+      const int shift = (tl & 1) ? 0 : 3;
+      auto chunk = [&](int i) { return (2 * i + half + shift) & 7; };
+      uint32_t r[3][32];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) tmem_ld32(acc + chunk(i) * 32, r[i]);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc_free);
+      auto finish = [&](int c, const uint32_t (&v)[32]) {
+        const int nc = tn * kBN + c * 32;
+        if (nc >= p.N) return;
+        uint32_t o[16];
+        const float4* cf = reinterpret_cast<const float4*>(col + c * 32);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+          const float4 f = cf[q];
+          o[q] = pack_out(p, fmaf(__uint_as_float(v[2 * q]) * ra, f.x, f.y),
+                          fmaf(__uint_as_float(v[2 * q + 1]) * ra, f.z, f.w));
+        }
+        store_chunk(p, sm.stage[ew], drow, m0, nc, o);
+      };
+      finish(chunk(0), r[0]);
+      tmem_ld32(acc + chunk(3) * 32, r[0]);
+      finish(chunk(1), r[1]);
+      finish(chunk(2), r[2]);
+      tmem_wait_ld();
+      finish(chunk(3), r[0]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the pair's barriers and tensor memory are no longer in use by the other CTA
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
 CUtensorMap code_map(const Fp4Matrix& x, uint32_t box_rows) {
   const uint64_t dims[2] = {(uint64_t)x.row_bytes(), (uint64_t)x.rows};
   const uint64_t strides[1] = {(uint64_t)x.row_bytes()};
@@ -308,15 +526,38 @@ CUtensorMap code_map(const Fp4Matrix& x, uint32_t box_rows) {
   return make_tmap_u8(x.data, 2, dims, strides, box);
 }
 
+// Raises a kernel's dynamic shared memory limit, once a device.
+template <auto Kernel>
+void configure(int smem, int device) {
+  static std::array<std::atomic<bool>, 64> done{};
+  if (device < 64 && done[device].load(std::memory_order_acquire)) return;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (device < 64) done[device].store(true, std::memory_order_release);
+}
+
+// Scales as a matrix of 8-byte elements, a row for each 128 rows of x, read in boxes of a stage's tiles.
+CUtensorMap scale_map(const Fp4Matrix& x) {
+  const uint64_t dims[2] = {(uint64_t)x.ktiles() * kFp4TileBytes / 8, (uint64_t)x.row_tiles()};
+  const uint64_t strides[1] = {(uint64_t)x.ktiles() * kFp4TileBytes};
+  const uint32_t box[2] = {(x.nv ? 4u : 2u) * kFp4TileBytes / 8, 1u};
+  return make_tmap(CU_TENSOR_MAP_DATA_TYPE_FLOAT64, x.scales, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
 template <bool NV>
-void launch(const CUtensorMap& ma, const CUtensorMap& mb, const Params& p, int device, cudaStream_t stream) {
-  const int smem = (int)sizeof(Smem) + 1024;
-  static std::array<std::atomic<bool>, 64> configured{};
-  if (device >= 64 || !configured[device].load(std::memory_order_acquire)) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(fp4_gemm_kernel<NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    if (device < 64) configured[device].store(true, std::memory_order_release);
+void launch(const Fp4Matrix& a, const Fp4Matrix& b, Params& p, int device, cudaStream_t stream) {
+  const int sms = sm_count(device);
+  if (p.M > 256) {
+    p.tiles_m = (p.M + kPairBM - 1) / kPairBM;
+    p.num_tiles = p.tiles_m * p.tiles_n;
+    const int smem = (int)sizeof(PairSmem) + 1024;
+    configure<fp4_gemm_pair_kernel<NV>>(smem, device);
+    fp4_gemm_pair_kernel<NV><<<2 * std::min(p.num_tiles, sms / 2), kPairThreads, smem, stream>>>(
+        code_map(a, kBM), code_map(b, kBM), scale_map(a), scale_map(b), p);
+  } else {
+    const int smem = (int)sizeof(Smem) + 1024;
+    configure<fp4_gemm_kernel<NV>>(smem, device);
+    fp4_gemm_kernel<NV><<<std::min(p.num_tiles, sms), 192, smem, stream>>>(code_map(a, kBM), code_map(b, kBN), p);
   }
-  fp4_gemm_kernel<NV><<<std::min(p.num_tiles, sm_count(device)), 192, smem, stream>>>(ma, mb, p);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -352,8 +593,7 @@ void gemm(const Fp4Matrix& a, const Fp4Matrix& b, const c10::optional<at::Tensor
   p.num_tiles = p.tiles_m * p.tiles_n;
   const int device = d.get_device();
   p.status = device_status_ptr(device);
-  const CUtensorMap ma = code_map(a, kBM), mb = code_map(b, kBN);
-  a.nv ? launch<true>(ma, mb, p, device, stream) : launch<false>(ma, mb, p, device, stream);
+  a.nv ? launch<true>(a, b, p, device, stream) : launch<false>(a, b, p, device, stream);
 }
 
 c10::optional<at::Tensor> checked_bias(const c10::optional<at::Tensor>& bias, int64_t N, const at::Device& device) {
