@@ -102,8 +102,25 @@ __device__ __forceinline__ void tile_coords(const Params& p, int t, int& tm, int
   tn = in / gm;
 }
 
-// Stores 32 columns from nc of this lane's row (a warp holds rows m0 .. m0 + 31).  Whole 32-byte sectors where the
-// rows of D allow it; other rows go through shared memory, so that a warp still writes runs of 32 bytes.
+// Stores 32 columns from nc of the warp's rows m0 .. m0 + 31 (o: the lane's row) to rows of D that are no multiple of
+// 16 bytes: through shared memory, so that a warp still writes runs of 32 bytes.
+__device__ __forceinline__ void store_unaligned(const Params& p, uint16_t (*stage)[18], int m0, int nc,
+                                                const uint32_t (&o)[16]) {
+  const int lane = lane_id();
+  uint16_t* d0 = static_cast<uint16_t*>(p.d) + (int64_t)m0 * p.ldd + nc;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 8; ++q) *reinterpret_cast<uint32_t*>(&stage[lane][2 * q]) = o[8 * h + q];
+    __syncwarp();
+    const int cc = lane & 15, n = 16 * h + cc;
+    for (int r = lane >> 4; r < 32; r += 2)
+      if (m0 + r < p.M && nc + n < p.N) d0[(int64_t)r * p.ldd + n] = stage[r][cc];
+  }
+}
+
+// The same to any rows: whole 32-byte sectors where they allow it.
 __device__ __forceinline__ void store_chunk(const Params& p, uint16_t (*stage)[18], uint16_t* drow, int m0, int nc,
                                             const uint32_t (&o)[16]) {
   const int lane = lane_id();
@@ -121,17 +138,7 @@ __device__ __forceinline__ void store_chunk(const Params& p, uint16_t (*stage)[1
           *reinterpret_cast<uint4*>(drow + nc + 8 * q) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
     }
   } else {
-    uint16_t* d0 = static_cast<uint16_t*>(p.d) + (int64_t)m0 * p.ldd + nc;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      __syncwarp();
-#pragma unroll
-      for (int q = 0; q < 8; ++q) *reinterpret_cast<uint32_t*>(&stage[lane][2 * q]) = o[8 * h + q];
-      __syncwarp();
-      const int cc = lane & 15, n = 16 * h + cc;
-      for (int r = lane >> 4; r < 32; r += 2)
-        if (m0 + r < p.M && nc + n < p.N) d0[(int64_t)r * p.ldd + n] = stage[r][cc];
-    }
+    store_unaligned(p, stage, m0, nc, o);
   }
 }
 
@@ -306,11 +313,13 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant_
 // loads 128 of B's 256 rows, so a stage moves 38 KB into an SM instead of 54 KB and the L2 is read a third less.
 //   warp 0      producer of its own CTA's operands and scales (all of B's scales: each CTA multiplies all of B), which
 //               all complete on the leader's barriers
-//   warp 1      leader CTA: the MMA thread, which also copies the scales of both CTAs to tensor memory
-//   warps 2..9  epilogue of the CTA's 128 rows: two warps a lane quarter, every other 32 columns each
-// Tensor memory: scale buffers in the last 144 columns (three of 48 for nvfp4, six of 24 for mxfp4, so that scales can
-// be copied while the MMAs of the stages before run), accumulators at 0 and 112.  The epilogue reads the 144 shared
-// columns into registers at once and then releases the accumulator.
+//   warp 1      leader CTA: the MMA thread, which also copies the scales of both CTAs to tensor memory.  A copy takes
+//               some 56 cycles of the tensor core's queue and a stage has 12 (nvfp4) or 6 (mxfp4), so the next
+//               stage's copies are issued between this stage's MMAs, where they run beside them
+//   warps 2..9  epilogue of the CTA's 128 rows: two warps a lane quarter, every other 32 columns each; rows leave
+//               through shared memory by TMA (direct stores of a lane's row cost the SM four times the cycles)
+// Tensor memory: scale buffers in the last 144 columns (three of 48 for nvfp4, six of 24 for mxfp4), accumulators at 0
+// and 112.  The epilogue reads the 144 shared columns into registers at once and then releases the accumulator.
 constexpr int kPairBM = 256, kPairStages = 5;
 constexpr int kPairAcc1 = 112, kPairSfCol = 368;
 constexpr int kEpiWarps = 8, kPairThreads = 64 + 32 * kEpiWarps;
@@ -320,8 +329,8 @@ struct PairSmem {
   uint8_t b[kPairStages][kABytes];
   uint8_t sa[kPairStages][kSaBytes];
   uint8_t sb[kPairStages][kSbBytes];
+  uint8_t stage[kEpiWarps][2048];  // a warp's 32 rows x 32 columns of D on their way out
   float2 col[2][kBN];
-  uint16_t stage[kEpiWarps][32][18];
   uint64_t full[kPairStages], empty[kPairStages];
   uint64_t acc_full[2], acc_free;
   uint64_t drain;
@@ -332,7 +341,8 @@ struct PairSmem {
 template <bool NV>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                     const __grid_constant__ CUtensorMap tm_sa, const __grid_constant__ CUtensorMap tm_sb, Params p) {
+                     const __grid_constant__ CUtensorMap tm_sa, const __grid_constant__ CUtensorMap tm_sb,
+                     const __grid_constant__ CUtensorMap tm_d, Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   PairSmem& sm = *reinterpret_cast<PairSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   volatile int* abort_flag = &sm.abort_flag;
@@ -362,6 +372,8 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&tm_a);
     prefetch_tmap(&tm_b);
+    prefetch_tmap(&tm_sa);
+    prefetch_tmap(&tm_sb);
   }
   tc_fence_before();
   __syncthreads();
@@ -408,9 +420,35 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader)
     if (elect_one()) {
-      int it = 0, tl = 0;
+      const int my_tiles = cluster < p.num_tiles ? (p.num_tiles - 1 - cluster) / clusters + 1 : 0;
+      const int total = my_tiles * p.ksteps;  // stages of all tiles
       bool ok = true;
-      for (int t = cluster; ok && t < p.num_tiles; t += clusters, ++tl) {
+      // waits for stage i's operands and for its scale buffer, last read by the MMAs of kSfBufs stages before (with
+      // as many buffers as stages the ring itself has waited for those)
+      auto stage_ready = [&](int i) {
+        return mbar_wait_cluster(&sm.full[i % kPairStages], (i / kPairStages) & 1, kStatusTimeoutTmaFull, abort_flag,
+                                 p.status) &&
+               (kSfBufs >= kPairStages || i < kSfBufs ||
+                mbar_wait(&sm.empty[(i - kSfBufs) % kPairStages], ((i - kSfBufs) / kPairStages) & 1, kStatusTimeoutMma,
+                          abort_flag, p.status));
+      };
+      auto stage_there = [&](int i) {  // the same without waiting
+        return mbar_try_wait(smem_u32(&sm.full[i % kPairStages]), (i / kPairStages) & 1) &&
+               (kSfBufs >= kPairStages || i < kSfBufs ||
+                mbar_try_wait(smem_u32(&sm.empty[(i - kSfBufs) % kPairStages]), ((i - kSfBufs) / kPairStages) & 1));
+      };
+      // scale tile j along K of stage i, to tensor memory
+      auto copy_scales = [&](int i, int j) {
+        const int s = i % kPairStages;
+        const uint32_t sfa = tmem + kPairSfCol + (i % kSfBufs) * kSfBufCols, sfb = sfa + 4 * kStageTiles;
+        tmem_cp_scales<2>(sfa + 4 * j, smem_desc_scales(smem_u32(sm.sa[s]) + j * kFp4TileBytes));
+        tmem_cp_scales<2>(sfb + 8 * j, smem_desc_scales(smem_u32(sm.sb[s]) + j * kFp4TileBytes));
+        tmem_cp_scales<2>(sfb + 8 * j + 4, smem_desc_scales(smem_u32(sm.sb[s]) + kSaBytes + j * kFp4TileBytes));
+      };
+      auto scale_tiles = [&](int k) { return min(kStageTiles, p.ktiles - k * kStageTiles); };
+      int it = 0;
+      bool copied = false;  // this stage's scales are on their way already
+      for (int tl = 0; ok && tl < my_tiles; ++tl) {
         // both CTAs have read the columns shared with the previous tile's accumulator
         if (tl > 0 &&
             !(ok = mbar_wait_cluster(&sm.acc_free, (tl - 1) & 1, kStatusTimeoutSoftmax, abort_flag, p.status)))
@@ -419,31 +457,27 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         const uint32_t d = tmem + ((tl & 1) ? kPairAcc1 : 0);
         for (int k = 0; k < p.ksteps; ++k, ++it) {
           const int s = it % kPairStages;
-          if (!(ok = mbar_wait_cluster(&sm.full[s], (it / kPairStages) & 1, kStatusTimeoutTmaFull, abort_flag, p.status)))
-            break;
-          // this stage's scale buffer was last read by the MMAs of kSfBufs stages ago (with as many buffers as
-          // stages the ring itself has waited for them)
-          if (kSfBufs < kPairStages && it >= kSfBufs &&
-              !(ok = mbar_wait(&sm.empty[(it - kSfBufs) % kPairStages], ((it - kSfBufs) / kPairStages) & 1,
-                               kStatusTimeoutMma, abort_flag, p.status)))
-            break;
+          if (!copied) {
+            if (!(ok = stage_ready(it))) break;
+            tc_fence_after();
+            for (int j = 0; j < scale_tiles(k); ++j) copy_scales(it, j);
+          }
+          const int knext = k + 1 < p.ksteps ? k + 1 : 0;
+          const int next_tiles = it + 1 < total && stage_there(it + 1) ? scale_tiles(knext) : 0;
           tc_fence_after();
           const uint32_t sfa = tmem + kPairSfCol + (it % kSfBufs) * kSfBufCols, sfb = sfa + 4 * kStageTiles;
-          const int nt = min(kStageTiles, p.ktiles - k * kStageTiles);
           const uint32_t aa = smem_u32(sm.a[s]), bb = smem_u32(sm.b[s]);
-          const uint32_t ssa = smem_u32(sm.sa[s]), ssb = smem_u32(sm.sb[s]);
-          for (int j = 0; j < nt; ++j) {
-            tmem_cp_scales<2>(sfa + 4 * j, smem_desc_scales(ssa + j * kFp4TileBytes));
-            tmem_cp_scales<2>(sfb + 8 * j, smem_desc_scales(ssb + j * kFp4TileBytes));
-            tmem_cp_scales<2>(sfb + 8 * j + 4, smem_desc_scales(ssb + kSaBytes + j * kFp4TileBytes));
-          }
           const int nk = min(4, (p.K - k * kBK + 63) / 64);
-          for (int kk = 0; kk < nk; ++kk) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
             const int j = NV ? kk : kk >> 1;
             const uint32_t idesc = idesc_fp4(NV, kPairBM, kBN, NV ? 0 : (kk & 1) * 2);
-            mma_fp4_ss<NV, 2>(d, smem_desc_sw128(aa + kk * 32, 16, 1024), smem_desc_sw128(bb + kk * 32, 16, 1024),
-                              idesc, sfa + 4 * j, sfb + 8 * j, (k > 0 || kk > 0) ? 1u : 0u);
+            if (kk < nk)
+              mma_fp4_ss<NV, 2>(d, smem_desc_sw128(aa + kk * 32, 16, 1024), smem_desc_sw128(bb + kk * 32, 16, 1024),
+                                idesc, sfa + 4 * j, sfb + 8 * j, (k > 0 || kk > 0) ? 1u : 0u);
+            if (kk < next_tiles) copy_scales(it + 1, kk);
           }
+          copied = next_tiles > 0;
           mma_commit_pair(&sm.empty[s]);
         }
         if (!ok) break;
@@ -459,24 +493,33 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
     const int et = threadIdx.x - 64;
     const uint32_t acc_free = cluster_map(&sm.acc_free, 0);
-    int tl = 0;
-    for (int t = cluster; t < p.num_tiles; t += clusters, ++tl) {
+    uint8_t* stage = sm.stage[ew];
+    // row of the warp's first lane, first column, and the factors of one tile
+    int m0 = 0, n0 = 0;
+    float ra = 1.f;
+    float2 cf = make_float2(1.f, 0.f);
+    auto fetch = [&](int t) {
       int tm, tn;
       tile_coords(p, t, tm, tn);
-      const int m0 = tm * kPairBM + (int)rank * kBM + wq * 32, m = m0 + lane;
-      // the tile's column factors and biases, read while its MMAs run (a buffer is written again only after the
-      // barrier of the tile in between)
-      float2* col = sm.col[tl & 1];
-      {
-        const int n = min(tn * kBN + et, p.N - 1);
-        col[et] = make_float2(NV ? __ldg(p.rb + n) : 1.f, p.bias != nullptr ? load_bias(p, n) : 0.f);
-      }
-      const float ra = (NV && m < p.M) ? __ldg(p.ra + m) : 1.f;
+      m0 = tm * kPairBM + (int)rank * kBM + wq * 32;
+      n0 = tn * kBN;
+      const int n = min(n0 + et, p.N - 1);
+      cf = make_float2(NV ? __ldg(p.rb + n) : 1.f, p.bias != nullptr ? load_bias(p, n) : 0.f);
+      ra = (NV && m0 + lane < p.M) ? __ldg(p.ra + m0 + lane) : 1.f;
+    };
+    if (cluster < p.num_tiles) {
+      fetch(cluster);
+      sm.col[0][et] = cf;
+    }
+    int tl = 0;
+    for (int t = cluster; t < p.num_tiles; t += clusters, ++tl) {
+      const float2* col = sm.col[tl & 1];
+      const int tm0 = m0, tn0 = n0;
+      const float tra = ra;
       const bool ok = mbar_wait(&sm.acc_full[tl & 1], (tl >> 1) & 1, kStatusTimeoutMma, abort_flag, p.status);
       // also the barrier of the column factors; all warps leave together, since it counts them
       if (named_bar_any(1, 32 * kEpiWarps, !ok)) break;
       tc_fence_after();
-      uint16_t* drow = static_cast<uint16_t*>(p.d) + (int64_t)m * p.ldd;
       const uint32_t acc = tmem + lane_base + ((tl & 1) ? kPairAcc1 : 0);
       // order of the 32-column chunks: the five that share columns with the other accumulator first (3..7 of the
       // first, 0..4 of the second); this warp takes every other one
@@ -485,22 +528,37 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
       uint32_t r[3][32];
 #pragma unroll
       for (int i = 0; i < 3; ++i) tmem_ld32(acc + chunk(i) * 32, r[i]);
+      // the next tile's factors are read while this tile is stored (all warps are past the tile before, whose
+      // buffer they go to)
+      if (t + clusters < p.num_tiles) fetch(t + clusters);
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(acc_free);
       auto finish = [&](int c, const uint32_t (&v)[32]) {
-        const int nc = tn * kBN + c * 32;
-        if (nc >= p.N) return;
+        const int nc = tn0 + c * 32;
+        if (nc >= p.N || tm0 >= p.M) return;
         uint32_t o[16];
-        const float4* cf = reinterpret_cast<const float4*>(col + c * 32);
+        const float4* f4 = reinterpret_cast<const float4*>(col + c * 32);
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-          const float4 f = cf[q];
-          o[q] = pack_out(p, fmaf(__uint_as_float(v[2 * q]) * ra, f.x, f.y),
-                          fmaf(__uint_as_float(v[2 * q + 1]) * ra, f.z, f.w));
+          const float4 f = f4[q];
+          o[q] = pack_out(p, fmaf(__uint_as_float(v[2 * q]) * tra, f.x, f.y),
+                          fmaf(__uint_as_float(v[2 * q + 1]) * tra, f.z, f.w));
         }
-        store_chunk(p, sm.stage[ew], drow, m0, nc, o);
+        if (p.vec >= 16) {  // rows of D are multiples of 16 bytes: a box of 32 x 32 by TMA, 64-byte swizzle
+          if (lane == 0) tma_store_wait_read();
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
+                make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) tma_store_2d(&tm_d, stage, nc, tm0);
+        } else {
+          store_unaligned(p, reinterpret_cast<uint16_t(*)[18]>(stage), tm0, nc, o);
+        }
       };
       finish(chunk(0), r[0]);
       tmem_ld32(acc + chunk(3) * 32, r[0]);
@@ -508,7 +566,9 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
       finish(chunk(2), r[2]);
       tmem_wait_ld();
       finish(chunk(3), r[0]);
+      sm.col[(tl + 1) & 1][et] = cf;
     }
+    if (lane == 0) tma_store_wait_read();
   }
   tc_fence_before();
   __syncthreads();
@@ -543,6 +603,14 @@ CUtensorMap scale_map(const Fp4Matrix& x) {
   return make_tmap(CU_TENSOR_MAP_DATA_TYPE_FLOAT64, x.scales, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// D in boxes of 32 x 32, swizzled over 64 bytes in shared memory.
+CUtensorMap out_map(const Params& p) {
+  const uint64_t dims[2] = {(uint64_t)p.N, (uint64_t)p.M};
+  const uint64_t strides[1] = {(uint64_t)p.ldd * 2};
+  const uint32_t box[2] = {32u, 32u};
+  return make_tmap_bf16(p.d, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 template <bool NV>
 void launch(const Fp4Matrix& a, const Fp4Matrix& b, Params& p, int device, cudaStream_t stream) {
   const int sms = sm_count(device);
@@ -550,9 +618,10 @@ void launch(const Fp4Matrix& a, const Fp4Matrix& b, Params& p, int device, cudaS
     p.tiles_m = (p.M + kPairBM - 1) / kPairBM;
     p.num_tiles = p.tiles_m * p.tiles_n;
     const int smem = (int)sizeof(PairSmem) + 1024;
+    const CUtensorMap ma = code_map(a, kBM), mb = code_map(b, kBM), sa = scale_map(a), sb = scale_map(b);
     configure<fp4_gemm_pair_kernel<NV>>(smem, device);
     fp4_gemm_pair_kernel<NV><<<2 * std::min(p.num_tiles, sms / 2), kPairThreads, smem, stream>>>(
-        code_map(a, kBM), code_map(b, kBM), scale_map(a), scale_map(b), p);
+        ma, mb, sa, sb, p.vec >= 16 ? out_map(p) : ma, p);
   } else {
     const int smem = (int)sizeof(Smem) + 1024;
     configure<fp4_gemm_kernel<NV>>(smem, device);
