@@ -528,13 +528,13 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
       uint32_t r[3][32];
 #pragma unroll
       for (int i = 0; i < 3; ++i) tmem_ld32(acc + chunk(i) * 32, r[i]);
-      // the next tile's factors are read while this tile is stored (all warps are past the tile before, whose
-      // buffer they go to)
-      if (t + clusters < p.num_tiles) fetch(t + clusters);
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(acc_free);
+      // the next tile's factors are read while this tile is stored (all warps are past the tile before, whose
+      // buffer they go to)
+      if (t + clusters < p.num_tiles) fetch(t + clusters);
       auto finish = [&](int c, const uint32_t (&v)[32]) {
         const int nc = tn0 + c * 32;
         if (nc >= p.N || tm0 >= p.M) return;

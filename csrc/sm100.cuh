@@ -348,8 +348,10 @@ __device__ __forceinline__ uint32_t cluster_map(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
+// Relaxed: it orders tensor-memory accesses only, by the tcgen05 fences around it and after the wait (a release at
+// cluster scope waits some 1100 cycles for the thread's earlier stores).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // mbar_wait for a barrier on which other CTAs of the cluster arrive.
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, int code, volatile int* abort,
