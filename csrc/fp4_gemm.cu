@@ -45,20 +45,6 @@ constexpr int kAcc1 = 160;               // first column of the second accumulat
 constexpr int kSfCol = 416;              // first column of the scales
 constexpr int kSfCols = 48;              // columns of one scale buffer
 
-struct Smem {
-  uint8_t a[kStages][kABytes];
-  uint8_t b[kStages][kBBytes];
-  uint8_t sa[kStages][kSaBytes];
-  uint8_t sb[kStages][kSbBytes];
-  float2 col[2][kBN];                  // row factor of B and bias of a tile's columns, by tile parity
-  uint16_t stage[4][32][18];           // a warp's 32 rows x 16 columns on their way to unaligned rows of D
-  uint64_t full[kStages], empty[kStages];
-  uint64_t acc_full[2], acc_free;
-  uint64_t drain;
-  uint32_t tmem_base;
-  int abort_flag;
-};
-
 struct Params {
   void* d;
   int64_t ldd;
@@ -120,202 +106,12 @@ __device__ __forceinline__ void store_unaligned(const Params& p, uint16_t (*stag
   }
 }
 
-// The same to any rows: whole 32-byte sectors where they allow it.
-__device__ __forceinline__ void store_chunk(const Params& p, uint16_t (*stage)[18], uint16_t* drow, int m0, int nc,
-                                            const uint32_t (&o)[16]) {
-  const int lane = lane_id();
-  if (p.vec == 32) {  // N % 16 == 0: a group of 16 columns is inside the row or past it
-    if (m0 + lane < p.M) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-        if (nc + 16 * q < p.N) st256(drow + nc + 16 * q, o + 8 * q);
-    }
-  } else if (p.vec == 16) {
-    if (m0 + lane < p.M) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (nc + 8 * q < p.N)
-          *reinterpret_cast<uint4*>(drow + nc + 8 * q) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
-    }
-  } else {
-    store_unaligned(p, stage, m0, nc, o);
-  }
-}
-
-template <bool NV>
-__global__ void __launch_bounds__(192, 1)
-fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b, Params p) {
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  volatile int* abort_flag = &sm.abort_flag;
-  const int warp = warp_id(), lane = lane_id();
-  constexpr int kStageTiles = NV ? 4 : 2;  // scale tiles along K of a whole stage
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&sm.full[s], 1);
-      mbar_init(&sm.empty[s], 1);
-    }
-    mbar_init(&sm.acc_full[0], 1);
-    mbar_init(&sm.acc_full[1], 1);
-    mbar_init(&sm.acc_free, 128);
-    mbar_init(&sm.drain, 1);
-    sm.abort_flag = 0;
-    fence_barrier_init();
-  }
-  if (warp == 1) {
-    tmem_alloc(&sm.tmem_base, 512);
-    tmem_relinquish();
-  }
-  if (warp == 0 && lane == 0) {
-    prefetch_tmap(&tm_a);
-    prefetch_tmap(&tm_b);
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = sm.tmem_base;
-
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    if (elect_one()) {
-      int it = 0;  // global stage counter (ring position)
-      bool ok = true;
-      const int sb_rows = (p.N + kFp4TileRows - 1) / kFp4TileRows;
-      for (int t = blockIdx.x; ok && t < p.num_tiles; t += gridDim.x) {
-        int tm, tn;
-        tile_coords(p, t, tm, tn);
-        const bool second = tn * 2 + 1 < sb_rows;  // whether B's tile has rows in a second scale tile
-        for (int k = 0; k < p.ksteps; ++k, ++it) {
-          const int s = it % kStages;
-          const uint32_t ph = (it / kStages) & 1;
-          if (!(ok = mbar_wait(&sm.empty[s], ph ^ 1, kStatusTimeoutEmpty, abort_flag, p.status))) break;
-          const int kt = k * kStageTiles;
-          const uint32_t bytes = (uint32_t)min(kStageTiles, p.ktiles - kt) * kFp4TileBytes;
-          mbar_arrive_expect_tx(&sm.full[s], kABytes + kBBytes + bytes * (second ? 3 : 2));
-          tma_load_2d(sm.a[s], &tm_a, &sm.full[s], k * 128, tm * kBM);
-          tma_load_2d(sm.b[s], &tm_b, &sm.full[s], k * 128, tn * kBN);
-          bulk_load(sm.sa[s], p.sa + ((int64_t)tm * p.ktiles + kt) * kFp4TileBytes, bytes, &sm.full[s]);
-          const uint8_t* sb = p.sb + ((int64_t)(2 * tn) * p.ktiles + kt) * kFp4TileBytes;
-          bulk_load(sm.sb[s], sb, bytes, &sm.full[s]);
-          if (second) bulk_load(sm.sb[s] + kSaBytes, sb + (int64_t)p.ktiles * kFp4TileBytes, bytes, &sm.full[s]);
-        }
-      }
-      // all issued copies land before the CTA's shared memory goes away
-      for (int j = max(0, it - kStages); j < it; ++j)
-        mbar_wait(&sm.full[j % kStages], (j / kStages) & 1, kStatusTimeoutTmaFull, nullptr, p.status);
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (elect_one()) {
-      int it = 0, tl = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; ok && t < p.num_tiles; t += gridDim.x, ++tl) {
-        // the columns shared with the previous tile's accumulator have been drained
-        if (tl > 0 && !(ok = mbar_wait(&sm.acc_free, (tl - 1) & 1, kStatusTimeoutSoftmax, abort_flag, p.status))) break;
-        tc_fence_after();
-        const uint32_t d = tmem + ((tl & 1) ? kAcc1 : 0);
-        for (int k = 0; k < p.ksteps; ++k, ++it) {
-          const int s = it % kStages;
-          if (!(ok = mbar_wait(&sm.full[s], (it / kStages) & 1, kStatusTimeoutTmaFull, abort_flag, p.status))) break;
-          // this stage's scale buffer was last read by the MMAs of two stages ago
-          if (it >= 2 && !(ok = mbar_wait(&sm.empty[(it - 2) % kStages], ((it - 2) / kStages) & 1, kStatusTimeoutMma,
-                                          abort_flag, p.status)))
-            break;
-          tc_fence_after();
-          const uint32_t sfa = tmem + kSfCol + (it & 1) * kSfCols, sfb = sfa + 16;
-          const int nt = min(kStageTiles, p.ktiles - k * kStageTiles);
-          const uint32_t aa = smem_u32(sm.a[s]), bb = smem_u32(sm.b[s]);
-          const uint32_t ssa = smem_u32(sm.sa[s]), ssb = smem_u32(sm.sb[s]);
-          for (int j = 0; j < nt; ++j) {
-            tmem_cp_scales<1>(sfa + 4 * j, smem_desc_scales(ssa + j * kFp4TileBytes));
-            tmem_cp_scales<1>(sfb + 8 * j, smem_desc_scales(ssb + j * kFp4TileBytes));
-            tmem_cp_scales<1>(sfb + 8 * j + 4, smem_desc_scales(ssb + kSaBytes + j * kFp4TileBytes));
-          }
-          const int nk = min(4, (p.K - k * kBK + 63) / 64);
-          for (int kk = 0; kk < nk; ++kk) {
-            const int j = NV ? kk : kk >> 1;
-            const uint32_t idesc = idesc_fp4(NV, kBM, kBN, NV ? 0 : (kk & 1) * 2);
-            mma_fp4_ss<NV, 1>(d, smem_desc_sw128(aa + kk * 32, 16, 1024), smem_desc_sw128(bb + kk * 32, 16, 1024), idesc,
-                           sfa + 4 * j, sfb + 8 * j, (k > 0 || kk > 0) ? 1u : 0u);
-          }
-          mma_commit(&sm.empty[s]);
-        }
-        if (!ok) break;
-        mma_commit(&sm.acc_full[tl & 1]);
-      }
-      if (!ok) *abort_flag = 1;
-      mma_commit(&sm.drain);
-      mbar_wait(&sm.drain, 0, kStatusTimeoutMma, nullptr, p.status);
-    }
-  } else {
-    // ------------------------------------------------------------ epilogue (warps 2..5)
-    const int wq = warp & 3;  // TMEM lane quarter this warp may access
-    const int row = wq * 32 + lane;
-    const uint32_t lane_base = (uint32_t)(wq * 32) << 16;
-    const int et = threadIdx.x - 64;
-    int tl = 0;
-    for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x, ++tl) {
-      int tm, tn;
-      tile_coords(p, t, tm, tn);
-      const int m = tm * kBM + row;
-      // the tile's column factors and biases, read while its MMAs run (a buffer is written again only after
-      // the barrier of the tile in between)
-      float2* col = sm.col[tl & 1];
-#pragma unroll
-      for (int i = et; i < kBN; i += 128) {
-        const int n = min(tn * kBN + i, p.N - 1);
-        col[i] = make_float2(NV ? __ldg(p.rb + n) : 1.f, p.bias != nullptr ? load_bias(p, n) : 0.f);
-      }
-      const float ra = (NV && m < p.M) ? __ldg(p.ra + m) : 1.f;
-      const bool ok = mbar_wait(&sm.acc_full[tl & 1], (tl >> 1) & 1, kStatusTimeoutMma, abort_flag, p.status);
-      // also the barrier of the column factors; all four warps leave together, since it counts them
-      if (named_bar_any(1, 128, !ok)) break;
-      tc_fence_after();
-      uint16_t* drow = static_cast<uint16_t*>(p.d) + (int64_t)m * p.ldd;
-      const uint32_t acc = tmem + lane_base + ((tl & 1) ? kAcc1 : 0);
-      // chunks of 32 columns, the ones shared with the other accumulator first: the last three of the
-      // first accumulator, the first three of the second
-#pragma unroll 1
-      for (int i = 0; i < kBN / 32; ++i) {
-        const int c = (tl & 1) ? i : (i < 3 ? 5 + i : i - 3);
-        uint32_t r[32];
-        tmem_ld32(acc + c * 32, r);
-        tmem_wait_ld();
-        if (i == 2) {
-          tc_fence_before();
-          mbar_arrive(&sm.acc_free);
-        }
-        const int nc = tn * kBN + c * 32;
-        if (nc >= p.N) continue;
-        uint32_t o[16];
-        const float4* cf = reinterpret_cast<const float4*>(col + c * 32);
-#pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const float4 f = cf[q];
-          o[q] = pack_out(p, fmaf(__uint_as_float(r[2 * q]) * ra, f.x, f.y),
-                          fmaf(__uint_as_float(r[2 * q + 1]) * ra, f.z, f.w));
-        }
-        store_chunk(p, sm.stage[wq], drow, m - lane, nc, o);
-      }
-    }
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem, 512);
-  }
-}
-
 // ---------------------------------------------------------------- CTA pairs
 // The same product with a pair of CTAs on each 256 x 256 tile (cta_group::2): each CTA holds 128 rows of A and of D and
 // loads 128 of B's 256 rows, so a stage moves 38 KB into an SM instead of 54 KB and the L2 is read a third less.
 //   warp 0      producer of its own CTA's operands and scales (all of B's scales: each CTA multiplies all of B), which
 //               all complete on the leader's barriers
-//   warp 1      leader CTA: the MMA thread, which also copies the scales of both CTAs to tensor memory.  A copy takes
-//               some 56 cycles of the tensor core's queue and a stage has 12 (nvfp4) or 6 (mxfp4), so the next
-//               stage's copies are issued between this stage's MMAs, where they run beside them
+//   warp 1      leader CTA: issues the MMAs, and before them the copies of both CTAs' scales to tensor memory
 //   warps 2..9  epilogue of the CTA's 128 rows: two warps a lane quarter, every other 32 columns each; rows leave
 //               through shared memory by TMA (direct stores of a lane's row cost the SM four times the cycles)
 // Tensor memory: scale buffers in the last 144 columns (three of 48 for nvfp4, six of 24 for mxfp4), accumulators at 0
@@ -419,70 +215,61 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     // the leader issues the pair's MMAs
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader)
-    if (elect_one()) {
-      const int my_tiles = cluster < p.num_tiles ? (p.num_tiles - 1 - cluster) / clusters + 1 : 0;
-      const int total = my_tiles * p.ksteps;  // stages of all tiles
-      bool ok = true;
-      // waits for stage i's operands and for its scale buffer, last read by the MMAs of kSfBufs stages before (with
-      // as many buffers as stages the ring itself has waited for those)
-      auto stage_ready = [&](int i) {
-        return mbar_wait_cluster(&sm.full[i % kPairStages], (i / kPairStages) & 1, kStatusTimeoutTmaFull, abort_flag,
-                                 p.status) &&
-               (kSfBufs >= kPairStages || i < kSfBufs ||
-                mbar_wait(&sm.empty[(i - kSfBufs) % kPairStages], ((i - kSfBufs) / kPairStages) & 1, kStatusTimeoutMma,
-                          abort_flag, p.status));
-      };
-      auto stage_there = [&](int i) {  // the same without waiting
-        return mbar_try_wait(smem_u32(&sm.full[i % kPairStages]), (i / kPairStages) & 1) &&
-               (kSfBufs >= kPairStages || i < kSfBufs ||
-                mbar_try_wait(smem_u32(&sm.empty[(i - kSfBufs) % kPairStages]), ((i - kSfBufs) / kPairStages) & 1));
-      };
-      // scale tile j along K of stage i, to tensor memory
-      auto copy_scales = [&](int i, int j) {
-        const int s = i % kPairStages;
-        const uint32_t sfa = tmem + kPairSfCol + (i % kSfBufs) * kSfBufCols, sfb = sfa + 4 * kStageTiles;
-        tmem_cp_scales<2>(sfa + 4 * j, smem_desc_scales(smem_u32(sm.sa[s]) + j * kFp4TileBytes));
-        tmem_cp_scales<2>(sfb + 8 * j, smem_desc_scales(smem_u32(sm.sb[s]) + j * kFp4TileBytes));
-        tmem_cp_scales<2>(sfb + 8 * j + 4, smem_desc_scales(smem_u32(sm.sb[s]) + kSaBytes + j * kFp4TileBytes));
-      };
-      auto scale_tiles = [&](int k) { return min(kStageTiles, p.ktiles - k * kStageTiles); };
-      int it = 0;
-      bool copied = false;  // this stage's scales are on their way already
-      for (int tl = 0; ok && tl < my_tiles; ++tl) {
-        // both CTAs have read the columns shared with the previous tile's accumulator
-        if (tl > 0 &&
-            !(ok = mbar_wait_cluster(&sm.acc_free, (tl - 1) & 1, kStatusTimeoutSoftmax, abort_flag, p.status)))
-          break;
+    // The whole warp runs the loop and one lane issues, so that the descriptors stay in uniform registers.  (Inside a
+    // branch of one lane every operand of every instruction is moved there first: 955 cycles a stage of nvfp4.)
+    const uint64_t da = smem_desc_sw128(smem_u32(sm.a[0]), 16, 1024), db = smem_desc_sw128(smem_u32(sm.b[0]), 16, 1024);
+    const uint64_t dsa = smem_desc_scales(smem_u32(sm.sa[0])), dsb = smem_desc_scales(smem_u32(sm.sb[0]));
+    int s = 0, s_old = 0, buf = 0;   // stage, that of kSfBufs stages before, scale buffer
+    uint32_t ph = 0, ph_old = 0;
+    int it = 0, tl = 0;
+    bool ok = true;
+    for (int t = cluster; ok && t < p.num_tiles; t += clusters, ++tl) {
+      // both CTAs have read the columns shared with the previous tile's accumulator
+      if (tl > 0) {
+        ok = mbar_wait_cluster(&sm.acc_free, (tl - 1) & 1, kStatusTimeoutSoftmax, abort_flag, p.status);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      }
+      const uint32_t d = tmem + ((tl & 1) ? kPairAcc1 : 0);
+      for (int k = 0; k < p.ksteps; ++k, ++it) {
+        ok = mbar_wait_cluster(&sm.full[s], ph, kStatusTimeoutTmaFull, abort_flag, p.status);
+        // this stage's scale buffer was last read by the MMAs of kSfBufs stages before (with as many buffers as stages
+        // the ring itself has waited for those)
+        if (kSfBufs < kPairStages && it >= kSfBufs) {
+          ok = ok && mbar_wait(&sm.empty[s_old], ph_old, kStatusTimeoutMma, abort_flag, p.status);
+          if (++s_old == kPairStages) s_old = 0, ph_old ^= 1;
+        }
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
-        const uint32_t d = tmem + ((tl & 1) ? kPairAcc1 : 0);
-        for (int k = 0; k < p.ksteps; ++k, ++it) {
-          const int s = it % kPairStages;
-          if (!copied) {
-            if (!(ok = stage_ready(it))) break;
-            tc_fence_after();
-            for (int j = 0; j < scale_tiles(k); ++j) copy_scales(it, j);
-          }
-          const int knext = k + 1 < p.ksteps ? k + 1 : 0;
-          const int next_tiles = it + 1 < total && stage_there(it + 1) ? scale_tiles(knext) : 0;
-          tc_fence_after();
-          const uint32_t sfa = tmem + kPairSfCol + (it % kSfBufs) * kSfBufCols, sfb = sfa + 4 * kStageTiles;
-          const uint32_t aa = smem_u32(sm.a[s]), bb = smem_u32(sm.b[s]);
-          const int nk = min(4, (p.K - k * kBK + 63) / 64);
+        const uint32_t sfa = tmem + kPairSfCol + buf * kSfBufCols, sfb = sfa + 4 * kStageTiles;
+        const int nt = min(kStageTiles, p.ktiles - k * kStageTiles), nk = min(4, (p.K - k * kBK + 63) / 64);
+        const uint64_t oa = (uint64_t)(s * (kABytes >> 4)), osa = (uint64_t)(s * (kSaBytes >> 4)),
+                       osb = (uint64_t)(s * (kSbBytes >> 4));
+        if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const int j = NV ? kk : kk >> 1;
-            const uint32_t idesc = idesc_fp4(NV, kPairBM, kBN, NV ? 0 : (kk & 1) * 2);
-            if (kk < nk)
-              mma_fp4_ss<NV, 2>(d, smem_desc_sw128(aa + kk * 32, 16, 1024), smem_desc_sw128(bb + kk * 32, 16, 1024),
-                                idesc, sfa + 4 * j, sfb + 8 * j, (k > 0 || kk > 0) ? 1u : 0u);
-            if (kk < next_tiles) copy_scales(it + 1, kk);
-          }
-          copied = next_tiles > 0;
+          for (int j = 0; j < kStageTiles; ++j)
+            if (j < nt) {
+              tmem_cp_scales<2>(sfa + 4 * j, dsa + osa + j * (kFp4TileBytes >> 4));
+              tmem_cp_scales<2>(sfb + 8 * j, dsb + osb + j * (kFp4TileBytes >> 4));
+              tmem_cp_scales<2>(sfb + 8 * j + 4, dsb + osb + (kSaBytes >> 4) + j * (kFp4TileBytes >> 4));
+            }
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            if (kk < nk) {
+              const int j = NV ? kk : kk >> 1;
+              mma_fp4_ss<NV, 2>(d, da + oa + 2 * kk, db + oa + 2 * kk, idesc_fp4(NV, kPairBM, kBN, NV ? 0 : (kk & 1) * 2),
+                                sfa + 4 * j, sfb + 8 * j, (k > 0 || kk > 0) ? 1u : 0u);
+            }
           mma_commit_pair(&sm.empty[s]);
         }
-        if (!ok) break;
-        mma_commit_pair(&sm.acc_full[tl & 1]);
+        __syncwarp();
+        if (++s == kPairStages) s = 0, ph ^= 1;
+        if (++buf == kSfBufs) buf = 0;
       }
+      if (!ok) break;
+      if (elect_one()) mma_commit_pair(&sm.acc_full[tl & 1]);
+      __syncwarp();
+    }
+    if (elect_one()) {
       if (!ok) *abort_flag = 1;
       mma_commit_pair(&sm.drain);
       mbar_wait(&sm.drain, 0, kStatusTimeoutMma, nullptr, p.status);
@@ -579,6 +366,242 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
   }
 }
 
+// ---------------------------------------------------------------- few rows
+// For few rows of x, D^T = B A^T: 128 rows of the weight B are the MMA's 128 rows and a tile of x's rows its N, so one
+// token costs a tile of 32 columns, and the K loop of a tile is split over a cluster of up to eight CTAs.  Each leaves
+// its fp32 part in its shared memory, [column of x's tile][128 rows], and adds a share of the columns over all
+// parts in rank order (the same sums every time), applies factors and bias and stores runs of the output row.
+//   warp 0      producer (ring of as many stages as fit, up to eight); with `early` the grid was launched to overlap
+//               the quantiser of x: the weight's part of the first stages is loaded before waiting for it
+//   warp 1      TMEM owner, scale copies and MMAs; scales in four buffers of 64 columns behind the accumulator
+//   warps 2..5  accumulator to shared memory; all warps add and store
+// Bound by the weight's bytes for one token, by the latency of a few K steps for small products.
+constexpr int kSmallThreads = 192, kSmallStages = 8, kSmallSfCol = 256, kSmallSfCols = 64;
+
+struct SmallBars {
+  uint64_t full[kSmallStages], empty[kSmallStages];
+  uint64_t acc_full;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct SmallParams {
+  Params g;          // M rows of x, N rows of the weight
+  int bn;            // rows of x of a tile: a multiple of 32 up to 256, of 128 where there are several tiles
+  int stages, stage_bytes;
+  int tiles_x;       // tiles along x
+  int split, per_split;  // CTAs of a cluster, K steps of each
+  int early;
+};
+
+template <bool NV>
+__global__ void __launch_bounds__(kSmallThreads, 1)
+fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                      const __grid_constant__ SmallParams sp) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ SmallBars sm;
+  const Params& p = sp.g;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  volatile int* abort_flag = &sm.abort_flag;
+  const int warp = warp_id(), lane = lane_id();
+  constexpr int kStageTiles = NV ? 4 : 2;
+  const int tile = blockIdx.x / sp.split, rank = blockIdx.x % sp.split;  // rank = rank in the cluster
+  const int tw = tile / sp.tiles_x, tx = tile % sp.tiles_x;
+  const int k0 = rank * sp.per_split, k1 = min(p.ksteps, k0 + sp.per_split), steps = max(0, k1 - k0);
+  const int x0 = tx * sp.bn;
+  // scale tiles of x's rows.  (A tile of x starts on a scale tile: in tensor memory the MMA wants its scales to start on
+  // an even column, of 32 rows each, and stops with "misaligned address" elsewhere.)
+  const int xt0 = x0 / kFp4TileRows;
+  const int xtiles = min((sp.bn + kFp4TileRows - 1) / kFp4TileRows, (p.M + kFp4TileRows - 1) / kFp4TileRows - xt0);
+  uint8_t *const sA = ring, *const sB = ring + kABytes, *const sSa = sB + sp.bn * 128, *const sSb = sSa + kSaBytes;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSmallStages; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    mbar_init(&sm.acc_full, 1);
+    sm.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_base, 512);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_x);
+  }
+  // factors and biases of the four weight rows that this thread stores, read while the operands come in
+  const int n = tw * kBM + lane * 4;
+  float rb[4], bias[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int nn = min(n + q, p.N - 1);
+    rb[q] = NV ? __ldg(p.rb + nn) : 1.f;
+    bias[q] = p.bias != nullptr ? load_bias(p, nn) : 0.f;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (elect_one()) {
+      auto bytes_of = [&](int i) { return (uint32_t)min(kStageTiles, p.ktiles - (k0 + i) * kStageTiles) * kFp4TileBytes; };
+      auto load_w = [&](int i, int s) {
+        const int kt = (k0 + i) * kStageTiles;
+        uint8_t* at = ring + s * sp.stage_bytes;
+        const uint32_t bytes = bytes_of(i);
+        mbar_arrive_expect_tx(&sm.full[s], kABytes + sp.bn * 128 + bytes * (1 + xtiles));
+        tma_load_2d(at, &tm_w, &sm.full[s], (k0 + i) * 128, tw * kBM);
+        bulk_load(at + (sSa - sA), p.sb + ((int64_t)tw * p.ktiles + kt) * kFp4TileBytes, bytes, &sm.full[s]);
+      };
+      auto load_x = [&](int i, int s) {
+        const int kt = (k0 + i) * kStageTiles;
+        uint8_t* at = ring + s * sp.stage_bytes;
+        tma_load_2d(at + kABytes, &tm_x, &sm.full[s], (k0 + i) * 128, x0);
+        for (int r = 0; r < xtiles; ++r)
+          bulk_load(at + (sSb - sA) + r * kSaBytes, p.sa + ((int64_t)(xt0 + r) * p.ktiles + kt) * kFp4TileBytes,
+                    bytes_of(i), &sm.full[s]);
+      };
+      const int first = min(steps, sp.stages);
+      for (int i = 0; i < first; ++i) load_w(i, i);
+      if (sp.early) wait_for_previous_grid();
+      for (int i = 0; i < first; ++i) load_x(i, i);
+      int i = first, s = 0;
+      uint32_t ph = 0;
+      for (; i < steps; ++i) {
+        if (!mbar_wait(&sm.empty[s], ph, kStatusTimeoutEmpty, abort_flag, p.status)) break;
+        load_w(i, s);
+        load_x(i, s);
+        if (++s == sp.stages) s = 0, ph ^= 1;
+      }
+      for (int j = max(0, i - sp.stages); j < i; ++j)  // all copies land before the ring is used for the sums
+        mbar_wait(&sm.full[j % sp.stages], (j / sp.stages) & 1, kStatusTimeoutTmaFull, nullptr, p.status);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    // The whole warp runs the loop and one lane issues: the descriptors stay in uniform registers.  (Inside a branch of
+    // one lane every operand of every instruction is moved there first, some 200 cycles an MMA and 40 a copy.)
+    const uint64_t da = smem_desc_sw128(smem_u32(ring), 16, 1024), db = smem_desc_sw128(smem_u32(ring) + kABytes, 16, 1024);
+    const uint64_t dsa = smem_desc_scales(smem_u32(ring) + (uint32_t)(sSa - sA));
+    const uint64_t dsb = smem_desc_scales(smem_u32(ring) + (uint32_t)(sSb - sA));
+    const bool two = xtiles > 1;
+    bool ok = true;
+    int s = 0, s4 = 0;           // the step's stage, and that of four steps before
+    uint32_t ph = 0, ph4 = 0;    // their parities
+    for (int i = 0; i < steps; ++i) {
+      const int k = k0 + i;
+      ok = mbar_wait(&sm.full[s], ph, kStatusTimeoutTmaFull, abort_flag, p.status);
+      if (i >= 4) {  // the scale buffer was last read by the MMAs of four steps ago
+        ok = ok && mbar_wait(&sm.empty[s4], ph4, kStatusTimeoutMma, abort_flag, p.status);
+        if (++s4 == sp.stages) s4 = 0, ph4 ^= 1;
+      }
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      tc_fence_after();
+      const uint64_t off = (uint64_t)(s * sp.stage_bytes) >> 4;
+      const uint32_t sfa = tmem + kSmallSfCol + (i & 3) * kSmallSfCols, sfb = sfa + 16;
+      const int nt = min(kStageTiles, p.ktiles - k * kStageTiles), nk = min(4, (p.K - k * kBK + 63) / 64);
+      if (elect_one()) {
+#pragma unroll
+        for (int j = 0; j < kStageTiles; ++j)
+          if (j < nt) {
+            tmem_cp_scales<1>(sfa + 4 * j, dsa + off + j * (kFp4TileBytes >> 4));
+            tmem_cp_scales<1>(sfb + 8 * j, dsb + off + j * (kFp4TileBytes >> 4));
+            if (two) tmem_cp_scales<1>(sfb + 8 * j + 4, dsb + off + (kSaBytes >> 4) + j * (kFp4TileBytes >> 4));
+          }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          if (kk < nk) {
+            const int j = NV ? kk : kk >> 1;
+            mma_fp4_ss<NV, 1>(tmem, da + off + 2 * kk, db + off + 2 * kk, idesc_fp4(NV, kBM, sp.bn, NV ? 0 : (kk & 1) * 2),
+                              sfa + 4 * j, sfb + 8 * j, (i > 0 || kk > 0) ? 1u : 0u);
+          }
+        mma_commit(&sm.empty[s]);
+      }
+      __syncwarp();
+      if (++s == sp.stages) s = 0, ph ^= 1;
+    }
+    if (elect_one()) {
+      if (!ok) *abort_flag = 1;
+      mma_commit(&sm.acc_full);
+      mbar_wait(&sm.acc_full, 0, kStatusTimeoutMma, nullptr, p.status);
+    }
+  }
+  // the MMAs are done and every copy has landed: the ring becomes the part's fp32 sums
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  float* part = reinterpret_cast<float*>(ring);
+  if (warp >= 2) {
+    const int wq = warp & 3, row = wq * 32 + lane;
+    for (int c = 0; c < sp.bn; c += 32) {
+      uint32_t r[32];
+      tmem_ld32(tmem + ((uint32_t)(wq * 32) << 16) + c, r);
+      tmem_wait_ld();
+#pragma unroll
+      for (int q = 0; q < 32; ++q) part[(c + q) * kBM + row] = steps > 0 ? __uint_as_float(r[q]) : 0.f;
+    }
+  }
+  if (sp.early) wait_for_previous_grid();  // the row factors of x are read below
+  tc_fence_before();
+  __syncthreads();
+  if (sp.split > 1) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+  // this CTA's share of x's rows: a warp takes eight of them at a time (that many loads in flight), a lane four weight
+  // rows of each
+  const int per = (sp.bn + sp.split - 1) / sp.split, c_end = min(min(sp.bn, p.M - x0), (rank + 1) * per);
+  constexpr int kWarps = kSmallThreads / 32, kRows = 8;
+  for (int c0 = rank * per + warp; c0 < c_end; c0 += kWarps * kRows) {
+    float v[kRows][4];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[u][q] = 0.f;
+    for (int r = 0; r < sp.split; ++r) {
+      const uint32_t from = sp.split > 1 ? cluster_map(part + lane * 4, r) : smem_u32(part + lane * 4);
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        const int c = c0 + u * kWarps;
+        if (c < c_end) {
+          const float4 q = ld_cluster_float4(from + c * (kBM * 4));
+          v[u][0] += q.x;
+          v[u][1] += q.y;
+          v[u][2] += q.z;
+          v[u][3] += q.w;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int c = c0 + u * kWarps;
+      if (c >= c_end || n >= p.N) continue;
+      const float ra = NV ? p.ra[x0 + c] : 1.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[u][q] = fmaf(v[u][q] * ra, rb[q], bias[q]);
+      uint16_t* d = static_cast<uint16_t*>(p.d) + (int64_t)(x0 + c) * p.ldd + n;
+      const uint32_t lo = pack_out(p, v[u][0], v[u][1]), hi = pack_out(p, v[u][2], v[u][3]);
+      if (p.vec >= 16) {  // rows of D are multiples of 16 bytes, N a multiple of 8
+        *reinterpret_cast<uint2*>(d) = make_uint2(lo, hi);
+      } else {
+        d[0] = (uint16_t)lo;
+        if (n + 1 < p.N) d[1] = (uint16_t)(lo >> 16);
+        if (n + 2 < p.N) d[2] = (uint16_t)hi;
+        if (n + 3 < p.N) d[3] = (uint16_t)(hi >> 16);
+      }
+    }
+  }
+  if (sp.split > 1) {
+    __syncthreads();
+    cluster_sync();  // the other CTAs have read this one's part
+  }
+}
+
 CUtensorMap code_map(const Fp4Matrix& x, uint32_t box_rows) {
   const uint64_t dims[2] = {(uint64_t)x.row_bytes(), (uint64_t)x.rows};
   const uint64_t strides[1] = {(uint64_t)x.row_bytes()};
@@ -612,27 +635,80 @@ CUtensorMap out_map(const Params& p) {
 }
 
 template <bool NV>
-void launch(const Fp4Matrix& a, const Fp4Matrix& b, Params& p, int device, cudaStream_t stream) {
-  const int sms = sm_count(device);
-  if (p.M > 256) {
-    p.tiles_m = (p.M + kPairBM - 1) / kPairBM;
-    p.num_tiles = p.tiles_m * p.tiles_n;
-    const int smem = (int)sizeof(PairSmem) + 1024;
-    const CUtensorMap ma = code_map(a, kBM), mb = code_map(b, kBM), sa = scale_map(a), sb = scale_map(b);
-    configure<fp4_gemm_pair_kernel<NV>>(smem, device);
-    fp4_gemm_pair_kernel<NV><<<2 * std::min(p.num_tiles, sms / 2), kPairThreads, smem, stream>>>(
-        ma, mb, sa, sb, p.vec >= 16 ? out_map(p) : ma, p);
-  } else {
-    const int smem = (int)sizeof(Smem) + 1024;
-    configure<fp4_gemm_kernel<NV>>(smem, device);
-    fp4_gemm_kernel<NV><<<std::min(p.num_tiles, sms), 192, smem, stream>>>(code_map(a, kBM), code_map(b, kBN), p);
-  }
+void launch_pair(const Fp4Matrix& a, const Fp4Matrix& b, Params& p, int device, cudaStream_t stream) {
+  p.tiles_m = (p.M + kPairBM - 1) / kPairBM;
+  p.num_tiles = p.tiles_m * p.tiles_n;
+  const int smem = (int)sizeof(PairSmem) + 1024;
+  const CUtensorMap ma = code_map(a, kBM), mb = code_map(b, kBM), sa = scale_map(a), sb = scale_map(b);
+  configure<fp4_gemm_pair_kernel<NV>>(smem, device);
+  fp4_gemm_pair_kernel<NV><<<2 * std::min(p.num_tiles, sm_count(device) / 2), kPairThreads, smem, stream>>>(
+      ma, mb, sa, sb, p.vec >= 16 ? out_map(p) : ma, p);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+constexpr int kSmallSmem = 227 * 1024 - 1024;  // dynamic shared memory of the few-rows kernel, barriers aside
+
+// Tile width, stages and split of the few-rows kernel.
+SmallParams plan_small(const Params& p, int sms, int bn, int split) {
+  SmallParams sp;
+  sp.g = p;
+  sp.bn = bn;
+  sp.tiles_x = (p.M + bn - 1) / bn;
+  TORCH_CHECK(bn % 32 == 0 && bn >= 32 && bn <= 256 && (sp.tiles_x == 1 || bn % kFp4TileRows == 0) && split >= 1 && split <= 8,
+              "fp4_linear: bad tile");
+  sp.stage_bytes = kABytes + bn * 128 + kSaBytes * (1 + (bn + kFp4TileRows - 1) / kFp4TileRows);
+  sp.stages = std::min(kSmallStages, (kSmallSmem - 1024) / sp.stage_bytes);
+  sp.split = split;
+  sp.per_split = (p.ksteps + split - 1) / split;
+  sp.early = 0;
+  return sp;
+}
+
+template <bool NV>
+void launch_small(const Fp4Matrix& a, const Fp4Matrix& b, const SmallParams& sp, int device, cudaStream_t stream) {
+  const int tiles = ((sp.g.N + kBM - 1) / kBM) * sp.tiles_x;
+  const CUtensorMap mw = code_map(b, kBM), mx = code_map(a, sp.bn);
+  // the ring, and the fp32 sums that take its place
+  const int smem = std::max(sp.stages * sp.stage_bytes, sp.bn * kBM * 4) + 1024;
+  configure<fp4_gemm_small_kernel<NV>>(kSmallSmem, device);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * sp.split));
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)sp.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = sp.early ? 2 : 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, fp4_gemm_small_kernel<NV>, mw, mx, sp));
+}
+
+// early: the kernel before this one on the stream is the quantiser that wrote a, launched without overlap itself.
+template <bool NV>
+void launch(const Fp4Matrix& a, const Fp4Matrix& b, Params& p, int device, cudaStream_t stream, bool early) {
+  const int sms = sm_count(device);
+  const char* force = getenv("FP4_FORCE");
+  int bn = 0, split = 0;
+  if (force && sscanf(force, "%d,%d", &bn, &split) == 2 && bn == 0) return launch_pair<NV>(a, b, p, device, stream);
+  if (!force && p.M > 512) return launch_pair<NV>(a, b, p, device, stream);
+  if (bn == 0) {
+    const int tx = (p.M + 255) / 256;
+    bn = tx > 1 ? 256 : (p.M + 31) / 32 * 32;
+    const int tiles = ((p.N + kBM - 1) / kBM) * tx;
+    split = std::max(1, std::min({8, sms / tiles, p.ksteps}));
+  }
+  SmallParams sp = plan_small(p, sms, bn, split);
+  sp.early = early ? 1 : 0;
+  launch_small<NV>(a, b, sp, device, stream);
 }
 
 // d [a.rows, b.rows] (bf16 or fp16, contiguous) = a b^T + bias, on the current device and stream.
 void gemm(const Fp4Matrix& a, const Fp4Matrix& b, const c10::optional<at::Tensor>& bias, at::Tensor& d,
-          cudaStream_t stream) {
+          cudaStream_t stream, bool early) {
   const int64_t M = a.rows, N = b.rows, K = a.cols;
   if (M == 0 || N == 0) return;
   Params p;
@@ -662,7 +738,7 @@ void gemm(const Fp4Matrix& a, const Fp4Matrix& b, const c10::optional<at::Tensor
   p.num_tiles = p.tiles_m * p.tiles_n;
   const int device = d.get_device();
   p.status = device_status_ptr(device);
-  a.nv ? launch<true>(a, b, p, device, stream) : launch<false>(a, b, p, device, stream);
+  a.nv ? launch<true>(a, b, p, device, stream, early) : launch<false>(a, b, p, device, stream, early);
 }
 
 c10::optional<at::Tensor> checked_bias(const c10::optional<at::Tensor>& bias, int64_t N, const at::Device& device) {
@@ -701,7 +777,7 @@ at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& data, const at::Ten
   at::Tensor y = at::empty(shape, plain.dtype(out_type == 0 ? at::kBFloat16 : out_type == 1 ? at::kHalf : dt));
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
   fp4_quantize_launch(x2, q, stream);
-  gemm(q, w, b, y, stream);
+  gemm(q, w, b, y, stream, true);
   return y;
 }
 
@@ -715,7 +791,7 @@ at::Tensor fp4_matmul(const at::Tensor& xdata, const at::Tensor& xscales, c10::o
   const auto b = checked_bias(bias, N, data.device());
   c10::cuda::CUDAGuard guard(data.device());
   at::Tensor y = at::empty({M, N}, data.options().dtype(out_type == 1 ? at::kHalf : at::kBFloat16));
-  gemm(q, w, b, y, at::cuda::getCurrentCUDAStream());
+  gemm(q, w, b, y, at::cuda::getCurrentCUDAStream(), false);
   return y;
 }
 

@@ -21,6 +21,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include "common.cuh"
 #include "fp4_host.h"
+#include "sm100.cuh"
 
 namespace dmad {
 namespace {
@@ -171,6 +172,7 @@ struct QuantParams {
 template <typename T, bool NV, bool ALIGNED, int UPT>
 __global__ void __launch_bounds__(512) quant_kernel(QuantParams p) {
   __shared__ uint32_t red[16];
+  launch_dependents();  // a product that reads the codes may set itself up meanwhile (it waits for this grid's end)
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   const int TX = blockDim.x;
   const int units = p.ktiles * kFp4TileBlocks * (fp4_block(NV) / 16);
