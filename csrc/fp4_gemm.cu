@@ -1,20 +1,14 @@
-// Persistent tcgen05 GEMM of block-scaled 4-bit operands for sm_100a.
+// tcgen05 GEMMs of block-scaled 4-bit operands for sm_100a.
 //
 //   D[M, N] = ra[m] rb[n] * sum_k A[m, k] B[n, k] + bias[n]          (bf16 or fp16 out, fp32 accumulation)
 //
 // A and B are e2m1 codes with one scale per 32 (mxfp4) or 16 (nvfp4) columns of K, multiplied on the tensor core
-// (kind::mxf4 / kind::mxf4nvf4), ra / rb the nvfp4 row scales applied to the accumulator in the epilogue.
-// The storage layout is described in fp4.cuh.
+// (kind::mxf4 / kind::mxf4nvf4), ra / rb the nvfp4 row scales applied to the accumulator in the epilogue, and one
+// rounding at the end.  The storage layout is described in fp4.cuh.  Two kernels: pairs of CTAs on 256 x 256 tiles, and
+// one for few rows (few_rows() says which).
 //
-// Structure (one CTA per SM, persistent over 128 x 256 output tiles):
-//   warp 0      producer: a ring of stages of 256 columns of K: A 128 x 128 bytes and B 256 x 128 bytes by TMA
-//               (128-byte swizzle), and their scale tiles by plain bulk copies
-//   warp 1      TMEM owner; one thread copies a stage's scale tiles to tensor memory (tcgen05.cp) and issues its
-//               four K = 64 MMAs
-//   warps 2..5  epilogue: tcgen05.ld (thread = output row), row scales, bias, stores
-// Tensor memory: scales of a stage take up to 48 columns, double-buffered in the last 96 columns; the two 256-column
-// accumulators overlap in columns [160, 256).  The epilogue drains the shared columns first and then releases the
-// accumulator, so the next tile's MMAs start while five eighths of the tile are still being stored.
+// Both step through K in stages of 256 columns (128 bytes of a row): codes by TMA with a 128-byte swizzle, scale tiles to
+// shared memory and from there by tcgen05.cp to tensor memory, then four K = 64 MMAs (fewer at the end of K).
 // Every mbarrier wait is bounded (2 s), records a status code and makes all roles leave.
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
@@ -34,16 +28,12 @@ at::Tensor fp4_rows(const at::Tensor& x, const char* name);
 
 namespace {
 
-constexpr int kBM = 128, kBN = 256, kStages = 4;
-constexpr int kBK = 256;                 // columns of K of a stage: 128 bytes of codes
-constexpr int kABytes = kBM * 128;       // 16 KB
-constexpr int kBBytes = kBN * 128;       // 32 KB
-constexpr int kMaxTiles = 4;             // scale tiles along K of a stage (nvfp4; mxfp4 has two)
+constexpr int kBM = 128, kBN = 256;
+constexpr int kBK = 256;            // columns of K of a stage: 128 bytes of codes
+constexpr int kABytes = kBM * 128;  // 16 KB
+constexpr int kMaxTiles = 4;        // scale tiles along K of a stage (nvfp4; mxfp4 has two)
 constexpr int kSaBytes = kMaxTiles * kFp4TileBytes;      // 2 KB
 constexpr int kSbBytes = 2 * kMaxTiles * kFp4TileBytes;  // 4 KB
-constexpr int kAcc1 = 160;               // first column of the second accumulator
-constexpr int kSfCol = 416;              // first column of the scales
-constexpr int kSfCols = 48;              // columns of one scale buffer
 
 struct Params {
   void* d;
@@ -69,8 +59,9 @@ __device__ __forceinline__ float load_bias(const Params& p, int n) {
   return __half2float(static_cast<const __half*>(p.bias)[n]);
 }
 
-__device__ __forceinline__ uint32_t pack_out(const Params& p, float lo, float hi) {
-  if (p.out_fp16) {
+template <bool FP16>
+__device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
+  if constexpr (FP16) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
   }
@@ -107,8 +98,9 @@ __device__ __forceinline__ void store_unaligned(const Params& p, uint16_t (*stag
 }
 
 // ---------------------------------------------------------------- CTA pairs
-// The same product with a pair of CTAs on each 256 x 256 tile (cta_group::2): each CTA holds 128 rows of A and of D and
-// loads 128 of B's 256 rows, so a stage moves 38 KB into an SM instead of 54 KB and the L2 is read a third less.
+// A pair of CTAs on each 256 x 256 tile (cta_group::2), persistent, one CTA an SM: each CTA holds 128 rows of A and of D
+// and loads 128 of B's 256 rows, so a stage moves 38 KB into an SM (one CTA with a 128 x 256 tile: 54 KB, more than the
+// some 64 bytes a cycle that the L2 gives an SM in the time of its MMAs).
 //   warp 0      producer of its own CTA's operands and scales (all of B's scales: each CTA multiplies all of B), which
 //               all complete on the leader's barriers
 //   warp 1      leader CTA: issues the MMAs, and before them the copies of both CTAs' scales to tensor memory
@@ -116,6 +108,9 @@ __device__ __forceinline__ void store_unaligned(const Params& p, uint16_t (*stag
 //               through shared memory by TMA (direct stores of a lane's row cost the SM four times the cycles)
 // Tensor memory: scale buffers in the last 144 columns (three of 48 for nvfp4, six of 24 for mxfp4), accumulators at 0
 // and 112.  The epilogue reads the 144 shared columns into registers at once and then releases the accumulator.
+// Measured: 37966 x 30720 x 5120 nvfp4 2.55 ms, 4.7 PFLOP/s at the 1.5 GHz that the power limit leaves (770 cycles a
+// stage of the tensor core's queue: the four MMAs and twelve scale copies); mxfp4 32760 x 8960 x 1536 0.22 ms, where
+// six stages of K are shorter than the epilogue of the tile.
 constexpr int kPairBM = 256, kPairStages = 5;
 constexpr int kPairAcc1 = 112, kPairSfCol = 368;
 constexpr int kEpiWarps = 8, kPairThreads = 64 + 32 * kEpiWarps;
@@ -134,7 +129,7 @@ struct PairSmem {
   int abort_flag;
 };
 
-template <bool NV>
+template <bool NV, bool FP16>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                      const __grid_constant__ CUtensorMap tm_sa, const __grid_constant__ CUtensorMap tm_sb,
@@ -330,8 +325,8 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
           const float4 f = f4[q];
-          o[q] = pack_out(p, fmaf(__uint_as_float(v[2 * q]) * tra, f.x, f.y),
-                          fmaf(__uint_as_float(v[2 * q + 1]) * tra, f.z, f.w));
+          o[q] = pack_out<FP16>(fmaf(__uint_as_float(v[2 * q]) * tra, f.x, f.y),
+                                fmaf(__uint_as_float(v[2 * q + 1]) * tra, f.z, f.w));
         }
         if (p.vec >= 16) {  // rows of D are multiples of 16 bytes: a box of 32 x 32 by TMA, 64-byte swizzle
           if (lane == 0) tma_store_wait_read();
@@ -373,12 +368,18 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
 // parts in rank order (the same sums every time), applies factors and bias and stores runs of the output row.
 //   warp 0      producer (ring of as many stages as fit, up to eight); with `early` the grid was launched to overlap
 //               the quantiser of x: the weight's part of the first stages is loaded before waiting for it
-//   warp 1      TMEM owner, scale copies and MMAs; scales in four buffers of 64 columns behind the accumulator
+//   warp 1      TMEM owner, scale copies and MMAs; the scales of each stage have their own columns
 //   warps 2..5  accumulator to shared memory; all warps add and store
+// Two CTAs share an SM (half the tensor memory each): a stage is some 12 instructions to the tensor core, which one warp
+// issues slower than the SM could load the stage (one token, 15360 x 5120: 15.5 us with one CTA, 12.9 us with two).
 // Bound by the weight's bytes for one token, by the latency of a few K steps for small products.
-constexpr int kSmallThreads = 192, kSmallStages = 8, kSmallSfCol = 256, kSmallSfCols = 64;
+// A tile of x starts on a scale tile: in tensor memory the MMA's scales have to start on an even column (of 32 rows
+// each), an odd one is a "misaligned address".
+constexpr int kSmallThreads = 192, kSmallStages = 8;
+constexpr int kSmallBN = 128, kSmallTmem = 256, kSmallSfCol = 128;  // scales behind the accumulator's 128 columns
 
 struct SmallBars {
+  float2 col[kBM];  // factor and bias of the tile's weight rows
   uint64_t full[kSmallStages], empty[kSmallStages];
   uint64_t acc_full;
   uint32_t tmem_base;
@@ -387,7 +388,7 @@ struct SmallBars {
 
 struct SmallParams {
   Params g;          // M rows of x, N rows of the weight
-  int bn;            // rows of x of a tile: a multiple of 32 up to 256, of 128 where there are several tiles
+  int bn;            // rows of x of a tile: a multiple of 32 up to 128, and 128 where there are several tiles
   int stages, stage_bytes;
   int tiles_x;       // tiles along x
   int split, per_split;  // CTAs of a cluster, K steps of each
@@ -395,7 +396,7 @@ struct SmallParams {
 };
 
 template <bool NV>
-__global__ void __launch_bounds__(kSmallThreads, 1)
+__global__ void __launch_bounds__(kSmallThreads, 2)
 fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                       const __grid_constant__ SmallParams sp) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -409,10 +410,7 @@ fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
   const int tw = tile / sp.tiles_x, tx = tile % sp.tiles_x;
   const int k0 = rank * sp.per_split, k1 = min(p.ksteps, k0 + sp.per_split), steps = max(0, k1 - k0);
   const int x0 = tx * sp.bn;
-  // scale tiles of x's rows.  (A tile of x starts on a scale tile: in tensor memory the MMA wants its scales to start on
-  // an even column, of 32 rows each, and stops with "misaligned address" elsewhere.)
-  const int xt0 = x0 / kFp4TileRows;
-  const int xtiles = min((sp.bn + kFp4TileRows - 1) / kFp4TileRows, (p.M + kFp4TileRows - 1) / kFp4TileRows - xt0);
+  constexpr int kSfCols = 8 * kStageTiles;  // columns of a stage's scales
   uint8_t *const sA = ring, *const sB = ring + kABytes, *const sSa = sB + sp.bn * 128, *const sSb = sSa + kSaBytes;
 
   if (threadIdx.x == 0) {
@@ -425,21 +423,12 @@ fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(&sm.tmem_base, 512);
+    tmem_alloc(&sm.tmem_base, kSmallTmem);
     tmem_relinquish();
   }
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&tm_w);
     prefetch_tmap(&tm_x);
-  }
-  // factors and biases of the four weight rows that this thread stores, read while the operands come in
-  const int n = tw * kBM + lane * 4;
-  float rb[4], bias[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int nn = min(n + q, p.N - 1);
-    rb[q] = NV ? __ldg(p.rb + nn) : 1.f;
-    bias[q] = p.bias != nullptr ? load_bias(p, nn) : 0.f;
   }
   tc_fence_before();
   __syncthreads();
@@ -454,7 +443,7 @@ fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
         const int kt = (k0 + i) * kStageTiles;
         uint8_t* at = ring + s * sp.stage_bytes;
         const uint32_t bytes = bytes_of(i);
-        mbar_arrive_expect_tx(&sm.full[s], kABytes + sp.bn * 128 + bytes * (1 + xtiles));
+        mbar_arrive_expect_tx(&sm.full[s], kABytes + sp.bn * 128 + 2 * bytes);
         tma_load_2d(at, &tm_w, &sm.full[s], (k0 + i) * 128, tw * kBM);
         bulk_load(at + (sSa - sA), p.sb + ((int64_t)tw * p.ktiles + kt) * kFp4TileBytes, bytes, &sm.full[s]);
       };
@@ -462,9 +451,7 @@ fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
         const int kt = (k0 + i) * kStageTiles;
         uint8_t* at = ring + s * sp.stage_bytes;
         tma_load_2d(at + kABytes, &tm_x, &sm.full[s], (k0 + i) * 128, x0);
-        for (int r = 0; r < xtiles; ++r)
-          bulk_load(at + (sSb - sA) + r * kSaBytes, p.sa + ((int64_t)(xt0 + r) * p.ktiles + kt) * kFp4TileBytes,
-                    bytes_of(i), &sm.full[s]);
+        bulk_load(at + (sSb - sA), p.sa + ((int64_t)tx * p.ktiles + kt) * kFp4TileBytes, bytes_of(i), &sm.full[s]);
       };
       const int first = min(steps, sp.stages);
       for (int i = 0; i < first; ++i) load_w(i, i);
@@ -488,36 +475,31 @@ fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     const uint64_t da = smem_desc_sw128(smem_u32(ring), 16, 1024), db = smem_desc_sw128(smem_u32(ring) + kABytes, 16, 1024);
     const uint64_t dsa = smem_desc_scales(smem_u32(ring) + (uint32_t)(sSa - sA));
     const uint64_t dsb = smem_desc_scales(smem_u32(ring) + (uint32_t)(sSb - sA));
-    const bool two = xtiles > 1;
     bool ok = true;
-    int s = 0, s4 = 0;           // the step's stage, and that of four steps before
-    uint32_t ph = 0, ph4 = 0;    // their parities
+    int s = 0;  // the step's stage
+    uint32_t ph = 0;
     for (int i = 0; i < steps; ++i) {
       const int k = k0 + i;
       ok = mbar_wait(&sm.full[s], ph, kStatusTimeoutTmaFull, abort_flag, p.status);
-      if (i >= 4) {  // the scale buffer was last read by the MMAs of four steps ago
-        ok = ok && mbar_wait(&sm.empty[s4], ph4, kStatusTimeoutMma, abort_flag, p.status);
-        if (++s4 == sp.stages) s4 = 0, ph4 ^= 1;
-      }
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       tc_fence_after();
       const uint64_t off = (uint64_t)(s * sp.stage_bytes) >> 4;
-      const uint32_t sfa = tmem + kSmallSfCol + (i & 3) * kSmallSfCols, sfb = sfa + 16;
+      // (the stage's columns were last read by the MMAs for which the ring has waited)
+      const uint32_t sfa = tmem + kSmallSfCol + s * kSfCols, sfb = sfa + 4 * kStageTiles;
       const int nt = min(kStageTiles, p.ktiles - k * kStageTiles), nk = min(4, (p.K - k * kBK + 63) / 64);
       if (elect_one()) {
 #pragma unroll
         for (int j = 0; j < kStageTiles; ++j)
           if (j < nt) {
             tmem_cp_scales<1>(sfa + 4 * j, dsa + off + j * (kFp4TileBytes >> 4));
-            tmem_cp_scales<1>(sfb + 8 * j, dsb + off + j * (kFp4TileBytes >> 4));
-            if (two) tmem_cp_scales<1>(sfb + 8 * j + 4, dsb + off + (kSaBytes >> 4) + j * (kFp4TileBytes >> 4));
+            tmem_cp_scales<1>(sfb + 4 * j, dsb + off + j * (kFp4TileBytes >> 4));
           }
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
           if (kk < nk) {
             const int j = NV ? kk : kk >> 1;
             mma_fp4_ss<NV, 1>(tmem, da + off + 2 * kk, db + off + 2 * kk, idesc_fp4(NV, kBM, sp.bn, NV ? 0 : (kk & 1) * 2),
-                              sfa + 4 * j, sfb + 8 * j, (i > 0 || kk > 0) ? 1u : 0u);
+                              sfa + 4 * j, sfb + 4 * j, (i > 0 || kk > 0) ? 1u : 0u);
           }
         mma_commit(&sm.empty[s]);
       }
@@ -531,18 +513,34 @@ fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
     }
   }
   // the MMAs are done and every copy has landed: the ring becomes the part's fp32 sums
+  if (warp >= 2) {  // factors and biases of the weight rows, read while the operands come in
+    const int r = threadIdx.x - 64, n = min(tw * kBM + r, p.N - 1);
+    sm.col[r] = make_float2(NV ? __ldg(p.rb + n) : 1.f, p.bias != nullptr ? load_bias(p, n) : 0.f);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   float* part = reinterpret_cast<float*>(ring);
   if (warp >= 2) {
     const int wq = warp & 3, row = wq * 32 + lane;
-    for (int c = 0; c < sp.bn; c += 32) {
-      uint32_t r[32];
-      tmem_ld32(tmem + ((uint32_t)(wq * 32) << 16) + c, r);
-      tmem_wait_ld();
+    const uint32_t acc = tmem + ((uint32_t)(wq * 32) << 16);
+    auto put = [&](int c, const uint32_t (&r)[32]) {
 #pragma unroll
       for (int q = 0; q < 32; ++q) part[(c + q) * kBM + row] = steps > 0 ? __uint_as_float(r[q]) : 0.f;
+    };
+    uint32_t r0[32], r1[32];
+    int c = 0;
+    for (; c + 64 <= sp.bn; c += 64) {
+      tmem_ld32(acc + c, r0);
+      tmem_ld32(acc + c + 32, r1);
+      tmem_wait_ld();
+      put(c, r0);
+      put(c + 32, r1);
+    }
+    if (c < sp.bn) {
+      tmem_ld32(acc + c, r0);
+      tmem_wait_ld();
+      put(c, r0);
     }
   }
   if (sp.early) wait_for_previous_grid();  // the row factors of x are read below
@@ -551,12 +549,16 @@ fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
   if (sp.split > 1) cluster_sync();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, kSmallTmem);
   }
   // this CTA's share of x's rows: a warp takes eight of them at a time (that many loads in flight), a lane four weight
   // rows of each
   const int per = (sp.bn + sp.split - 1) / sp.split, c_end = min(min(sp.bn, p.M - x0), (rank + 1) * per);
   constexpr int kWarps = kSmallThreads / 32, kRows = 8;
+  const int n = tw * kBM + lane * 4;
+  float2 cf[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) cf[q] = sm.col[lane * 4 + q];
   for (int c0 = rank * per + warp; c0 < c_end; c0 += kWarps * kRows) {
     float v[kRows][4];
 #pragma unroll
@@ -583,9 +585,10 @@ fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       if (c >= c_end || n >= p.N) continue;
       const float ra = NV ? p.ra[x0 + c] : 1.f;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[u][q] = fmaf(v[u][q] * ra, rb[q], bias[q]);
+      for (int q = 0; q < 4; ++q) v[u][q] = fmaf(v[u][q] * ra, cf[q].x, cf[q].y);
       uint16_t* d = static_cast<uint16_t*>(p.d) + (int64_t)(x0 + c) * p.ldd + n;
-      const uint32_t lo = pack_out(p, v[u][0], v[u][1]), hi = pack_out(p, v[u][2], v[u][3]);
+      const uint32_t lo = p.out_fp16 ? pack_out<true>(v[u][0], v[u][1]) : pack_out<false>(v[u][0], v[u][1]);
+      const uint32_t hi = p.out_fp16 ? pack_out<true>(v[u][2], v[u][3]) : pack_out<false>(v[u][2], v[u][3]);
       if (p.vec >= 16) {  // rows of D are multiples of 16 bytes, N a multiple of 8
         *reinterpret_cast<uint2*>(d) = make_uint2(lo, hi);
       } else {
@@ -634,34 +637,44 @@ CUtensorMap out_map(const Params& p) {
   return make_tmap_bf16(p.d, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-template <bool NV>
+template <bool NV, bool FP16>
 void launch_pair(const Fp4Matrix& a, const Fp4Matrix& b, Params& p, int device, cudaStream_t stream) {
   p.tiles_m = (p.M + kPairBM - 1) / kPairBM;
   p.num_tiles = p.tiles_m * p.tiles_n;
   const int smem = (int)sizeof(PairSmem) + 1024;
   const CUtensorMap ma = code_map(a, kBM), mb = code_map(b, kBM), sa = scale_map(a), sb = scale_map(b);
-  configure<fp4_gemm_pair_kernel<NV>>(smem, device);
-  fp4_gemm_pair_kernel<NV><<<2 * std::min(p.num_tiles, sm_count(device) / 2), kPairThreads, smem, stream>>>(
+  configure<fp4_gemm_pair_kernel<NV, FP16>>(smem, device);
+  fp4_gemm_pair_kernel<NV, FP16><<<2 * std::min(p.num_tiles, sm_count(device) / 2), kPairThreads, smem, stream>>>(
       ma, mb, sa, sb, p.vec >= 16 ? out_map(p) : ma, p);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-constexpr int kSmallSmem = 227 * 1024 - 1024;  // dynamic shared memory of the few-rows kernel, barriers aside
+constexpr int kSmallSmem = 109 * 1024;  // dynamic shared memory of a CTA of the few-rows kernel: two fit an SM
 
-// Tile width, stages and split of the few-rows kernel.
-SmallParams plan_small(const Params& p, int sms, int bn, int split) {
+// Tiles, stages and split of the few-rows kernel.
+SmallParams plan_small(const Params& p, bool nv, int sms, bool early) {
   SmallParams sp;
   sp.g = p;
-  sp.bn = bn;
-  sp.tiles_x = (p.M + bn - 1) / bn;
-  TORCH_CHECK(bn % 32 == 0 && bn >= 32 && bn <= 256 && (sp.tiles_x == 1 || bn % kFp4TileRows == 0) && split >= 1 && split <= 8,
-              "fp4_linear: bad tile");
-  sp.stage_bytes = kABytes + bn * 128 + kSaBytes * (1 + (bn + kFp4TileRows - 1) / kFp4TileRows);
-  sp.stages = std::min(kSmallStages, (kSmallSmem - 1024) / sp.stage_bytes);
-  sp.split = split;
-  sp.per_split = (p.ksteps + split - 1) / split;
-  sp.early = 0;
+  sp.tiles_x = (p.M + kSmallBN - 1) / kSmallBN;
+  sp.bn = sp.tiles_x > 1 ? kSmallBN : (p.M + 31) / 32 * 32;
+  sp.stage_bytes = kABytes + sp.bn * 128 + 2 * kSaBytes;
+  sp.stages = std::min({kSmallStages, (kSmallSmem - 1024) / sp.stage_bytes, (kSmallTmem - kSmallSfCol) / (nv ? 32 : 16)});
+  // CTAs for four fifths of the places (two an SM): above that, and with clusters of more than six, they no longer
+  // all run at once (16 x 5120 x 5120 nvfp4: 10.0 us with 160 to 240 CTAs, 15.1 us with 280)
+  const int tiles = ((p.N + kBM - 1) / kBM) * sp.tiles_x;
+  sp.split = std::max(1, std::min({6, sms * 2 * 4 / 5 / std::max(tiles, 1), p.ksteps}));
+  sp.per_split = (p.ksteps + sp.split - 1) / sp.split;
+  sp.early = early ? 1 : 0;
   return sp;
+}
+
+// Which kernel: up to 128 rows of x the few-rows kernel reads the weight once and wastes no half of a 256-row tile; above
+// it stays ahead while its 128 x 128 tiles do not fill the GPU (256 x 5120 x 15360: 20.4 us against 27.3; 1024 x 1536 x
+// 1536: 10.2 against 11.1) and falls behind when they do (512 x 5120 x 5120: 20.1 against 18.6).
+bool few_rows(const Params& p, int sms) {
+  if (p.M <= kSmallBN) return true;
+  const int64_t tiles = (int64_t)((p.N + kBM - 1) / kBM) * ((p.M + kSmallBN - 1) / kSmallBN);
+  return tiles <= sms * 7 / 8;
 }
 
 template <bool NV>
@@ -691,19 +704,9 @@ void launch_small(const Fp4Matrix& a, const Fp4Matrix& b, const SmallParams& sp,
 template <bool NV>
 void launch(const Fp4Matrix& a, const Fp4Matrix& b, Params& p, int device, cudaStream_t stream, bool early) {
   const int sms = sm_count(device);
-  const char* force = getenv("FP4_FORCE");
-  int bn = 0, split = 0;
-  if (force && sscanf(force, "%d,%d", &bn, &split) == 2 && bn == 0) return launch_pair<NV>(a, b, p, device, stream);
-  if (!force && p.M > 512) return launch_pair<NV>(a, b, p, device, stream);
-  if (bn == 0) {
-    const int tx = (p.M + 255) / 256;
-    bn = tx > 1 ? 256 : (p.M + 31) / 32 * 32;
-    const int tiles = ((p.N + kBM - 1) / kBM) * tx;
-    split = std::max(1, std::min({8, sms / tiles, p.ksteps}));
-  }
-  SmallParams sp = plan_small(p, sms, bn, split);
-  sp.early = early ? 1 : 0;
-  launch_small<NV>(a, b, sp, device, stream);
+  if (few_rows(p, sms)) launch_small<NV>(a, b, plan_small(p, NV, sms, early), device, stream);
+  else if (p.out_fp16) launch_pair<NV, true>(a, b, p, device, stream);
+  else launch_pair<NV, false>(a, b, p, device, stream);
 }
 
 // d [a.rows, b.rows] (bf16 or fp16, contiguous) = a b^T + bias, on the current device and stream.
