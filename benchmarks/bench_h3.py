@@ -69,6 +69,9 @@ def main(argv=None):
     ap.add_argument("--num-frames", type=int, default=124)
     ap.add_argument("--text-tokens", type=int, default=256)
     ap.add_argument("--budget-gib", type=float, default=16.0)
+    ap.add_argument("--fused-qk-norm", action="store_true", help="q / k norms and RoPE as one kernel")
+    ap.add_argument("--weights-fp4", choices=["nvfp4", "mxfp4"], default=None,
+                    help="4-bit projections (resident or cp mode); not the headline's precision")
     ap.add_argument("--cp-impl", default="fused", choices=["fused", "nccl"])
     a = ap.parse_args(argv)
     from dmad_b200.inference.h3 import build_row_timesteps, rollout
@@ -137,6 +140,11 @@ def main(argv=None):
             broadcast_module(model)
             model.enable_context_parallel(cp)
         model.eval().requires_grad_(False)
+        if a.fused_qk_norm:
+            model.enable_fused_qk_norm()
+        if a.weights_fp4:
+            model.quantize_fp4_(a.weights_fp4)
+            torch.cuda.empty_cache()
     build_s = time.time() - t_build
 
     results = []
@@ -174,7 +182,7 @@ def main(argv=None):
            "gpus": cp.world if cp is not None else 1, "build_s": round(build_s, 1),
            "config": {"model": f"H3-shaped DiT, {cfg.num_layers} blocks, hidden {cfg.dim}, ffn {cfg.ffn_dim}",
                       "video": f"{a.num_frames} frames at {a.height}x{a.width}", "text_tokens": a.text_tokens,
-                      "dtype": "bf16", "weights": "random init"},
+                      "dtype": a.weights_fp4 or "bf16", "weights": "random init"},
            "reference_published": {"s_per_evaluation_h200": 9.0, "s_per_video_4step_h200": 37.0,
                                    "lowvram_peak_sampling_gib": 5.9}}
     if streamed is not None:

@@ -54,6 +54,10 @@ def parse_args(argv=None):
                    help="directory of the int8 copy streamed from disk (default ~/.cache/dmad_b200/<id>/int8)")
     p.add_argument("--chunk-rows", type=int, default=None,
                    help="row-chunked blocks: at most this many rows of every intermediate except k / v")
+    p.add_argument("--weights-fp4", choices=["nvfp4", "mxfp4"], default=None,
+                   help="resident 4-bit weights and activations of the blocks' projections (LoRA folded in first)")
+    p.add_argument("--fused-qk-norm", action="store_true",
+                   help="q / k norms and RoPE in one pass (last-bit differences; implied by --weights-fp4)")
     p.add_argument("--offload", action="store_true", help="same as --low-vram auto")
     # the H3 video / audio VAEs are Diffusers modules that this package does not rebuild; latents are
     # written instead of decoded video, and these two flags only keep reference command lines parsing
@@ -65,7 +69,10 @@ def parse_args(argv=None):
                    help="hybrid: Ulysses inside groups of --ulysses-size ranks, ring attention across them "
                         "(for head counts the CP size does not divide)")
     p.add_argument("--ulysses-size", type=int, default=None)
-    return p.parse_args(argv)
+    a = p.parse_args(argv)
+    if (a.weights_fp4 or a.fused_qk_norm) and (a.low_vram or a.offload):
+        p.error("--weights-fp4 and --fused-qk-norm run with resident weights: they exclude --low-vram / --offload")
+    return a
 
 
 def main(argv=None):
@@ -189,6 +196,12 @@ def main(argv=None):
         log(f"streaming {streamed.streamer.bytes_per_pass / 2**30:.1f} GiB of weights per model evaluation")
     else:
         model.to(device)
+        if args.fused_qk_norm:
+            model.enable_fused_qk_norm()
+        if args.weights_fp4:
+            n = model.quantize_fp4_(args.weights_fp4)
+            log(f"{n} projections quantised to {args.weights_fp4}")
+            peak("quantisation")
         if cp is not None:
             model.enable_context_parallel(cp)
     outs = []

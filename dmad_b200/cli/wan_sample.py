@@ -54,6 +54,8 @@ def parse(argv=None):
     p.add_argument("--negative_prompt", default=_NEG)
     p.add_argument("--timestep_shift", type=float, default=5.0)
     p.add_argument("--cp_size", type=int, default=1)
+    p.add_argument("--weights_fp4", choices=["nvfp4", "mxfp4"], default=None,
+                   help="4-bit weights and activations of the blocks' projections")
     p.add_argument("--tiny", action="store_true", help="tiny random model and shapes (smoke tests)")
     return p.parse_args(argv)
 
@@ -126,6 +128,9 @@ def main(argv=None):
         sd = {k[4:] if k.startswith("net.") else k: v for k, v in sd.items()}
         net.load_state_dict(sd)
     net = net.to(dev, dtype).eval()
+    if a.weights_fp4:
+        from ..models.layers import quantize_fp4_
+        quantize_fp4_(net.blocks, a.weights_fp4)
     if a.cp_size > 1:
         from ..parallel.cp import ContextParallel
         from ..train.trainer import make_cp_group

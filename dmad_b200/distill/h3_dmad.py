@@ -63,6 +63,7 @@ class H3DMADConfig:
     head_lr: float = 4e-5
     head_wd: float = 0.01
     gradient_checkpointing: bool = True
+    fused_qk_norm: bool = False       # q / k norms and RoPE as one kernel, forward and backward
     text_tokens: int = 256
     model_dir: str | None = None      # H3 release folder: transformer/config.json sets ``model``, shards load
     # shard the block weights over the ranks (FSDP-style, the reference's fully_shard per block,
@@ -122,6 +123,7 @@ class H3DMAD:
         if cfg.model_dir:
             from ..inference.h3 import load_transformer_weights
             load_transformer_weights(base, cfg.model_dir)
+        base.enable_fused_qk_norm(cfg.fused_qk_norm)
         self.student = base
         self.fake = copy.deepcopy(base)
         self.student.enable_lora(cfg.student_lora_rank)

@@ -32,7 +32,7 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..ops import attention as attn_ops
-from .layers import SegLinear, install_segment_key_remap
+from .layers import SegLinear, head_attention_core, install_segment_key_remap, quantize_fp4_
 from .sac import checkpoint_block
 
 
@@ -77,6 +77,7 @@ class _H3Attention(nn.Module):
     def __init__(self, dim, heads, eps):
         super().__init__()
         self.heads, self.head_dim, self.eps = heads, dim // heads, eps
+        self.fused_qk_norm = False  # q / k norms and RoPE in one pass (H3Model.enable_fused_qk_norm)
         self.qkv = SegLinear(dim, [("to_q", dim), ("to_k", dim), ("to_v", dim)], flat_name="qkv")
         self.to_out = nn.Module()
         self.to_out.add_module("0", SegLinear(dim, [("0", dim)], flat_name=""))
@@ -94,11 +95,19 @@ class _H3Attention(nn.Module):
         H, hd = self.heads, self.head_dim
         D = H * hd
         qkv = self.qkv(x)
-        q = ops.rms_norm(qkv[:, :D].reshape(L * H, hd), self.norm_q.weight, self.eps).reshape(L, D)
-        k = ops.rms_norm(qkv[:, D:2 * D].reshape(L * H, hd), self.norm_k.weight, self.eps).reshape(L, D)
-        if cos is not None:
-            q = ops.rope(q, cos, sin, hd)
-            k = ops.rope(k, cos, sin, hd)
+        if self.fused_qk_norm and (cp is None or cp.world == 1):
+            o = head_attention_core(qkv, self.norm_q.weight, self.norm_k.weight, cos, sin, 1, L, H, self.eps)
+            return getattr(self.to_out, "0")(o)
+        if self.fused_qk_norm:
+            q, k = ops.qk_head_norm_rope(qkv[:, :D].view(L, H, hd), qkv[:, D:2 * D].view(L, H, hd), self.norm_q.weight,
+                                         self.norm_k.weight, cos, sin, eps=self.eps)
+            q, k = q.view(L, D), k.view(L, D)
+        else:
+            q = ops.rms_norm(qkv[:, :D].reshape(L * H, hd), self.norm_q.weight, self.eps).reshape(L, D)
+            k = ops.rms_norm(qkv[:, D:2 * D].reshape(L * H, hd), self.norm_k.weight, self.eps).reshape(L, D)
+            if cos is not None:
+                q = ops.rope(q, cos, sin, hd)
+                k = ops.rope(k, cos, sin, hd)
         v = qkv[:, 2 * D:]
         if cp is not None and cp.world > 1 and torch.is_grad_enabled() and x.requires_grad:
             raise NotImplementedError("H3 context parallelism is inference-only (its exchanges carry no gradient)")
@@ -290,6 +299,18 @@ class H3Model(nn.Module):
     def enable_context_parallel(self, cp):
         """Shard the packed sequence over ``cp`` (a ``parallel.cp.ContextParallel``); None disables."""
         self.cp = cp
+
+    def enable_fused_qk_norm(self, on: bool = True):
+        """Per-head q / k norms and RoPE as one kernel (``ops.qk_head_norm_rope``), forward and backward, instead of
+        separate norm and rotation passes: one rounding to bf16 fewer, so results differ in the last bits."""
+        for b in [*self.token_refiner.refiner_blocks, *self.transformer_blocks]:
+            b.attn.fused_qk_norm = on
+
+    def quantize_fp4_(self, fmt: str = "nvfp4") -> int:
+        """4-bit inference: the attention and feed-forward projections of every block (0.34 of the 33B model's 0.6 B
+        parameters a block; adaLN projections, embeddings and heads stay) in place, with the fused q / k norm."""
+        self.enable_fused_qk_norm()
+        return quantize_fp4_(self.token_refiner, fmt) + quantize_fp4_(self.transformer_blocks, fmt)
 
     def lora_linears(self, targets=("to_q", "to_k", "to_v", "to_out.0", "ff.net.0.proj", "ff.net.2")):
         out = []

@@ -13,6 +13,7 @@
         train/image/main/edm/edm_guidance.py:54-80);
       * a rank-r LoRA adapter ``W x + (alpha/r) B A x`` in the Diffusers/PEFT
         layout (dmad_h3/lora.py:23-75).
+    ``quantize_fp4_`` turns the layer into a 4-bit inference layer (``ops.fp4_linear``).
 ``SelfAttnCore`` / ``CrossAttnCore``
     autograd functions that run q/k RMSNorm (+3D RoPE) and flash attention on
     the sm_100a kernels and produce the fused ``dqkv`` gradient directly.
@@ -74,6 +75,7 @@ class SegLinear(nn.Module):
         self.sn_enabled = False
         self.lora_rank = 0
         self.lora_scale = 0.0
+        self.fp4 = None  # an ops.Fp4Tensor once quantize_fp4_ has replaced the weight
         nn.init.xavier_uniform_(self.weight)
 
     # ------------------------------------------------------------------ segments
@@ -97,6 +99,7 @@ class SegLinear(nn.Module):
         Returns the number of segments wrapped.  Zero-initialised segments are
         skipped (sigma would be 0), as the reference does.
         """
+        self._refuse_fp4("spectral norm")
         n = 0
         dev = self.weight.device
         us, vs, gains, mask = [], [], [], []
@@ -165,6 +168,8 @@ class SegLinear(nn.Module):
         return torch.cat(scales)
 
     def effective_weight(self):
+        if self.fp4 is not None:
+            return ops.dequantize_fp4(self.fp4, self._fp4_dtype)
         if not self.sn_enabled:
             return self.weight
         if (self.weight.is_cuda and self.weight.dtype == torch.bfloat16 and self.in_features % 8 == 0
@@ -215,6 +220,7 @@ class SegLinear(nn.Module):
     # ------------------------------------------------------------------ LoRA
     def enable_lora(self, rank: int, alpha: float | None = None, segments: Sequence[str] | None = None):
         """Adds a LoRA adapter (A: [r, in] per segment, B: [out, r]) initialised so the output is unchanged."""
+        self._refuse_fp4("LoRA")
         self.lora_rank = int(rank)
         self.lora_alpha = float(alpha if alpha is not None else rank)
         self.lora_scale = self.lora_alpha / self.lora_rank
@@ -237,10 +243,47 @@ class SegLinear(nn.Module):
     def lora_delta_weight(self):
         return self.lora_scale * (self.lora_B * self.lora_mask) @ self.lora_A
 
+    # ------------------------------------------------------------------ 4-bit inference
+    @torch.no_grad()
+    def quantize_fp4_(self, fmt: str = "nvfp4"):
+        """Replaces the weight (spectral norm and LoRA folded in) by its 4-bit form, for inference: ``forward``
+        quantises its input and multiplies in 4 bits.  The layer can no longer be trained or saved."""
+        self._refuse_fp4("quantize_fp4_")
+        w = self.effective_weight()
+        if self.lora_rank:
+            w = w + self.lora_delta_weight().to(w.dtype)
+        self._fp4_dtype = w.dtype if w.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+        self.fp4 = ops.quantize_fp4(w.detach(), fmt)
+        self.weight = None
+        if self.lora_rank:
+            self.lora_A = self.lora_B = self.lora_mask = None
+            self.lora_rank = 0
+        if self.sn_enabled:
+            self.sn_u = self.sn_v = self.sn_gain = self.sn_mask = None
+            self.sn_enabled = False
+        return self
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        if self.fp4 is not None:  # devices follow the module; the stored numbers keep their types
+            q = self.fp4
+            rs = None if q.row_scale is None else fn(q.row_scale.view(torch.int32)).view(torch.float32)
+            self.fp4 = ops.Fp4Tensor(fn(q.data), fn(q.scales), rs, q.fmt, q.shape)
+        return self
+
+    def _refuse_fp4(self, what):
+        if self.fp4 is not None:
+            raise RuntimeError(f"{what}: the layer's weight has been replaced by its 4-bit form (quantize_fp4_)")
+
+    def _forward_fp4(self, x):
+        return ops.fp4_linear(x.to(self._fp4_dtype), self.fp4, self.bias)
+
     # ------------------------------------------------------------------ forward
     def forward_rows(self, x, start: int, stop: int):
         """Output columns ``[start, stop)`` of ``forward(x)``, computed from those weight rows only
         (one segment of a fused projection, for instance)."""
+        if self.fp4 is not None:
+            return self._forward_fp4(x)[..., start:stop]
         w = self.effective_weight()[start:stop]
         b = None if self.bias is None else self.bias[start:stop]
         if x.dtype != w.dtype:
@@ -254,6 +297,8 @@ class SegLinear(nn.Module):
         return F.linear(x, w, b)
 
     def forward(self, x):
+        if self.fp4 is not None:
+            return self._forward_fp4(x)
         w = self.effective_weight()
         b = self.bias
         if x.dtype != w.dtype:
@@ -273,6 +318,7 @@ class SegLinear(nn.Module):
         return prefix
 
     def _save_to_state_dict(self, destination, prefix, keep_vars):
+        self._refuse_fp4("state dict")
         base = self._split_prefix(prefix)
         w = self.weight if keep_vars else self.weight.detach()
         for i, (name, sl) in enumerate(self.seg_slices()):
@@ -298,6 +344,7 @@ class SegLinear(nn.Module):
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
         # keys arrive as <prefix><segment>.<name> (the parent's pre-hook maps the reference's
         # <parent>.<segment>.<name> layout under this module's prefix; see install_segment_key_remap)
+        self._refuse_fp4("loading a state dict")
         with torch.no_grad():
             consumed = set()
             for i, (name, sl) in enumerate(self.seg_slices()):
@@ -414,6 +461,70 @@ def self_attention_core(qkv, wq, wk, cos, sin, B, L, H, eps=1e-6):
         o = attn_ops.attention_reference(q.view(B, L, H, hd), k.view(B, L, H, hd), v.reshape(B, L, H, hd))
         return o.reshape(R, D)
     return _SelfAttnCore.apply(qkv, wq.float().contiguous(), wk.float().contiguous(), cos, sin, B, L, H, eps)
+
+
+class _HeadAttnCore(torch.autograd.Function):
+    """qkv [R, 3D] (pre-norm) -> attention output [R, D] with per-head q / k norms: the counterpart of
+    ``_SelfAttnCore`` on ``qk_head_norm_rope``'s kernels.  Only qkv, O and the LSE are kept."""
+
+    @staticmethod
+    def _heads(qkv, H):
+        R, D = qkv.shape[0], qkv.shape[1] // 3
+        return [qkv[:, i * D:(i + 1) * D].view(R, H, D // H) for i in range(3)]
+
+    @staticmethod
+    def forward(ctx, qkv, wq, wk, cos, sin, B, L, H, eps):
+        R, D = qkv.shape[0], qkv.shape[1] // 3
+        hd = D // H
+        q, k, v = _HeadAttnCore._heads(qkv, H)
+        q, k = ops.ext().head_norm_rope_fwd(q, k, wq, wk, cos, sin, None, eps, True)
+        scale = 1.0 / math.sqrt(hd)
+        o, lse = attn_ops.flash_attn_fwd(q.view(B, L, H, hd), k.view(B, L, H, hd), v.view(B, L, H, hd), scale)
+        ctx.save_for_backward(qkv, wq, wk, cos, sin, o, lse)
+        ctx.cfg = (B, L, H, hd, eps, scale)
+        return o.view(R, D)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        qkv, wq, wk, cos, sin, o, lse = ctx.saved_tensors
+        B, L, H, hd, eps, scale = ctx.cfg
+        e = ops.ext()
+        x, xk, v = _HeadAttnCore._heads(qkv, H)
+        q, k = e.head_norm_rope_fwd(x, xk, wq, wk, cos, sin, None, eps, True)
+        sh = (B, L, H, hd)
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        dq, dk, dv = _HeadAttnCore._heads(dqkv, H)
+        gq, gk = torch.empty_like(q), torch.empty_like(k)
+        attn_ops.flash_bwd_into(q.view(sh), k.view(sh), v.view(sh), o, do.contiguous().view(sh), lse, gq.view(sh), gk.view(sh),
+                                dv.view(sh), torch.empty_like(lse), scale)
+        dwq = torch.empty(wq.shape, dtype=wq.dtype, device=wq.device) if ctx.needs_input_grad[1] else None
+        dwk = torch.empty(wk.shape, dtype=wk.dtype, device=wk.device) if ctx.needs_input_grad[2] else None
+        e.head_norm_rope_bwd(gq, gk, x, xk, wq, wk, cos, sin, None, dq, dk, dwq, dwk, eps, True)
+        return dqkv, dwq, dwk, None, None, None, None, None, None
+
+
+def head_attention_core(qkv, wq, wk, cos, sin, B, L, H, eps=1e-6):
+    """Self-attention on a fused [B * L, 3D] projection with per-head q / k RMSNorm (weights [D / H]) and, with ``cos``
+    / ``sin`` [L, rot / 2], interleaved RoPE: one norm-and-rotation pass, flash attention, and a backward that writes
+    the fused gradient (bf16 CUDA; head size 64 or 128)."""
+    if not qkv.is_cuda:
+        R, D = qkv.shape[0], qkv.shape[1] // 3
+        q, k, v = (t.reshape(R, H, D // H) for t in qkv.split(D, dim=1))
+        q, k = ops.qk_head_norm_rope(q, k, wq, wk, cos, sin, eps=eps)
+        o = attn_ops.attention_reference(*(t.view(B, L, H, D // H) for t in (q, k, v)))
+        return o.reshape(R, D)
+    return _HeadAttnCore.apply(qkv, wq, wk, cos, sin, B, L, H, eps)
+
+
+def quantize_fp4_(module: nn.Module, fmt: str = "nvfp4") -> int:
+    """Quantises every ``SegLinear`` of ``module`` in place (``SegLinear.quantize_fp4_``); returns how many."""
+    n = 0
+    for m in module.modules():
+        if isinstance(m, SegLinear) and m.fp4 is None:
+            m.quantize_fp4_(fmt)
+            n += 1
+    return n
 
 
 class _CrossAttnCore(torch.autograd.Function):
