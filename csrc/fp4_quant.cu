@@ -4,7 +4,8 @@
 //   nvfp4:  g_r = the smallest 2^p with max_r |x| <= 6 * 448 * 2^p,
 //           s_b = e4m3(max_b |x| / (6 g_r)),                           code = e2m1(x / (s_b g_r))
 //
-// (e2m1 and e4m3 round to nearest with halves to the even code; e2m1 saturates at 6.)  A block that holds an
+// (e2m1 and e4m3 round to nearest with halves to the even code; e2m1 saturates at 6, and what rounds to zero has code
+// 0 whatever its sign.)  A block that holds an
 // infinity or a NaN gets the scale code NaN, so all its values read back as NaN; such blocks do not count
 // in g_r.  Scales are exact powers of two or quotients rounded once, so a code depends on nothing but the
 // numbers: the CPU restatement gives the same bytes.
@@ -61,41 +62,39 @@ __device__ __forceinline__ Unit<T> load_unit(const T* __restrict__ row, int c0, 
 }
 
 // max |x| of a unit as the bits of an fp32 number.  Non-negative numbers order as their bits do, with infinity
-// and NaN above all finite ones.
+// and NaN above all finite ones (16-bit maxima carry a NaN on).
 template <typename T>
 __device__ __forceinline__ uint32_t absmax_bits(const Unit<T>& u) {
-  uint32_t m = 0;
   if constexpr (sizeof(T) == 4) {
+    uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 16; ++i) m = max(m, u.w[i] & 0x7fffffffu);
     return m;
-  } else {
+  } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u.w[0]));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, u.w[i] & 0x7fff7fffu);
-    m = max(m & 0xffffu, m >> 16);
-    if constexpr (std::is_same_v<T, __nv_bfloat16>) return m << 16;
-    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+    for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&u.w[i])));
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&m) & 0x7fff7fffu;
+    return max(w & 0xffffu, w >> 16) << 16;
+  } else {
+    __half2 m = __habs2(*reinterpret_cast<const __half2*>(&u.w[0]));
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&u.w[i])));
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(&m) & 0x7fff7fffu;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(w & 0xffffu, w >> 16))));
   }
 }
 
+// Elements 2i and 2i + 1 of a unit as two packed floats.
 template <typename T>
-__device__ __forceinline__ void unit_to_float(const Unit<T>& u, float (&f)[16]) {
+__device__ __forceinline__ uint64_t unit_pair(const Unit<T>& u, int i) {
   if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(u.w[i]);
+    return f2(__uint_as_float(u.w[2 * i]), __uint_as_float(u.w[2 * i + 1]));
   } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[2 * i] = __uint_as_float(u.w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(u.w[i] & 0xffff0000u);
-    }
+    return f2(__uint_as_float(u.w[i] << 16), __uint_as_float(u.w[i] & 0xffff0000u));
   } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&u.w[i]));
-      f[2 * i] = h.x;
-      f[2 * i + 1] = h.y;
-    }
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&u.w[i]));
+    return f2(h.x, h.y);
   }
 }
 
@@ -107,6 +106,42 @@ __device__ __forceinline__ float row_scale_of(uint32_t amax_bits) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
+// Eight codes with those of -0 made +0.
+__device__ __forceinline__ uint32_t unsigned_zeros(uint32_t w) {
+  const uint32_t some = (w | (w >> 1) | (w >> 2)) & 0x11111111u;  // codes that are not zero
+  return w & (0x77777777u | (some << 3));
+}
+
+// Codes of 16 values x * m of 16-bit elements x.  Rounded to steps of 2^-15 first, by adding and subtracting 384: x m
+// differs from a border b of two codes by 2^-11 b or more unless x over the scale is b, and where m is a rounded
+// reciprocal it is off by no more than 2^-20; so the step moves such a product onto b and no other onto it.
+template <typename T>
+__device__ __forceinline__ void encode16(const Unit<T>& u, float m, uint32_t (&out)[2]) {
+  const uint64_t m2 = f2(m, m), c = f2(384.f, 384.f);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = f2_split(f2_sub(f2_fma(unit_pair(u, 4 * h + i), m2, c), c));
+      y[2 * i] = v.x;
+      y[2 * i + 1] = v.y;
+    }
+    out[h] = unsigned_zeros(float8_to_e2m1x8(y));
+  }
+}
+
+// The same for fp32 elements, given the values.
+__device__ __forceinline__ void encode32(const float (&v)[16], uint32_t (&out)[2]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = v[8 * h + i];
+    out[h] = unsigned_zeros(float8_to_e2m1x8(y));
+  }
+}
+
 // Codes of one unit for nvfp4; returns the block's scale code.
 template <typename T>
 __device__ __forceinline__ uint32_t encode_nv(const Unit<T>& u, uint32_t amax, float ginv, uint32_t (&out)[2]) {
@@ -114,28 +149,38 @@ __device__ __forceinline__ uint32_t encode_nv(const Unit<T>& u, uint32_t amax, f
     out[0] = out[1] = 0u;
     return 0x7fu;
   }
-  const uint32_t code = float_to_e4m3(__fdiv_rn(__uint_as_float(amax) * ginv, 6.f));
-  const float s = e4m3_to_float(code);
-  float f[16], y[8];
-  unit_to_float(u, f);
-  // 16-bit elements: x / s differs from a border b of two codes by 2^-11 b or more unless it is b, and then the
-  // product with the rounded 1 / s is off by 2^-23 of it; the addition and subtraction of 384 rounds to steps of
-  // 2^-15, which moves such a product onto b and no other onto it.  fp32 elements are divided.
-  const float r = s > 0.f ? __frcp_rn(s) : 0.f;
+  const float top = __uint_as_float(amax) * ginv;
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t code = float_to_e4m3(__fdiv_rn(top, 6.f));
+    const float s = e4m3_to_float(code);
+    float v[16];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+    for (int i = 0; i < 16; ++i) v[i] = s > 0.f ? __fdiv_rn(__uint_as_float(u.w[i]) * ginv, s) : 0.f;
+    encode32(v, out);
+    return code;
+  } else {
+    // top / 6 by the rounded 1 / 6, then rounded to 17 bits: as above, that puts what is half-way between two e4m3
+    // numbers (with an 11-bit top) back there and moves nothing else across
+    const uint32_t q = (__float_as_uint(top * (1.f / 6.f)) + 0x40u) & ~0x7fu;
+    const uint32_t code = float_to_e4m3(__uint_as_float(q));
+    const float s = e4m3_to_float(code);
+    float r;  // 1 / s to within 2^-23; 0 for a block without a scale
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+    r = s > 0.f ? r : 0.f;
+    if (ginv > 0x1p100f) {  // a row of tiny numbers: ginv r could overflow
+      Unit<float> big;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = f[8 * h + i], t = x * ginv;
-      if constexpr (sizeof(T) == 4) {
-        y[i] = s > 0.f ? __fdiv_rn(t, s) : t * 0.f;
-      } else {
-        y[i] = copysignf(fmaf(t, r, 384.f) - 384.f, x);
+      for (int i = 0; i < 8; ++i) {
+        const float2 x = f2_split(unit_pair(u, i));
+        big.w[2 * i] = __float_as_uint(x.x * ginv);
+        big.w[2 * i + 1] = __float_as_uint(x.y * ginv);
       }
+      encode16(big, r, out);
+    } else {
+      encode16(u, ginv * r, out);
     }
-    out[h] = float8_to_e2m1x8(y);
+    return code;
   }
-  return code;
 }
 
 // Codes of one unit for mxfp4 with the block's (two units') maximum; returns the scale code.
@@ -147,13 +192,13 @@ __device__ __forceinline__ uint32_t encode_mx(const Unit<T>& u, uint32_t amax, u
   }
   const uint32_t code = (uint32_t)max((int)(amax >> 23) - 2, 0);
   const float m = __uint_as_float((254u - code) << 23);  // 2^(127 - code)
-  float f[16], y[8];
-  unit_to_float(u, f);
+  if constexpr (sizeof(T) == 4) {
+    float v[16];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = f[8 * h + i] * m;
-    out[h] = float8_to_e2m1x8(y);
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(u.w[i]) * m;
+    encode32(v, out);
+  } else {
+    encode16(u, m, out);
   }
   return code;
 }
@@ -180,6 +225,7 @@ __global__ void __launch_bounds__(512) quant_kernel(QuantParams p) {
   const T* xr = static_cast<const T*>(p.x) + row * p.ld;
   const int chunks = (units + TX * UPT - 1) / (TX * UPT);
   Unit<T> v[UPT];
+  uint32_t top[UPT];  // maxima of the units
   auto load = [&](int c) {
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
@@ -194,8 +240,8 @@ __global__ void __launch_bounds__(512) quant_kernel(QuantParams p) {
       load(c);
 #pragma unroll
       for (int i = 0; i < UPT; ++i) {
-        const uint32_t a = absmax_bits(v[i]);
-        m = max(m, a < kInfBits ? a : 0u);
+        top[i] = absmax_bits(v[i]);
+        m = max(m, top[i] < kInfBits ? top[i] : 0u);
       }
     }
     m = __reduce_max_sync(0xffffffffu, m);
@@ -212,11 +258,15 @@ __global__ void __launch_bounds__(512) quant_kernel(QuantParams p) {
   // rows past R up to the scale tile's end have zero scales and no data
   const bool tile_row = row < ((int64_t)p.R + kFp4TileRows - 1) / kFp4TileRows * kFp4TileRows;
   for (int c = 0; c < chunks; ++c) {
-    if (!NV || chunks > 1) load(c);
+    if (!NV || chunks > 1) {
+      load(c);
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) top[i] = absmax_bits(v[i]);
+    }
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       const int u = threadIdx.x + (c * UPT + i) * TX;
-      uint32_t amax = absmax_bits(v[i]);
+      uint32_t amax = top[i];
       uint32_t codes[2], sc;
       if constexpr (NV) {
         sc = encode_nv(v[i], amax, ginv, codes);
@@ -269,11 +319,17 @@ __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict_
                                                       const uint8_t* __restrict__ scales, int ktiles,
                                                       const float* __restrict__ row_scale, O* __restrict__ out, int R,
                                                       int K) {
+  // rows of out that are no multiples of 32 bytes leave through shared memory, a warp's 512 columns at a time
+  __shared__ float turn[ALIGNED ? 1 : 8][ALIGNED ? 1 : 32 * 17];
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= R) return;
   const float g = NV ? row_scale[row] : 1.f;
   O* orow = out + row * K;
-  for (int u = threadIdx.x; u * 16 < K; u += blockDim.x) {
+  const int lane = threadIdx.x & 31;
+  // whole warps stay together: a lane past the row works on its last unit
+  for (int first = threadIdx.x - lane; first * 16 < K; first += blockDim.x) {
+    const int u = min(first + lane, (K - 1) / 16);
+    if (ALIGNED && first + lane != u) continue;
     const uint2 w = __ldg(reinterpret_cast<const uint2*>(data + row * row_bytes + (int64_t)u * 8));
     const uint32_t sc = __ldg(scales + fp4_scale_offset(row, NV ? u : u >> 1, ktiles));
     const float s = NV ? e4m3_to_float(sc) * g : ue8m0_to_float(sc);
@@ -306,13 +362,21 @@ __global__ void __launch_bounds__(256) dequant_kernel(const uint8_t* __restrict_
         st256(orow + u * 16, o);
       }
     } else {
+      float* t = turn[(threadIdx.y * blockDim.x + threadIdx.x) >> 5];
+      __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (u * 16 + i < K) {
-          if constexpr (sizeof(O) == 4) orow[u * 16 + i] = f[i];
-          else if constexpr (std::is_same_v<O, __nv_bfloat16>) orow[u * 16 + i] = __float2bfloat16_rn(f[i]);
-          else orow[u * 16 + i] = __float2half_rn(f[i]);
+      for (int i = 0; i < 16; ++i) t[lane * 17 + i] = f[i];
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int e = i * 32 + lane, c = first * 16 + e;
+        const float v = t[(e >> 4) * 17 + (e & 15)];
+        if (c < K) {
+          if constexpr (sizeof(O) == 4) orow[c] = v;
+          else if constexpr (std::is_same_v<O, __nv_bfloat16>) orow[c] = __float2bfloat16_rn(v);
+          else orow[c] = __float2half_rn(v);
         }
+      }
     }
   }
 }

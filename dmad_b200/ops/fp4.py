@@ -9,7 +9,7 @@ Formats (``fmt``), both of e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their nega
   weight may have any positive fp32 factors (one tensor-wide factor repeated, for instance).
 
 All roundings are to the nearest, halves to the even code; values above 6 scales become 6 (mxfp4 can clip the
-largest of a block by up to a quarter).  A block that holds an infinity or a NaN reads back as NaN.  The CPU
+largest of a block by up to a quarter), and zero is +0.  A block that holds an infinity or a NaN reads back as NaN.  The CPU
 path is a PyTorch restatement that gives the same bytes.
 
 Forward only: the codes have no gradient, so inputs that require one are refused while gradients are
@@ -151,7 +151,7 @@ def quantize_fp4_reference(x: torch.Tensor, fmt: str):
     step = torch.where(v < 2, 0.5, torch.where(v < 4, 1.0, 2.0))
     v = (torch.round(v / step) * step).clamp(max=6.0)  # round: halves to even multiples = even codes
     code = torch.where(v < 2, 2 * v, torch.where(v < 4, v + 2, v / 2 + 4)).to(torch.uint8)
-    code = torch.where(torch.signbit(xb), code + 8, code)
+    code = torch.where((xb < 0) & (code > 0), code + 8, code)  # zero has one code
     code = torch.where(bad[..., None], torch.zeros_like(code), code).reshape(R, nb * blk)[:, :K]
     code = torch.nn.functional.pad(code, (0, -K % 32))
     return (code[:, 0::2] | (code[:, 1::2] << 4)).contiguous(), _tile_scales(scale), row_scale
