@@ -9,10 +9,13 @@
 //
 // Bound by HBM: the forward reads and writes q and k once, the backward reads g and x and writes dx; the
 // statistics are taken again from x, which is in registers anyway, so nothing is kept between the passes.  A
-// head is held by a group of G lanes, eight elements a lane (16-byte accesses of 16-bit types), and a group
-// takes U heads of one row at a time: U loads in flight, one read of the row's angles.  gridDim.y separates q
-// from k, so a thread has one weight slice and one gradient accumulator.  dw: per-thread sums over the tasks
-// of a persistent grid, one partial row a block, and a second kernel that adds the partials in a fixed order.
+// head is held by a group of G lanes, eight elements a lane (16-byte accesses of 16-bit types, streamed past the
+// caches: nothing is read twice), and a group takes U heads of one row at a time: U loads in flight, one read of the
+// row's angles.  gridDim.y separates q from k, so a thread has one weight slice and one gradient accumulator.  dw:
+// per-thread sums over the tasks of a persistent grid, one partial row a block, and a second kernel that adds the
+// partials in a fixed order.
+// Measured at 37966 rows of 40 + 40 heads of 128, bf16: forward 256 us (6.1 TB/s), backward 414 us (5.6 TB/s; with
+// U = 4 instead of 8 and cached accesses 497 us; with the next task's loads issued ahead, U = 2, 690 us).
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -66,7 +69,7 @@ struct Raw8 {
 
   __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -96,8 +99,8 @@ struct Raw8 {
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
   if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    __stcs(reinterpret_cast<float4*>(p), make_float4(f[0], f[1], f[2], f[3]));
+    __stcs(reinterpret_cast<float4*>(p) + 1, make_float4(f[4], f[5], f[6], f[7]));
   } else {
     uint32_t w[4];
 #pragma unroll
@@ -109,7 +112,7 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
       }
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
   }
 }
 
@@ -600,9 +603,9 @@ void head_norm_rope_bwd(const at::Tensor& gq, const at::Tensor& gk, const at::Te
       using T = decltype(tag);
       dispatch_group(p.hd, [&](auto g) {
         dispatch_mode(mode, [&](auto m) {
-          constexpr int U = 4;
+          constexpr int U = sizeof(T) == 4 ? 4 : 8;
           for (Side& s : p.side) s.chunks = (s.H + U - 1) / U;
-          blocks = (int)blocks_for(p, g, (int64_t)sms * 4);
+          blocks = (int)blocks_for(p, g, (int64_t)sms * 2);
           if (want_dw) {
             partial = at::empty({2, blocks, p.hd}, q.options().dtype(at::kFloat));
             for (int i = 0; i < 2; ++i)
