@@ -87,6 +87,10 @@ std::tuple<at::Tensor, at::Tensor> head_norm_rope_fwd(const at::Tensor& q, const
                                                       c10::optional<at::Tensor> cosT, c10::optional<at::Tensor> sinT,
                                                       c10::optional<at::Tensor> positions, double eps,
                                                       bool interleaved);
+std::tuple<at::Tensor, at::Tensor> head_norm_rope(const at::Tensor& q, const at::Tensor& k, c10::optional<at::Tensor> wq,
+                                                  c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cosT,
+                                                  c10::optional<at::Tensor> sinT, c10::optional<at::Tensor> positions,
+                                                  double eps, bool interleaved);
 void head_norm_rope_bwd(const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q, const at::Tensor& k,
                         c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cosT,
                         c10::optional<at::Tensor> sinT, c10::optional<at::Tensor> positions, at::Tensor& dq,
@@ -144,6 +148,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp4_dequantize", &dmad::fp4_dequantize);
   m.def("fp4_linear", &dmad::fp4_linear);
   m.def("fp4_matmul", &dmad::fp4_matmul);
+  m.def("head_norm_rope", &dmad::head_norm_rope);
   m.def("head_norm_rope_fwd", &dmad::head_norm_rope_fwd);
   m.def("head_norm_rope_bwd", &dmad::head_norm_rope_bwd);
   m.def("fsdp_gather", &dmad::fsdp_gather);

@@ -50,25 +50,6 @@ def qk_head_norm_rope_reference(q, k, wq=None, wk=None, cos=None, sin=None, posi
     return tuple(outs)
 
 
-class _HeadNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, interleaved):
-        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
-        ctx.cfg = (eps, interleaved)
-        return ext().head_norm_rope_fwd(q, k, wq, wk, cos, sin, positions, eps, interleaved)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dwq = torch.empty(wq.shape, dtype=wq.dtype, device=wq.device) if ctx.needs_input_grad[2] else None
-        dwk = torch.empty(wk.shape, dtype=wk.dtype, device=wk.device) if ctx.needs_input_grad[3] else None
-        ext().head_norm_rope_bwd(gq, gk, q, k, wq, wk, cos, sin, positions, dq, dk, dwq, dwk, *ctx.cfg)
-        return dq, dk, dwq, dwk, None, None, None, None, None
-
-
 def _check(q, k, wq, wk, cos, sin, positions):
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"qk_head_norm_rope: q and k must be [R, heads, hd] with one R and hd, got {tuple(q.shape)} "
@@ -100,7 +81,7 @@ def _check(q, k, wq, wk, cos, sin, positions):
 def qk_head_norm_rope(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor | None = None, wk: torch.Tensor | None = None,
                       cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
                       positions: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = True):
-    """``(Rot(rmsnorm(q) * wq), Rot(rmsnorm(k) * wk))`` per head, contiguous; differentiable in q, k, wq and wk.
+    """``(Rot(rmsnorm(q) * wq), Rot(rmsnorm(k) * wk))`` per head, contiguous; differentiable once in q, k, wq and wk.
 
     ``q`` [R, Hq, hd], ``k`` [R, Hk, hd] (bf16, fp16 or fp32; any row and head strides, e.g. column ranges of one
     fused projection; hd a multiple of 8 up to 256; Hq and Hk independent).  ``wq`` / ``wk`` [hd] (None: ones).
@@ -114,5 +95,5 @@ def qk_head_norm_rope(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor | None 
         return qk_head_norm_rope_reference(q, k, wq, wk, cos, sin, positions, eps, interleaved)
     # on CUDA the same checks are the extension's
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, wq, wk)):
-        return _HeadNormRope.apply(q, k, wq, wk, cos, sin, positions, eps, interleaved)
+        return ext().head_norm_rope(q, k, wq, wk, cos, sin, positions, eps, interleaved)
     return ext().head_norm_rope_fwd(q, k, wq, wk, cos, sin, positions, eps, interleaved)

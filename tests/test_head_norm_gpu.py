@@ -181,3 +181,33 @@ def test_refusals_on_the_gpu():
               lambda: f(q, k, *w, c, s, p.float()), lambda: f(q, k, *w, c.cpu(), s.cpu())):
         with pytest.raises(ValueError):
             g()
+
+
+def test_autograd_corner_cases():
+    """One weight without a gradient, an unused output, gradients twice through one graph, no second derivative, and an
+    input changed between forward and backward."""
+    ops = _ops()
+    q, k, w, c, s = _case(5, 2, 1, 64, 64, 5, torch.bfloat16, torch.float32)
+    ql, kl, wl = q.detach().requires_grad_(True), k.detach(), w[0].detach().requires_grad_(True)
+    qo, ko = ops.qk_head_norm_rope(ql, kl, wl, w[1].detach(), c, s)
+    assert qo.requires_grad and ko.requires_grad
+    g = torch.randn(qo.shape, device=dev).bfloat16()
+    a = torch.autograd.grad(qo, (ql, wl), g, retain_graph=True)
+    b = torch.autograd.grad(qo, (ql, wl), g)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    ref, gref = _oracle(q, k, w, c, s, torch.arange(5, device=dev), 64, True, (g, torch.zeros_like(ko)))
+    assert (a[0].double() - gref[0]).norm() <= 2.0 ** -8 * gref[0].norm()
+    assert (a[1].double() - gref[2]).norm() <= 2.0 ** -16 * gref[2].norm()
+    qo, _ = ops.qk_head_norm_rope(ql, kl, wl, w[1].detach(), c, s)
+    first, = torch.autograd.grad(qo, ql, g, create_graph=True)
+    assert torch.equal(first, a[0])
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(first.float().sum(), ql)
+    x = q.clone().requires_grad_(True)
+    qo, _ = ops.qk_head_norm_rope(x, kl, wl, w[1].detach(), c, s)
+    with torch.no_grad():
+        x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(qo, x, g)
+    with torch.no_grad():
+        assert not ops.qk_head_norm_rope(ql, kl, wl)[0].requires_grad
