@@ -15,13 +15,24 @@ int* device_status_ptr(int device) {
   std::lock_guard<std::mutex> lock(mu);
   if ((int)ptrs.size() <= device) ptrs.resize(device + 1, nullptr);
   if (ptrs[device] == nullptr) {
+    // The first kernel of a process may be one that a graph captures: the word is made outside of the capture, on a
+    // stream of its own.
     int prev;
     C10_CUDA_CHECK(cudaGetDevice(&prev));
     C10_CUDA_CHECK(cudaSetDevice(device));
-    C10_CUDA_CHECK(cudaMalloc(&ptrs[device], sizeof(int)));
-    C10_CUDA_CHECK(cudaMemset(ptrs[device], 0, sizeof(int)));
-    C10_CUDA_CHECK(cudaDeviceSynchronize());
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    int* word = nullptr;
+    cudaStream_t stream = nullptr;
+    cudaError_t err = cudaMalloc(&word, sizeof(int));
+    if (err == cudaSuccess) err = cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking);
+    if (err == cudaSuccess) err = cudaMemsetAsync(word, 0, sizeof(int), stream);
+    if (err == cudaSuccess) err = cudaStreamSynchronize(stream);
+    if (stream != nullptr) cudaStreamDestroy(stream);
+    C10_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
     C10_CUDA_CHECK(cudaSetDevice(prev));
+    C10_CUDA_CHECK(err);
+    ptrs[device] = word;
   }
   return ptrs[device];
 }

@@ -89,6 +89,21 @@ def test_linear_matches_64_bits(fmt, M, N, K):
     _check_linear(_ops(), M, N, K, fmt, torch.bfloat16, torch.float32, seed=M)
 
 
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("M,N,K,dtype", [(700, 4500, 1000, torch.bfloat16), (1100, 3001, 520, torch.bfloat16),
+                                         (520, 8200, 65, torch.float16), (2500, 5120, 1536, torch.bfloat16),
+                                         (385, 16387, 257, torch.float16), (257, 40000, 4100, torch.bfloat16)])
+def test_linear_of_many_tiles(fmt, M, N, K, dtype):
+    """Sizes that the kernel for pairs of CTAs takes: several tiles a pair, tails of every kind, rows of the output that
+    are no multiples of 16 bytes."""
+    _check_linear(_ops(), M, N, K, fmt, dtype, torch.float32 if N % 2 else dtype, seed=M)
+
+
+@pytest.mark.parametrize("M,N", [(127, 128), (128, 129), (129, 128), (129, 4096), (129, 16384), (128, 16512), (256, 8192)])
+def test_linear_on_both_sides_of_the_kernel_choice(M, N):
+    _check_linear(_ops(), M, N, 320, "nvfp4", torch.bfloat16, None, seed=N)
+
+
 @pytest.mark.parametrize("fmt,dtype,bias", [("mxfp4", torch.float16, None), ("nvfp4", torch.float16, torch.float16),
                                             ("nvfp4", torch.bfloat16, torch.bfloat16)])
 def test_linear_types(fmt, dtype, bias):
@@ -96,15 +111,15 @@ def test_linear_types(fmt, dtype, bias):
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
-@pytest.mark.parametrize("M", [3, 700])
-def test_linear_non_finite_rows_stay_in_their_rows(fmt, M):
+@pytest.mark.parametrize("M,N", [(3, 300), (700, 300), (700, 5000)])
+def test_linear_non_finite_rows_stay_in_their_rows(fmt, M, N):
     ops = _ops()
     x = torch.randn(M, 512).bfloat16()
     x[1, 5] = float("inf")
-    w = torch.randn(300, 512)
+    w = torch.randn(N, 512)
     w[7, 100] = float("nan")
     y = ops.fp4_linear(x.to(dev), ops.quantize_fp4(w.to(dev), fmt)).cpu()
-    bad = torch.zeros(M, 300, dtype=torch.bool)
+    bad = torch.zeros(M, N, dtype=torch.bool)
     bad[1], bad[:, 7] = True, True
     assert torch.equal(torch.isnan(y), bad)
 

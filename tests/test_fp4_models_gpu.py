@@ -135,3 +135,86 @@ def test_h3_in_four_bits_runs_and_repeats(fmt):
         one = m(v.cuda(), a.cuda(), pe.cuda(), **kw)
         two = m(v.cuda(), a.cuda(), pe.cuda(), **kw)
     assert all(torch.isfinite(o).all() and torch.equal(o, t) for o, t in zip(one, two))
+
+
+_FIRST = """
+import torch
+from dmad_b200 import ops
+x = torch.randn(3, 256, device="cuda").bfloat16()
+big = torch.randn(300, 256, device="cuda").bfloat16()
+q = torch.randn(3, 2, 64, device="cuda").bfloat16()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):  # the first kernels of the process
+    w = ops.quantize_fp4(big)
+    y, z = ops.fp4_linear(x, w), ops.fp4_linear(big, w)
+    h = ops.qk_head_norm_rope(q, q)
+g.replay()
+torch.cuda.synchronize()
+w2 = ops.quantize_fp4(big)
+assert torch.equal(y, ops.fp4_linear(x, w2)) and torch.equal(z, ops.fp4_linear(big, w2))
+assert torch.equal(h[0], ops.qk_head_norm_rope(q, q)[0])
+ops.check_device_status()
+print("captured first")
+"""
+
+
+def test_first_calls_of_a_process_under_capture():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stdout + r.stderr
+
+
+def test_training_step_of_the_norm_in_a_graph():
+    """Forward and backward captured and replayed on new numbers, beside an eager graph of the same leaves."""
+    from dmad_b200 import ops
+    q = torch.randn(40, 4, 64, device=dev).bfloat16().requires_grad_(True)
+    k = torch.randn(40, 2, 64, device=dev).bfloat16().requires_grad_(True)
+    w = torch.rand(64, device=dev, requires_grad=True)
+    ang = torch.randn(40, 32, device=dev)
+    c, s = ang.cos(), ang.sin()
+    gq, gk = torch.randn_like(q).detach(), torch.randn_like(k).detach()
+
+    def step():
+        return torch.autograd.grad(ops.qk_head_norm_rope(q, k, w, w, c, s), (q, k, w), (gq, gk))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    alive = ops.qk_head_norm_rope(q, k, w, w, c, s)
+    for seed in range(2):
+        with torch.no_grad():
+            torch.manual_seed(seed)
+            gq.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.isfinite(t).all() for t in torch.autograd.grad(alive, (q, k, w), (gq, gk)))
+
+
+def test_results_do_not_depend_on_the_stream_or_repetition():
+    """The few-rows kernel splits K over clusters: the same sums every time, on any stream, beside other work."""
+    from dmad_b200 import ops
+    torch.manual_seed(0)
+    for M, N, K in ((1, 640, 5120), (100, 1000, 2048), (200, 256, 4096)):
+        x = torch.randn(M, K, device=dev).bfloat16()
+        w = ops.quantize_fp4(torch.randn(N, K, device=dev), "nvfp4")
+        want = ops.fp4_linear(x, w)
+        streams = [torch.cuda.Stream() for _ in range(3)]
+        torch.cuda.synchronize()
+        got = []
+        for i in range(12):
+            with torch.cuda.stream(streams[i % 3]):
+                got.append(ops.fp4_linear(x, w))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, want) for g in got)
+    ops.check_device_status()
