@@ -14,6 +14,9 @@
 // load of 16-bit elements, one 8-byte store of codes); a row is held by one block in registers between the
 // row maximum and the encoding, so nvfp4's two levels cost no second read while the row fits (32768 columns;
 // longer rows are read twice).
+// Measured at 37966 x 5120 bf16 nvfp4: quantiser 110 us (4.5 TB/s; 71 % of the issue slots: some 230 instructions for a
+// thread's 16 columns; with IEEE divisions and one element an instruction 127 us; one unit a thread instead of two 123
+// us), inverse to bf16 82 us (6.1 TB/s).
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
