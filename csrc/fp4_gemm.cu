@@ -108,9 +108,10 @@ __device__ __forceinline__ void store_unaligned(const Params& p, uint16_t (*stag
 //               through shared memory by TMA (direct stores of a lane's row cost the SM four times the cycles)
 // Tensor memory: scale buffers in the last 144 columns (three of 48 for nvfp4, six of 24 for mxfp4), accumulators at 0
 // and 112.  The epilogue reads the 144 shared columns into registers at once and then releases the accumulator.
-// Measured: 37966 x 30720 x 5120 nvfp4 2.55 ms, 4.7 PFLOP/s at the 1.5 GHz that the power limit leaves (770 cycles a
-// stage of the tensor core's queue: the four MMAs and twelve scale copies); mxfp4 32760 x 8960 x 1536 0.22 ms, where
-// six stages of K are shorter than the epilogue of the tile.
+// Measured: 37966 x 30720 x 5120 nvfp4 2.42 ms (4.9 PFLOP/s at the 1.5 GHz that the power limit leaves), mxfp4 1.99 ms
+// (6.0 PFLOP/s); bound by the tensor core's queue, where a scale copy holds up the MMAs behind it for some 40 cycles
+// (nvfp4 has twelve a stage beside four MMAs, mxfp4 six).  mxfp4 32760 x 8960 x 1536 0.22 ms, where six stages of K are
+// shorter than the epilogue of the tile.
 constexpr int kPairBM = 256, kPairStages = 5;
 constexpr int kPairAcc1 = 112, kPairSfCol = 368;
 constexpr int kEpiWarps = 8, kPairThreads = 64 + 32 * kEpiWarps;
@@ -214,10 +215,35 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     // branch of one lane every operand of every instruction is moved there first: 955 cycles a stage of nvfp4.)
     const uint64_t da = smem_desc_sw128(smem_u32(sm.a[0]), 16, 1024), db = smem_desc_sw128(smem_u32(sm.b[0]), 16, 1024);
     const uint64_t dsa = smem_desc_scales(smem_u32(sm.sa[0])), dsb = smem_desc_scales(smem_u32(sm.sb[0]));
-    int s = 0, s_old = 0, buf = 0;   // stage, that of kSfBufs stages before, scale buffer
-    uint32_t ph = 0, ph_old = 0;
-    int it = 0, tl = 0;
-    bool ok = true;
+    // (s, ph): the stage whose MMAs are next; (sn, phn): the stage whose scales are copied next, at most one ahead, into
+    // buffer bufn, last read by the MMAs of stage s_old (kSfBufs before; with as many buffers as stages the ring itself
+    // has waited for those)
+    int s = 0, buf = 0, sn = 0, bufn = 0, s_old = 0;
+    uint32_t ph = 0, phn = 0, ph_old = 0;
+    const int my_tiles = cluster < p.num_tiles ? (p.num_tiles - 1 - cluster) / clusters + 1 : 0;
+    int64_t left = (int64_t)my_tiles * p.ksteps;  // stages whose scales have not been copied
+    int64_t copied = 0;
+    int kn = 0;  // K step of stage sn
+    auto copy_tile = [&](int j, int nt) {  // scale tile j along K of stage sn (the elected lane)
+      const uint32_t sfa = tmem + kPairSfCol + bufn * kSfBufCols, sfb = sfa + 4 * kStageTiles;
+      const uint64_t osa = (uint64_t)(sn * (kSaBytes >> 4)), osb = (uint64_t)(sn * (kSbBytes >> 4));
+      if (j < nt) {
+        tmem_cp_scales<2>(sfa + 4 * j, dsa + osa + j * (kFp4TileBytes >> 4));
+        tmem_cp_scales<2>(sfb + 8 * j, dsb + osb + j * (kFp4TileBytes >> 4));
+        tmem_cp_scales<2>(sfb + 8 * j + 4, dsb + osb + (kSaBytes >> 4) + j * (kFp4TileBytes >> 4));
+      }
+    };
+    auto advance = [&] {  // stage sn's copies have been issued
+      if (kSfBufs < kPairStages && copied >= kSfBufs)
+        if (++s_old == kPairStages) s_old = 0, ph_old ^= 1;
+      ++copied;
+      --left;
+      if (++sn == kPairStages) sn = 0, phn ^= 1;
+      if (++bufn == kSfBufs) bufn = 0;
+      if (++kn == p.ksteps) kn = 0;
+    };
+    int tl = 0;
+    bool ok = true, ahead = false;  // ahead: the scales of stage s have been copied
     for (int t = cluster; ok && t < p.num_tiles; t += clusters, ++tl) {
       // both CTAs have read the columns shared with the previous tile's accumulator
       if (tl > 0) {
@@ -225,38 +251,45 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
       }
       const uint32_t d = tmem + ((tl & 1) ? kPairAcc1 : 0);
-      for (int k = 0; k < p.ksteps; ++k, ++it) {
-        ok = mbar_wait_cluster(&sm.full[s], ph, kStatusTimeoutTmaFull, abort_flag, p.status);
-        // this stage's scale buffer was last read by the MMAs of kSfBufs stages before (with as many buffers as stages
-        // the ring itself has waited for those)
-        if (kSfBufs < kPairStages && it >= kSfBufs) {
-          ok = ok && mbar_wait(&sm.empty[s_old], ph_old, kStatusTimeoutMma, abort_flag, p.status);
-          if (++s_old == kPairStages) s_old = 0, ph_old ^= 1;
+      for (int k = 0; k < p.ksteps; ++k) {
+        if (!ahead) {
+          ok = mbar_wait_cluster(&sm.full[sn], phn, kStatusTimeoutTmaFull, abort_flag, p.status);
+          if (kSfBufs < kPairStages && copied >= kSfBufs)
+            ok = ok && mbar_wait(&sm.empty[s_old], ph_old, kStatusTimeoutMma, abort_flag, p.status);
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          tc_fence_after();
+          const int nt = min(kStageTiles, p.ktiles - kn * kStageTiles);
+          if (elect_one()) {
+#pragma unroll
+            for (int j = 0; j < kStageTiles; ++j) copy_tile(j, nt);
+          }
+          __syncwarp();
+          advance();
         }
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        // nvfp4: the next stage's scales go between this stage's MMAs if it has landed and its buffer is free (9472 x
+        // 16384 x 5120: 317 us against 341 with all copies first; mxfp4, with half as many, 286 us against 277)
+        bool next = NV && left > 0 && mbar_try_wait(smem_u32(&sm.full[sn]), phn);
+        if (kSfBufs < kPairStages && copied >= kSfBufs) next = next && mbar_try_wait(smem_u32(&sm.empty[s_old]), ph_old);
+        next = __all_sync(0xffffffffu, next);
         tc_fence_after();
         const uint32_t sfa = tmem + kPairSfCol + buf * kSfBufCols, sfb = sfa + 4 * kStageTiles;
-        const int nt = min(kStageTiles, p.ktiles - k * kStageTiles), nk = min(4, (p.K - k * kBK + 63) / 64);
-        const uint64_t oa = (uint64_t)(s * (kABytes >> 4)), osa = (uint64_t)(s * (kSaBytes >> 4)),
-                       osb = (uint64_t)(s * (kSbBytes >> 4));
+        const int nk = min(4, (p.K - k * kBK + 63) / 64), nt = next ? min(kStageTiles, p.ktiles - kn * kStageTiles) : 0;
+        const uint64_t oa = (uint64_t)(s * (kABytes >> 4));
         if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < kStageTiles; ++j)
-            if (j < nt) {
-              tmem_cp_scales<2>(sfa + 4 * j, dsa + osa + j * (kFp4TileBytes >> 4));
-              tmem_cp_scales<2>(sfb + 8 * j, dsb + osb + j * (kFp4TileBytes >> 4));
-              tmem_cp_scales<2>(sfb + 8 * j + 4, dsb + osb + (kSaBytes >> 4) + j * (kFp4TileBytes >> 4));
-            }
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
+          for (int kk = 0; kk < 4; ++kk) {
             if (kk < nk) {
               const int j = NV ? kk : kk >> 1;
               mma_fp4_ss<NV, 2>(d, da + oa + 2 * kk, db + oa + 2 * kk, idesc_fp4(NV, kPairBM, kBN, NV ? 0 : (kk & 1) * 2),
                                 sfa + 4 * j, sfb + 8 * j, (k > 0 || kk > 0) ? 1u : 0u);
             }
+            if (kk < kStageTiles) copy_tile(kk, nt);
+          }
           mma_commit_pair(&sm.empty[s]);
         }
         __syncwarp();
+        if (next) advance();
+        ahead = next;
         if (++s == kPairStages) s = 0, ph ^= 1;
         if (++buf == kSfBufs) buf = 0;
       }
