@@ -14,9 +14,9 @@
 // load of 16-bit elements, one 8-byte store of codes); a row is held by one block in registers between the
 // row maximum and the encoding, so nvfp4's two levels cost no second read while the row fits (32768 columns;
 // longer rows are read twice).
-// Measured at 37966 x 5120 bf16 nvfp4: quantiser 110 us (4.5 TB/s; 71 % of the issue slots: some 230 instructions for a
-// thread's 16 columns; with IEEE divisions and one element an instruction 127 us; one unit a thread instead of two 123
-// us), inverse to bf16 82 us (6.1 TB/s).
+// Measured at 37966 x 5120 bf16 nvfp4: quantiser 105 us (4.7 TB/s; some 230 instructions for a thread's 16 columns take
+// 71 % of the issue slots; with 64 registers a thread instead of 40 110 us; with IEEE divisions 127 us; one unit a thread
+// instead of two 123 us), inverse to bf16 82 us (6.1 TB/s).
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -218,7 +218,7 @@ struct QuantParams {
 
 // blockDim = (threads of a row, rows); more than one warp a row means one row a block.
 template <typename T, bool NV, bool ALIGNED, int UPT>
-__global__ void __launch_bounds__(512) quant_kernel(QuantParams p) {
+__global__ void __launch_bounds__(512, sizeof(T) == 4 || UPT > 2 ? 1 : 3) quant_kernel(QuantParams p) {
   __shared__ uint32_t red[16];
   launch_dependents();  // a product that reads the codes may set itself up meanwhile (it waits for this grid's end)
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
