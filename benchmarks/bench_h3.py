@@ -74,6 +74,8 @@ def main(argv=None):
                     help="4-bit projections (resident or cp mode); not the headline's precision")
     ap.add_argument("--cp-impl", default="fused", choices=["fused", "nccl"])
     a = ap.parse_args(argv)
+    if a.mode == "lowvram" and (a.weights_fp4 or a.fused_qk_norm):
+        ap.error("--weights-fp4 and --fused-qk-norm run with resident weights")
     from dmad_b200.inference.h3 import build_row_timesteps, rollout
     from dmad_b200.models.h3 import H3Config, H3Model
 
