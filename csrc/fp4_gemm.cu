@@ -207,6 +207,9 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
       if (rank == 0)
         for (int j = max(0, it - kPairStages); j < it; ++j)
           mbar_wait_cluster(&sm.full[j % kPairStages], (j / kPairStages) & 1, kStatusTimeoutTmaFull, nullptr, p.status);
+      // and so do the leader's arrivals for the last stages, which nobody else waits for
+      for (int j = max(0, it - kPairStages); ok && j < it; ++j)
+        ok = mbar_wait(&sm.empty[j % kPairStages], (j / kPairStages) & 1, kStatusTimeoutMma, abort_flag, p.status);
     }
   } else if (warp == 1 && rank != 0) {
     // the leader issues the pair's MMAs
@@ -388,6 +391,13 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
   }
   tc_fence_before();
   __syncthreads();
+  // The leader's last commit arrives in both CTAs, at some time after it is issued: neither leaves, or lets its shared
+  // memory go, before its own barrier has been reached.  (The leader has waited; here the CTA's last tile is stored, so
+  // the arrival is at most moments away.)
+  if (rank != 0 && warp == 1) {
+    if (elect_one()) mbar_wait(&sm.drain, 0, kStatusTimeoutMma, nullptr, p.status);
+    __syncwarp();
+  }
   cluster_sync();  // the pair's barriers and tensor memory are no longer in use by the other CTA
   if (warp == 1) {
     tc_fence_after();
