@@ -68,6 +68,20 @@ __device__ __forceinline__ uint32_t pack_out(float lo, float hi) {
   return pack_bf16x2(lo, hi);
 }
 
+// acc ra rb + bias for nvfp4's factors of the row and of the column, without an overflow or a lost digit where the result
+// has none.  An accumulator is 0 or of a size from 2^-20 (two codes and two scales) to 2^47 (K <= 2^24 products of at
+// most (6 * 448)^2), so acc ra is an ordinary number for ra from 2^-80 to 2^80 and the last step rounds once.  For rows
+// further out (elements above 1e27, or all below 1e-20) rb comes first, on acc c with c = 2^+-64, and ra / c last: acc c rb
+// is larger than fp32 only if the result is, and small enough to lose digits only if the result is below 2^-140.
+__device__ __forceinline__ bool far_out(float ra) { return !(ra >= 0x1p-80f && ra <= 0x1p80f); }
+__device__ __forceinline__ float apply_factors(float acc, float ra, float rb, float bias) {
+  return fmaf(acc * ra, rb, bias);
+}
+__device__ __forceinline__ float apply_factors_far(float acc, float ra, float rb, float bias) {
+  const bool big = ra > 1.f;
+  return fmaf(acc * (big ? 0x1p64f : 0x1p-64f) * rb, ra * (big ? 0x1p-64f : 0x1p64f), bias);
+}
+
 __device__ __forceinline__ void tile_coords(const Params& p, int t, int& tm, int& tn) {
   // column-major raster within groups of 8 M-tiles: neighbouring CTAs share B tiles in L2
   constexpr int kGroup = 8;
@@ -359,11 +373,20 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         if (nc >= p.N || tm0 >= p.M) return;
         uint32_t o[16];
         const float4* f4 = reinterpret_cast<const float4*>(col + c * 32);
+        if (NV && far_out(tra)) {
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          const float4 f = f4[q];
-          o[q] = pack_out<FP16>(fmaf(__uint_as_float(v[2 * q]) * tra, f.x, f.y),
-                                fmaf(__uint_as_float(v[2 * q + 1]) * tra, f.z, f.w));
+          for (int q = 0; q < 16; ++q) {
+            const float4 f = f4[q];
+            o[q] = pack_out<FP16>(apply_factors_far(__uint_as_float(v[2 * q]), tra, f.x, f.y),
+                                  apply_factors_far(__uint_as_float(v[2 * q + 1]), tra, f.z, f.w));
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 16; ++q) {
+            const float4 f = f4[q];
+            o[q] = pack_out<FP16>(apply_factors(__uint_as_float(v[2 * q]), tra, f.x, f.y),
+                                  apply_factors(__uint_as_float(v[2 * q + 1]), tra, f.z, f.w));
+          }
         }
         if (p.vec >= 16) {  // rows of D are multiples of 16 bytes: a box of 32 x 32 by TMA, 64-byte swizzle
           if (lane == 0) tma_store_wait_read();
@@ -628,8 +651,10 @@ fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       const int c = c0 + u * kWarps;
       if (c >= c_end || n >= p.N) continue;
       const float ra = NV ? p.ra[x0 + c] : 1.f;
+      const bool far = NV && far_out(ra);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[u][q] = fmaf(v[u][q] * ra, cf[q].x, cf[q].y);
+      for (int q = 0; q < 4; ++q)
+        v[u][q] = far ? apply_factors_far(v[u][q], ra, cf[q].x, cf[q].y) : apply_factors(v[u][q], ra, cf[q].x, cf[q].y);
       uint16_t* d = static_cast<uint16_t*>(p.d) + (int64_t)(x0 + c) * p.ldd + n;
       const uint32_t lo = p.out_fp16 ? pack_out<true>(v[u][0], v[u][1]) : pack_out<false>(v[u][0], v[u][1]);
       const uint32_t hi = p.out_fp16 ? pack_out<true>(v[u][2], v[u][3]) : pack_out<false>(v[u][2], v[u][3]);
