@@ -12,8 +12,8 @@ All roundings are to the nearest, halves to the even code; values above 6 scales
 largest of a block by up to a quarter), and zero is +0.  A block that holds an infinity or a NaN reads back as NaN.  The CPU
 path is a PyTorch restatement that gives the same bytes.
 
-Forward only: the codes have no gradient, so inputs that require one are refused while gradients are
-recorded.  It stands beside the int8 weights of the low-VRAM path (``inference.lowmem.int8_rows``): weights
+Forward only: the codes have no derivative, so inputs that require a gradient are refused while gradients are
+recorded, and dual tensors (forward mode) always.  It stands beside the int8 weights of the low-VRAM path (``inference.lowmem.int8_rows``): weights
 take 4.25 (mxfp4) or 4.5 (nvfp4) bits an element and the product runs on the tensor core's 4-bit kind.
 """
 from __future__ import annotations
@@ -24,6 +24,7 @@ from dataclasses import dataclass
 import torch
 
 from . import ext
+from .tangent import carries_tangent
 
 FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -97,6 +98,8 @@ def _check(q: Fp4Tensor, name: str):
 def _no_grad(what: str, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} is forward only: 4-bit codes have no gradient (call it under torch.no_grad)")
+    if carries_tangent(*tensors):
+        raise RuntimeError(f"{what} is forward only: 4-bit codes have no forward-mode derivative (unpack the dual tensor)")
 
 
 # ----------------------------------------------------------------------------- reference math
@@ -178,8 +181,7 @@ def dequantize_fp4_reference(q: Fp4Tensor) -> torch.Tensor:
 def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4") -> Fp4Tensor:
     """The 4-bit form of ``x`` [..., K] (bf16, fp16 or fp32), quantised along the last dimension."""
     nv = _block(fmt) == 16
-    if x.requires_grad:
-        _no_grad("quantize_fp4", x)
+    _no_grad("quantize_fp4", x)
     if x.is_cuda:  # the same checks are the extension's
         return Fp4Tensor(*ext().fp4_quantize(x, nv), fmt, tuple(x.shape))
     if x.dtype not in _DTYPES:
@@ -218,8 +220,7 @@ def fp4_linear(x: torch.Tensor | Fp4Tensor, w: Fp4Tensor, bias: torch.Tensor | N
     coded = isinstance(x, Fp4Tensor)
     if coded and x.fmt != w.fmt:
         raise ValueError(f"fp4_linear: x is {x.fmt}, w is {w.fmt}")
-    if torch.is_grad_enabled():
-        _no_grad("fp4_linear", None if coded else x, bias)
+    _no_grad("fp4_linear", None if coded else x, bias)
     if w.data.is_cuda:  # the same checks are the extension's
         out = -1 if out_dtype is None else _DTYPES.index(out_dtype)
         if not coded:

@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import ext
+from .tangent import carries_tangent
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
@@ -81,7 +82,8 @@ def _check(q, k, wq, wk, cos, sin, positions):
 def qk_head_norm_rope(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor | None = None, wk: torch.Tensor | None = None,
                       cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
                       positions: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = True):
-    """``(Rot(rmsnorm(q) * wq), Rot(rmsnorm(k) * wk))`` per head, contiguous; differentiable once in q, k, wq and wk.
+    """``(Rot(rmsnorm(q) * wq), Rot(rmsnorm(k) * wk))`` per head, contiguous; differentiable once in q, k, wq and wk
+    (reverse mode; dual tensors are refused on CUDA).
 
     ``q`` [R, Hq, hd], ``k`` [R, Hk, hd] (bf16, fp16 or fp32; any row and head strides, e.g. column ranges of one
     fused projection; hd a multiple of 8 up to 256; Hq and Hk independent).  ``wq`` / ``wk`` [hd] (None: ones).
@@ -94,6 +96,8 @@ def qk_head_norm_rope(q: torch.Tensor, k: torch.Tensor, wq: torch.Tensor | None 
         _check(q, k, wq, wk, cos, sin, positions)
         return qk_head_norm_rope_reference(q, k, wq, wk, cos, sin, positions, eps, interleaved)
     # on CUDA the same checks are the extension's
+    if carries_tangent(q, k, wq, wk, cos, sin):
+        raise RuntimeError("qk_head_norm_rope: the CUDA kernels have no forward-mode derivative (unpack the dual tensor)")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, wq, wk)):
         return ext().head_norm_rope(q, k, wq, wk, cos, sin, positions, eps, interleaved)
     return ext().head_norm_rope_fwd(q, k, wq, wk, cos, sin, positions, eps, interleaved)
