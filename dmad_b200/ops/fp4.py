@@ -197,6 +197,7 @@ def dequantize_fp4(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.T
     significant bits of a scale by two of a code) above bf16's subnormals; fp16 rounds and can overflow."""
     if dtype not in _DTYPES:
         raise ValueError(f"dequantize_fp4: dtype must be bf16, fp16 or fp32, got {dtype}")
+    _no_grad("dequantize_fp4", q.row_scale)
     if not q.data.is_cuda:
         return dequantize_fp4_reference(q).to(dtype).reshape(q.shape)
     out = ext().fp4_dequantize(q.data, q.scales, q.row_scale, math.prod(q.shape[:-1]), q.shape[-1], _block(q.fmt) == 16,
@@ -220,7 +221,7 @@ def fp4_linear(x: torch.Tensor | Fp4Tensor, w: Fp4Tensor, bias: torch.Tensor | N
     coded = isinstance(x, Fp4Tensor)
     if coded and x.fmt != w.fmt:
         raise ValueError(f"fp4_linear: x is {x.fmt}, w is {w.fmt}")
-    _no_grad("fp4_linear", None if coded else x, bias)
+    _no_grad("fp4_linear", x.row_scale if coded else x, w.row_scale, bias)
     if w.data.is_cuda:  # the same checks are the extension's
         out = -1 if out_dtype is None else _DTYPES.index(out_dtype)
         if not coded:

@@ -29,3 +29,8 @@ def test_dual_tensors_are_refused():
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.func.jvp(f, (x,), (torch.ones_like(x),))
     assert torch.isfinite(ops.fp4_linear(x, wq)).all()
+
+
+def test_row_factors_have_no_derivative():
+    from tests.test_op_derivatives_cpu import check_row_scale_refusals
+    check_row_scale_refusals(dev)
