@@ -86,6 +86,7 @@ class SegLinear(nn.Module):
             off += o
 
     def seg_weight(self, name):
+        self._refuse_fp4("seg_weight")
         for n, sl in self.seg_slices():
             if n == name:
                 return self.weight[sl]
@@ -281,9 +282,11 @@ class SegLinear(nn.Module):
     # ------------------------------------------------------------------ forward
     def forward_rows(self, x, start: int, stop: int):
         """Output columns ``[start, stop)`` of ``forward(x)``, computed from those weight rows only
-        (one segment of a fused projection, for instance)."""
-        if self.fp4 is not None:
-            return self._forward_fp4(x)[..., start:stop]
+        (one segment of a fused projection, for instance; 4-bit weights: from the multiple of 128 before them)."""
+        if self.fp4 is not None:  # from the tile of 128 rows on in which they begin
+            first, stop = start // 128 * 128, min(stop, self.out_features)
+            b = None if self.bias is None else self.bias[first:stop]
+            return ops.fp4_linear(x.to(self._fp4_dtype), self.fp4.row_slice(first, stop), b)[..., start - first:]
         w = self.effective_weight()[start:stop]
         b = None if self.bias is None else self.bias[start:stop]
         if x.dtype != w.dtype:

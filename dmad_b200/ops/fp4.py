@@ -58,6 +58,15 @@ class Fp4Tensor:
     def nbytes(self) -> int:
         return self.data.numel() + self.scales.numel() + (4 * self.rows if self.row_scale is not None else 0)
 
+    def row_slice(self, start: int, stop: int) -> "Fp4Tensor":
+        """Rows [start, stop) of a matrix, sharing its storage; ``start`` is a multiple of 128, the rows of a tile of
+        scales.  (The scales of the rows behind ``stop`` in its last tile stay; nothing reads them.)"""
+        if len(self.shape) != 2 or start % 128 or not 0 <= start <= stop <= self.shape[0]:
+            raise ValueError(f"row_slice: rows [{start}, {stop}) of shape {tuple(self.shape)} (a matrix, start a multiple of 128)")
+        rs = None if self.row_scale is None else self.row_scale[start:stop]
+        return Fp4Tensor(self.data[start:stop], self.scales[start // 128:start // 128 - (start - stop) // 128], rs, self.fmt,
+                         (stop - start, self.shape[1]))
+
     def to(self, device) -> "Fp4Tensor":
         rs = None if self.row_scale is None else self.row_scale.to(device)
         return Fp4Tensor(self.data.to(device), self.scales.to(device), rs, self.fmt, self.shape)
