@@ -510,7 +510,11 @@ class _HeadAttnCore(torch.autograd.Function):
 def head_attention_core(qkv, wq, wk, cos, sin, B, L, H, eps=1e-6):
     """Self-attention on a fused [B * L, 3D] projection with per-head q / k RMSNorm (weights [D / H]) and, with ``cos``
     / ``sin`` [L, rot / 2], interleaved RoPE: one norm-and-rotation pass, flash attention, and a backward that writes
-    the fused gradient (bf16 CUDA; head size 64 or 128)."""
+    the fused gradient (bf16 CUDA; head size 64 or 128).  Longer tables: their first L rows."""
+    if cos is not None:
+        if cos.shape[0] < L:
+            raise ValueError(f"head_attention_core: cos and sin must have L = {L} rows, got {tuple(cos.shape)}")
+        cos, sin = cos[:L], sin[:L]  # a sequence's row r turns by table row r (the norm's kernel counts r modulo the table)
     if not qkv.is_cuda:
         R, D = qkv.shape[0], qkv.shape[1] // 3
         q, k, v = (t.reshape(R, H, D // H) for t in qkv.split(D, dim=1))
