@@ -91,6 +91,7 @@ std::tuple<at::Tensor, at::Tensor> head_norm_rope(const at::Tensor& q, const at:
                                                   c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cosT,
                                                   c10::optional<at::Tensor> sinT, c10::optional<at::Tensor> positions,
                                                   double eps, bool interleaved);
+void check_captured_backward(const std::string& op);
 void head_norm_rope_bwd(const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q, const at::Tensor& k,
                         c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk, c10::optional<at::Tensor> cosT,
                         c10::optional<at::Tensor> sinT, c10::optional<at::Tensor> positions, at::Tensor& dq,
@@ -148,6 +149,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp4_dequantize", &dmad::fp4_dequantize);
   m.def("fp4_linear", &dmad::fp4_linear);
   m.def("fp4_matmul", &dmad::fp4_matmul);
+  m.def("check_captured_backward", &dmad::check_captured_backward);
   m.def("head_norm_rope", &dmad::head_norm_rope);
   m.def("head_norm_rope_fwd", &dmad::head_norm_rope_fwd);
   m.def("head_norm_rope_bwd", &dmad::head_norm_rope_bwd);

@@ -1,7 +1,12 @@
 // Autograd of qk_head_norm_rope in C++: a backward through a Python function costs the host some 50 us more, which for
 // few rows is most of the step.
 #include <torch/extension.h>
+#include <c10/cuda/CUDAStream.h>
+#include <cuda_runtime.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <stdexcept>
+#include <string>
 
 namespace dmad {
 
@@ -13,6 +18,31 @@ std::tuple<at::Tensor, at::Tensor> head_norm_rope_fwd(const at::Tensor& q, const
 void head_norm_rope_bwd(const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q, const at::Tensor& k, OptTensor wq,
                         OptTensor wk, OptTensor cosT, OptTensor sinT, OptTensor positions, at::Tensor& dq, at::Tensor& dk,
                         OptTensor dwq, OptTensor dwk, double eps, bool interleaved);
+
+// In a backward that a CUDA graph captures: an error where the gradient of a leaf would leave the capture.  While an
+// eager graph of the same leaves lives, they keep the accumulators that it made, and with them the stream on which it
+// made them; the engine then makes that stream, which nothing captures, wait for the captured one: no capture survives
+// that, and the process may not either.
+void check_captured_backward(const std::string& op) {
+  const auto capturing = [](const c10::cuda::CUDAStream& s) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (s.stream() == nullptr) return false;  // the default stream is never captured, nor may it be asked meanwhile
+    if (cudaStreamIsCapturing(s.stream(), &status) == cudaSuccess) return status == cudaStreamCaptureStatusActive;
+    cudaGetLastError();
+    return false;
+  };
+  const auto current = c10::cuda::getCurrentCUDAStream();
+  const auto node = torch::autograd::get_current_node();
+  if (node == nullptr || !capturing(current)) return;
+  for (const auto& edge : node->next_edges()) {
+    auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
+    if (leaf == nullptr) continue;
+    const auto stream = leaf->stream();
+    if (stream.has_value() && !capturing(c10::cuda::CUDAStream(*stream)))
+      throw std::runtime_error(op + ": this backward is being captured while a graph of the same leaves, recorded outside "
+                                    "of the capture, is alive; release that graph first, or record it on the captured stream");
+  }
+}
 
 namespace {
 
@@ -33,6 +63,7 @@ struct HeadNormRope : torch::autograd::Function<HeadNormRope> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list g) {
+    check_captured_backward("qk_head_norm_rope");
     const auto s = ctx->get_saved_variables();
     torch::autograd::variable_list out(9);
     {

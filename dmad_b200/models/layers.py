@@ -493,6 +493,7 @@ class _HeadAttnCore(torch.autograd.Function):
         qkv, wq, wk, cos, sin, o, lse = ctx.saved_tensors
         B, L, H, hd, eps, scale = ctx.cfg
         e = ops.ext()
+        e.check_captured_backward("head_attention_core")
         x, xk, v = _HeadAttnCore._heads(qkv, H)
         q, k = e.head_norm_rope_fwd(x, xk, wq, wk, cos, sin, None, eps, True)
         sh = (B, L, H, hd)
