@@ -84,7 +84,14 @@ def fp4_storage_shapes(rows: int, cols: int, fmt: str) -> tuple[tuple, tuple]:
     return (rows, -(-cols // 32) * 16), (-(-rows // 128), -(-blocks // 4), 512)
 
 
+def _columns(shape, what: str):
+    """A ValueError for the shape of a single number, which has no columns."""
+    if len(shape) < 1:
+        raise ValueError(f"{what} must have at least one dimension, got shape {tuple(shape)}")
+
+
 def _check(q: Fp4Tensor, name: str):
+    _columns(q.shape, name)
     blk = _block(q.fmt)
     cols, rows = int(q.shape[-1]), 1
     for s in q.shape[:-1]:
@@ -207,6 +214,7 @@ def dequantize_fp4(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.T
     if dtype not in _DTYPES:
         raise ValueError(f"dequantize_fp4: dtype must be bf16, fp16 or fp32, got {dtype}")
     _no_grad("dequantize_fp4", q.row_scale)
+    _columns(q.shape, "dequantize_fp4: q")
     if not q.data.is_cuda:
         return dequantize_fp4_reference(q).to(dtype).reshape(q.shape)
     out = ext().fp4_dequantize(q.data, q.scales, q.row_scale, math.prod(q.shape[:-1]), q.shape[-1], _block(q.fmt) == 16,
@@ -225,6 +233,7 @@ def fp4_linear(x: torch.Tensor | Fp4Tensor, w: Fp4Tensor, bias: torch.Tensor | N
         raise ValueError(f"fp4_linear: w must be a matrix, got shape {tuple(w.shape)}")
     if out_dtype not in (None, torch.bfloat16, torch.float16):
         raise ValueError(f"fp4_linear: out_dtype must be bf16 or fp16, got {out_dtype}")
+    _columns(x.shape, "fp4_linear: x")
     N, K = w.shape
     nv = _block(w.fmt) == 16
     coded = isinstance(x, Fp4Tensor)
