@@ -93,3 +93,40 @@ def test_large_rows_match_the_cpu():
     # both round fp32 sums of the same values once: a bf16 step apart at most, and the sums' own rounding
     size = want.abs().amax()
     assert ((got - want).abs() <= 2.0 ** -7 * want.abs() + 1000 * 2.0 ** -22 * size).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 300, 512), (9, 640, 2048), (300, 16500, 704)])
+@pytest.mark.parametrize("wsize", [1e-37, 1e-30, 1e30])
+def test_mxfp4_scales_at_the_ends_of_fp32(M, N, K, wsize):
+    """Block scales of 2^120 and of 2^-127 on either side: the products are those of the values."""
+    ops = _ops()
+    x = ops.quantize_fp4(_ends(M, K, torch.bfloat16), "mxfp4")
+    w = ops.quantize_fp4(wsize * torch.randn(N, K, device=dev, generator=torch.Generator(device=dev).manual_seed(N)), "mxfp4")
+    y = ops.fp4_linear(x, w).double()
+    ops.check_device_status()
+    xv, wv = (ops.dequantize_fp4(q, torch.float32).double() for q in (x, w))
+    ref, size = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    # half a bf16 step (2^-134 of the smallest) and a truncation of the running size, or of fp32's smallest step (or its
+    # smallest normal number, should the accumulator have no smaller ones), at each product
+    bound = 2.0 ** -8 * ref.abs() + 2.0 ** -134 + (K + 8) * (2.0 ** -23 * size + 2.0 ** -126)
+    fits = size < 2.0 ** 127  # no partial sum leaves fp32
+    assert fits.any() and torch.isfinite(y[fits]).all()
+    assert ((y - ref).abs()[fits] <= bound[fits]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+def test_non_finite_blocks_of_16_bit_rows(fmt, dtype):
+    """The bytes of rows with infinities, NaN of either sign and zeros, against the CPU."""
+    ops = _ops()
+    x = torch.randn(200, 100, generator=torch.Generator().manual_seed(0)).to(dtype)
+    x[0, 3], x[1, 40], x[2, 99] = float("inf"), -float("inf"), float("nan")
+    x[3] = float("nan")
+    x[4] = 0.0
+    x[5, ::2] = -0.0
+    x[6] = torch.finfo(dtype).max
+    x[7] = torch.finfo(dtype).smallest_normal / 4
+    x.view(torch.int16)[8, 5] = -1  # a NaN with its sign set
+    got, want = ops.quantize_fp4(x.to(dev), fmt), ops.quantize_fp4(x, fmt)
+    assert torch.equal(got.data.cpu(), want.data) and torch.equal(got.scales.cpu(), want.scales)
+    assert want.row_scale is None or torch.equal(got.row_scale.cpu(), want.row_scale)
