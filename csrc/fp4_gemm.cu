@@ -45,11 +45,11 @@ struct Params {
   const void* bias;
   int bias_type;  // 0 fp32, 1 bf16, 2 fp16
   int out_fp16;
-  int vec;        // bytes of a store: 32, 16 or 2, by the alignment of D's rows
+  bool rows16;    // D's rows start on 16 bytes (and N is a multiple of 8)
   int M, N, K;
   int ktiles;     // scale tiles along K
   int ksteps;     // stages along K
-  int tiles_m, tiles_n, num_tiles;
+  int tiles_m, tiles_n, num_tiles;  // of the pair kernel
   int* status;
 };
 
@@ -233,11 +233,11 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
     // branch of one lane every operand of every instruction is moved there first: 955 cycles a stage of nvfp4.)
     const uint64_t da = smem_desc_sw128(smem_u32(sm.a[0]), 16, 1024), db = smem_desc_sw128(smem_u32(sm.b[0]), 16, 1024);
     const uint64_t dsa = smem_desc_scales(smem_u32(sm.sa[0])), dsb = smem_desc_scales(smem_u32(sm.sb[0]));
-    // (s, ph): the stage whose MMAs are next; (sn, phn): the stage whose scales are copied next, at most one ahead, into
+    // s: the stage whose MMAs are next; (sn, phn): the stage whose scales are copied next, at most one ahead, into
     // buffer bufn, last read by the MMAs of stage s_old (kSfBufs before; with as many buffers as stages the ring itself
     // has waited for those)
     int s = 0, buf = 0, sn = 0, bufn = 0, s_old = 0;
-    uint32_t ph = 0, phn = 0, ph_old = 0;
+    uint32_t phn = 0, ph_old = 0;
     const int my_tiles = cluster < p.num_tiles ? (p.num_tiles - 1 - cluster) / clusters + 1 : 0;
     int64_t left = (int64_t)my_tiles * p.ksteps;  // stages whose scales have not been copied
     int64_t copied = 0;
@@ -308,7 +308,7 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
         __syncwarp();
         if (next) advance();
         ahead = next;
-        if (++s == kPairStages) s = 0, ph ^= 1;
+        if (++s == kPairStages) s = 0;
         if (++buf == kSfBufs) buf = 0;
       }
       if (!ok) break;
@@ -388,7 +388,7 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
                                   apply_factors(__uint_as_float(v[2 * q + 1]), tra, f.z, f.w));
           }
         }
-        if (p.vec >= 16) {  // rows of D are multiples of 16 bytes: a box of 32 x 32 by TMA, 64-byte swizzle
+        if (p.rows16) {  // a box of 32 x 32 by TMA, 64-byte swizzle
           if (lane == 0) tma_store_wait_read();
           __syncwarp();
 #pragma unroll
@@ -430,11 +430,12 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
 
 // ---------------------------------------------------------------- few rows
 // For few rows of x, D^T = B A^T: 128 rows of the weight B are the MMA's 128 rows and a tile of x's rows its N, so one
-// token costs a tile of 32 columns, and the K loop of a tile is split over a cluster of up to eight CTAs.  Each leaves
+// token costs a tile of 32 columns, and the K loop of a tile is split over a cluster of up to six CTAs.  Each leaves
 // its fp32 part in its shared memory, [column of x's tile][128 rows], and adds a share of the columns over all
 // parts in rank order (the same sums every time), applies factors and bias and stores runs of the output row.
-//   warp 0      producer (ring of as many stages as fit, up to eight); with `early` the grid was launched to overlap
-//               the quantiser of x: the weight's part of the first stages is loaded before waiting for it
+//   warp 0      producer (ring of four stages, three for more than 32 rows of x: what fits); with `early` the grid was
+//               launched to overlap the quantiser of x: the weight's part of the first stages is loaded before waiting
+//               for it
 //   warp 1      TMEM owner, scale copies and MMAs; the scales of each stage have their own columns
 //   warps 2..5  accumulator to shared memory; all warps add and store
 // Two CTAs share an SM (half the tensor memory each): a stage is some 12 instructions to the tensor core, which one warp
@@ -442,8 +443,9 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
 // Bound by the weight's bytes for one token, by the latency of a few K steps for small products.
 // A tile of x starts on a scale tile: in tensor memory the MMA's scales have to start on an even column (of 32 rows
 // each), an odd one is a "misaligned address".
-constexpr int kSmallThreads = 192, kSmallStages = 8;
+constexpr int kSmallThreads = 192, kSmallStages = 4;
 constexpr int kSmallBN = 128, kSmallTmem = 256, kSmallSfCol = 128;  // scales behind the accumulator's 128 columns
+static_assert(kSmallSfCol + kSmallStages * 8 * kMaxTiles <= kSmallTmem, "columns of the stages' scales");
 
 struct SmallBars {
   float2 col[kBM];  // factor and bias of the tile's weight rows
@@ -658,7 +660,7 @@ fp4_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_con
       uint16_t* d = static_cast<uint16_t*>(p.d) + (int64_t)(x0 + c) * p.ldd + n;
       const uint32_t lo = p.out_fp16 ? pack_out<true>(v[u][0], v[u][1]) : pack_out<false>(v[u][0], v[u][1]);
       const uint32_t hi = p.out_fp16 ? pack_out<true>(v[u][2], v[u][3]) : pack_out<false>(v[u][2], v[u][3]);
-      if (p.vec >= 16) {  // rows of D are multiples of 16 bytes, N a multiple of 8
+      if (p.rows16) {
         *reinterpret_cast<uint2*>(d) = make_uint2(lo, hi);
       } else {
         d[0] = (uint16_t)lo;
@@ -708,26 +710,24 @@ CUtensorMap out_map(const Params& p) {
 
 template <bool NV, bool FP16>
 void launch_pair(const Fp4Matrix& a, const Fp4Matrix& b, Params& p, int device, cudaStream_t stream) {
-  p.tiles_m = (p.M + kPairBM - 1) / kPairBM;
-  p.num_tiles = p.tiles_m * p.tiles_n;
   const int smem = (int)sizeof(PairSmem) + 1024;
   const CUtensorMap ma = code_map(a, kBM), mb = code_map(b, kBM), sa = scale_map(a), sb = scale_map(b);
   configure<fp4_gemm_pair_kernel<NV, FP16>>(smem, device);
   fp4_gemm_pair_kernel<NV, FP16><<<2 * std::min(p.num_tiles, sm_count(device) / 2), kPairThreads, smem, stream>>>(
-      ma, mb, sa, sb, p.vec >= 16 ? out_map(p) : ma, p);
+      ma, mb, sa, sb, p.rows16 ? out_map(p) : ma, p);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 constexpr int kSmallSmem = 109 * 1024;  // dynamic shared memory of a CTA of the few-rows kernel: two fit an SM
 
 // Tiles, stages and split of the few-rows kernel.
-SmallParams plan_small(const Params& p, bool nv, int sms, bool early) {
+SmallParams plan_small(const Params& p, int sms, bool early) {
   SmallParams sp;
   sp.g = p;
   sp.tiles_x = (p.M + kSmallBN - 1) / kSmallBN;
   sp.bn = sp.tiles_x > 1 ? kSmallBN : (p.M + 31) / 32 * 32;
   sp.stage_bytes = kABytes + sp.bn * 128 + 2 * kSaBytes;
-  sp.stages = std::min({kSmallStages, (kSmallSmem - 1024) / sp.stage_bytes, (kSmallTmem - kSmallSfCol) / (nv ? 32 : 16)});
+  sp.stages = std::min(kSmallStages, (kSmallSmem - 1024) / sp.stage_bytes);
   // CTAs for four fifths of the places (two an SM): above that, and with clusters of more than six, they no longer
   // all run at once (16 x 5120 x 5120 nvfp4: 10.0 us with 160 to 240 CTAs, 15.1 us with 280)
   const int tiles = ((p.N + kBM - 1) / kBM) * sp.tiles_x;
@@ -773,7 +773,7 @@ void launch_small(const Fp4Matrix& a, const Fp4Matrix& b, const SmallParams& sp,
 template <bool NV>
 void launch(const Fp4Matrix& a, const Fp4Matrix& b, Params& p, int device, cudaStream_t stream, bool early) {
   const int sms = sm_count(device);
-  if (few_rows(p, sms)) launch_small<NV>(a, b, plan_small(p, NV, sms, early), device, stream);
+  if (few_rows(p, sms)) launch_small<NV>(a, b, plan_small(p, sms, early), device, stream);
   else if (p.out_fp16) launch_pair<NV, true>(a, b, p, device, stream);
   else launch_pair<NV, false>(a, b, p, device, stream);
 }
@@ -797,14 +797,13 @@ void gemm(const Fp4Matrix& a, const Fp4Matrix& b, const c10::optional<at::Tensor
   p.ra = a.row_scale;
   p.rb = b.row_scale;
   p.out_fp16 = d.scalar_type() == at::kHalf ? 1 : 0;
-  const uintptr_t align = reinterpret_cast<uintptr_t>(p.d) | (uintptr_t)(2 * N);
-  p.vec = align % 32 == 0 ? 32 : align % 16 == 0 ? 16 : 2;
+  p.rows16 = (reinterpret_cast<uintptr_t>(p.d) | (uintptr_t)(2 * N)) % 16 == 0;
   p.M = (int)M;
   p.N = (int)N;
   p.K = (int)K;
   p.ktiles = (int)a.ktiles();
   p.ksteps = (int)((K + kBK - 1) / kBK);
-  p.tiles_m = (int)((M + kBM - 1) / kBM);
+  p.tiles_m = (int)((M + kPairBM - 1) / kPairBM);
   p.tiles_n = (int)((N + kBN - 1) / kBN);
   DMAD_VALUE_CHECK((int64_t)p.tiles_m * p.tiles_n <= INT32_MAX, "fp4_linear: too many output tiles");
   p.num_tiles = p.tiles_m * p.tiles_n;
