@@ -276,24 +276,34 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
             ok = ok && mbar_wait(&sm.empty[s_old], ph_old, kStatusTimeoutMma, abort_flag, p.status);
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
           tc_fence_after();
-          const int nt = min(kStageTiles, p.ktiles - kn * kStageTiles);
-          if (elect_one()) {
+          if constexpr (NV) {
+            const int nt = min(kStageTiles, p.ktiles - kn * kStageTiles);
+            if (elect_one()) {
+#pragma unroll
+              for (int j = 0; j < kStageTiles; ++j) copy_tile(j, nt);
+            }
+            __syncwarp();
+            advance();
+          }
+        }
+        // nvfp4: the next stage's scales go between this stage's MMAs if it has landed and its buffer is free (9472 x
+        // 16384 x 5120: 317 us against 341 with all copies first).  mxfp4, with half as many, has them first, in one
+        // go with its MMAs: 274 us there, 286 with the copies between, and 311 with no more than the votes and fences here.
+        bool next = false;
+        if constexpr (NV) {
+          next = left > 0 && mbar_try_wait(smem_u32(&sm.full[sn]), phn);
+          if (kSfBufs < kPairStages && copied >= kSfBufs) next = next && mbar_try_wait(smem_u32(&sm.empty[s_old]), ph_old);
+          next = __all_sync(0xffffffffu, next);
+          tc_fence_after();
+        }
+        const uint32_t sfa = tmem + kPairSfCol + buf * kSfBufCols, sfb = sfa + 4 * kStageTiles;
+        const int nk = min(4, (p.K - k * kBK + 63) / 64), nt = !NV || next ? min(kStageTiles, p.ktiles - kn * kStageTiles) : 0;
+        const uint64_t oa = (uint64_t)(s * (kABytes >> 4));
+        if (elect_one()) {
+          if constexpr (!NV) {
 #pragma unroll
             for (int j = 0; j < kStageTiles; ++j) copy_tile(j, nt);
           }
-          __syncwarp();
-          advance();
-        }
-        // nvfp4: the next stage's scales go between this stage's MMAs if it has landed and its buffer is free (9472 x
-        // 16384 x 5120: 317 us against 341 with all copies first; mxfp4, with half as many, 286 us against 277)
-        bool next = NV && left > 0 && mbar_try_wait(smem_u32(&sm.full[sn]), phn);
-        if (kSfBufs < kPairStages && copied >= kSfBufs) next = next && mbar_try_wait(smem_u32(&sm.empty[s_old]), ph_old);
-        next = __all_sync(0xffffffffu, next);
-        tc_fence_after();
-        const uint32_t sfa = tmem + kPairSfCol + buf * kSfBufCols, sfb = sfa + 4 * kStageTiles;
-        const int nk = min(4, (p.K - k * kBK + 63) / 64), nt = next ? min(kStageTiles, p.ktiles - kn * kStageTiles) : 0;
-        const uint64_t oa = (uint64_t)(s * (kABytes >> 4));
-        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk) {
             if (kk < nk) {
@@ -301,12 +311,12 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
               mma_fp4_ss<NV, 2>(d, da + oa + 2 * kk, db + oa + 2 * kk, idesc_fp4(NV, kPairBM, kBN, NV ? 0 : (kk & 1) * 2),
                                 sfa + 4 * j, sfb + 8 * j, (k > 0 || kk > 0) ? 1u : 0u);
             }
-            if (kk < kStageTiles) copy_tile(kk, nt);
+            if (NV && kk < kStageTiles) copy_tile(kk, nt);
           }
           mma_commit_pair(&sm.empty[s]);
         }
         __syncwarp();
-        if (next) advance();
+        if (!NV || next) advance();
         ahead = next;
         if (++s == kPairStages) s = 0;
         if (++buf == kSfBufs) buf = 0;
