@@ -270,6 +270,10 @@ class SegLinear(nn.Module):
             q = self.fp4
             rs = None if q.row_scale is None else fn(q.row_scale.view(torch.int32)).view(torch.float32)
             self.fp4 = ops.Fp4Tensor(fn(q.data), fn(q.scales), rs, q.fmt, q.shape)
+            # what the layer computes in follows a conversion to another 16-bit type, as its bias and the other layers do
+            kind = fn(torch.empty(0, dtype=self._fp4_dtype, device=q.device)).dtype
+            if kind in (torch.bfloat16, torch.float16):
+                self._fp4_dtype = kind
         return self
 
     def _refuse_fp4(self, what):
