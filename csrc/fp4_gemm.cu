@@ -94,8 +94,8 @@ __device__ __forceinline__ void tile_coords(const Params& p, int t, int& tm, int
 }
 
 // Stores 32 columns from nc of the warp's rows m0 .. m0 + 31 (o: the lane's row) to rows of D that are no multiple of
-// 16 bytes: through shared memory, so that a warp still writes runs of 32 bytes.  (8192 x 8191 x 1536: 117 us, 53 with
-// 8192 columns; words of 4 bytes, shifted in every other row, 146 to 166 us.)
+// 16 bytes: through shared memory, so that a warp still writes runs of 32 bytes.  (8192 x 8191 x 1536 mxfp4: 118 us, 58
+// with 8192 columns; words of 4 bytes, shifted in every other row, 146 to 166 us.)
 __device__ __forceinline__ void store_unaligned(const Params& p, uint16_t (*stage)[18], int m0, int nc,
                                                 const uint32_t (&o)[16]) {
   const int lane = lane_id();
@@ -123,10 +123,11 @@ __device__ __forceinline__ void store_unaligned(const Params& p, uint16_t (*stag
 //               through shared memory by TMA (direct stores of a lane's row cost the SM four times the cycles)
 // Tensor memory: scale buffers in the last 144 columns (three of 48 for nvfp4, six of 24 for mxfp4), accumulators at 0
 // and 112.  The epilogue reads the 144 shared columns into registers at once and then releases the accumulator.
-// Measured: 37966 x 30720 x 5120 nvfp4 2.42 ms (4.9 PFLOP/s at the 1.5 GHz that the power limit leaves), mxfp4 1.99 ms
-// (6.0 PFLOP/s); bound by the tensor core's queue, where a scale copy holds up the MMAs behind it for some 40 cycles
-// (nvfp4 has twelve a stage beside four MMAs, mxfp4 six).  mxfp4 32760 x 8960 x 1536 0.22 ms, where six stages of K are
-// shorter than the epilogue of the tile.
+// Measured, two passes after a pause and 3 s of passes at the power limit: 37966 x 30720 x 5120 nvfp4 2.43 to 2.50 ms (4.9
+// PFLOP/s) and 2.81 ms at 1.40 GHz, mxfp4 2.07 to 2.13 ms (5.7 PFLOP/s) and 2.41 ms at 1.24 GHz.  In cycles bound by the
+// tensor core's queue, where a scale copy holds up the MMAs behind it for some 40 (nvfp4 has twelve a stage beside four
+// MMAs, mxfp4 six); the clock is what the power limit leaves.  32760 x 8960 x 1536 mxfp4 0.22 ms, nvfp4 0.24 ms, where six
+// stages of K are shorter than the epilogue of the tile.
 constexpr int kPairBM = 256, kPairStages = 5;
 constexpr int kPairAcc1 = 112, kPairSfCol = 368;
 constexpr int kEpiWarps = 8, kPairThreads = 64 + 32 * kEpiWarps;
@@ -451,9 +452,10 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_cons
 //               for it
 //   warp 1      TMEM owner, scale copies and MMAs; the scales of each stage have their own columns
 //   warps 2..5  accumulator to shared memory; all warps add and store
-// Two CTAs share an SM (half the tensor memory each): a stage is some 12 instructions to the tensor core, which one warp
-// issues slower than the SM could load the stage (one token, 15360 x 5120: 15.5 us with one CTA, 12.9 us with two).
-// Bound by the weight's bytes for one token, by the latency of a few K steps for small products.
+// Two CTAs fit an SM (half the tensor memory each): a stage is some 12 instructions to the tensor core, which one warp
+// issues slower than the SM could load the stage.  (One token, 15360 x 5120, in 240 CTAs: 15.5 us with room for one CTA an
+// SM, 12.9 us for two.  plan_small() now makes 120 CTAs of it, one an SM, in 12.0 us.)
+// Bound by the latency of a CTA's K steps (twenty for that token) and of the start; the weight's bytes take 6.8 us from HBM.
 // A tile of x starts on a scale tile: in tensor memory the MMA's scales have to start on an even column (of 32 rows
 // each), an odd one is a "misaligned address".
 constexpr int kSmallThreads = 192, kSmallStages = 4;
@@ -741,8 +743,8 @@ SmallParams plan_small(const Params& p, int sms, bool early) {
   sp.bn = sp.tiles_x > 1 ? kSmallBN : (p.M + 31) / 32 * 32;
   sp.stage_bytes = kABytes + sp.bn * 128 + 2 * kSaBytes;
   sp.stages = std::min(kSmallStages, (kSmallSmem - 1024) / sp.stage_bytes);
-  // CTAs for four fifths of the places (two an SM): above that, and with clusters of more than six, they no longer
-  // all run at once (16 x 5120 x 5120 nvfp4: 10.0 us with 160 to 240 CTAs, 15.1 us with 280)
+  // CTAs for up to four fifths of the places (two an SM; 236 of 148 SMs): above that, and with clusters of more than six,
+  // they no longer all run at once (16 x 5120 x 5120 nvfp4: 10.0 us with 160 to 240 CTAs, 15.1 us with 280)
   const int tiles = ((p.N + kBM - 1) / kBM) * sp.tiles_x;
   sp.split = std::max(1, std::min({6, sms * 2 * 4 / 5 / std::max(tiles, 1), p.ksteps}));
   sp.per_split = (p.ksteps + sp.split - 1) / sp.split;

@@ -14,9 +14,11 @@
 // load of 16-bit elements, one 8-byte store of codes); a row is held by one block in registers between the
 // row maximum and the encoding, so nvfp4's two levels cost no second read while the row fits (32768 columns;
 // longer rows are read twice).
-// Measured at 37966 x 5120 bf16 nvfp4: quantiser 105 us (4.7 TB/s; some 230 instructions for a thread's 16 columns take
-// 71 % of the issue slots; with 64 registers a thread instead of 40 110 us; with IEEE divisions 127 us; one unit a thread
-// instead of two 123 us), inverse to bf16 82 us (6.1 TB/s).
+// Measured at 37966 x 5120 bf16: nvfp4 quantiser 105 us (4.7 TB/s; bound by its instructions, some 230 for a thread's 16
+// columns, which take 80 % of the issue slots; with 64 registers a thread 110 us, the bound to 40 for a third block of 512
+// threads costs 96 bytes of spills; with IEEE divisions 127 us; one unit a thread instead of two 123 us), mxfp4 91 us (5.4
+// TB/s), fp32 nvfp4 251 us (3.5 TB/s); inverse to bf16 82 us (6.1 TB/s).  Rows off 32 bytes are loaded by elements, one
+// sector a lane: 37966 x 5121 248 us.
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

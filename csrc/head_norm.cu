@@ -14,8 +14,10 @@
 // row's angles.  gridDim.y separates q from k, so a thread has one weight slice and one gradient accumulator.  dw:
 // per-thread sums over the tasks of a persistent grid, one partial row a block, and a second kernel that adds the
 // partials in a fixed order.
-// Measured at 37966 rows of 40 + 40 heads of 128, bf16: forward 256 us (6.1 TB/s), backward 414 us (5.6 TB/s; with
-// U = 4 instead of 8 and cached accesses 497 us; with the next task's loads issued ahead, U = 2, 690 us).
+// Measured at 37966 rows of 40 + 40 heads of 128, bf16, pairs: forward 255 us (6.1 TB/s), backward 404 us (5.8 TB/s; with
+// U = 4 instead of 8 and cached accesses 497 us; with the next task's loads issued ahead, U = 2, 690 us).  Halves, whose
+// partners come by shuffles: 300 and 459 us.  fp32, half as many rows: pairs 245 and 362 us, halves 262 and 364 us (the
+// forward of these holds four heads of fp32 in 64 registers and spills 132 bytes).
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
