@@ -19,28 +19,25 @@ void head_norm_rope_bwd(const at::Tensor& gq, const at::Tensor& gk, const at::Te
                         OptTensor wk, OptTensor cosT, OptTensor sinT, OptTensor positions, at::Tensor& dq, at::Tensor& dk,
                         OptTensor dwq, OptTensor dwk, double eps, bool interleaved);
 
-// In a backward that a CUDA graph captures: an error where the gradient of a leaf would leave the capture.  While an
-// eager graph of the same leaves lives, they keep the accumulators that it made, and with them the stream on which it
-// made them; the engine then makes that stream, which nothing captures, wait for the captured one: no capture survives
-// that, and the process may not either.
+// In a backward that a CUDA graph captures: an error where a leaf's gradient belongs to the default stream.  While an eager
+// graph of the same leaves lives, they keep the accumulators that it made, and with them the stream on which it made
+// them; the engine then makes that stream wait for the captured one.  Another stream joins the capture by that and is
+// joined again at the end; the default stream cannot: no capture survives it, and the process may not either.
 void check_captured_backward(const std::string& op) {
-  const auto capturing = [](const c10::cuda::CUDAStream& s) {
-    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-    if (s.stream() == nullptr) return false;  // the default stream is never captured, nor may it be asked meanwhile
-    if (cudaStreamIsCapturing(s.stream(), &status) == cudaSuccess) return status == cudaStreamCaptureStatusActive;
-    cudaGetLastError();
-    return false;
-  };
   const auto current = c10::cuda::getCurrentCUDAStream();
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (current.stream() == nullptr || cudaStreamIsCapturing(current.stream(), &status) != cudaSuccess ||
+      status != cudaStreamCaptureStatusActive)
+    return;
   const auto node = torch::autograd::get_current_node();
-  if (node == nullptr || !capturing(current)) return;
+  if (node == nullptr) return;
   for (const auto& edge : node->next_edges()) {
     auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
     if (leaf == nullptr) continue;
     const auto stream = leaf->stream();
-    if (stream.has_value() && !capturing(c10::cuda::CUDAStream(*stream)))
-      throw std::runtime_error(op + ": this backward is being captured while a graph of the same leaves, recorded outside "
-                                    "of the capture, is alive; release that graph first, or record it on the captured stream");
+    if (stream.has_value() && c10::cuda::CUDAStream(*stream).stream() == nullptr)
+      throw std::runtime_error(op + ": this backward is being captured while a graph of the same leaves, recorded on the "
+                                    "default stream, is alive; release that graph first, or record it on another stream");
   }
 }
 
