@@ -288,7 +288,9 @@ class SegLinear(nn.Module):
         """Output columns ``[start, stop)`` of ``forward(x)``, computed from those weight rows only
         (one segment of a fused projection, for instance; 4-bit weights: from the multiple of 128 before them)."""
         if self.fp4 is not None:  # from the tile of 128 rows on in which they begin
-            first, stop = start // 128 * 128, min(stop, self.out_features)
+            stop = min(stop, self.out_features)
+            start = min(start, stop)
+            first = start // 128 * 128
             b = None if self.bias is None else self.bias[first:stop]
             return ops.fp4_linear(x.to(self._fp4_dtype), self.fp4.row_slice(first, stop), b)[..., start - first:]
         w = self.effective_weight()[start:stop]
