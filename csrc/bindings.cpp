@@ -82,6 +82,12 @@ at::Tensor fp4_linear(const at::Tensor& x, const at::Tensor& data, const at::Ten
 at::Tensor fp4_matmul(const at::Tensor& xdata, const at::Tensor& xscales, c10::optional<at::Tensor> xrow_scale,
                       int64_t M, const at::Tensor& data, const at::Tensor& scales, c10::optional<at::Tensor> row_scale,
                       c10::optional<at::Tensor> bias, int64_t N, int64_t K, bool nv, int64_t out_type);
+std::tuple<at::Tensor, at::Tensor> int8_quantize(const at::Tensor& x, bool blocks);
+at::Tensor int8_dequantize(const at::Tensor& data, const at::Tensor& scale, int64_t R, int64_t K, bool blocks, int64_t type);
+at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& data, const at::Tensor& scale, c10::optional<at::Tensor> bias,
+                       int64_t N, int64_t K, int64_t out_type);
+at::Tensor int8_matmul(const at::Tensor& xdata, const at::Tensor& xscale, int64_t M, const at::Tensor& data,
+                       const at::Tensor& scale, c10::optional<at::Tensor> bias, int64_t N, int64_t K, int64_t out_type);
 std::tuple<at::Tensor, at::Tensor> head_norm_rope_fwd(const at::Tensor& q, const at::Tensor& k,
                                                       c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk,
                                                       c10::optional<at::Tensor> cosT, c10::optional<at::Tensor> sinT,
@@ -149,6 +155,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp4_dequantize", &dmad::fp4_dequantize);
   m.def("fp4_linear", &dmad::fp4_linear);
   m.def("fp4_matmul", &dmad::fp4_matmul);
+  m.def("int8_quantize", &dmad::int8_quantize);
+  m.def("int8_dequantize", &dmad::int8_dequantize);
+  m.def("int8_linear", &dmad::int8_linear);
+  m.def("int8_matmul", &dmad::int8_matmul);
   m.def("check_captured_backward", &dmad::check_captured_backward);
   m.def("head_norm_rope", &dmad::head_norm_rope);
   m.def("head_norm_rope_fwd", &dmad::head_norm_rope_fwd);

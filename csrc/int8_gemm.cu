@@ -1,0 +1,447 @@
+// tcgen05 GEMMs of 8-bit integers for sm_100a.
+//
+//   D[M, N] = ra[m] rb[n] * sum_k A[m, k] B[n, k] + bias[n]          (bf16 or fp16 out)
+//
+// A and B are codes of -127 .. 127 with a scale a row (int8.cuh), multiplied on the tensor core (kind::i8) with exact int32
+// sums (K <= 133144: 2^31 / 127^2), so the only roundings are the epilogue's: the factors, the bias, and one to the result's
+// type.  Two kernels: pairs of CTAs on 256 x 256 tiles (gemm_pair.cuh), and one for few rows (few_rows() says which).
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include "common.cuh"
+#include "gemm_pair.cuh"
+#include "int8_host.h"
+#include "row_factors.cuh"
+
+namespace dmad {
+namespace {
+
+constexpr int64_t kMaxK = 133144;
+constexpr int kBM = 128;            // weight rows of a tile of the few-rows kernel
+constexpr int kBK = 128;            // columns of K of a stage
+constexpr int kABytes = kBM * 128;  // 16 KB
+
+struct Factors {
+  const float* ra;
+  const float* rb;
+  FloatRow bias;
+};
+
+// ---------------------------------------------------------------- CTA pairs
+template <bool FP16>
+struct ScaleEpilogue {
+  static constexpr int kStages = 6, kOutBytes = 2048;
+  static constexpr bool kShared = true;
+  struct Args {
+    CUtensorMap map;
+    OutRows out;
+    Factors f;
+  };
+  const Args& a;
+  const PairGemm& p;
+  const EpiPlace at;
+  int m0, n0, m0_next, n0_next;
+  float ra, ra_next;
+  float2 cf;
+  bool far;
+  const float2* col;
+
+  __device__ __forceinline__ ScaleEpilogue(const Args& a, const PairGemm& p, const EpiPlace& at) : a(a), p(p), at(at) {}
+  __device__ __forceinline__ void fetch(int item) {
+    int tm, tn;
+    p.tile(item, tm, tn);
+    m0_next = tm * kPairM + (int)at.rank * kPairHalf + at.wq * 32;
+    n0_next = tn * kPairN;
+    const int n = min(n0_next + at.thread, p.N - 1);
+    cf = make_float2(__ldg(a.f.rb + n), a.f.bias.at(n));
+    ra_next = m0_next + at.lane < p.M ? __ldg(a.f.ra + m0_next + at.lane) : 1.f;
+  }
+  __device__ __forceinline__ void first(int item) { fetch(item); }
+  __device__ __forceinline__ void begin(int, int, int parity) {
+    // (the buffer's last readers are two tiles back, behind the barrier between)
+    col = at.col + parity * kPairN;
+    at.col[parity * kPairN + at.thread] = cf;
+    m0 = m0_next;
+    n0 = n0_next;
+    ra = ra_next;
+    far = __any_sync(0xffffffffu, far_out(ra));
+  }
+  __device__ __forceinline__ void met(int next) {  // the next tile's factors are read while this one is stored
+    if (next >= 0) fetch(next);
+  }
+  __device__ __forceinline__ void chunk(int, int c, const uint32_t (&v)[32]) {
+    const int nc = n0 + c * 32;
+    if (nc >= p.N || m0 >= p.M) return;
+    uint32_t o[16];
+    const float4* f4 = reinterpret_cast<const float4*>(col + c * 32);
+    if (far) {  // one vote a tile, so that the warp stays together
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const float4 f = f4[q];
+        const float x = __int2float_rn((int)v[2 * q]), y = __int2float_rn((int)v[2 * q + 1]);
+        const bool out = far_out(ra);
+        o[q] = pack16<FP16>(out ? apply_factors_far(x, ra, f.x, f.y) : apply_factors(x, ra, f.x, f.y),
+                            out ? apply_factors_far(y, ra, f.z, f.w) : apply_factors(y, ra, f.z, f.w));
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 16; ++q) {
+        const float4 f = f4[q];
+        o[q] = pack16<FP16>(apply_factors(__int2float_rn((int)v[2 * q]), ra, f.x, f.y),
+                            apply_factors(__int2float_rn((int)v[2 * q + 1]), ra, f.z, f.w));
+      }
+    }
+    if (at.lane == 0) tma_store_wait_read();
+    __syncwarp();
+    store_rows(a.out, &a.map, at.stage, m0, nc, o);
+  }
+  __device__ __forceinline__ void done() {
+    if (at.lane == 0) tma_store_wait_read();
+  }
+};
+
+// ---------------------------------------------------------------- few rows
+// For few rows of x, D^T = B A^T: 128 rows of the weight B are the MMA's 128 rows and a tile of x's rows its N, so one
+// token costs a tile of 32 columns, and the K loop of a tile is split over a cluster of up to six CTAs.  Each leaves its
+// int32 part in its shared memory, [column of x's tile][128 rows], and adds a share of the columns over all parts (exactly,
+// whatever the order), applies factors and bias and stores runs of the output row.
+//   warp 0      producer (a ring of as many stages as fit); with `early` the grid was launched to overlap the quantiser of
+//               x: the weight's part of the first stages is loaded before waiting for it
+//   warp 1      TMEM owner and MMAs
+//   warps 2..5  accumulator to shared memory; all warps add and store
+// Two CTAs fit an SM.
+constexpr int kSmallThreads = 192, kSmallStages = 5;
+constexpr int kSmallBN = 128;
+
+struct SmallBars {
+  float2 col[kBM];  // factor and bias of the tile's weight rows
+  uint64_t full[kSmallStages], empty[kSmallStages];
+  uint64_t acc_full;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct SmallParams {
+  void* d;
+  int64_t ldd;
+  Factors f;
+  int out_fp16;
+  bool rows8;        // D's rows start on 8 bytes
+  int M, N;          // rows of x, rows of the weight
+  int ksteps, k_last;
+  int bn;            // rows of x of a tile: a multiple of 32 up to 128, and 128 where there are several tiles
+  int stages, stage_bytes;
+  int tiles_x;       // tiles along x
+  int split, per_split;  // CTAs of a cluster, K steps of each
+  int early;
+  int* status;
+};
+
+__global__ void __launch_bounds__(kSmallThreads, 2)
+int8_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                       const __grid_constant__ SmallParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ SmallBars sm;
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  volatile int* abort_flag = &sm.abort_flag;
+  const int warp = warp_id(), lane = lane_id();
+  const int tile = blockIdx.x / p.split, rank = blockIdx.x % p.split;  // rank = rank in the cluster
+  const int tw = tile / p.tiles_x, tx = tile % p.tiles_x;
+  const int k0 = rank * p.per_split, steps = max(0, min(p.ksteps, k0 + p.per_split) - k0);
+  const int x0 = tx * p.bn;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSmallStages; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    mbar_init(&sm.acc_full, 1);
+    sm.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_base, kSmallBN);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_x);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem_base;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (elect_one()) {
+      auto load_w = [&](int i, int s) {
+        mbar_arrive_expect_tx(&sm.full[s], kABytes + p.bn * 128);
+        tma_load_2d(ring + s * p.stage_bytes, &tm_w, &sm.full[s], (k0 + i) * kBK, tw * kBM);
+      };
+      auto load_x = [&](int i, int s) {
+        tma_load_2d(ring + s * p.stage_bytes + kABytes, &tm_x, &sm.full[s], (k0 + i) * kBK, x0);
+      };
+      const int first = min(steps, p.stages);
+      for (int i = 0; i < first; ++i) load_w(i, i);
+      if (p.early) wait_for_previous_grid();
+      for (int i = 0; i < first; ++i) load_x(i, i);
+      int i = first, s = 0;
+      uint32_t ph = 0;
+      for (; i < steps; ++i) {
+        if (!mbar_wait(&sm.empty[s], ph, kStatusTimeoutEmpty, abort_flag, p.status)) break;
+        load_w(i, s);
+        load_x(i, s);
+        if (++s == p.stages) s = 0, ph ^= 1;
+      }
+      for (int j = max(0, i - p.stages); j < i; ++j)  // all copies land before the ring is used for the sums
+        mbar_wait(&sm.full[j % p.stages], (j / p.stages) & 1, kStatusTimeoutTmaFull, nullptr, p.status);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    // The whole warp runs the loop and one lane issues: the descriptors stay in uniform registers.
+    const uint64_t da = smem_desc_sw128(smem_u32(ring), 16, 1024), db = smem_desc_sw128(smem_u32(ring) + kABytes, 16, 1024);
+    const uint32_t idesc = idesc_of(Mma::kI8, kBM, p.bn, false, false);
+    bool ok = true;
+    int s = 0;  // the step's stage
+    uint32_t ph = 0;
+    for (int i = 0; i < steps; ++i) {
+      ok = mbar_wait(&sm.full[s], ph, kStatusTimeoutTmaFull, abort_flag, p.status);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      tc_fence_after();
+      const uint64_t off = (uint64_t)(s * p.stage_bytes) >> 4;
+      const int nk = k0 + i == p.ksteps - 1 ? p.k_last : 4;
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          if (kk < nk) mma_ss<Mma::kI8, 1>(tmem, da + off + 2 * kk, db + off + 2 * kk, idesc, (i > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(&sm.empty[s]);
+      }
+      __syncwarp();
+      if (++s == p.stages) s = 0, ph ^= 1;
+    }
+    if (elect_one()) {
+      if (!ok) *abort_flag = 1;
+      mma_commit(&sm.acc_full);
+      mbar_wait(&sm.acc_full, 0, kStatusTimeoutMma, nullptr, p.status);
+    }
+  } else {  // factors and biases of the weight rows, read while the operands come in
+    const int r = threadIdx.x - 64, n = min(tw * kBM + r, p.N - 1);
+    sm.col[r] = make_float2(__ldg(p.f.rb + n), p.f.bias.at(n));
+  }
+  // the MMAs are done and every copy has landed: the ring becomes the part's sums
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  int* part = reinterpret_cast<int*>(ring);
+  if (warp >= 2) {
+    const int wq = warp & 3, row = wq * 32 + lane;
+    const uint32_t acc = tmem + ((uint32_t)(wq * 32) << 16);
+    for (int c = 0; c < p.bn; c += 32) {
+      uint32_t r[32];
+      tmem_ld32(acc + c, r);
+      tmem_wait_ld();
+#pragma unroll
+      for (int q = 0; q < 32; ++q) part[(c + q) * kBM + row] = steps > 0 ? (int)r[q] : 0;
+    }
+  }
+  if (p.early) wait_for_previous_grid();  // the row factors of x are read below
+  tc_fence_before();
+  __syncthreads();
+  if (p.split > 1) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kSmallBN);
+  }
+  // this CTA's share of x's rows: a warp takes eight of them at a time (that many loads in flight), a lane four weight
+  // rows of each
+  const int per = (p.bn + p.split - 1) / p.split, c_end = min(min(p.bn, p.M - x0), (rank + 1) * per);
+  constexpr int kWarps = kSmallThreads / 32, kRows = 8;
+  const int n = tw * kBM + lane * 4;
+  float2 cf[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) cf[q] = sm.col[lane * 4 + q];
+  for (int c0 = rank * per + warp; c0 < c_end; c0 += kWarps * kRows) {
+    int v[kRows][4];
+#pragma unroll
+    for (int u = 0; u < kRows; ++u)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[u][q] = 0;
+    for (int r = 0; r < p.split; ++r) {
+      const uint32_t from = p.split > 1 ? cluster_map(part + lane * 4, r) : smem_u32(part + lane * 4);
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) {
+        const int c = c0 + u * kWarps;
+        if (c < c_end) {
+          const float4 q = ld_cluster_float4(from + c * (kBM * 4));
+          v[u][0] += __float_as_int(q.x);
+          v[u][1] += __float_as_int(q.y);
+          v[u][2] += __float_as_int(q.z);
+          v[u][3] += __float_as_int(q.w);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kRows; ++u) {
+      const int c = c0 + u * kWarps;
+      if (c >= c_end || n >= p.N) continue;
+      const float ra = p.f.ra[x0 + c];
+      const bool far = far_out(ra);
+      float y[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float s = __int2float_rn(v[u][q]);
+        y[q] = far ? apply_factors_far(s, ra, cf[q].x, cf[q].y) : apply_factors(s, ra, cf[q].x, cf[q].y);
+      }
+      uint16_t* d = static_cast<uint16_t*>(p.d) + (int64_t)(x0 + c) * p.ldd + n;
+      const uint32_t lo = p.out_fp16 ? pack16<true>(y[0], y[1]) : pack16<false>(y[0], y[1]);
+      const uint32_t hi = p.out_fp16 ? pack16<true>(y[2], y[3]) : pack16<false>(y[2], y[3]);
+      if (p.rows8) {
+        *reinterpret_cast<uint2*>(d) = make_uint2(lo, hi);
+      } else {
+        d[0] = (uint16_t)lo;
+        if (n + 1 < p.N) d[1] = (uint16_t)(lo >> 16);
+        if (n + 2 < p.N) d[2] = (uint16_t)hi;
+        if (n + 3 < p.N) d[3] = (uint16_t)(hi >> 16);
+      }
+    }
+  }
+  if (p.split > 1) {
+    __syncthreads();
+    cluster_sync();  // the other CTAs have read this one's part
+  }
+}
+
+constexpr int kSmallSmem = 109 * 1024;  // dynamic shared memory of a CTA of the few-rows kernel: two fit an SM
+
+CUtensorMap code_map(const Int8Matrix& x, uint32_t box_rows) {  // zeros past column K, whatever is stored there
+  const uint64_t dims[2] = {(uint64_t)x.cols, (uint64_t)x.rows};
+  const uint64_t strides[1] = {(uint64_t)x.row_bytes()};
+  const uint32_t box[2] = {128u, box_rows};
+  return make_tmap_u8(x.data, 2, dims, strides, box);
+}
+
+// Which kernel: up to 128 rows of x the few-rows kernel reads the weight once and wastes no half of a 256-row tile; above
+// it stays ahead while its 128 x 128 tiles do not fill the GPU.
+bool few_rows(int64_t M, int64_t N, int sms) {
+  if (M <= kSmallBN) return true;
+  return ((N + kBM - 1) / kBM) * ((M + kSmallBN - 1) / kSmallBN) <= sms * 7 / 8;
+}
+
+void launch_small(const Int8Matrix& a, const Int8Matrix& b, const Factors& f, at::Tensor& d, int device, cudaStream_t stream,
+                  bool early) {
+  const int sms = sm_count(device);
+  SmallParams p;
+  p.d = d.data_ptr();
+  p.ldd = b.rows;
+  p.f = f;
+  p.out_fp16 = d.scalar_type() == at::kHalf ? 1 : 0;
+  p.rows8 = (reinterpret_cast<uintptr_t>(p.d) | (uintptr_t)(2 * p.ldd)) % 8 == 0;
+  p.M = (int)a.rows;
+  p.N = (int)b.rows;
+  p.ksteps = (int)((a.cols + kBK - 1) / kBK);
+  p.k_last = (int)((a.cols - (int64_t)(p.ksteps - 1) * kBK + 31) / 32);
+  p.tiles_x = (p.M + kSmallBN - 1) / kSmallBN;
+  p.bn = p.tiles_x > 1 ? kSmallBN : (p.M + 31) / 32 * 32;
+  p.stage_bytes = kABytes + p.bn * 128;
+  p.stages = std::min(kSmallStages, (kSmallSmem - 1024) / p.stage_bytes);
+  // CTAs for up to four fifths of the places (two an SM): above that, and with clusters of more than six, they no longer
+  // all run at once
+  const int tiles = ((p.N + kBM - 1) / kBM) * p.tiles_x;
+  p.split = std::max(1, std::min({6, sms * 2 * 4 / 5 / std::max(tiles, 1), p.ksteps}));
+  p.per_split = (p.ksteps + p.split - 1) / p.split;
+  p.early = early ? 1 : 0;
+  p.status = device_status_ptr(device);
+  const CUtensorMap mw = code_map(b, kBM), mx = code_map(a, p.bn);
+  // the ring, and the int32 sums that take its place
+  const int smem = std::max(p.stages * p.stage_bytes, p.bn * kBM * 4) + 1024;
+  raise_smem<int8_gemm_small_kernel>(kSmallSmem, device);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * p.split));
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 2 : 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, int8_gemm_small_kernel, mw, mx, p));
+}
+
+template <bool FP16>
+void launch_pair(const Int8Matrix& a, const Int8Matrix& b, const Factors& f, at::Tensor& d, int device, cudaStream_t stream) {
+  const PairGemm p = pair_gemm(a.rows, b.rows, a.cols, 1, false, false, 1, device);
+  const CUtensorMap ma = code_map(a, kPairHalf), mb = code_map(b, kPairHalf);
+  const OutRows out = out_rows(d.data_ptr(), b.rows, a.rows, b.rows);
+  const typename ScaleEpilogue<FP16>::Args args{out.tma ? out_rows_map(out) : ma, out, f};
+  launch_pair_gemm<Mma::kI8, ScaleEpilogue<FP16>>(ma, mb, args, p, device, stream);
+}
+
+// d [a.rows, b.rows] (bf16 or fp16, contiguous) = a b^T + bias, on the current device and stream.  early: the kernel before
+// this one on the stream is the quantiser that wrote a, launched without overlap itself.
+void gemm(const Int8Matrix& a, const Int8Matrix& b, const c10::optional<at::Tensor>& bias, at::Tensor& d, cudaStream_t stream,
+          bool early) {
+  if (a.rows == 0 || b.rows == 0) return;
+  const Factors f{a.row_scale, b.row_scale, float_row(bias)};
+  const int device = d.get_device();
+  if (few_rows(a.rows, b.rows, sm_count(device))) launch_small(a, b, f, d, device, stream, early);
+  else if (d.scalar_type() == at::kHalf) launch_pair<true>(a, b, f, d, device, stream);
+  else launch_pair<false>(a, b, f, d, device, stream);
+}
+
+void check_sum(int64_t K) {
+  DMAD_VALUE_CHECK(K <= kMaxK, "int8_linear: " + num(K) + " columns: int32 sums hold " + num(kMaxK) + " at most");
+}
+
+}  // namespace
+
+// x W^T + bias for x [..., K] (bf16 or fp16), quantised here by rows, and W [N, K] stored in 8 bits by rows; the result in
+// bf16 (0), fp16 (1) or x's type (-1).
+at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& data, const at::Tensor& scale, c10::optional<at::Tensor> bias,
+                       int64_t N, int64_t K, int64_t out_type) {
+  const auto dt = x.scalar_type();
+  DMAD_VALUE_CHECK(x.is_cuda() && (dt == at::kBFloat16 || dt == at::kHalf), "int8_linear: x must be bf16 or fp16 on CUDA");
+  DMAD_VALUE_CHECK(x.dim() >= 1 && x.size(-1) == K, "int8_linear: x " + shape_text(x) + " must have " + num(K) + " columns");
+  const Int8Matrix w = int8_matrix(data, scale, N, K, false, x.device(), "int8_linear: w");
+  check_sum(K);
+  const auto b = checked_bias(bias, N, x.device(), "int8_linear");
+  c10::cuda::CUDAGuard guard(x.device());
+  const at::Tensor x2 = int8_rows(x, "int8_linear");
+  Int8Matrix q{nullptr, nullptr, nullptr, x2.size(0), K};
+  // codes and scales of x in one piece, freed to the stream's pool when the call returns
+  const int64_t at_scales = (q.rows * q.row_bytes() + 511) / 512 * 512;
+  const auto plain = x.options().requires_grad(false);
+  at::Tensor work = at::empty({at_scales + 4 * q.rows}, plain.dtype(at::kByte));
+  q.data = reinterpret_cast<int8_t*>(work.data_ptr());
+  q.row_scale = reinterpret_cast<float*>(work.data_ptr<uint8_t>() + at_scales);
+  c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  at::Tensor y = at::empty(shape, plain.dtype(out_type == 0 ? at::kBFloat16 : out_type == 1 ? at::kHalf : dt));
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  int8_quantize_launch(x2, q, stream);
+  gemm(q, w, b, y, stream, true);
+  return y;
+}
+
+// The same for an x [M, K] that is stored in 8 bits by rows; the result [M, N] in bf16 (0) or fp16 (1).
+at::Tensor int8_matmul(const at::Tensor& xdata, const at::Tensor& xscale, int64_t M, const at::Tensor& data,
+                       const at::Tensor& scale, c10::optional<at::Tensor> bias, int64_t N, int64_t K, int64_t out_type) {
+  DMAD_VALUE_CHECK(data.is_cuda(), "int8_linear: the native kernel takes CUDA tensors");
+  const Int8Matrix w = int8_matrix(data, scale, N, K, false, data.device(), "int8_linear: w");
+  const Int8Matrix q = int8_matrix(xdata, xscale, M, K, false, data.device(), "int8_linear: x");
+  check_sum(K);
+  const auto b = checked_bias(bias, N, data.device(), "int8_linear");
+  c10::cuda::CUDAGuard guard(data.device());
+  at::Tensor y = at::empty({M, N}, data.options().dtype(out_type == 1 ? at::kHalf : at::kBFloat16));
+  gemm(q, w, b, y, at::cuda::getCurrentCUDAStream(), false);
+  return y;
+}
+
+}  // namespace dmad

@@ -63,6 +63,7 @@ from .attention import flash_attention, attention_reference, flash_attention_jvp
 from .norm import ln_mod, gate_residual, qk_norm_rope, rope, rope_apply, rms_norm, layer_norm_affine  # noqa: E402
 from .activation import gelu_tanh  # noqa: E402
 from .fp4 import Fp4Tensor, quantize_fp4, dequantize_fp4, fp4_linear  # noqa: E402
+from .int8 import Int8Tensor, quantize_int8, dequantize_int8, int8_linear  # noqa: E402
 from .head_norm import qk_head_norm_rope  # noqa: E402
 from .temb import sinusoidal_embedding, small_linear  # noqa: E402
 
@@ -87,6 +88,10 @@ __all__ = [
     "quantize_fp4",
     "dequantize_fp4",
     "fp4_linear",
+    "Int8Tensor",
+    "quantize_int8",
+    "dequantize_int8",
+    "int8_linear",
     "qk_head_norm_rope",
     "sinusoidal_embedding",
     "small_linear",
