@@ -1,0 +1,763 @@
+// A linear layer with an activation in front of it that keeps its input for the backward pass in 8 bits.
+//
+//   y = a W^T + bias,   a = act(x)                               x [R, F] (SwiGLU: [R, 2 F], value and gate), W [N, F]
+//   kept: the codes of x in blocks of 32 columns (int8.cuh; a SwiGLU's halves each from their start), x' their values
+//   dW = g^T act(x'),   dx = (g W) act'(x'),   db = sum g
+//
+//   gelu    v p with p = 1 / (1 + exp(-2 u)), u = sqrt(2 / pi) (v + 0.044715 v^3)      (0.5 (1 + tanh u) = p)
+//           derivative p + 2 v p (1 - p) u'
+//   SwiGLU  v u p with p = 1 / (1 + exp(-u)); derivatives u p and v p (1 + u (1 - p))
+//
+// The products run on gemm_pair.cuh; operands that lie transposed are read MN-major where they are.  a is rounded to the
+// operands' 16 bits, as the tensor core takes it; sums, activations and derivatives are fp32, rounded once.
+//   forward     one pass over x writes a and the codes, then the product.  (Without an activation x itself is the operand.)
+//   backward    the epilogue of g W reads the codes (1 byte an element) and writes dx and act(x') in one go: g W never
+//               reaches memory and x' is decoded once for both; then g^T act(x').  Without an activation x' is decoded for
+//               that product.
+// Few output tiles: the K steps of a tile are spread over several pairs, whose fp32 parts are added in order by a second
+// kernel, so that the sums are the same every time.
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include "act8.h"
+#include "common.cuh"
+#include "gemm_pair.cuh"
+#include "int8_host.h"
+
+namespace dmad {
+namespace {
+
+// ---------------------------------------------------------------- activations
+__device__ __forceinline__ float rcp_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// 1 / (1 + 2^z): 2^z of 2^128 and more is infinity, and the quotient 0
+__device__ __forceinline__ float logistic2(float z) { return rcp_fast(1.f + ex2_approx(z)); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGeluA = -2.f * 0.7978845608028654f * kLog2e, kGeluB = 0.044715f;
+
+template <int ACT>
+__device__ __forceinline__ float act_value(float v, float u) {
+  if constexpr (ACT == kActGelu) return v * logistic2(kGeluA * v * fmaf(kGeluB * v, v, 1.f));
+  else if constexpr (ACT == kActSwiglu) return v * u * logistic2(-kLog2e * u);
+  else return v;
+}
+
+// act(x') and da act'(x'): dv, and for a SwiGLU du.
+template <int ACT>
+__device__ __forceinline__ void act_backward(float da, float v, float u, float& a, float& dv, float& du) {
+  if constexpr (ACT == kActGelu) {
+    const float w = kGeluB * v * v, p = logistic2(kGeluA * v * (1.f + w));
+    a = v * p;
+    // 2 u' = -kGeluA / log2(e) (1 + 3 w)
+    dv = da * fmaf(a * (1.f - p), (-kGeluA / kLog2e) * fmaf(3.f, w, 1.f), p);
+    du = 0.f;
+  } else if constexpr (ACT == kActSwiglu) {
+    const float p = logistic2(-kLog2e * u), up = u * p;
+    a = v * up;
+    dv = da * up;
+    du = da * v * fmaf(up, 1.f - p, p);
+  } else {
+    a = v;
+    dv = da;
+    du = 0.f;
+  }
+}
+
+// Kept input: H = 2 for a SwiGLU (row r's halves are rows 2 r and 2 r + 1 of the codes), else 1.
+struct Kept {
+  int8_t* data;
+  uint8_t* exponents;
+};
+
+// ---------------------------------------------------------------- forward pass over x
+struct EncodeParams {
+  const void* x;
+  int64_t ld;
+  int R, F;
+  void* a;
+  int64_t lda;
+  Kept kept;  // data null: nothing is kept
+};
+
+// Codes of a unit in spread order: a block of 32 columns is element j of all lanes.  Returns the scale byte of block `lane`.
+template <typename T>
+__device__ __forceinline__ uint32_t encode_spread(const Unit<T>& u, uint32_t (&codes)[4]) {
+  const int lane = lane_id();
+  uint32_t mine = 0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    codes[q] = 0u;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int j = 4 * q + h;
+      const uint32_t e = int8_block_code(__reduce_max_sync(0xffffffffu, abs_bits(u, j)));
+      if (lane == j) mine = e;
+      codes[q] |= int8_block_byte(u, j, e) << (8 * h);
+    }
+  }
+  return mine;
+}
+
+template <typename T, int ACT, bool ALIGNED>
+__global__ void __launch_bounds__(256) act_encode_kernel(EncodeParams p) {
+  constexpr bool FP16 = std::is_same_v<T, __half>;
+  constexpr int H = ACT == kActSwiglu ? 2 : 1;
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= p.R) return;  // whole warps
+  const int lane = threadIdx.x & 31;
+  const int row_bytes = (int)int8_row_bytes(p.F), nb = row_bytes / kInt8Block;
+  const T* xr = static_cast<const T*>(p.x) + row * p.ld;
+  uint16_t* ar = static_cast<uint16_t*>(p.a) + row * p.lda;
+  for (int first = threadIdx.x - lane; first * 16 < row_bytes; first += blockDim.x) {
+    const int col = ALIGNED ? (first + lane) * 16 : first * 16;
+    Unit<T> v[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      if constexpr (ALIGNED) v[h] = load_unit<T, true>(xr + h * p.F, col, p.F);
+      else v[h] = load_spread<T>(xr + h * p.F, col, p.F);
+    }
+    uint32_t o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 a = f2_split(unit_pair(v[0], i)), b = f2_split(unit_pair(v[H - 1], i));
+      o[i] = pack16<FP16>(act_value<ACT>(a.x, b.x), act_value<ACT>(a.y, b.y));
+    }
+    if constexpr (ALIGNED) {
+      if (col < p.F) st256(ar + col, o);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (col + 32 * j + lane < p.F) ar[col + 32 * j + lane] = (uint16_t)(o[j >> 1] >> (16 * (j & 1)));
+    }
+    if (p.kept.data == nullptr) continue;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      int8_t* dr = p.kept.data + (row * H + h) * row_bytes;
+      uint8_t* er = p.kept.exponents + (row * H + h) * nb;
+      uint32_t codes[4];
+      if constexpr (ALIGNED) {  // a block is two lanes' units
+        uint32_t amax = absmax_bits(v[h]);
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        const uint32_t e = int8_block_code(amax);
+        int8_encode_block(v[h], e, codes);
+        if (col < row_bytes) {
+          *reinterpret_cast<uint4*>(dr + col) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+          if ((lane & 1) == 0) er[col / kInt8Block] = (uint8_t)e;
+        }
+      } else {
+        const uint32_t e = encode_spread(v[h], codes);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (col + 32 * j < row_bytes) dr[col + 32 * j + lane] = (int8_t)(codes[j >> 2] >> (8 * (j & 3)));
+        if (lane < 16 && col / kInt8Block + lane < nb) er[col / kInt8Block + lane] = (uint8_t)e;
+      }
+    }
+  }
+}
+
+// act(x') [R, F] of the kept codes, for a backward pass without dx.  A thread takes four columns (a has room for them).
+template <bool FP16, int ACT>
+__global__ void __launch_bounds__(256) act_decode_kernel(Kept kept, uint16_t* a, int64_t lda, int R, int F) {
+  constexpr int H = ACT == kActSwiglu ? 2 : 1;
+  const int row_bytes = (int)int8_row_bytes(F), nb = row_bytes / kInt8Block;
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= R) return;
+  for (int c = threadIdx.x * 4; c < F; c += blockDim.x * 4) {
+    float2 v[H][2];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int64_t r = row * H + h;
+      const float s = int8_block_scale(__ldg(kept.exponents + r * nb + c / kInt8Block));
+      uint64_t lo, hi;
+      bytes_to_float(__ldg(reinterpret_cast<const uint32_t*>(kept.data + r * row_bytes + c)), lo, hi);
+      v[h][0] = f2_split(f2_mul(lo, f2(s, s)));
+      v[h][1] = f2_split(f2_mul(hi, f2(s, s)));
+    }
+    uint32_t o[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      o[i] = pack16<FP16>(act_value<ACT>(v[0][i].x, v[H - 1][i].x), act_value<ACT>(v[0][i].y, v[H - 1][i].y));
+    *reinterpret_cast<uint2*>(a + row * lda + c) = make_uint2(o[0], o[1]);
+  }
+}
+
+// ---------------------------------------------------------------- epilogues
+// acc + bias -> 16 bits.
+template <bool FP16>
+struct BiasEpilogue {
+  static constexpr int kStages = 6, kOutBytes = 2048;
+  static constexpr bool kShared = true;
+  struct Args {
+    CUtensorMap map;
+    OutRows out;
+    FloatRow bias;
+  };
+  const Args& a;
+  const PairGemm& p;
+  const EpiPlace at;
+  int m0, n0;
+  float next_bias;
+  const float* col;
+
+  __device__ __forceinline__ BiasEpilogue(const Args& a, const PairGemm& p, const EpiPlace& at) : a(a), p(p), at(at) {}
+  __device__ __forceinline__ void fetch(int item) {
+    int tm, tn;
+    p.tile(item, tm, tn);
+    next_bias = a.bias.at(min(tn * kPairN + at.thread, p.N - 1));
+  }
+  __device__ __forceinline__ void first(int item) { fetch(item); }
+  __device__ __forceinline__ void begin(int item, int, int parity) {
+    int tm, tn;
+    p.tile(item, tm, tn);
+    m0 = tm * kPairM + (int)at.rank * kPairHalf + at.wq * 32;
+    n0 = tn * kPairN;
+    float* mine = reinterpret_cast<float*>(at.col) + parity * kPairN;
+    col = mine;
+    mine[at.thread] = next_bias;
+  }
+  __device__ __forceinline__ void met(int next) {
+    if (next >= 0) fetch(next);
+  }
+  __device__ __forceinline__ void chunk(int, int c, const uint32_t (&v)[32]) {
+    const int nc = n0 + c * 32;
+    if (nc >= p.N || m0 >= p.M) return;
+    uint32_t o[16];
+    const float4* f4 = reinterpret_cast<const float4*>(col + c * 32);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float4 f = f4[q];
+      o[2 * q] = pack16<FP16>(__uint_as_float(v[4 * q]) + f.x, __uint_as_float(v[4 * q + 1]) + f.y);
+      o[2 * q + 1] = pack16<FP16>(__uint_as_float(v[4 * q + 2]) + f.z, __uint_as_float(v[4 * q + 3]) + f.w);
+    }
+    if (at.lane == 0) tma_store_wait_read();
+    __syncwarp();
+    store_rows(a.out, &a.map, at.stage, m0, nc, o);
+  }
+  __device__ __forceinline__ void done() {
+    if (at.lane == 0) tma_store_wait_read();
+  }
+};
+
+// fp32 parts [split, M, N] of tiles whose K steps several pairs share, in boxes of 32 x 32 (128-byte swizzle).
+struct PartEpilogue {
+  static constexpr int kStages = 5, kOutBytes = 4096;
+  static constexpr bool kShared = false;
+  struct Args {
+    CUtensorMap map;
+  };
+  const Args& a;
+  const PairGemm& p;
+  const EpiPlace at;
+  int m0, n0, part;
+
+  __device__ __forceinline__ PartEpilogue(const Args& a, const PairGemm& p, const EpiPlace& at) : a(a), p(p), at(at) {}
+  __device__ __forceinline__ void first(int) {}
+  __device__ __forceinline__ void begin(int item, int, int) {
+    int tm, tn;
+    p.tile(item, tm, tn);
+    m0 = tm * kPairM + (int)at.rank * kPairHalf + at.wq * 32;
+    n0 = tn * kPairN;
+    part = item % p.split;
+  }
+  __device__ __forceinline__ void met(int) {}
+  __device__ __forceinline__ void chunk(int, int c, const uint32_t (&v)[32]) {
+    const int nc = n0 + c * 32;
+    if (nc >= p.N || m0 >= p.M) return;
+    if (at.lane == 0) tma_store_wait_read();
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<uint4*>(at.stage + at.lane * 128 + ((q ^ (at.lane & 7)) << 4)) =
+          make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (at.lane == 0) tma_store_3d(&a.map, at.stage, nc, m0, part);
+  }
+  __device__ __forceinline__ void done() {
+    if (at.lane == 0) tma_store_wait_read();
+  }
+};
+
+// dx = acc act'(x') and act(x'), from the accumulator (g W) and the kept codes.  A lane reads its row's 32 codes of a chunk
+// (one sector) while the chunk before is computed.
+template <bool FP16, int ACT>
+struct ActGradEpilogue {
+  static constexpr int H = ACT == kActSwiglu ? 2 : 1;
+  static constexpr int kStages = 5, kOutBytes = 2048 * (H + 1);
+  static constexpr bool kShared = false;
+  struct Args {
+    CUtensorMap map_dx[H], map_a;
+    OutRows dx[H], act;
+    bool want_act;
+    Kept kept;
+  };
+  struct Codes {
+    uint4 lo, hi;
+    uint32_t e;
+  };
+  const Args& a;
+  const PairGemm& p;
+  const EpiPlace at;
+  int m0, n0;
+  Codes q[2][H];
+
+  __device__ __forceinline__ ActGradEpilogue(const Args& a, const PairGemm& p, const EpiPlace& at) : a(a), p(p), at(at) {}
+  __device__ __forceinline__ void first(int) {}
+  __device__ __forceinline__ void load(Codes (&to)[H], int c) {
+    const int nc = n0 + c * 32, m = m0 + at.lane;
+    const int row_bytes = (int)int8_row_bytes(p.N), nb = row_bytes / kInt8Block;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      to[h] = Codes{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0), 0u};
+      if (m < p.M && nc < p.N) {
+        const int64_t r = (int64_t)m * H + h;
+        const uint4* d = reinterpret_cast<const uint4*>(a.kept.data + r * row_bytes + nc);
+        to[h].lo = __ldg(d);
+        to[h].hi = __ldg(d + 1);
+        to[h].e = __ldg(a.kept.exponents + r * nb + nc / kInt8Block);
+      }
+    }
+  }
+  __device__ __forceinline__ void begin(int item, int, int) {
+    int tm, tn;
+    p.tile(item, tm, tn);
+    m0 = tm * kPairM + (int)at.rank * kPairHalf + at.wq * 32;
+    n0 = tn * kPairN;
+    load(q[0], at.half);
+  }
+  __device__ __forceinline__ void met(int) {}
+  __device__ __forceinline__ void chunk(int i, int c, const uint32_t (&v)[32]) {
+    const int nc = n0 + c * 32;
+    if (i < 3) load(q[(i + 1) & 1], c + 2);
+    if (nc >= p.N || m0 >= p.M) return;
+    const Codes(&k)[H] = q[i & 1];
+    uint32_t od[H][16], oa[16];
+    uint64_t s[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const float f = int8_block_scale(k[h].e);
+      s[h] = f2(f, f);
+    }
+#pragma unroll
+    for (int w = 0; w < 8; ++w) {
+      float2 x[H][2];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        const uint32_t bytes = w == 0 ? k[h].lo.x : w == 1 ? k[h].lo.y : w == 2 ? k[h].lo.z : w == 3 ? k[h].lo.w
+                               : w == 4 ? k[h].hi.x : w == 5 ? k[h].hi.y : w == 6 ? k[h].hi.z : k[h].hi.w;
+        uint64_t lo, hi;
+        bytes_to_float(bytes, lo, hi);
+        x[h][0] = f2_split(f2_mul(lo, s[h]));
+        x[h][1] = f2_split(f2_mul(hi, s[h]));
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float a0, v0, u0, a1, v1, u1;
+        act_backward<ACT>(__uint_as_float(v[4 * w + 2 * j]), x[0][j].x, x[H - 1][j].x, a0, v0, u0);
+        act_backward<ACT>(__uint_as_float(v[4 * w + 2 * j + 1]), x[0][j].y, x[H - 1][j].y, a1, v1, u1);
+        oa[2 * w + j] = pack16<FP16>(a0, a1);
+        od[0][2 * w + j] = pack16<FP16>(v0, v1);
+        if constexpr (H == 2) od[1][2 * w + j] = pack16<FP16>(u0, u1);
+      }
+    }
+    if (at.lane == 0) tma_store_wait_read();
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < H; ++h) store_rows(a.dx[h], &a.map_dx[h], at.stage + 2048 * h, m0, nc, od[h]);
+    if (a.want_act) store_rows(a.act, &a.map_a, at.stage + 2048 * H, m0, nc, oa);
+  }
+  __device__ __forceinline__ void done() {
+    if (at.lane == 0) tma_store_wait_read();
+  }
+};
+
+// ---------------------------------------------------------------- sums of parts
+struct PartSum {
+  const float* parts;  // [split, M, ldp]
+  int split, M, N;
+  int64_t ldp;
+  OutRows out[2];      // the result, or dx (of a SwiGLU: its halves)
+  FloatRow bias;
+  OutRows act;         // act(x'), if wanted
+  bool want_act;
+  Kept kept;
+};
+
+template <bool FP16>
+__device__ __forceinline__ void store4(const OutRows& o, int m, int n, const float (&v)[4]) {
+  uint16_t* d = o.d + (int64_t)m * o.ld + n;
+  const uint32_t lo = pack16<FP16>(v[0], v[1]), hi = pack16<FP16>(v[2], v[3]);
+  if (o.tma && n + 4 <= o.N) {
+    *reinterpret_cast<uint2*>(d) = make_uint2(lo, hi);
+  } else {
+    d[0] = (uint16_t)lo;
+    if (n + 1 < o.N) d[1] = (uint16_t)(lo >> 16);
+    if (n + 2 < o.N) d[2] = (uint16_t)hi;
+    if (n + 3 < o.N) d[3] = (uint16_t)(hi >> 16);
+  }
+}
+
+// Four columns a thread: the parts added in order, then what the epilogue of an undivided tile does.
+template <bool FP16, int ACT>
+__global__ void __launch_bounds__(256) part_sum_kernel(const __grid_constant__ PartSum p) {
+  constexpr int H = ACT == kActSwiglu ? 2 : 1;
+  const int n = (blockIdx.x * blockDim.x + threadIdx.x) * 4, m = blockIdx.y * blockDim.y + threadIdx.y;
+  if (n >= p.N || m >= p.M) return;
+  const float* at = p.parts + (int64_t)m * p.ldp + n;
+  float4 sum = __ldg(reinterpret_cast<const float4*>(at));
+  for (int s = 1; s < p.split; ++s) {
+    const float4 f = __ldg(reinterpret_cast<const float4*>(at + (int64_t)s * p.M * p.ldp));
+    sum.x += f.x;
+    sum.y += f.y;
+    sum.z += f.z;
+    sum.w += f.w;
+  }
+  float v[4] = {sum.x, sum.y, sum.z, sum.w};
+  if constexpr (ACT == kActNone) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += p.bias.at(min(n + i, p.N - 1));
+    store4<FP16>(p.out[0], m, n, v);
+  } else {
+    const int row_bytes = (int)int8_row_bytes(p.N), nb = row_bytes / kInt8Block;
+    float x[H][4];
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int64_t r = (int64_t)m * H + h;
+      const float s = int8_block_scale(__ldg(p.kept.exponents + r * nb + n / kInt8Block));
+      uint64_t lo, hi;
+      bytes_to_float(__ldg(reinterpret_cast<const uint32_t*>(p.kept.data + r * row_bytes + n)), lo, hi);
+      const float2 a = f2_split(f2_mul(lo, f2(s, s))), b = f2_split(f2_mul(hi, f2(s, s)));
+      x[h][0] = a.x, x[h][1] = a.y, x[h][2] = b.x, x[h][3] = b.y;
+    }
+    float act[4], dv[4], du[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) act_backward<ACT>(v[i], x[0][i], x[H - 1][i], act[i], dv[i], du[i]);
+    store4<FP16>(p.out[0], m, n, dv);
+    if constexpr (H == 2) store4<FP16>(p.out[1], m, n, du);
+    if (p.want_act) store4<FP16>(p.act, m, n, act);
+  }
+}
+
+// ---------------------------------------------------------------- sums of columns
+// out[slice, n] = sum of rows slice * per .. of g: 256 columns a block, eight a lane, the block's warps on every eighth row.
+template <bool FP16>
+__global__ void __launch_bounds__(256) column_sum_kernel(const uint16_t* g, int64_t ld, int R, int N, int per, void* out, int type) {
+  __shared__ float red[8][256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.x * 256 + lane * 8;
+  const int r0 = blockIdx.y * per, r1 = min(R, r0 + per);
+  float s[8] = {};
+  if (n + 8 <= N) {
+    for (int r = r0 + warp; r < r1; r += 8) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(g + (int64_t)r * ld + n));
+      const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = FP16 ? __half22float2(*reinterpret_cast<const __half2*>(&q[i])) : unpack_bf16x2(q[i]);
+        s[2 * i] += f.x;
+        s[2 * i + 1] += f.y;
+      }
+    }
+  } else {
+    for (int r = r0 + warp; r < r1; r += 8)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + i < N) {
+          const uint16_t w = g[(int64_t)r * ld + n + i];
+          s[i] += FP16 ? __half2float(__ushort_as_half(w)) : __uint_as_float((uint32_t)w << 16);
+        }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) red[warp][lane * 8 + i] = s[i];
+  __syncthreads();
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= N) return;
+  float t = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) t += red[w][threadIdx.x];
+  const int64_t to = (int64_t)blockIdx.y * N + c;
+  if (type == 0) static_cast<float*>(out)[to] = t;
+  else if (type == 1) static_cast<__nv_bfloat16*>(out)[to] = __float2bfloat16_rn(t);
+  else static_cast<__half*>(out)[to] = __float2half_rn(t);
+}
+
+__global__ void __launch_bounds__(256) slice_sum_kernel(const float* parts, int slices, int N, void* out, int type) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= N) return;
+  float t = 0.f;
+  for (int s = 0; s < slices; ++s) t += parts[(int64_t)s * N + c];
+  if (type == 0) static_cast<float*>(out)[c] = t;
+  else if (type == 1) static_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(t);
+  else static_cast<__half*>(out)[c] = __float2half_rn(t);
+}
+
+int type_index(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : 2; }
+
+at::Tensor column_sum(const at::Tensor& g, at::ScalarType type, cudaStream_t stream) {
+  const int R = (int)g.size(0), N = (int)g.size(1), nb = (N + 255) / 256, device = g.get_device();
+  at::Tensor out = at::empty({N}, g.options().dtype(type));
+  // slices for two blocks an SM, of 64 rows at least
+  const int slices = std::max(1, std::min(2 * sm_count(device) / nb, R / 64)), per = (R + slices - 1) / slices;
+  at::Tensor parts = slices > 1 ? at::empty({slices, N}, g.options().dtype(at::kFloat)) : out;
+  void* to = parts.data_ptr();
+  const int first = slices > 1 ? 0 : type_index(type);
+  const uint16_t* gp = static_cast<const uint16_t*>(g.data_ptr());
+  if (g.scalar_type() == at::kHalf)
+    column_sum_kernel<true><<<dim3(nb, slices), 256, 0, stream>>>(gp, g.stride(0), R, N, per, to, first);
+  else
+    column_sum_kernel<false><<<dim3(nb, slices), 256, 0, stream>>>(gp, g.stride(0), R, N, per, to, first);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (slices > 1) {
+    slice_sum_kernel<<<nb, 256, 0, stream>>>(parts.data_ptr<float>(), slices, N, out.data_ptr(), type_index(type));
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  return out;
+}
+
+// ---------------------------------------------------------------- products
+// Rows that TMA can read: contiguous columns, rows on 16 bytes; copied where t is laid out otherwise.
+at::Tensor tma_rows(const at::Tensor& t) {
+  if (t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)
+    return t;
+  at::Tensor p = at::empty({t.size(0), (t.size(1) + 7) / 8 * 8}, t.options().requires_grad(false)).narrow(1, 0, t.size(1));
+  p.copy_(t);
+  return p;
+}
+
+// Items for each tile along K: where the tiles leave half of the pairs or more without work, as many as fill them, of four
+// stages at least.
+int split_of(int64_t M, int64_t N, int64_t K, int device) {
+  const int64_t tiles = ((M + kPairM - 1) / kPairM) * ((N + kPairN - 1) / kPairN), pairs = sm_count(device) / 2;
+  const int64_t stages = (K + 63) / 64;
+  return tiles * 2 > pairs ? 1 : (int)std::max<int64_t>(1, std::min(pairs / tiles, stages / 4));
+}
+
+struct Operand {  // [rows, K], or stored [K, rows]
+  const at::Tensor& t;
+  bool mn;
+  int64_t rows() const { return t.size(mn ? 1 : 0); }
+  int64_t K() const { return t.size(mn ? 0 : 1); }
+  CUtensorMap map() const { return operand_map(t.data_ptr(), rows(), K(), t.stride(0), 2, mn); }
+};
+
+// What becomes of the product: out = acc + bias, or (act) out = acc act'(x') and act(x').
+struct Result {
+  OutRows out[2];
+  FloatRow bias{nullptr, 0};
+  int act = kActNone;
+  Kept kept{nullptr, nullptr};
+  OutRows value{};
+  bool want_value = false;
+};
+
+template <bool FP16, int ACT>
+void product_typed(const Operand& A, const Operand& B, const Result& r, int device, cudaStream_t stream) {
+  constexpr Mma KIND = FP16 ? Mma::kF16 : Mma::kBf16;
+  const int64_t M = A.rows(), N = B.rows(), K = A.K();
+  const PairGemm p = pair_gemm(M, N, K, 2, A.mn, B.mn, split_of(M, N, K, device), device);
+  const CUtensorMap ma = A.map(), mb = B.map();
+  auto map_of = [&](const OutRows& o) { return o.tma && o.d != nullptr ? out_rows_map(o) : ma; };
+  if (p.split > 1) {
+    const int64_t ldp = (N + 3) / 4 * 4;
+    at::Tensor parts = at::empty({p.split, M, ldp}, A.t.options().dtype(at::kFloat).requires_grad(false));
+    const uint64_t dims[3] = {(uint64_t)N, (uint64_t)M, (uint64_t)p.split};
+    const uint64_t strides[2] = {(uint64_t)ldp * 4, (uint64_t)(M * ldp) * 4};
+    const uint32_t box[3] = {32u, 32u, 1u};
+    const PartEpilogue::Args args{make_tmap(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, parts.data_ptr(), 3, dims, strides, box,
+                                            CU_TENSOR_MAP_SWIZZLE_128B)};
+    launch_pair_gemm<KIND, PartEpilogue>(ma, mb, args, p, device, stream);
+    const PartSum s{parts.data_ptr<float>(), p.split, (int)M, (int)N, ldp, {r.out[0], r.out[1]}, r.bias, r.value,
+                    r.want_value, r.kept};
+    const int tx = N > 128 ? 64 : 32, ty = 256 / tx;
+    DMAD_VALUE_CHECK((M + ty - 1) / ty <= 65535, "linear_act8: too many rows");  // (split tiles are few)
+    part_sum_kernel<FP16, ACT><<<dim3((unsigned)((N + 4 * tx - 1) / (4 * tx)), (unsigned)((M + ty - 1) / ty)), dim3(tx, ty), 0,
+                                 stream>>>(s);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  } else if constexpr (ACT == kActNone) {
+    const typename BiasEpilogue<FP16>::Args args{map_of(r.out[0]), r.out[0], r.bias};
+    launch_pair_gemm<KIND, BiasEpilogue<FP16>>(ma, mb, args, p, device, stream);
+  } else {
+    typename ActGradEpilogue<FP16, ACT>::Args args;
+    for (int h = 0; h < ActGradEpilogue<FP16, ACT>::H; ++h) {
+      args.map_dx[h] = map_of(r.out[h]);
+      args.dx[h] = r.out[h];
+    }
+    args.map_a = map_of(r.value);
+    args.act = r.value;
+    args.want_act = r.want_value;
+    args.kept = r.kept;
+    launch_pair_gemm<KIND, ActGradEpilogue<FP16, ACT>>(ma, mb, args, p, device, stream);
+  }
+}
+
+void product(const Operand& A, const Operand& B, const Result& r, cudaStream_t stream) {
+  const bool fp16 = A.t.scalar_type() == at::kHalf;
+  const int device = A.t.get_device();
+  if (r.act == kActGelu) fp16 ? product_typed<true, kActGelu>(A, B, r, device, stream) : product_typed<false, kActGelu>(A, B, r, device, stream);
+  else if (r.act == kActSwiglu) fp16 ? product_typed<true, kActSwiglu>(A, B, r, device, stream) : product_typed<false, kActSwiglu>(A, B, r, device, stream);
+  else fp16 ? product_typed<true, kActNone>(A, B, r, device, stream) : product_typed<false, kActNone>(A, B, r, device, stream);
+}
+
+dim3 row_block(int64_t units) {  // threads of a row, rows
+  const int tx = (int)std::min<int64_t>(256, (units + 31) / 32 * 32);
+  return dim3(tx, 256 / tx);
+}
+
+int halves(int64_t act) { return act == kActSwiglu ? 2 : 1; }
+
+Kept kept_of(const at::Tensor& data, const at::Tensor& exponents) {
+  return Kept{reinterpret_cast<int8_t*>(data.data_ptr()), exponents.data_ptr<uint8_t>()};
+}
+
+// act(x) [R, F] with rows on 32 bytes, and the codes of x.
+at::Tensor encode(const at::Tensor& x2, int64_t F, int64_t act, const Kept& kept, cudaStream_t stream) {
+  const int64_t R = x2.size(0), lda = (F + 15) / 16 * 16;
+  at::Tensor a = at::empty({R, lda}, x2.options().requires_grad(false));
+  if (R > 0) {
+    const EncodeParams p{x2.data_ptr(), x2.stride(0), (int)R, (int)F, a.data_ptr(), lda, kept};
+    const bool aligned = F % 16 == 0 && x2.stride(0) % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 32 == 0;
+    const dim3 block = row_block(int8_row_bytes(F) / 16);
+    const unsigned grid = (unsigned)((R + block.y - 1) / block.y);
+    auto go = [&](auto tag, auto which) {
+      using T = decltype(tag);
+      constexpr int ACT = decltype(which)::value;
+      if (aligned) act_encode_kernel<T, ACT, true><<<grid, block, 0, stream>>>(p);
+      else act_encode_kernel<T, ACT, false><<<grid, block, 0, stream>>>(p);
+    };
+    auto typed = [&](auto tag) {
+      if (act == kActGelu) go(tag, std::integral_constant<int, kActGelu>{});
+      else go(tag, std::integral_constant<int, kActSwiglu>{});
+    };
+    if (x2.scalar_type() == at::kHalf) typed(__half{});
+    else typed(__nv_bfloat16{});
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  return a.narrow(1, 0, F);
+}
+
+// act(x') [R, F] of the codes.
+at::Tensor decode(const Kept& kept, int64_t R, int64_t F, int64_t act, const at::TensorOptions& options, cudaStream_t stream) {
+  const int64_t lda = (F + 15) / 16 * 16;
+  at::Tensor a = at::empty({R, lda}, options).narrow(1, 0, F);
+  if (act == kActNone) {
+    int8_dequantize_launch(Int8Matrix{kept.data, nullptr, kept.exponents, R, F}, a, stream);
+    return a;
+  }
+  const dim3 block = row_block((F + 3) / 4);
+  const unsigned grid = (unsigned)((R + block.y - 1) / block.y);
+  uint16_t* to = static_cast<uint16_t*>(a.data_ptr());
+  if (options.dtype() == at::kHalf) {
+    if (act == kActGelu) act_decode_kernel<true, kActGelu><<<grid, block, 0, stream>>>(kept, to, lda, (int)R, (int)F);
+    else act_decode_kernel<true, kActSwiglu><<<grid, block, 0, stream>>>(kept, to, lda, (int)R, (int)F);
+  } else {
+    if (act == kActGelu) act_decode_kernel<false, kActGelu><<<grid, block, 0, stream>>>(kept, to, lda, (int)R, (int)F);
+    else act_decode_kernel<false, kActSwiglu><<<grid, block, 0, stream>>>(kept, to, lda, (int)R, (int)F);
+  }
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return a;
+}
+
+}  // namespace
+
+void act8_check(const at::Tensor& x, const at::Tensor& w, const c10::optional<at::Tensor>& bias, int64_t act) {
+  const auto dt = x.scalar_type();
+  DMAD_VALUE_CHECK(x.is_cuda() && (dt == at::kBFloat16 || dt == at::kHalf), "linear_act8: x must be bf16 or fp16 on CUDA");
+  DMAD_VALUE_CHECK(w.dim() == 2 && w.scalar_type() == dt && w.device() == x.device(),
+                   "linear_act8: w must be a matrix of x's type on its device, got " + std::string(dtype_name(w.scalar_type())) +
+                       " " + shape_text(w));
+  const int64_t F = w.size(1);
+  DMAD_VALUE_CHECK(F >= 1 && F <= (1 << 23) && w.size(0) <= (1 << 24), "linear_act8: w " + shape_text(w) + ": sizes out of range");
+  DMAD_VALUE_CHECK(x.dim() >= 1 && x.size(-1) == halves(act) * F,
+                   "linear_act8: x " + shape_text(x) + " must have " + num(halves(act) * F) + " columns for w " + shape_text(w));
+  checked_bias(bias, w.size(0), x.device(), "linear_act8");
+}
+
+// (y, codes, exponents) of x [..., H F], W [N, F] (checked); the codes [R H, ..] where `keep` is set.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_forward(const at::Tensor& x, const at::Tensor& w,
+                                                            const c10::optional<at::Tensor>& bias, int64_t act, bool keep) {
+  c10::cuda::CUDAGuard guard(x.device());
+  const int64_t N = w.size(0), F = w.size(1), H = halves(act);
+  const at::Tensor x2 = int8_rows(x, "linear_act8");
+  const int64_t R = x2.size(0);
+  DMAD_VALUE_CHECK(R * H <= INT32_MAX - 256, "linear_act8: too many rows");
+  const auto plain = x.options().requires_grad(false);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  at::Tensor data, exponents;
+  Kept kept{nullptr, nullptr};
+  if (keep) {
+    data = at::empty({R * H, int8_row_bytes(F)}, plain.dtype(at::kChar));
+    exponents = at::empty({R * H, (F + kInt8Block - 1) / kInt8Block}, plain.dtype(at::kByte));
+    kept = kept_of(data, exponents);
+  }
+  at::Tensor a;
+  if (act == kActNone) {
+    if (keep) int8_quantize_launch(x2, Int8Matrix{kept.data, nullptr, kept.exponents, R, F}, stream);
+    a = tma_rows(x2);
+  } else {
+    a = encode(x2, F, act, kept, stream);
+  }
+  c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = N;
+  at::Tensor y = at::empty(shape, plain);
+  if (R > 0 && N > 0) {
+    const at::Tensor wt = tma_rows(w);
+    const auto b = bias.has_value() && bias->defined() ? c10::optional<at::Tensor>(bias->contiguous()) : c10::nullopt;
+    Result r;
+    r.out[0] = out_rows(y.data_ptr(), N, R, N);
+    r.bias = float_row(b);
+    product(Operand{a, false}, Operand{wt, false}, r, stream);
+  }
+  return {y, data, exponents};
+}
+
+// Gradients of x (shape [R, H F]), w and bias (undefined where they are not wanted).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_backward(const at::Tensor& g, const at::Tensor& w, const at::Tensor& data,
+                                                             const at::Tensor& exponents, int64_t act, int64_t R,
+                                                             bool want_x, bool want_w, bool want_b, at::ScalarType bias_type) {
+  c10::cuda::CUDAGuard guard(g.device());
+  const int64_t N = w.size(0), F = w.size(1), H = halves(act);
+  const auto plain = w.options().requires_grad(false);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  at::Tensor dx, dw, db;
+  if (want_x) dx = at::empty({R, H * F}, plain);
+  if (R == 0 || N == 0) {
+    if (want_x) dx.zero_();
+    if (want_w) dw = at::zeros({N, F}, plain);
+    if (want_b) db = at::zeros({N}, plain.dtype(bias_type));
+    return {dx, dw, db};
+  }
+  const at::Tensor gt = tma_rows(g.dim() == 2 ? g : g.reshape({R, N}));
+  const Kept kept = data.defined() ? kept_of(data, exponents) : Kept{nullptr, nullptr};
+  at::Tensor a;  // act(x')
+  if (want_x) {
+    const at::Tensor wt = tma_rows(w);
+    Result r;
+    for (int h = 0; h < H; ++h) r.out[h] = out_rows(static_cast<uint16_t*>(dx.data_ptr()) + h * F, H * F, R, F);
+    r.act = (int)act;
+    r.kept = kept;
+    if (act != kActNone && want_w) {
+      a = at::empty({R, (F + 15) / 16 * 16}, plain);
+      r.value = out_rows(a.data_ptr(), a.stride(0), R, a.size(1));  // columns past F may be written, nothing reads them
+      a = a.narrow(1, 0, F);
+      r.want_value = true;
+    }
+    product(Operand{gt, false}, Operand{wt, true}, r, stream);
+  }
+  if (want_w) {
+    if (!a.defined()) a = decode(kept, R, F, act, plain, stream);
+    dw = at::empty({N, F}, plain);
+    Result r;
+    r.out[0] = out_rows(dw.data_ptr(), F, N, F);
+    product(Operand{gt, true}, Operand{a, true}, r, stream);
+  }
+  if (want_b) db = column_sum(gt, bias_type, stream);
+  return {dx, dw, db};
+}
+
+}  // namespace dmad

@@ -88,6 +88,7 @@ at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& data, const at::Te
                        int64_t N, int64_t K, int64_t out_type);
 at::Tensor int8_matmul(const at::Tensor& xdata, const at::Tensor& xscale, int64_t M, const at::Tensor& data,
                        const at::Tensor& scale, c10::optional<at::Tensor> bias, int64_t N, int64_t K, int64_t out_type);
+at::Tensor linear_act8(const at::Tensor& x, const at::Tensor& w, c10::optional<at::Tensor> bias, int64_t act);
 std::tuple<at::Tensor, at::Tensor> head_norm_rope_fwd(const at::Tensor& q, const at::Tensor& k,
                                                       c10::optional<at::Tensor> wq, c10::optional<at::Tensor> wk,
                                                       c10::optional<at::Tensor> cosT, c10::optional<at::Tensor> sinT,
@@ -159,6 +160,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("int8_dequantize", &dmad::int8_dequantize);
   m.def("int8_linear", &dmad::int8_linear);
   m.def("int8_matmul", &dmad::int8_matmul);
+  m.def("linear_act8", &dmad::linear_act8);
   m.def("check_captured_backward", &dmad::check_captured_backward);
   m.def("head_norm_rope", &dmad::head_norm_rope);
   m.def("head_norm_rope_fwd", &dmad::head_norm_rope_fwd);

@@ -375,8 +375,11 @@ inline CUtensorMap out_rows_map(const OutRows& o) {  // 16-bit elements, whichev
   return make_tmap_bf16(o.d, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
+// TMA writes whole pieces of 16 bytes, so the columns that it may write have to end on one: where N does not (one half of a
+// row beside the other), runs of 32 bytes are stored instead.
 inline OutRows out_rows(void* d, int64_t ld, int64_t M, int64_t N) {
-  return OutRows{static_cast<uint16_t*>(d), ld, (int)M, (int)N, (reinterpret_cast<uintptr_t>(d) | (uintptr_t)(2 * ld)) % 16 == 0};
+  return OutRows{static_cast<uint16_t*>(d), ld, (int)M, (int)N,
+                 (reinterpret_cast<uintptr_t>(d) | (uintptr_t)(2 * ld) | (uintptr_t)(2 * N)) % 16 == 0};
 }
 
 // An operand's map: rows x 128 bytes of a K-major matrix, or 64 x 64 of an MN-major one.

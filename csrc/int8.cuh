@@ -146,4 +146,13 @@ __device__ __forceinline__ uint32_t abs_bits(const Unit<T>& u, int i) {
   return __float_as_uint(i & 1 ? v.y : v.x) & 0x7fffffffu;
 }
 
+// Element i of a unit in a block with the scale byte e, as a byte.
+template <typename T>
+__device__ __forceinline__ uint32_t int8_block_byte(const Unit<T>& u, int i, uint32_t e) {
+  const float2 x = f2_split(unit_pair(u, i >> 1));
+  const float m = __uint_as_float((254u - min(e, 254u)) << 23);
+  const float t = clamp127((i & 1 ? x.y : x.x) * m) + kRoundMagic;
+  return e == 0xffu ? 0u : __float_as_uint(t) & 0xffu;
+}
+
 }  // namespace dmad

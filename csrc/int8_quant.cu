@@ -87,10 +87,7 @@ __global__ void __launch_bounds__(512, sizeof(T) == 4 || UPT > 2 ? 1 : 2) int8_q
               const int j = 4 * q + h;
               const uint32_t e = int8_block_code(__reduce_max_sync(0xffffffffu, abs_bits(v[i], j)));
               if (lane == j) mine = e;
-              const float2 x = f2_split(unit_pair(v[i], j >> 1));
-              const float m = __uint_as_float((254u - min(e, 254u)) << 23);
-              const float t = clamp127((j & 1 ? x.y : x.x) * m) + kRoundMagic;
-              if (e != 0xffu) codes[q] |= (__float_as_uint(t) & 0xffu) << (8 * h);
+              codes[q] |= int8_block_byte(v[i], j, e) << (8 * h);
             }
           }
           if (live && lane < 16 && col / kInt8Block + lane < nb) er[col / kInt8Block + lane] = (uint8_t)mine;

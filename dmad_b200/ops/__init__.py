@@ -64,6 +64,7 @@ from .norm import ln_mod, gate_residual, qk_norm_rope, rope, rope_apply, rms_nor
 from .activation import gelu_tanh  # noqa: E402
 from .fp4 import Fp4Tensor, quantize_fp4, dequantize_fp4, fp4_linear  # noqa: E402
 from .int8 import Int8Tensor, quantize_int8, dequantize_int8, int8_linear  # noqa: E402
+from .act8 import linear_act8  # noqa: E402
 from .head_norm import qk_head_norm_rope  # noqa: E402
 from .temb import sinusoidal_embedding, small_linear  # noqa: E402
 
@@ -92,6 +93,7 @@ __all__ = [
     "quantize_int8",
     "dequantize_int8",
     "int8_linear",
+    "linear_act8",
     "qk_head_norm_rope",
     "sinusoidal_embedding",
     "small_linear",
