@@ -72,10 +72,14 @@ def main(argv=None):
     ap.add_argument("--fused-qk-norm", action="store_true", help="q / k norms and RoPE as one kernel")
     ap.add_argument("--weights-fp4", choices=["nvfp4", "mxfp4"], default=None,
                     help="4-bit projections (resident or cp mode); not the headline's precision")
+    ap.add_argument("--linear-int8", action="store_true",
+                    help="8-bit integer projections (resident or cp mode); not the headline's precision")
     ap.add_argument("--cp-impl", default="fused", choices=["fused", "nccl"])
     a = ap.parse_args(argv)
-    if a.mode == "lowvram" and (a.weights_fp4 or a.fused_qk_norm):
-        ap.error("--weights-fp4 and --fused-qk-norm run with resident weights")
+    if a.mode == "lowvram" and (a.weights_fp4 or a.linear_int8 or a.fused_qk_norm):
+        ap.error("--weights-fp4, --linear-int8 and --fused-qk-norm run with resident weights")
+    if a.weights_fp4 and a.linear_int8:
+        ap.error("--weights-fp4 and --linear-int8 exclude each other")
     from dmad_b200.inference.h3 import build_row_timesteps, rollout
     from dmad_b200.models.h3 import H3Config, H3Model
 
@@ -147,6 +151,9 @@ def main(argv=None):
         if a.weights_fp4:
             model.quantize_fp4_(a.weights_fp4)
             torch.cuda.empty_cache()
+        if a.linear_int8:
+            model.quantize_int8_()
+            torch.cuda.empty_cache()
     build_s = time.time() - t_build
 
     results = []
@@ -184,7 +191,7 @@ def main(argv=None):
            "gpus": cp.world if cp is not None else 1, "build_s": round(build_s, 1),
            "config": {"model": f"H3-shaped DiT, {cfg.num_layers} blocks, hidden {cfg.dim}, ffn {cfg.ffn_dim}",
                       "video": f"{a.num_frames} frames at {a.height}x{a.width}", "text_tokens": a.text_tokens,
-                      "dtype": a.weights_fp4 or "bf16", "weights": "random init"},
+                      "dtype": a.weights_fp4 or ("int8" if a.linear_int8 else "bf16"), "weights": "random init"},
            "reference_published": {"s_per_evaluation_h200": 9.0, "s_per_video_4step_h200": 37.0,
                                    "lowvram_peak_sampling_gib": 5.9}}
     if streamed is not None:

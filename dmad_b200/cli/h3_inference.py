@@ -56,8 +56,10 @@ def parse_args(argv=None):
                    help="row-chunked blocks: at most this many rows of every intermediate except k / v")
     p.add_argument("--weights-fp4", choices=["nvfp4", "mxfp4"], default=None,
                    help="resident 4-bit weights and activations of the blocks' projections (LoRA folded in first)")
+    p.add_argument("--linear-int8", action="store_true",
+                   help="resident 8-bit integer weights and activations of the blocks' projections (LoRA folded in first)")
     p.add_argument("--fused-qk-norm", action="store_true",
-                   help="q / k norms and RoPE in one pass (last-bit differences; implied by --weights-fp4)")
+                   help="q / k norms and RoPE in one pass (last-bit differences; implied by --weights-fp4 and --linear-int8)")
     p.add_argument("--offload", action="store_true", help="same as --low-vram auto")
     # the H3 video / audio VAEs are Diffusers modules that this package does not rebuild; latents are
     # written instead of decoded video, and these two flags only keep reference command lines parsing
@@ -70,8 +72,10 @@ def parse_args(argv=None):
                         "(for head counts the CP size does not divide)")
     p.add_argument("--ulysses-size", type=int, default=None)
     a = p.parse_args(argv)
-    if (a.weights_fp4 or a.fused_qk_norm) and (a.low_vram or a.offload):
-        p.error("--weights-fp4 and --fused-qk-norm run with resident weights: they exclude --low-vram / --offload")
+    if (a.weights_fp4 or a.linear_int8 or a.fused_qk_norm) and (a.low_vram or a.offload):
+        p.error("--weights-fp4, --linear-int8 and --fused-qk-norm run with resident weights: they exclude --low-vram / --offload")
+    if a.weights_fp4 and a.linear_int8:
+        p.error("--weights-fp4 and --linear-int8 exclude each other")
     return a
 
 
@@ -201,6 +205,9 @@ def main(argv=None):
         if args.weights_fp4:
             n = model.quantize_fp4_(args.weights_fp4)
             log(f"{n} projections quantised to {args.weights_fp4}")
+            peak("quantisation")
+        if args.linear_int8:
+            log(f"{model.quantize_int8_()} projections quantised to int8")
             peak("quantisation")
         if cp is not None:
             model.enable_context_parallel(cp)

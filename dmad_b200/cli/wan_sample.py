@@ -56,8 +56,13 @@ def parse(argv=None):
     p.add_argument("--cp_size", type=int, default=1)
     p.add_argument("--weights_fp4", choices=["nvfp4", "mxfp4"], default=None,
                    help="4-bit weights and activations of the blocks' projections")
+    p.add_argument("--linear_int8", action="store_true",
+                   help="8-bit integer weights and activations of the blocks' projections")
     p.add_argument("--tiny", action="store_true", help="tiny random model and shapes (smoke tests)")
-    return p.parse_args(argv)
+    a = p.parse_args(argv)
+    if a.weights_fp4 and a.linear_int8:
+        p.error("--weights_fp4 and --linear_int8 exclude each other")
+    return a
 
 
 def load_prompts(a) -> list[str]:
@@ -131,6 +136,9 @@ def main(argv=None):
     if a.weights_fp4:
         from ..models.layers import quantize_fp4_
         quantize_fp4_(net.blocks, a.weights_fp4)
+    if a.linear_int8:
+        from ..models.layers import quantize_int8_
+        quantize_int8_(net.blocks)
     if a.cp_size > 1:
         from ..parallel.cp import ContextParallel
         from ..train.trainer import make_cp_group

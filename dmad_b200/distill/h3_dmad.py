@@ -63,6 +63,8 @@ class H3DMADConfig:
     head_lr: float = 4e-5
     head_wd: float = 0.01
     gradient_checkpointing: bool = True
+    checkpoint_policy: str = "block_wise"  # "mm_only": keep matmul / attention outputs; "block_int8": block inputs in 8 bits
+    act8: bool = False                # without checkpointing: linear layers without LoRA keep their inputs in 8 bits
     fused_qk_norm: bool = False       # q / k norms and RoPE as one kernel, forward and backward
     text_tokens: int = 256
     model_dir: str | None = None      # H3 release folder: transformer/config.json sets ``model``, shards load
@@ -124,6 +126,8 @@ class H3DMAD:
             from ..inference.h3 import load_transformer_weights
             load_transformer_weights(base, cfg.model_dir)
         base.enable_fused_qk_norm(cfg.fused_qk_norm)
+        base.enable_act8(cfg.act8)
+        base.checkpoint_policy = cfg.checkpoint_policy
         self.student = base
         self.fake = copy.deepcopy(base)
         self.student.enable_lora(cfg.student_lora_rank)

@@ -71,8 +71,11 @@ class WanDMADConfig:
     checkpoint_student_blocks: int = 0
     checkpoint_critic_blocks: int = 0
     checkpoint_critic_blocks_student_phase: int | None = None
-    checkpoint_student_policy: str = "block_wise"  # "mm_only": keep matmul / attention outputs
+    # "mm_only": keep matmul / attention outputs; "block_int8": block inputs in 8 bits
+    checkpoint_student_policy: str = "block_wise"
     checkpoint_critic_policy: str = "block_wise"
+    # linear layers of the blocks that are not checkpointed keep their inputs in 8 bits (those with LoRA: as they are)
+    act8: bool = False
     rectified_flow_t_scaling_factor: float = 1000.0
     # rCM consistency term (0 = pure DMAD, as the reference's DMAD experiments; > 0 adds the sCM /
     # dCM loss of the rCM recipe in the student phase, which needs the teacher network)
@@ -155,6 +158,8 @@ class WanDMAD(nn.Module):
         self.net_fake_score.checkpoint_blocks = cfg.checkpoint_critic_blocks
         self.net.checkpoint_policy = cfg.checkpoint_student_policy
         self.net_fake_score.checkpoint_policy = cfg.checkpoint_critic_policy
+        self.net.enable_act8(cfg.act8)
+        self.net_fake_score.enable_act8(cfg.act8)
         broadcast_module(self.net)
         broadcast_module(self.net_fake_score)
         broadcast_module(self.critic_heads)

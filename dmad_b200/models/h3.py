@@ -32,7 +32,8 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..ops import attention as attn_ops
-from .layers import SegLinear, head_attention_core, install_segment_key_remap, quantize_fp4_
+from .layers import (SegLinear, enable_act8, head_attention_core, install_segment_key_remap, quantize_fp4_,
+                     quantize_int8_)
 from .sac import checkpoint_block
 
 
@@ -135,9 +136,7 @@ class _SwiGLU(nn.Module):
         self.ffn_dim = ffn_dim
 
     def forward(self, x):
-        h = getattr(self.net, "0").proj(x)
-        value, gate = h[:, : self.ffn_dim], h[:, self.ffn_dim:]
-        return getattr(self.net, "2")(value * F.silu(gate))
+        return getattr(self.net, "2")(getattr(self.net, "0").proj(x), act="swiglu")
 
 
 class H3Block(nn.Module):
@@ -198,7 +197,7 @@ class H3Model(nn.Module):
         self.proj_out = nn.Linear(D, cfg.in_channels * math.prod(cfg.patch_size))
         self.audio_proj_out = nn.Linear(D, cfg.audio_in_channels)
         self.checkpoint_blocks = 0
-        self.checkpoint_policy = "block_wise"  # or "mm_only" (keep matmul / attention outputs)
+        self.checkpoint_policy = "block_wise"  # "mm_only" (keep matmul / attention outputs), "block_int8" (inputs in 8 bits)
         self._rope_cache = {}
         self.cp = None  # parallel.cp.ContextParallel: shard the packed sequence over a CP group
         self.init_weights()
@@ -311,6 +310,17 @@ class H3Model(nn.Module):
         parameters a block; adaLN projections, embeddings and heads stay) in place, with the fused q / k norm."""
         self.enable_fused_qk_norm()
         return quantize_fp4_(self.token_refiner, fmt) + quantize_fp4_(self.transformer_blocks, fmt)
+
+    def quantize_int8_(self) -> int:
+        """8-bit integer inference of the same projections (a scale for each token and each output channel), in place, with
+        the fused q / k norm."""
+        self.enable_fused_qk_norm()
+        return quantize_int8_(self.token_refiner) + quantize_int8_(self.transformer_blocks)
+
+    def enable_act8(self, on: bool = True) -> int:
+        """The blocks' projections keep their inputs (the SwiGLU's: its value and gate) in 8 bits for the backward pass;
+        those with a LoRA adapter keep them as they are."""
+        return enable_act8(self.transformer_blocks, on)
 
     def lora_linears(self, targets=("to_q", "to_k", "to_v", "to_out.0", "ff.net.0.proj", "ff.net.2")):
         out = []

@@ -13,7 +13,9 @@
         train/image/main/edm/edm_guidance.py:54-80);
       * a rank-r LoRA adapter ``W x + (alpha/r) B A x`` in the Diffusers/PEFT
         layout (dmad_h3/lora.py:23-75).
-    ``quantize_fp4_`` turns the layer into a 4-bit inference layer (``ops.fp4_linear``).
+    ``quantize_fp4_`` turns the layer into a 4-bit inference layer (``ops.fp4_linear``), ``quantize_int8_`` into one of
+    8-bit integers (``ops.int8_linear``).  ``act8`` makes a trained layer keep its input in 8 bits for the backward pass
+    (``ops.linear_act8``; layers with a LoRA adapter keep it as it is).
 ``SelfAttnCore`` / ``CrossAttnCore``
     autograd functions that run q/k RMSNorm (+3D RoPE) and flash attention on
     the sm_100a kernels and produce the fused ``dqkv`` gradient directly.
@@ -76,6 +78,8 @@ class SegLinear(nn.Module):
         self.lora_rank = 0
         self.lora_scale = 0.0
         self.fp4 = None  # an ops.Fp4Tensor once quantize_fp4_ has replaced the weight
+        self.int8 = None  # an ops.Int8Tensor once quantize_int8_ has
+        self.act8 = False
         nn.init.xavier_uniform_(self.weight)
 
     # ------------------------------------------------------------------ segments
@@ -171,6 +175,8 @@ class SegLinear(nn.Module):
     def effective_weight(self):
         if self.fp4 is not None:
             return ops.dequantize_fp4(self.fp4, self._fp4_dtype)
+        if self.int8 is not None:
+            return ops.dequantize_int8(self.int8, self._fp4_dtype)
         if not self.sn_enabled:
             return self.weight
         if (self.weight.is_cuda and self.weight.dtype == torch.bfloat16 and self.in_features % 8 == 0
@@ -244,17 +250,31 @@ class SegLinear(nn.Module):
     def lora_delta_weight(self):
         return self.lora_scale * (self.lora_B * self.lora_mask) @ self.lora_A
 
-    # ------------------------------------------------------------------ 4-bit inference
+    # ------------------------------------------------------------------ 4-bit and 8-bit inference
     @torch.no_grad()
     def quantize_fp4_(self, fmt: str = "nvfp4"):
         """Replaces the weight (spectral norm and LoRA folded in) by its 4-bit form, for inference: ``forward``
         quantises its input and multiplies in 4 bits.  The layer can no longer be trained or saved."""
-        self._refuse_fp4("quantize_fp4_")
+        self.fp4 = ops.quantize_fp4(self._folded("quantize_fp4_"), fmt)
+        return self._drop_weight()
+
+    @torch.no_grad()
+    def quantize_int8_(self):
+        """Replaces the weight (spectral norm and LoRA folded in) by 8-bit integers with a scale for each output row, for
+        inference: ``forward`` codes its input with a scale for each token and multiplies the integers.  The layer can no
+        longer be trained or saved."""
+        self.int8 = ops.quantize_int8(self._folded("quantize_int8_"))
+        return self._drop_weight()
+
+    def _folded(self, what):
+        self._refuse_fp4(what)
         w = self.effective_weight()
         if self.lora_rank:
             w = w + self.lora_delta_weight().to(w.dtype)
-        self._fp4_dtype = w.dtype if w.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
-        self.fp4 = ops.quantize_fp4(w.detach(), fmt)
+        self._fp4_dtype = w.dtype if w.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16  # what the layer computes in
+        return w.detach()
+
+    def _drop_weight(self):
         self.weight = None
         if self.lora_rank:
             self.lora_A = self.lora_B = self.lora_mask = None
@@ -266,12 +286,17 @@ class SegLinear(nn.Module):
 
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
-        if self.fp4 is not None:  # devices follow the module; the stored numbers keep their types
+        # devices follow the module; the stored numbers keep their types
+        as_is = lambda t: None if t is None else fn(t.view(torch.int32)).view(torch.float32)
+        if self.fp4 is not None:
             q = self.fp4
-            rs = None if q.row_scale is None else fn(q.row_scale.view(torch.int32)).view(torch.float32)
-            self.fp4 = ops.Fp4Tensor(fn(q.data), fn(q.scales), rs, q.fmt, q.shape)
+            self.fp4 = ops.Fp4Tensor(fn(q.data), fn(q.scales), as_is(q.row_scale), q.fmt, q.shape)
+        if self.int8 is not None:
+            q = self.int8
+            self.int8 = ops.Int8Tensor(fn(q.data), as_is(q.scale), q.block, q.shape)
+        if self.fp4 is not None or self.int8 is not None:
             # what the layer computes in follows a conversion to another 16-bit type, as its bias and the other layers do
-            kind = fn(torch.empty(0, dtype=self._fp4_dtype, device=q.device)).dtype
+            kind = fn(torch.empty(0, dtype=self._fp4_dtype, device=(self.fp4 or self.int8).device)).dtype
             if kind in (torch.bfloat16, torch.float16):
                 self._fp4_dtype = kind
         return self
@@ -279,9 +304,14 @@ class SegLinear(nn.Module):
     def _refuse_fp4(self, what):
         if self.fp4 is not None:
             raise RuntimeError(f"{what}: the layer's weight has been replaced by its 4-bit form (quantize_fp4_)")
+        if self.int8 is not None:
+            raise RuntimeError(f"{what}: the layer's weight has been replaced by its 8-bit form (quantize_int8_)")
 
     def _forward_fp4(self, x):
         return ops.fp4_linear(x.to(self._fp4_dtype), self.fp4, self.bias)
+
+    def _forward_int8(self, x):
+        return ops.int8_linear(x.to(self._fp4_dtype), self.int8, self.bias)
 
     # ------------------------------------------------------------------ forward
     def forward_rows(self, x, start: int, stop: int):
@@ -293,6 +323,11 @@ class SegLinear(nn.Module):
             first = start // 128 * 128
             b = None if self.bias is None else self.bias[first:stop]
             return ops.fp4_linear(x.to(self._fp4_dtype), self.fp4.row_slice(first, stop), b)[..., start - first:]
+        if self.int8 is not None:
+            stop = min(stop, self.out_features)
+            start = min(start, stop)
+            b = None if self.bias is None else self.bias[start:stop]
+            return ops.int8_linear(x.to(self._fp4_dtype), self.int8.row_slice(start, stop), b)
         w = self.effective_weight()[start:stop]
         b = None if self.bias is None else self.bias[start:stop]
         if x.dtype != w.dtype:
@@ -305,9 +340,21 @@ class SegLinear(nn.Module):
             return F.linear(x, w, b) + self.lora_scale * F.linear(F.linear(x, self.lora_A), bm)
         return F.linear(x, w, b)
 
-    def forward(self, x):
+    def forward(self, x, act: str | None = None):
+        """The layer on ``act(x)``; ``act`` None, "gelu_tanh" or "swiglu" (``x`` is ``[value | gate]``)."""
+        if act is not None and not self._keeps_act8():
+            if act == "gelu_tanh":
+                x = ops.gelu_tanh(x)
+            elif act == "swiglu":
+                value, gate = x[..., :self.in_features], x[..., self.in_features:]
+                x = value * F.silu(gate)
+            else:
+                raise ValueError(f"act must be None, 'gelu_tanh' or 'swiglu', got {act!r}")
+            act = None
         if self.fp4 is not None:
             return self._forward_fp4(x)
+        if self.int8 is not None:
+            return self._forward_int8(x)
         w = self.effective_weight()
         b = self.bias
         if x.dtype != w.dtype:
@@ -318,7 +365,13 @@ class SegLinear(nn.Module):
                 return lora_linear(x, w, b, self.lora_A, self.lora_B * self.lora_mask, self.lora_scale)
             y = F.linear(x, w, b)
             return y + self.lora_scale * F.linear(F.linear(x, self.lora_A), self.lora_B * self.lora_mask)
+        if self._keeps_act8():
+            return ops.linear_act8(x, w, b, act)
         return F.linear(x, w, b)
+
+    def _keeps_act8(self):
+        """Whether ``forward`` keeps its input in 8 bits: not under ``torch.no_grad``, with an adapter or coded weights."""
+        return self.act8 and not self.lora_rank and self.weight is not None and torch.is_grad_enabled()
 
     # ------------------------------------------------------------------ state dict (per-segment keys)
     def _split_prefix(self, prefix):
@@ -537,6 +590,28 @@ def quantize_fp4_(module: nn.Module, fmt: str = "nvfp4") -> int:
     for m in module.modules():
         if isinstance(m, SegLinear) and m.fp4 is None:
             m.quantize_fp4_(fmt)
+            n += 1
+    return n
+
+
+def quantize_int8_(module: nn.Module) -> int:
+    """``SegLinear.quantize_int8_`` of every ``SegLinear`` of ``module``; returns how many."""
+    n = 0
+    for m in module.modules():
+        if isinstance(m, SegLinear) and m.int8 is None:
+            m.quantize_int8_()
+            n += 1
+    return n
+
+
+def enable_act8(module: nn.Module, on: bool = True) -> int:
+    """Makes every ``SegLinear`` of ``module`` keep its input in 8 bits for the backward pass (``SegLinear.act8``), or the
+    16 bits that it was given; returns how many.  For blocks that are not recomputed: one under activation checkpointing
+    keeps nothing anyway."""
+    n = 0
+    for m in module.modules():
+        if isinstance(m, SegLinear):
+            m.act8 = bool(on)
             n += 1
     return n
 

@@ -24,7 +24,7 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..ops import norm as norm_ops
-from .layers import SegLinear, cross_attention_core, install_segment_key_remap, self_attention_core
+from .layers import SegLinear, cross_attention_core, enable_act8, install_segment_key_remap, self_attention_core
 from .sac import checkpoint_block
 
 
@@ -161,8 +161,7 @@ class WanBlock(nn.Module):
                                  cfg.eps)
         x = x + self.cross_attn.o(c)
         h2 = ops.ln_mod(x, e[:, 4], e[:, 3], a_add=1.0, eps=cfg.eps, **grp)
-        f = ops.gelu_tanh(getattr(self.ffn, "0")(h2))
-        y2 = getattr(self.ffn, "2")(f)
+        y2 = getattr(self.ffn, "2")(getattr(self.ffn, "0")(h2), act="gelu_tanh")
         return ops.gate_residual(x, y2, e[:, 5], **grp)
 
 
@@ -230,7 +229,7 @@ class WanModel(nn.Module):
         self.blocks = nn.ModuleList([WanBlock(cfg) for _ in range(cfg.num_layers)])
         self.head = _Head(cfg)
         self.checkpoint_blocks = 0  # activation-checkpoint the first N blocks
-        self.checkpoint_policy = "block_wise"  # or "mm_only" (keep matmul / attention outputs)
+        self.checkpoint_policy = "block_wise"  # "mm_only" (keep matmul / attention outputs), "block_int8" (inputs in 8 bits)
         self._rope_cache: dict = {}
         self.cp = None  # ContextParallel (sequence sharding) or None
         self.init_weights()
@@ -375,6 +374,11 @@ class WanModel(nn.Module):
         """Shard the token sequence over ``cp`` (a ``parallel.cp.ContextParallel``); None disables.
         Features returned for the critic are this rank's token slice (pool with ``cp.all_reduce_sum``)."""
         self.cp = cp
+
+    def enable_act8(self, on: bool = True) -> int:
+        """The blocks' linear layers keep their inputs (the feed-forward's: what the GELU reads) in 8 bits for the backward
+        pass; those with a LoRA adapter keep them as they are."""
+        return enable_act8(self.blocks, on)
 
     # --------------------------------------------------------------- utilities
     def seg_linears(self):
