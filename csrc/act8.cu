@@ -109,6 +109,7 @@ template <typename T, int ACT, bool ALIGNED>
 __global__ void __launch_bounds__(256) act_encode_kernel(EncodeParams p) {
   constexpr bool FP16 = std::is_same_v<T, __half>;
   constexpr int H = ACT == kActSwiglu ? 2 : 1;
+  launch_dependents();
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= p.R) return;  // whole warps
   const int lane = threadIdx.x & 31;
@@ -166,6 +167,7 @@ __global__ void __launch_bounds__(256) act_encode_kernel(EncodeParams p) {
 template <bool FP16, int ACT>
 __global__ void __launch_bounds__(256) act_decode_kernel(Kept kept, uint16_t* a, int64_t lda, int R, int F) {
   constexpr int H = ACT == kActSwiglu ? 2 : 1;
+  launch_dependents();
   const int row_bytes = (int)int8_row_bytes(F), nb = row_bytes / kInt8Block;
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= R) return;
@@ -239,49 +241,6 @@ struct BiasEpilogue {
     if (at.lane == 0) tma_store_wait_read();
     __syncwarp();
     store_rows(a.out, &a.map, at.stage, m0, nc, o);
-  }
-  __device__ __forceinline__ void done() {
-    if (at.lane == 0) tma_store_wait_read();
-  }
-};
-
-// fp32 parts [split, M, N] of tiles whose K steps several pairs share, in boxes of 32 x 32 (128-byte swizzle).
-struct PartEpilogue {
-  static constexpr int kStages = 5, kOutBytes = 4096;
-  static constexpr bool kShared = false;
-  struct Args {
-    CUtensorMap map;
-  };
-  const Args& a;
-  const PairGemm& p;
-  const EpiPlace at;
-  int m0, n0, part;
-
-  __device__ __forceinline__ PartEpilogue(const Args& a, const PairGemm& p, const EpiPlace& at) : a(a), p(p), at(at) {}
-  __device__ __forceinline__ void first(int) {}
-  __device__ __forceinline__ void begin(int item, int, int) {
-    int tm, tn;
-    p.tile(item, tm, tn);
-    m0 = tm * kPairM + (int)at.rank * kPairHalf + at.wq * 32;
-    n0 = tn * kPairN;
-    part = item % p.split;
-  }
-  __device__ __forceinline__ void met(int) {}
-  __device__ __forceinline__ void chunk(int, int c, const uint32_t (&v)[32]) {
-    const int nc = n0 + c * 32;
-    if (nc >= p.N || m0 >= p.M) return;
-    if (at.lane == 0) tma_store_wait_read();
-    __syncwarp();
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      *reinterpret_cast<uint4*>(at.stage + at.lane * 128 + ((q ^ (at.lane & 7)) << 4)) =
-          make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (at.lane == 0) tma_store_3d(&a.map, at.stage, nc, m0, part);
-  }
-  __device__ __forceinline__ void done() {
-    if (at.lane == 0) tma_store_wait_read();
   }
 };
 
@@ -373,16 +332,12 @@ struct ActGradEpilogue {
     for (int h = 0; h < H; ++h) store_rows(a.dx[h], &a.map_dx[h], at.stage + 2048 * h, m0, nc, od[h]);
     if (a.want_act) store_rows(a.act, &a.map_a, at.stage + 2048 * H, m0, nc, oa);
   }
-  __device__ __forceinline__ void done() {
-    if (at.lane == 0) tma_store_wait_read();
-  }
 };
 
 // ---------------------------------------------------------------- sums of parts
 struct PartSum {
-  const float* parts;  // [split, M, ldp]
-  int split, M, N;
-  int64_t ldp;
+  const float* parts;
+  PairGemm g;
   OutRows out[2];      // the result, or dx (of a SwiGLU: its halves)
   FloatRow bias;
   OutRows act;         // act(x'), if wanted
@@ -390,30 +345,18 @@ struct PartSum {
   Kept kept;
 };
 
-template <bool FP16>
-__device__ __forceinline__ void store4(const OutRows& o, int m, int n, const float (&v)[4]) {
-  uint16_t* d = o.d + (int64_t)m * o.ld + n;
-  const uint32_t lo = pack16<FP16>(v[0], v[1]), hi = pack16<FP16>(v[2], v[3]);
-  if (o.tma && n + 4 <= o.N) {
-    *reinterpret_cast<uint2*>(d) = make_uint2(lo, hi);
-  } else {
-    d[0] = (uint16_t)lo;
-    if (n + 1 < o.N) d[1] = (uint16_t)(lo >> 16);
-    if (n + 2 < o.N) d[2] = (uint16_t)hi;
-    if (n + 3 < o.N) d[3] = (uint16_t)(hi >> 16);
-  }
-}
-
 // Four columns a thread: the parts added in order, then what the epilogue of an undivided tile does.
 template <bool FP16, int ACT>
-__global__ void __launch_bounds__(256) part_sum_kernel(const __grid_constant__ PartSum p) {
+__global__ void __launch_bounds__(kPartThreads) part_sum_kernel(const __grid_constant__ PartSum p) {
   constexpr int H = ACT == kActSwiglu ? 2 : 1;
-  const int n = (blockIdx.x * blockDim.x + threadIdx.x) * 4, m = blockIdx.y * blockDim.y + threadIdx.y;
-  if (n >= p.N || m >= p.M) return;
-  const float* at = p.parts + (int64_t)m * p.ldp + n;
-  float4 sum = __ldg(reinterpret_cast<const float4*>(at));
-  for (int s = 1; s < p.split; ++s) {
-    const float4 f = __ldg(reinterpret_cast<const float4*>(at + (int64_t)s * p.M * p.ldp));
+  launch_dependents();
+  wait_for_previous_grid();
+  int m, n;
+  int64_t at;
+  if (!part_place(p.g, m, n, at)) return;
+  float4 sum = *reinterpret_cast<const float4*>(p.parts + at);
+  for (int s = 1; s < p.g.split; ++s) {
+    const float4 f = *reinterpret_cast<const float4*>(p.parts + at + s * kPartStep);
     sum.x += f.x;
     sum.y += f.y;
     sum.z += f.z;
@@ -422,10 +365,10 @@ __global__ void __launch_bounds__(256) part_sum_kernel(const __grid_constant__ P
   float v[4] = {sum.x, sum.y, sum.z, sum.w};
   if constexpr (ACT == kActNone) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += p.bias.at(min(n + i, p.N - 1));
+    for (int i = 0; i < 4; ++i) v[i] += p.bias.at(min(n + i, p.g.N - 1));
     store4<FP16>(p.out[0], m, n, v);
   } else {
-    const int row_bytes = (int)int8_row_bytes(p.N), nb = row_bytes / kInt8Block;
+    const int row_bytes = (int)int8_row_bytes(p.g.N), nb = row_bytes / kInt8Block;
     float x[H][4];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
@@ -450,6 +393,7 @@ __global__ void __launch_bounds__(256) part_sum_kernel(const __grid_constant__ P
 template <bool FP16>
 __global__ void __launch_bounds__(256) column_sum_kernel(const uint16_t* g, int64_t ld, int R, int N, int per, void* out, int type) {
   __shared__ float red[8][256];
+  launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockIdx.x * 256 + lane * 8;
   const int r0 = blockIdx.y * per, r1 = min(R, r0 + per);
   float s[8] = {};
@@ -488,6 +432,8 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const uint16_t* g, int6
 }
 
 __global__ void __launch_bounds__(256) slice_sum_kernel(const float* parts, int slices, int N, void* out, int type) {
+  launch_dependents();
+  wait_for_previous_grid();
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= N) return;
   float t = 0.f;
@@ -513,10 +459,9 @@ at::Tensor column_sum(const at::Tensor& g, at::ScalarType type, cudaStream_t str
   else
     column_sum_kernel<false><<<dim3(nb, slices), 256, 0, stream>>>(gp, g.stride(0), R, N, per, to, first);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  if (slices > 1) {
-    slice_sum_kernel<<<nb, 256, 0, stream>>>(parts.data_ptr<float>(), slices, N, out.data_ptr(), type_index(type));
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-  }
+  if (slices > 1)
+    launch_overlapping(slice_sum_kernel, dim3(nb), dim3(256), 0, stream, true, (const float*)parts.data_ptr<float>(), slices, N,
+                       out.data_ptr(), type_index(type));
   return out;
 }
 
@@ -530,14 +475,6 @@ at::Tensor tma_rows(const at::Tensor& t) {
   return p;
 }
 
-// Items for each tile along K: where the tiles leave half of the pairs or more without work, as many as fill them, of four
-// stages at least.
-int split_of(int64_t M, int64_t N, int64_t K, int device) {
-  const int64_t tiles = ((M + kPairM - 1) / kPairM) * ((N + kPairN - 1) / kPairN), pairs = sm_count(device) / 2;
-  const int64_t stages = (K + 63) / 64;
-  return tiles * 2 > pairs ? 1 : (int)std::max<int64_t>(1, std::min(pairs / tiles, stages / 4));
-}
-
 struct Operand {  // [rows, K], or stored [K, rows]
   const at::Tensor& t;
   bool mn;
@@ -546,7 +483,7 @@ struct Operand {  // [rows, K], or stored [K, rows]
   CUtensorMap map() const { return operand_map(t.data_ptr(), rows(), K(), t.stride(0), 2, mn); }
 };
 
-// What becomes of the product: out = acc + bias, or (act) out = acc act'(x') and act(x').
+// What becomes of the product (early: as PairGemm has it): out = acc + bias, or (act) out = acc act'(x') and act(x').
 struct Result {
   OutRows out[2];
   FloatRow bias{nullptr, 0};
@@ -554,34 +491,21 @@ struct Result {
   Kept kept{nullptr, nullptr};
   OutRows value{};
   bool want_value = false;
+  int early = 0;
 };
 
 template <bool FP16, int ACT>
 void product_typed(const Operand& A, const Operand& B, const Result& r, int device, cudaStream_t stream) {
   constexpr Mma KIND = FP16 ? Mma::kF16 : Mma::kBf16;
   const int64_t M = A.rows(), N = B.rows(), K = A.K();
-  const PairGemm p = pair_gemm(M, N, K, 2, A.mn, B.mn, split_of(M, N, K, device), device);
+  PairGemm p = pair_gemm(M, N, K, 2, A.mn, B.mn, device);
+  p.early = r.early;
+  const at::Tensor parts = part_memory(p, A.t.options());
   const CUtensorMap ma = A.map(), mb = B.map();
   auto map_of = [&](const OutRows& o) { return o.tma && o.d != nullptr ? out_rows_map(o) : ma; };
-  if (p.split > 1) {
-    const int64_t ldp = (N + 3) / 4 * 4;
-    at::Tensor parts = at::empty({p.split, M, ldp}, A.t.options().dtype(at::kFloat).requires_grad(false));
-    const uint64_t dims[3] = {(uint64_t)N, (uint64_t)M, (uint64_t)p.split};
-    const uint64_t strides[2] = {(uint64_t)ldp * 4, (uint64_t)(M * ldp) * 4};
-    const uint32_t box[3] = {32u, 32u, 1u};
-    const PartEpilogue::Args args{make_tmap(CU_TENSOR_MAP_DATA_TYPE_FLOAT32, parts.data_ptr(), 3, dims, strides, box,
-                                            CU_TENSOR_MAP_SWIZZLE_128B)};
-    launch_pair_gemm<KIND, PartEpilogue>(ma, mb, args, p, device, stream);
-    const PartSum s{parts.data_ptr<float>(), p.split, (int)M, (int)N, ldp, {r.out[0], r.out[1]}, r.bias, r.value,
-                    r.want_value, r.kept};
-    const int tx = N > 128 ? 64 : 32, ty = 256 / tx;
-    DMAD_VALUE_CHECK((M + ty - 1) / ty <= 65535, "linear_act8: too many rows");  // (split tiles are few)
-    part_sum_kernel<FP16, ACT><<<dim3((unsigned)((N + 4 * tx - 1) / (4 * tx)), (unsigned)((M + ty - 1) / ty)), dim3(tx, ty), 0,
-                                 stream>>>(s);
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-  } else if constexpr (ACT == kActNone) {
+  if constexpr (ACT == kActNone) {
     const typename BiasEpilogue<FP16>::Args args{map_of(r.out[0]), r.out[0], r.bias};
-    launch_pair_gemm<KIND, BiasEpilogue<FP16>>(ma, mb, args, p, device, stream);
+    launch_pair_gemm<KIND, BiasEpilogue<FP16>>(ma, mb, parts, args, p, device, stream);
   } else {
     typename ActGradEpilogue<FP16, ACT>::Args args;
     for (int h = 0; h < ActGradEpilogue<FP16, ACT>::H; ++h) {
@@ -592,8 +516,12 @@ void product_typed(const Operand& A, const Operand& B, const Result& r, int devi
     args.act = r.value;
     args.want_act = r.want_value;
     args.kept = r.kept;
-    launch_pair_gemm<KIND, ActGradEpilogue<FP16, ACT>>(ma, mb, args, p, device, stream);
+    launch_pair_gemm<KIND, ActGradEpilogue<FP16, ACT>>(ma, mb, parts, args, p, device, stream);
   }
+  if (p.split > 1)
+    launch_overlapping(part_sum_kernel<FP16, ACT>, part_grid(p), dim3(kPartThreads), 0, stream, true,
+                       PartSum{reinterpret_cast<const float*>(parts.data_ptr()), p, {r.out[0], r.out[1]}, r.bias, r.value,
+                               r.want_value, r.kept});
 }
 
 void product(const Operand& A, const Operand& B, const Result& r, cudaStream_t stream) {
@@ -688,6 +616,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_forward(const at::Tensor& x,
   DMAD_VALUE_CHECK(R * H <= INT32_MAX - 256, "linear_act8: too many rows");
   const auto plain = x.options().requires_grad(false);
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  const auto b = bias.has_value() && bias->defined() ? c10::optional<at::Tensor>(bias->contiguous()) : c10::nullopt;
   at::Tensor data, exponents;
   Kept kept{nullptr, nullptr};
   if (keep) {
@@ -695,22 +624,24 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_forward(const at::Tensor& x,
     exponents = at::empty({R * H, (F + kInt8Block - 1) / kInt8Block}, plain.dtype(at::kByte));
     kept = kept_of(data, exponents);
   }
+  // copies before the pass over x, so that the product may overlap that pass without reading anything younger
+  const bool some = R > 0 && N > 0;
+  const at::Tensor wt = some ? tma_rows(w) : w;
   at::Tensor a;
   if (act == kActNone) {
+    if (some) a = tma_rows(x2);
     if (keep) int8_quantize_launch(x2, Int8Matrix{kept.data, nullptr, kept.exponents, R, F}, stream);
-    a = tma_rows(x2);
   } else {
     a = encode(x2, F, act, kept, stream);
   }
   c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = N;
   at::Tensor y = at::empty(shape, plain);
-  if (R > 0 && N > 0) {
-    const at::Tensor wt = tma_rows(w);
-    const auto b = bias.has_value() && bias->defined() ? c10::optional<at::Tensor>(bias->contiguous()) : c10::nullopt;
+  if (some) {
     Result r;
     r.out[0] = out_rows(y.data_ptr(), N, R, N);
     r.bias = float_row(b);
+    r.early = act != kActNone ? 1 : keep ? 2 : 0;
     product(Operand{a, false}, Operand{wt, false}, r, stream);
   }
   return {y, data, exponents};
@@ -732,12 +663,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_backward(const at::Tensor& g
     if (want_b) db = at::zeros({N}, plain.dtype(bias_type));
     return {dx, dw, db};
   }
+  // Copies, then the passes that only read them and the codes, then the products, each overlapping the end of the kernel
+  // before it: the first one reads nothing that those passes write (early 2) or, for want_w, what the one before did.
   const at::Tensor gt = tma_rows(g.dim() == 2 ? g : g.reshape({R, N}));
+  const at::Tensor wt = want_x ? tma_rows(w) : w;
   const Kept kept = data.defined() ? kept_of(data, exponents) : Kept{nullptr, nullptr};
   at::Tensor a;  // act(x')
+  if (want_b) db = column_sum(gt, bias_type, stream);
+  if (want_w && (act == kActNone || !want_x)) a = decode(kept, R, F, act, plain, stream);
   if (want_x) {
-    const at::Tensor wt = tma_rows(w);
     Result r;
+    r.early = want_b || a.defined() ? 2 : 0;
     for (int h = 0; h < H; ++h) r.out[h] = out_rows(static_cast<uint16_t*>(dx.data_ptr()) + h * F, H * F, R, F);
     r.act = (int)act;
     r.kept = kept;
@@ -750,13 +686,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_backward(const at::Tensor& g
     product(Operand{gt, false}, Operand{wt, true}, r, stream);
   }
   if (want_w) {
-    if (!a.defined()) a = decode(kept, R, F, act, plain, stream);
     dw = at::empty({N, F}, plain);
     Result r;
+    r.early = 1;
     r.out[0] = out_rows(dw.data_ptr(), F, N, F);
     product(Operand{gt, true}, Operand{a, true}, r, stream);
   }
-  if (want_b) db = column_sum(gt, bias_type, stream);
   return {dx, dw, db};
 }
 

@@ -11,8 +11,10 @@
 //               in uniform registers
 //   warps 2..9  epilogue of the CTA's 128 rows: two warps a lane quarter, every other 32 columns each
 // The two accumulators take the 512 columns of tensor memory, so that a tile's epilogue runs beside the next one's MMAs.
-// An operand is read K-major ([rows, K]) or, 16-bit types, MN-major ([K, rows]) where it lies.  split > 1: the K steps of
-// a tile are spread over several work items, whose epilogue gets the item's part.
+// An operand is read K-major ([rows, K]) or, 16-bit types, MN-major ([K, rows]) where it lies.
+// Tiles that would leave half of the pairs or more without work (all of them, where they are few; those of the last round
+// else) have their K steps spread over several pairs: these store the accumulators as they are, 256 x 256 numbers an item, and
+// a second kernel adds a tile's parts in order and does what the epilogue does.  (tile_split() says when.)
 // Every mbarrier wait is bounded (2 s), records a status code and makes all roles leave.
 #pragma once
 #include <cuda_runtime.h>
@@ -64,23 +66,26 @@ struct PairGemm {
   int M, N;
   int ksteps;             // stages along K: 128 bytes each
   int k_last;             // MMAs (32 bytes) of the last stage
-  int tiles_m, tiles_n, items;  // work items: tiles x split
-  int split, per_split;   // K steps of an item
+  int tiles_m, tiles_n, items;  // work items: `whole` tiles, then `split` of each other tile
+  int whole, split, per_split;  // per_split: K steps of a part
   int a_mn, b_mn;         // 1: stored [K, rows]
+  int early;              // launched to overlap the kernel before it: 1 reads what that writes, 2 does not (operands and
+                          // epilogue's inputs older); either way results are stored after its end
   int* status;
 
   __device__ __forceinline__ void tile(int item, int& tm, int& tn) const {
     // column-major raster within groups of 8 M-tiles: neighbouring pairs share B tiles in L2
     constexpr int kGroup = 8;
-    const int t = item / split, group = t / (kGroup * tiles_n), first = group * kGroup;
+    const int t = item < whole ? item : whole + (item - whole) / split, group = t / (kGroup * tiles_n), first = group * kGroup;
     const int gm = min(kGroup, tiles_m - first), in = t % (kGroup * tiles_n);
     tm = first + in % gm;
     tn = in / gm;
   }
   __device__ __forceinline__ void steps(int item, int& k0, int& k1) const {
-    k0 = item % split * per_split;
-    k1 = min(ksteps, k0 + per_split);
+    k0 = item < whole ? 0 : (item - whole) % split * per_split;
+    k1 = item < whole ? ksteps : min(ksteps, k0 + per_split);
   }
+  __host__ __device__ __forceinline__ int split_tiles() const { return (items - whole) / split; }
 };
 
 // What an epilogue warp knows of its place.
@@ -122,11 +127,28 @@ __device__ __forceinline__ void load_pair_operand(uint8_t* dst, const CUtensorMa
 //   begin(item, next, parity)   before the tile's accumulator is waited for; next: the item after it, or -1
 //   met(next)                   behind the warps' barrier (kShared)
 //   chunk(i, c, v)              the accumulator's columns 32 c .. 32 c + 31 of the lane's row; i = 0 .. 3
-//   done()                      before the warp leaves
+// (of a part only the calls that the barrier's warps share are made)
+// Columns 32 c .. of the lane's row of a part, through 2 KB of shared memory: twice 16 columns of 32 rows (64-byte swizzle).
+__device__ __forceinline__ void store_part(const CUtensorMap* map, const EpiPlace& at, int part, int c, const uint32_t (&v)[32]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (at.lane == 0) tma_store_wait_read();
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<uint4*>(at.stage + at.lane * 64 + ((q ^ ((at.lane >> 1) & 3)) << 4)) =
+          make_uint4(v[16 * h + 4 * q], v[16 * h + 4 * q + 1], v[16 * h + 4 * q + 2], v[16 * h + 4 * q + 3]);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (at.lane == 0) tma_store_2d(map, at.stage, c * 32 + h * 16, part * kPairM + (int)at.rank * kPairHalf + at.wq * 32);
+  }
+}
+
 template <Mma KIND, class Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairGemmThreads, 1)
 pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                 const __grid_constant__ typename Epi::Args args, const PairGemm p) {
+                 const __grid_constant__ CUtensorMap tm_parts, const __grid_constant__ typename Epi::Args args,
+                 const PairGemm p) {
   constexpr int kStages = Epi::kStages;
   using Smem = PairGemmSmem<kStages, Epi::kOutBytes>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -158,11 +180,13 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     prefetch_tmap(&tm_a);
     prefetch_tmap(&tm_b);
   }
+  launch_dependents();
   tc_fence_before();
   __syncthreads();
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
+  if (p.early == 1 ? warp != 1 : p.early == 2 && warp > 1) wait_for_previous_grid();
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -248,7 +272,8 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     int tl = 0;
     for (int t = pair; t < p.items; t += pairs, ++tl) {
       const int next = t + pairs < p.items ? t + pairs : -1;
-      epi.begin(t, next, tl & 1);
+      const bool part = t >= p.whole;
+      if (Epi::kShared || !part) epi.begin(t, next, tl & 1);
       bool ok = mbar_wait(&sm.acc_full[tl & 1], (tl >> 1) & 1, kStatusTimeoutMma, abort_flag, p.status);
       if constexpr (Epi::kShared) {  // all warps leave together, since the barrier counts them
         if (named_bar_any(1, 32 * kPairEpiWarps, !ok)) break;
@@ -271,10 +296,11 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(freed);
         }
-        epi.chunk(i, 2 * i + place.half, r[i & 1]);
+        if (part) store_part(&tm_parts, place, t - p.whole, 2 * i + place.half, r[i & 1]);
+        else epi.chunk(i, 2 * i + place.half, r[i & 1]);
       }
     }
-    epi.done();
+    if (lane == 0) tma_store_wait_read();
   }
   tc_fence_before();
   __syncthreads();
@@ -340,6 +366,33 @@ __device__ __forceinline__ void store_rows(const OutRows& out, const CUtensorMap
   }
 }
 
+// Row m and first column n of a thread of such a kernel, and where the first part's four numbers are; false past the matrix.
+__device__ __forceinline__ bool part_place(const PairGemm& p, int& m, int& n, int64_t& at) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), col = (threadIdx.x & 63) * 4;
+  int tm, tn;
+  p.tile(p.whole + blockIdx.y * p.split, tm, tn);
+  m = tm * kPairM + row;
+  n = tn * kPairN + col;
+  at = ((int64_t)blockIdx.y * p.split * kPairM + row) * kPairN + col;
+  return m < p.M && n < p.N;
+}
+constexpr int64_t kPartStep = (int64_t)kPairM * kPairN;  // from one part to the next
+
+// Four columns from n of row m of a 16-bit matrix.
+template <bool FP16>
+__device__ __forceinline__ void store4(const OutRows& o, int m, int n, const float (&v)[4]) {
+  uint16_t* d = o.d + (int64_t)m * o.ld + n;
+  const uint32_t lo = pack16<FP16>(v[0], v[1]), hi = pack16<FP16>(v[2], v[3]);
+  if (o.tma && n + 4 <= o.N) {
+    *reinterpret_cast<uint2*>(d) = make_uint2(lo, hi);
+  } else {
+    d[0] = (uint16_t)lo;
+    if (n + 1 < o.N) d[1] = (uint16_t)(lo >> 16);
+    if (n + 2 < o.N) d[2] = (uint16_t)hi;
+    if (n + 3 < o.N) d[3] = (uint16_t)(hi >> 16);
+  }
+}
+
 // A row of numbers of any of three types: 0 fp32, 1 bf16, 2 fp16; none: zeros.
 struct FloatRow {
   const void* p;
@@ -390,7 +443,15 @@ inline CUtensorMap operand_map(const void* base, int64_t rows, int64_t K, int64_
   return bytes == 1 ? make_tmap_u8(base, 2, dims, strides, box) : make_tmap_bf16(base, 2, dims, strides, box);
 }
 
-inline PairGemm pair_gemm(int64_t M, int64_t N, int64_t K, int bytes, bool a_mn, bool b_mn, int split, int device) {
+// Parts of each tile of a round that fills no more than half of the pairs: as many as fill them, of four stages at least.
+// After whole rounds only where that saves twelve stages (some 3 us), for which the parts' kernel is paid.
+inline int tile_split(int64_t tiles, int64_t stages, int pairs, bool only) {
+  if (tiles == 0 || 2 * tiles > pairs) return 1;
+  const int64_t split = std::max<int64_t>(1, std::min(pairs / tiles, stages / 4));
+  return only || stages - stages / split >= 12 ? (int)split : 1;
+}
+
+inline PairGemm pair_gemm(int64_t M, int64_t N, int64_t K, int bytes, bool a_mn, bool b_mn, int device) {
   PairGemm p;
   const int64_t step = 128 / bytes, per_mma = 32 / bytes;
   p.M = (int)M;
@@ -399,12 +460,18 @@ inline PairGemm pair_gemm(int64_t M, int64_t N, int64_t K, int bytes, bool a_mn,
   p.k_last = (int)((K - (int64_t)(p.ksteps - 1) * step + per_mma - 1) / per_mma);
   p.tiles_m = (int)((M + kPairM - 1) / kPairM);
   p.tiles_n = (int)((N + kPairN - 1) / kPairN);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  DMAD_VALUE_CHECK(tiles <= INT32_MAX / 4, "too many output tiles");
+  const int pairs = sm_count(device) / 2;
+  p.whole = (int)(tiles / pairs * pairs);
+  const int split = tile_split(tiles - p.whole, p.ksteps, pairs, p.whole == 0);
   p.per_split = (p.ksteps + split - 1) / split;
-  p.split = (p.ksteps + p.per_split - 1) / p.per_split;  // every item has a step
-  DMAD_VALUE_CHECK((int64_t)p.tiles_m * p.tiles_n * p.split <= INT32_MAX / 2, "too many output tiles");
-  p.items = p.tiles_m * p.tiles_n * p.split;
+  p.split = (p.ksteps + p.per_split - 1) / p.per_split;  // every part has a step
+  if (p.split == 1) p.whole = (int)tiles;
+  p.items = p.whole + (int)(tiles - p.whole) * p.split;
   p.a_mn = a_mn ? 1 : 0;
   p.b_mn = b_mn ? 1 : 0;
+  p.early = 0;
   p.status = device_status_ptr(device);
   return p;
 }
@@ -418,14 +485,48 @@ void raise_smem(int smem, int device) {
   if (device < 64) done[device].store(true, std::memory_order_release);
 }
 
-template <Mma KIND, class Epi>
-void launch_pair_gemm(const CUtensorMap& a, const CUtensorMap& b, const typename Epi::Args& args, const PairGemm& p, int device,
-                      cudaStream_t stream) {
-  constexpr int smem = (int)sizeof(PairGemmSmem<Epi::kStages, Epi::kOutBytes>) + 1024;
-  static_assert(smem <= 232448, "shared memory of an SM");
-  raise_smem<pair_gemm_kernel<KIND, Epi>>(smem, device);
-  pair_gemm_kernel<KIND, Epi><<<2 * std::min(p.items, sm_count(device) / 2), kPairGemmThreads, smem, stream>>>(a, b, args, p);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+// Launch of a kernel that may overlap the end of the one before it (and then waits for it by itself).
+template <class... Params, class... Args>
+void launch_overlapping(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool early,
+                        const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = early ? 1 : 0;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
+
+// Memory for the parts of p's divided tiles (undefined where there are none): [items, 256, 256] 32-bit numbers.
+inline at::Tensor part_memory(const PairGemm& p, const at::TensorOptions& options) {
+  if (p.split == 1) return at::Tensor();
+  return at::empty({(int64_t)(p.items - p.whole) * kPairM, kPairN}, options.dtype(at::kInt).requires_grad(false));
+}
+
+template <Mma KIND, class Epi>
+void launch_pair_gemm(const CUtensorMap& a, const CUtensorMap& b, const at::Tensor& parts, const typename Epi::Args& args,
+                      const PairGemm& p, int device, cudaStream_t stream) {
+  constexpr int smem = (int)sizeof(PairGemmSmem<Epi::kStages, Epi::kOutBytes>) + 1024;
+  static_assert(smem <= 232448 && Epi::kOutBytes >= 2048, "shared memory of an SM, of a part's rows");
+  CUtensorMap mp = a;
+  if (parts.defined()) {
+    const uint64_t dims[2] = {(uint64_t)kPairN, (uint64_t)parts.size(0)};
+    const uint64_t strides[1] = {(uint64_t)kPairN * 4};
+    const uint32_t box[2] = {16u, 32u};
+    mp = make_tmap(CU_TENSOR_MAP_DATA_TYPE_INT32, parts.data_ptr(), 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+  }
+  raise_smem<pair_gemm_kernel<KIND, Epi>>(smem, device);
+  launch_overlapping(pair_gemm_kernel<KIND, Epi>, dim3(2 * std::min(p.items, sm_count(device) / 2)), dim3(kPairGemmThreads), smem,
+                     stream, p.early != 0, a, b, mp, args, p);
+}
+
+// Blocks of a kernel that adds parts, four columns a thread: four rows of a tile each.
+inline dim3 part_grid(const PairGemm& p) { return dim3(kPairM / 4, (unsigned)p.split_tiles()); }
+constexpr int kPartThreads = 256;
 
 }  // namespace dmad

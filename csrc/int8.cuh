@@ -29,6 +29,17 @@ __device__ __forceinline__ uint32_t pack_bytes(uint64_t ab, uint64_t cd) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
+// Scale of a row with the maximum amax (bits of an fp32 number); inv: 1 / s, rounded, and 0 for a row that is not finite.
+__device__ __forceinline__ float int8_row_scale(uint32_t amax, float& inv) {
+  if (amax >= kInfBits) {
+    inv = 0.f;
+    return __uint_as_float(0x7fffffffu);
+  }
+  const float s = amax == 0u ? 1.f : fminf(fmaxf(__fdiv_rn(__uint_as_float(amax), 127.f), kInt8MinScale), kInt8MaxScale);
+  inv = __frcp_rn(s);
+  return s;
+}
+
 // Four signed bytes -> two pairs of floats: the byte plus 128 in the low bits of 2^23, less 2^23 + 128.
 __device__ __forceinline__ void bytes_to_float(uint32_t w, uint64_t& lo, uint64_t& hi) {
   const uint32_t u = w ^ 0x80808080u;

@@ -4,7 +4,8 @@
 //
 // A and B are codes of -127 .. 127 with a scale a row (int8.cuh), multiplied on the tensor core (kind::i8) with exact int32
 // sums (K <= 133144: 2^31 / 127^2), so the only roundings are the epilogue's: the factors, the bias, and one to the result's
-// type.  Two kernels: pairs of CTAs on 256 x 256 tiles (gemm_pair.cuh), and one for few rows (few_rows() says which).
+// type.  Three kernels, by the rows of A: for one, dot products that stream the weight; up to kSmallBN, MMAs whose rows are the
+// weight's; above that, pairs of CTAs on 256 x 256 tiles (gemm_pair.cuh).
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -98,10 +99,175 @@ struct ScaleEpilogue {
     __syncwarp();
     store_rows(a.out, &a.map, at.stage, m0, nc, o);
   }
-  __device__ __forceinline__ void done() {
-    if (at.lane == 0) tma_store_wait_read();
-  }
 };
+
+// Sum of a tile's int32 parts (exact, whatever the order), factors, bias and the result's type: four columns a thread.
+struct PartSum {
+  const int* parts;
+  PairGemm g;
+  OutRows out;
+  Factors f;
+};
+
+template <bool FP16>
+__global__ void __launch_bounds__(kPartThreads) int8_part_sum_kernel(const __grid_constant__ PartSum p) {
+  wait_for_previous_grid();
+  int m, n;
+  int64_t at;
+  if (!part_place(p.g, m, n, at)) return;
+  int4 sum = make_int4(0, 0, 0, 0);
+  for (int s = 0; s < p.g.split; ++s) {
+    const int4 v = *reinterpret_cast<const int4*>(p.parts + at + s * kPartStep);
+    sum.x += v.x;
+    sum.y += v.y;
+    sum.z += v.z;
+    sum.w += v.w;
+  }
+  const float ra = __ldg(p.f.ra + m);
+  const bool far = far_out(ra);
+  const int acc[4] = {sum.x, sum.y, sum.z, sum.w};
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = min(n + i, p.g.N - 1);
+    const float x = __int2float_rn(acc[i]), rb = __ldg(p.f.rb + c), b = p.f.bias.at(c);
+    y[i] = far ? apply_factors_far(x, ra, rb, b) : apply_factors(x, ra, rb, b);
+  }
+  store4<FP16>(p.out, m, n, y);
+}
+
+// ---------------------------------------------------------------- one row
+// The weight's bytes are all there is.  A block takes a run of the weight's rows, its warps equal shares of the run's 512-byte
+// pieces, eight loads in flight each all the time (across rows), and multiplies them with the codes of x by four-way dot
+// products; no matrix instruction has to be fed, no second grid waits.  A row that two warps share is added up in shared
+// memory (whole numbers: the same in any order).  x is coded by every block for itself, from registers into shared memory (a
+// few KB from the L2), while the first loads of the weight are on their way.
+constexpr int kVectorThreads = 256, kVectorDepth = 8;
+constexpr int kVectorUnits = 4;                                            // units of 16 columns of x a thread
+constexpr int kVectorMaxK = kVectorThreads * kVectorUnits * 16;            // 16384
+constexpr int kVectorBlocks = 2;                                           // of an SM
+constexpr int kVectorMaxRows = 8192;                                       // of a block: 32 KB of sums
+constexpr int kVectorSmem = kVectorMaxK + 512 + 4 * kVectorMaxRows;
+
+struct VectorParams {
+  const void* x;    // 16 bits, or codes
+  const int8_t* w;
+  void* d;
+  Factors f;        // ra: of codes
+  int out_fp16;
+  int N, K;
+};
+
+// T: the type of x, int8_t where it is coded.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(kVectorThreads, kVectorBlocks) int8_vector_kernel(const VectorParams p) {
+  extern __shared__ __align__(16) int8_t codes[];  // whole pieces of 512 columns, then the sums of the block's rows
+  __shared__ uint32_t red[kVectorThreads / 32];
+  constexpr int kWarps = kVectorThreads / 32;
+  const int warp = warp_id(), lane = lane_id();
+  const int row_bytes = (int)int8_row_bytes(p.K), pieces = (row_bytes + 511) / 512, tail = row_bytes - (pieces - 1) * 512;
+  int* sums = reinterpret_cast<int*>(codes + pieces * 512);
+  // rows n0 .. n0 + rows - 1 of the block, and pieces begin .. end - 1 of them of the warp
+  const int n0 = (int)((int64_t)p.N * blockIdx.x / gridDim.x), rows = (int)((int64_t)p.N * (blockIdx.x + 1) / gridDim.x) - n0;
+  const int total = rows * pieces;
+  const int begin = (int)((int64_t)total * warp / kWarps), end = (int)((int64_t)total * (warp + 1) / kWarps);
+  const int first_row = begin / pieces, first_piece = begin % pieces;
+  // rows lie one behind the other: the next piece is 512 bytes on, or `tail` at a row's end
+  const int8_t* at = p.w + (int64_t)(n0 + first_row) * row_bytes + first_piece * 512 + lane * 16;
+  int to_load = end - begin, lp = pieces - 1 - first_piece;  // loads left; pieces of the row behind the next one
+  const bool in_tail = lane * 16 < tail;
+  uint4 w[kVectorDepth];
+  auto load = [&](uint4& to) {
+    to = make_uint4(0u, 0u, 0u, 0u);
+    if (to_load > 0 && (lp > 0 || in_tail)) to = ld_stream(at);
+    --to_load;
+    at += lp > 0 ? 512 : tail;
+    lp = lp > 0 ? lp - 1 : pieces - 1;
+  };
+#pragma unroll
+  for (int i = 0; i < kVectorDepth; ++i) load(w[i]);
+
+  for (int r = threadIdx.x; r < rows; r += kVectorThreads) sums[r] = 0;
+  float ra;
+  if constexpr (std::is_same_v<T, int8_t>) {
+    for (int c = threadIdx.x * 16; c < pieces * 512; c += kVectorThreads * 16) {
+      uint32_t q[4] = {0u, 0u, 0u, 0u};
+      if (c < row_bytes) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const int8_t*>(p.x) + c));
+        q[0] = v.x, q[1] = v.y, q[2] = v.z, q[3] = v.w;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // zeros past the columns, whatever is stored there
+        const int left = p.K - c - 4 * i;
+        if (left < 4) q[i] = left <= 0 ? 0u : q[i] & ((1u << (8 * left)) - 1u);
+      }
+      *reinterpret_cast<uint4*>(codes + c) = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+    ra = __ldg(p.f.ra);
+  } else {
+    const T* x = static_cast<const T*>(p.x);
+    Unit<T> u[kVectorUnits];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < kVectorUnits; ++i) {
+      const int unit = threadIdx.x + i * kVectorThreads;
+      if constexpr (ALIGNED) u[i] = load_unit<T, true>(x, unit * 16, p.K);
+      else u[i] = load_spread<T>(x, (unit - lane) * 16, p.K);
+      top = max(top, absmax_bits(u[i]));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, lane < kWarps ? red[lane] : 0u);
+    float inv;
+    ra = int8_row_scale(top, inv);
+#pragma unroll
+    for (int i = 0; i < kVectorUnits; ++i) {
+      const int unit = threadIdx.x + i * kVectorThreads, col = ALIGNED ? unit * 16 : (unit - lane) * 16;
+      if (col >= pieces * 512) break;  // (units past the columns are zeros)
+      uint32_t q[4] = {0u, 0u, 0u, 0u};
+      if (top < kInfBits) int8_encode_row(u[i], ra, inv, q);
+      if constexpr (ALIGNED) {
+        *reinterpret_cast<uint4*>(codes + col) = make_uint4(q[0], q[1], q[2], q[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) codes[col + 32 * j + lane] = (int8_t)(q[j >> 2] >> (8 * (j & 3)));
+      }
+    }
+  }
+  __syncthreads();
+
+  int acc = 0, left = end - begin, cp = pieces - 1 - first_piece, row = first_row;  // pieces left; of the row behind this one
+  const int8_t *x0 = codes + lane * 16, *xc = x0 + first_piece * 512;
+  while (left > 0) {
+#pragma unroll
+    for (int i = 0; i < kVectorDepth; ++i) {
+      const uint4 v = w[i];  // (zeros past the end)
+      load(w[i]);
+      const uint4 x = *reinterpret_cast<const uint4*>(xc);
+      acc = __dp4a((int)v.x, (int)x.x, __dp4a((int)v.y, (int)x.y, __dp4a((int)v.z, (int)x.z, __dp4a((int)v.w, (int)x.w, acc))));
+      xc += 512;
+      --left;
+      if (cp == 0 || left == 0) {  // the same for the whole warp
+        const int sum = __reduce_add_sync(0xffffffffu, acc);
+        if (lane == 0) atomicAdd(&sums[row], sum);
+        acc = 0;
+        if (left == 0) break;
+        ++row;
+        cp = pieces;
+        xc = x0;
+      }
+      --cp;
+    }
+  }
+  __syncthreads();
+  for (int r = threadIdx.x; r < rows; r += kVectorThreads) {
+    const int n = n0 + r;
+    const float s = __int2float_rn(sums[r]), rb = __ldg(p.f.rb + n), b = p.f.bias.at(n);
+    const float y = far_out(ra) ? apply_factors_far(s, ra, rb, b) : apply_factors(s, ra, rb, b);
+    static_cast<uint16_t*>(p.d)[n] = (uint16_t)(p.out_fp16 ? pack16<true>(y, 0.f) : pack16<false>(y, 0.f));
+  }
+}
 
 // ---------------------------------------------------------------- few rows
 // For few rows of x, D^T = B A^T: 128 rows of the weight B are the MMA's 128 rows and a tile of x's rows its N, so one
@@ -324,13 +490,6 @@ CUtensorMap code_map(const Int8Matrix& x, uint32_t box_rows) {  // zeros past co
   return make_tmap_u8(x.data, 2, dims, strides, box);
 }
 
-// Which kernel: up to 128 rows of x the few-rows kernel reads the weight once and wastes no half of a 256-row tile; above
-// it stays ahead while its 128 x 128 tiles do not fill the GPU.
-bool few_rows(int64_t M, int64_t N, int sms) {
-  if (M <= kSmallBN) return true;
-  return ((N + kBM - 1) / kBM) * ((M + kSmallBN - 1) / kSmallBN) <= sms * 7 / 8;
-}
-
 void launch_small(const Int8Matrix& a, const Int8Matrix& b, const Factors& f, at::Tensor& d, int device, cudaStream_t stream,
                   bool early) {
   const int sms = sm_count(device);
@@ -376,12 +535,47 @@ void launch_small(const Int8Matrix& a, const Int8Matrix& b, const Factors& f, at
 }
 
 template <bool FP16>
-void launch_pair(const Int8Matrix& a, const Int8Matrix& b, const Factors& f, at::Tensor& d, int device, cudaStream_t stream) {
-  const PairGemm p = pair_gemm(a.rows, b.rows, a.cols, 1, false, false, 1, device);
+void launch_pair(const Int8Matrix& a, const Int8Matrix& b, const Factors& f, at::Tensor& d, int device, cudaStream_t stream,
+                 bool early) {
+  const int64_t M = a.rows, N = b.rows;
+  PairGemm p = pair_gemm(M, N, a.cols, 1, false, false, device);
+  p.early = early ? 1 : 0;
   const CUtensorMap ma = code_map(a, kPairHalf), mb = code_map(b, kPairHalf);
-  const OutRows out = out_rows(d.data_ptr(), b.rows, a.rows, b.rows);
+  const OutRows out = out_rows(d.data_ptr(), N, M, N);
   const typename ScaleEpilogue<FP16>::Args args{out.tma ? out_rows_map(out) : ma, out, f};
-  launch_pair_gemm<Mma::kI8, ScaleEpilogue<FP16>>(ma, mb, args, p, device, stream);
+  const at::Tensor parts = part_memory(p, d.options());
+  launch_pair_gemm<Mma::kI8, ScaleEpilogue<FP16>>(ma, mb, parts, args, p, device, stream);
+  if (p.split > 1)
+    launch_overlapping(int8_part_sum_kernel<FP16>, part_grid(p), dim3(kPartThreads), 0, stream, true,
+                       PartSum{parts.data_ptr<int>(), p, out, f});
+}
+
+template <typename T, bool ALIGNED>
+void launch_vector_as(const VectorParams& p, int device, cudaStream_t stream) {
+  // a row for each warp at least, and as many blocks as run at once
+  const int grid = std::max(1, std::min(p.N / (kVectorThreads / 32), kVectorBlocks * sm_count(device)));
+  const int smem = (int)((int8_row_bytes(p.K) + 511) / 512 * 512) + 4 * ((p.N + grid - 1) / grid);
+  raise_smem<int8_vector_kernel<T, ALIGNED>>(kVectorSmem, device);
+  int8_vector_kernel<T, ALIGNED><<<grid, kVectorThreads, smem, stream>>>(p);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+// One row, whose codes and the sums of a block's rows of the weight fit into shared memory.
+bool one_row(int64_t M, const Int8Matrix& w, int device) {
+  return M == 1 && w.cols <= kVectorMaxK && w.rows <= (int64_t)sm_count(device) * kVectorBlocks * kVectorMaxRows;
+}
+
+// d = x b^T + bias for one row x of 16 bits, or coded with the scale x_scale.
+void launch_vector(const void* x, at::ScalarType type, const float* x_scale, const Int8Matrix& b,
+                   const c10::optional<at::Tensor>& bias, at::Tensor& d, cudaStream_t stream) {
+  if (b.rows == 0) return;
+  const VectorParams p{x, b.data, d.data_ptr(), Factors{x_scale, b.row_scale, float_row(bias)}, d.scalar_type() == at::kHalf ? 1 : 0,
+                 (int)b.rows, (int)b.cols};
+  const bool aligned = b.cols % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 32 == 0;
+  const int device = d.get_device();
+  if (type == at::kChar) launch_vector_as<int8_t, true>(p, device, stream);
+  else if (type == at::kHalf) aligned ? launch_vector_as<__half, true>(p, device, stream) : launch_vector_as<__half, false>(p, device, stream);
+  else aligned ? launch_vector_as<__nv_bfloat16, true>(p, device, stream) : launch_vector_as<__nv_bfloat16, false>(p, device, stream);
 }
 
 // d [a.rows, b.rows] (bf16 or fp16, contiguous) = a b^T + bias, on the current device and stream.  early: the kernel before
@@ -391,9 +585,9 @@ void gemm(const Int8Matrix& a, const Int8Matrix& b, const c10::optional<at::Tens
   if (a.rows == 0 || b.rows == 0) return;
   const Factors f{a.row_scale, b.row_scale, float_row(bias)};
   const int device = d.get_device();
-  if (few_rows(a.rows, b.rows, sm_count(device))) launch_small(a, b, f, d, device, stream, early);
-  else if (d.scalar_type() == at::kHalf) launch_pair<true>(a, b, f, d, device, stream);
-  else launch_pair<false>(a, b, f, d, device, stream);
+  if (a.rows <= kSmallBN) launch_small(a, b, f, d, device, stream, early);
+  else if (d.scalar_type() == at::kHalf) launch_pair<true>(a, b, f, d, device, stream, early);
+  else launch_pair<false>(a, b, f, d, device, stream, early);
 }
 
 void check_sum(int64_t K) {
@@ -415,16 +609,20 @@ at::Tensor int8_linear(const at::Tensor& x, const at::Tensor& data, const at::Te
   c10::cuda::CUDAGuard guard(x.device());
   const at::Tensor x2 = int8_rows(x, "int8_linear");
   Int8Matrix q{nullptr, nullptr, nullptr, x2.size(0), K};
-  // codes and scales of x in one piece, freed to the stream's pool when the call returns
-  const int64_t at_scales = (q.rows * q.row_bytes() + 511) / 512 * 512;
   const auto plain = x.options().requires_grad(false);
-  at::Tensor work = at::empty({at_scales + 4 * q.rows}, plain.dtype(at::kByte));
-  q.data = reinterpret_cast<int8_t*>(work.data_ptr());
-  q.row_scale = reinterpret_cast<float*>(work.data_ptr<uint8_t>() + at_scales);
   c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = N;
   at::Tensor y = at::empty(shape, plain.dtype(out_type == 0 ? at::kBFloat16 : out_type == 1 ? at::kHalf : dt));
   cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  if (one_row(q.rows, w, y.get_device())) {
+    launch_vector(x2.data_ptr(), dt, nullptr, w, b, y, stream);
+    return y;
+  }
+  // codes and scales of x in one piece, freed to the stream's pool when the call returns
+  const int64_t at_scales = (q.rows * q.row_bytes() + 511) / 512 * 512;
+  at::Tensor work = at::empty({at_scales + 4 * q.rows}, plain.dtype(at::kByte));
+  q.data = reinterpret_cast<int8_t*>(work.data_ptr());
+  q.row_scale = reinterpret_cast<float*>(work.data_ptr<uint8_t>() + at_scales);
   int8_quantize_launch(x2, q, stream);
   gemm(q, w, b, y, stream, true);
   return y;
@@ -440,7 +638,9 @@ at::Tensor int8_matmul(const at::Tensor& xdata, const at::Tensor& xscale, int64_
   const auto b = checked_bias(bias, N, data.device(), "int8_linear");
   c10::cuda::CUDAGuard guard(data.device());
   at::Tensor y = at::empty({M, N}, data.options().dtype(out_type == 1 ? at::kHalf : at::kBFloat16));
-  gemm(q, w, b, y, at::cuda::getCurrentCUDAStream(), false);
+  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+  if (one_row(M, w, y.get_device())) launch_vector(q.data, at::kChar, q.row_scale, w, b, y, stream);
+  else gemm(q, w, b, y, stream, false);
   return y;
 }
 

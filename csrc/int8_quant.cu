@@ -109,8 +109,8 @@ __global__ void __launch_bounds__(512, sizeof(T) == 4 || UPT > 2 ? 1 : 2) int8_q
       m = __reduce_max_sync(0xffffffffu, lane < (TX >> 5) ? red[lane] : 0u);
     }
     const bool bad = m >= kInfBits;
-    const float s = bad ? __uint_as_float(0x7fffffffu) : m == 0u ? 1.f : fminf(fmaxf(__fdiv_rn(__uint_as_float(m), 127.f), kInt8MinScale), kInt8MaxScale);
-    const float inv = bad ? 0.f : __frcp_rn(s);
+    float inv;
+    const float s = int8_row_scale(m, inv);
     if (threadIdx.x == 0 && live) p.row_scale[row] = s;
     for (int c = 0; c < chunks; ++c) {
       if (chunks > 1) load(c);
@@ -163,6 +163,7 @@ template <typename O, bool BLOCKS, bool ALIGNED>
 __global__ void __launch_bounds__(256) int8_dequant_kernel(const int8_t* __restrict__ data, const float* __restrict__ row_scale,
                                                            const uint8_t* __restrict__ exponents, O* __restrict__ out, int64_t ld,
                                                            int R, int K) {
+  launch_dependents();
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= R) return;
   const int row_bytes = (int)int8_row_bytes(K), nb = row_bytes / kInt8Block;

@@ -21,6 +21,13 @@ __device__ __forceinline__ void st256(void* p, const uint32_t* w) {
                : "memory");
 }
 
+// 16 bytes that are read once: past the L1.
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 constexpr uint32_t kInfBits = 0x7f800000u;  // non-negative fp32 numbers from here on are infinity and NaN
 
 template <typename T>
