@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(256) act_decode_kernel(Kept kept, uint16_t* a,
 // acc + bias -> 16 bits.
 template <bool FP16>
 struct BiasEpilogue {
-  static constexpr int kStages = 6, kOutBytes = 2048;
-  static constexpr bool kShared = true;
+  static constexpr int kStages = 6, kWarps = 8, kOutBytes = 2048;
+  static constexpr bool kShared = true, kAhead = true;
   struct Args {
     CUtensorMap map;
     OutRows out;
@@ -227,7 +227,7 @@ struct BiasEpilogue {
   __device__ __forceinline__ void met(int next) {
     if (next >= 0) fetch(next);
   }
-  __device__ __forceinline__ void chunk(int, int c, const uint32_t (&v)[32]) {
+  __device__ __forceinline__ void chunk(int c, const uint32_t (&v)[32]) {
     const int nc = n0 + c * 32;
     if (nc >= p.N || m0 >= p.M) return;
     uint32_t o[16];
@@ -244,13 +244,15 @@ struct BiasEpilogue {
   }
 };
 
-// dx = acc act'(x') and act(x'), from the accumulator (g W) and the kept codes.  A lane reads its row's 32 codes of a chunk
-// (one sector) while the chunk before is computed.
+// dx = acc act'(x') and act(x'), from the accumulator (g W) and the kept codes.  Some thirty instructions an element, with
+// chains of dependent ones: sixteen warps, four a scheduler, and one copy of the code (eight warps with four unrolled
+// chunks: 32760 x 1536 -> 8960 GELU 826 us, stalled on results and on the instruction cache).  A lane reads its row's 32
+// codes of a chunk (one sector) while the chunk before is computed.
 template <bool FP16, int ACT>
 struct ActGradEpilogue {
   static constexpr int H = ACT == kActSwiglu ? 2 : 1;
-  static constexpr int kStages = 5, kOutBytes = 2048 * (H + 1);
-  static constexpr bool kShared = false;
+  static constexpr int kStages = 5, kWarps = 16, kOutBytes = 2048;
+  static constexpr bool kShared = false, kAhead = false;
   struct Args {
     CUtensorMap map_dx[H], map_a;
     OutRows dx[H], act;
@@ -265,22 +267,22 @@ struct ActGradEpilogue {
   const PairGemm& p;
   const EpiPlace at;
   int m0, n0;
-  Codes q[2][H];
+  Codes next[H];
 
   __device__ __forceinline__ ActGradEpilogue(const Args& a, const PairGemm& p, const EpiPlace& at) : a(a), p(p), at(at) {}
   __device__ __forceinline__ void first(int) {}
-  __device__ __forceinline__ void load(Codes (&to)[H], int c) {
+  __device__ __forceinline__ void load(int c) {
     const int nc = n0 + c * 32, m = m0 + at.lane;
     const int row_bytes = (int)int8_row_bytes(p.N), nb = row_bytes / kInt8Block;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      to[h] = Codes{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0), 0u};
-      if (m < p.M && nc < p.N) {
+      next[h] = Codes{make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0), 0u};
+      if (m < p.M && nc < p.N && c < kPairN / 32) {
         const int64_t r = (int64_t)m * H + h;
         const uint4* d = reinterpret_cast<const uint4*>(a.kept.data + r * row_bytes + nc);
-        to[h].lo = __ldg(d);
-        to[h].hi = __ldg(d + 1);
-        to[h].e = __ldg(a.kept.exponents + r * nb + nc / kInt8Block);
+        next[h].lo = __ldg(d);
+        next[h].hi = __ldg(d + 1);
+        next[h].e = __ldg(a.kept.exponents + r * nb + nc / kInt8Block);
       }
     }
   }
@@ -289,14 +291,16 @@ struct ActGradEpilogue {
     p.tile(item, tm, tn);
     m0 = tm * kPairM + (int)at.rank * kPairHalf + at.wq * 32;
     n0 = tn * kPairN;
-    load(q[0], at.half);
+    load(at.group);
   }
   __device__ __forceinline__ void met(int) {}
-  __device__ __forceinline__ void chunk(int i, int c, const uint32_t (&v)[32]) {
+  __device__ __forceinline__ void chunk(int c, const uint32_t (&v)[32]) {
     const int nc = n0 + c * 32;
-    if (i < 3) load(q[(i + 1) & 1], c + 2);
+    Codes k[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) k[h] = next[h];
+    load(c + kWarps / 4);
     if (nc >= p.N || m0 >= p.M) return;
-    const Codes(&k)[H] = q[i & 1];
     uint32_t od[H][16], oa[16];
     uint64_t s[H];
 #pragma unroll
@@ -326,11 +330,14 @@ struct ActGradEpilogue {
         if constexpr (H == 2) od[1][2 * w + j] = pack16<FP16>(u0, u1);
       }
     }
-    if (at.lane == 0) tma_store_wait_read();
-    __syncwarp();
+    auto store = [&](const OutRows& out, const CUtensorMap* map, const uint32_t (&o)[16]) {
+      if (at.lane == 0) tma_store_wait_read();
+      __syncwarp();
+      store_rows(out, map, at.stage, m0, nc, o);
+    };
 #pragma unroll
-    for (int h = 0; h < H; ++h) store_rows(a.dx[h], &a.map_dx[h], at.stage + 2048 * h, m0, nc, od[h]);
-    if (a.want_act) store_rows(a.act, &a.map_a, at.stage + 2048 * H, m0, nc, oa);
+    for (int h = 0; h < H; ++h) store(a.dx[h], &a.map_dx[h], od[h]);
+    if (a.want_act) store(a.act, &a.map_a, oa);
   }
 };
 
@@ -398,6 +405,7 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const uint16_t* g, int6
   const int r0 = blockIdx.y * per, r1 = min(R, r0 + per);
   float s[8] = {};
   if (n + 8 <= N) {
+#pragma unroll 4
     for (int r = r0 + warp; r < r1; r += 8) {
       const uint4 w = __ldg(reinterpret_cast<const uint4*>(g + (int64_t)r * ld + n));
       const uint32_t q[4] = {w.x, w.y, w.z, w.w};
@@ -448,8 +456,8 @@ int type_index(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat
 at::Tensor column_sum(const at::Tensor& g, at::ScalarType type, cudaStream_t stream) {
   const int R = (int)g.size(0), N = (int)g.size(1), nb = (N + 255) / 256, device = g.get_device();
   at::Tensor out = at::empty({N}, g.options().dtype(type));
-  // slices for two blocks an SM, of 64 rows at least
-  const int slices = std::max(1, std::min(2 * sm_count(device) / nb, R / 64)), per = (R + slices - 1) / slices;
+  // slices for eight blocks an SM, of 64 rows at least
+  const int slices = std::max(1, std::min(8 * sm_count(device) / nb, R / 64)), per = (R + slices - 1) / slices;
   at::Tensor parts = slices > 1 ? at::empty({slices, N}, g.options().dtype(at::kFloat)) : out;
   void* to = parts.data_ptr();
   const int first = slices > 1 ? 0 : type_index(type);
@@ -532,10 +540,6 @@ void product(const Operand& A, const Operand& B, const Result& r, cudaStream_t s
   else fp16 ? product_typed<true, kActNone>(A, B, r, device, stream) : product_typed<false, kActNone>(A, B, r, device, stream);
 }
 
-dim3 row_block(int64_t units) {  // threads of a row, rows
-  const int tx = (int)std::min<int64_t>(256, (units + 31) / 32 * 32);
-  return dim3(tx, 256 / tx);
-}
 
 int halves(int64_t act) { return act == kActSwiglu ? 2 : 1; }
 

@@ -9,7 +9,7 @@
 //   warp 0      producer of its own CTA's operands, which complete on the leader's barriers
 //   warp 1      leader CTA: issues the MMAs.  The whole warp runs the loop and one lane issues, so that the descriptors stay
 //               in uniform registers
-//   warps 2..9  epilogue of the CTA's 128 rows: two warps a lane quarter, every other 32 columns each
+//   warps 2..   epilogue of the CTA's 128 rows: two or four warps a lane quarter, every second or fourth 32 columns each
 // The two accumulators take the 512 columns of tensor memory, so that a tile's epilogue runs beside the next one's MMAs.
 // An operand is read K-major ([rows, K]) or, 16-bit types, MN-major ([K, rows]) where it lies.
 // Tiles that would leave half of the pairs or more without work (all of them, where they are few; those of the last round
@@ -60,7 +60,6 @@ __device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_
 
 constexpr int kPairM = 256, kPairN = 256, kPairHalf = 128;
 constexpr int kPairTileBytes = kPairHalf * 128;  // an operand's rows of a stage in one CTA: 16 KB
-constexpr int kPairEpiWarps = 8, kPairGemmThreads = 64 + 32 * kPairEpiWarps;
 
 struct PairGemm {
   int M, N;
@@ -92,15 +91,15 @@ struct PairGemm {
 struct EpiPlace {
   uint8_t* stage;   // the warp's shared memory
   float2* col;      // [2][256], shared by the epilogue warps
-  int wq, half, lane, thread;
+  int wq, group, lane, thread;  // lane quarter; the warp's chunks of 32 columns: group, group + kWarps / 4, ..
   uint32_t rank;
 };
 
-template <int STAGES, int OUT_BYTES>
+template <int STAGES, int WARPS, int OUT_BYTES>
 struct PairGemmSmem {
   uint8_t a[STAGES][kPairTileBytes];
   uint8_t b[STAGES][kPairTileBytes];
-  uint8_t out[kPairEpiWarps][OUT_BYTES];
+  uint8_t out[WARPS][OUT_BYTES];
   float2 col[2][kPairN];
   uint64_t full[STAGES], empty[STAGES];
   uint64_t acc_full[2], acc_free[2];
@@ -120,13 +119,14 @@ __device__ __forceinline__ void load_pair_operand(uint8_t* dst, const CUtensorMa
   }
 }
 
-// Epi: kStages, kOutBytes (shared memory of a warp), kShared (the column factors are used: the epilogue's warps meet once a
-// tile), Args (passed to the kernel), and
+// Epi: kStages, kWarps (8 or 16), kOutBytes (shared memory of a warp), kShared (the column factors are used: the epilogue's
+// warps, eight of them, meet once a tile), kAhead (a chunk is read from tensor memory while the one before is worked on; short
+// epilogues), Args (passed to the kernel), and
 //   Epi(args, gemm, place)
 //   first(item)                 before the first tile
 //   begin(item, next, parity)   before the tile's accumulator is waited for; next: the item after it, or -1
 //   met(next)                   behind the warps' barrier (kShared)
-//   chunk(i, c, v)              the accumulator's columns 32 c .. 32 c + 31 of the lane's row; i = 0 .. 3
+//   chunk(c, v)                 the accumulator's columns 32 c .. 32 c + 31 of the lane's row
 // (of a part only the calls that the barrier's warps share are made)
 // Columns 32 c .. of the lane's row of a part, through 2 KB of shared memory: twice 16 columns of 32 rows (64-byte swizzle).
 __device__ __forceinline__ void store_part(const CUtensorMap* map, const EpiPlace& at, int part, int c, const uint32_t (&v)[32]) {
@@ -145,12 +145,13 @@ __device__ __forceinline__ void store_part(const CUtensorMap* map, const EpiPlac
 }
 
 template <Mma KIND, class Epi>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairGemmThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * Epi::kWarps, 1)
 pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                  const __grid_constant__ CUtensorMap tm_parts, const __grid_constant__ typename Epi::Args args,
                  const PairGemm p) {
-  constexpr int kStages = Epi::kStages;
-  using Smem = PairGemmSmem<kStages, Epi::kOutBytes>;
+  constexpr int kStages = Epi::kStages, kWarps = Epi::kWarps, kGroups = kWarps / 4, kChunks = kPairN / 32 / kGroups;
+  static_assert(!Epi::kShared || 32 * kWarps == kPairN, "a column a thread");
+  using Smem = PairGemmSmem<kStages, kWarps, Epi::kOutBytes>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   volatile int* abort_flag = &sm.abort_flag;
@@ -166,7 +167,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&sm.acc_full[b], 1);
-      mbar_init(&sm.acc_free[b], 2 * kPairEpiWarps);
+      mbar_init(&sm.acc_free[b], 2 * kWarps);
     }
     mbar_init(&sm.drain, 1);
     sm.abort_flag = 0;
@@ -263,7 +264,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       mbar_wait(&sm.drain, 0, kStatusTimeoutMma, nullptr, p.status);
     }
   } else {
-    // ------------------------------------------------------------ epilogue (warps 2..9)
+    // ------------------------------------------------------------ epilogue (warps 2..)
     const int ew = warp - 2;
     const EpiPlace place{sm.out[ew], &sm.col[0][0], warp & 3, ew >> 2, lane, (int)threadIdx.x - 64, rank};
     const uint32_t lane_base = (uint32_t)(place.wq * 32) << 16;
@@ -276,7 +277,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       if (Epi::kShared || !part) epi.begin(t, next, tl & 1);
       bool ok = mbar_wait(&sm.acc_full[tl & 1], (tl >> 1) & 1, kStatusTimeoutMma, abort_flag, p.status);
       if constexpr (Epi::kShared) {  // all warps leave together, since the barrier counts them
-        if (named_bar_any(1, 32 * kPairEpiWarps, !ok)) break;
+        if (named_bar_any(1, 32 * kWarps, !ok)) break;
         epi.met(next);
       } else {
         if (!__all_sync(0xffffffffu, ok)) break;
@@ -284,20 +285,34 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
       tc_fence_after();
       const uint32_t acc = tmem + lane_base + (tl & 1) * kPairN;
       const uint32_t freed = cluster_map(&sm.acc_free[tl & 1], 0);
-      uint32_t r[2][32];
-      tmem_ld32(acc + place.half * 32, r[0]);
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(freed);
+      };
+      auto finish = [&](int c, const uint32_t (&v)[32]) {
+        if (part) store_part(&tm_parts, place, t - p.whole, c, v);
+        else epi.chunk(c, v);
+      };
+      if constexpr (Epi::kAhead) {
+        uint32_t r[2][32];
+        tmem_ld32(acc + place.group * 32, r[0]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        tmem_wait_ld();
-        if (i < 3) {
-          tmem_ld32(acc + (2 * i + 2 + place.half) * 32, r[(i + 1) & 1]);
-        } else {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(freed);
+        for (int i = 0; i < kChunks; ++i) {
+          tmem_wait_ld();
+          if (i + 1 < kChunks) tmem_ld32(acc + (kGroups * (i + 1) + place.group) * 32, r[(i + 1) & 1]);
+          else release();
+          finish(kGroups * i + place.group, r[i & 1]);
         }
-        if (part) store_part(&tm_parts, place, t - p.whole, 2 * i + place.half, r[i & 1]);
-        else epi.chunk(i, 2 * i + place.half, r[i & 1]);
+      } else {
+#pragma unroll 1
+        for (int c = place.group; c < kPairN / 32; c += kGroups) {
+          uint32_t r[32];
+          tmem_ld32(acc + c * 32, r);
+          tmem_wait_ld();
+          if (c + kGroups >= kPairN / 32) release();
+          finish(c, r);
+        }
       }
     }
     if (lane == 0) tma_store_wait_read();
@@ -511,7 +526,7 @@ inline at::Tensor part_memory(const PairGemm& p, const at::TensorOptions& option
 template <Mma KIND, class Epi>
 void launch_pair_gemm(const CUtensorMap& a, const CUtensorMap& b, const at::Tensor& parts, const typename Epi::Args& args,
                       const PairGemm& p, int device, cudaStream_t stream) {
-  constexpr int smem = (int)sizeof(PairGemmSmem<Epi::kStages, Epi::kOutBytes>) + 1024;
+  constexpr int smem = (int)sizeof(PairGemmSmem<Epi::kStages, Epi::kWarps, Epi::kOutBytes>) + 1024;
   static_assert(smem <= 232448 && Epi::kOutBytes >= 2048, "shared memory of an SM, of a part's rows");
   CUtensorMap mp = a;
   if (parts.defined()) {
@@ -521,7 +536,7 @@ void launch_pair_gemm(const CUtensorMap& a, const CUtensorMap& b, const at::Tens
     mp = make_tmap(CU_TENSOR_MAP_DATA_TYPE_INT32, parts.data_ptr(), 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
   }
   raise_smem<pair_gemm_kernel<KIND, Epi>>(smem, device);
-  launch_overlapping(pair_gemm_kernel<KIND, Epi>, dim3(2 * std::min(p.items, sm_count(device) / 2)), dim3(kPairGemmThreads), smem,
+  launch_overlapping(pair_gemm_kernel<KIND, Epi>, dim3(2 * std::min(p.items, sm_count(device) / 2)), dim3(64 + 32 * Epi::kWarps), smem,
                      stream, p.early != 0, a, b, mp, args, p);
 }
 

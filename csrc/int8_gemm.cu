@@ -34,8 +34,8 @@ struct Factors {
 // ---------------------------------------------------------------- CTA pairs
 template <bool FP16>
 struct ScaleEpilogue {
-  static constexpr int kStages = 6, kOutBytes = 2048;
-  static constexpr bool kShared = true;
+  static constexpr int kStages = 6, kWarps = 8, kOutBytes = 2048;
+  static constexpr bool kShared = true, kAhead = true;
   struct Args {
     CUtensorMap map;
     OutRows out;
@@ -73,7 +73,7 @@ struct ScaleEpilogue {
   __device__ __forceinline__ void met(int next) {  // the next tile's factors are read while this one is stored
     if (next >= 0) fetch(next);
   }
-  __device__ __forceinline__ void chunk(int, int c, const uint32_t (&v)[32]) {
+  __device__ __forceinline__ void chunk(int c, const uint32_t (&v)[32]) {
     const int nc = n0 + c * 32;
     if (nc >= p.N || m0 >= p.M) return;
     uint32_t o[16];

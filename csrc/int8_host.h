@@ -5,6 +5,13 @@
 
 namespace dmad {
 
+// Threads of a row (whole warps, as even a share of the row's units each as there is) and rows of a block of up to 256.
+inline dim3 row_block(int64_t units) {
+  const int64_t passes = (units + 255) / 256;
+  const unsigned tx = (unsigned)std::max<int64_t>(32, ((units + passes - 1) / passes + 31) / 32 * 32);
+  return dim3(tx, 256 / tx);
+}
+
 struct Int8Matrix {  // storage as int8.cuh describes it
   int8_t* data;
   float* row_scale;    // one scale a row

@@ -222,14 +222,14 @@ __global__ void __launch_bounds__(256) int8_dequant_kernel(const int8_t* __restr
 template <typename O, bool BLOCKS>
 void launch_dequant(const Int8Matrix& q, void* out, int64_t ld, cudaStream_t stream) {
   const int R = (int)q.rows, K = (int)q.cols, units = (K + 15) / 16;
-  const int tx = std::min(256, (units + 31) / 32 * 32), ty = 256 / tx;
-  const unsigned grid = (unsigned)(((int64_t)R + ty - 1) / ty);
+  const dim3 block = row_block(units);
+  const unsigned grid = (unsigned)(((int64_t)R + block.y - 1) / block.y);
   const bool aligned = K % 16 == 0 && (ld * sizeof(O)) % 32 == 0 && reinterpret_cast<uintptr_t>(out) % 32 == 0;
   O* o = static_cast<O*>(out);
   if (aligned)
-    int8_dequant_kernel<O, BLOCKS, true><<<grid, dim3(tx, ty), 0, stream>>>(q.data, q.row_scale, q.exponents, o, ld, R, K);
+    int8_dequant_kernel<O, BLOCKS, true><<<grid, block, 0, stream>>>(q.data, q.row_scale, q.exponents, o, ld, R, K);
   else
-    int8_dequant_kernel<O, BLOCKS, false><<<grid, dim3(tx, ty), 0, stream>>>(q.data, q.row_scale, q.exponents, o, ld, R, K);
+    int8_dequant_kernel<O, BLOCKS, false><<<grid, block, 0, stream>>>(q.data, q.row_scale, q.exponents, o, ld, R, K);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
