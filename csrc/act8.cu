@@ -86,25 +86,6 @@ struct EncodeParams {
   Kept kept;  // data null: nothing is kept
 };
 
-// Codes of a unit in spread order: a block of 32 columns is element j of all lanes.  Returns the scale byte of block `lane`.
-template <typename T>
-__device__ __forceinline__ uint32_t encode_spread(const Unit<T>& u, uint32_t (&codes)[4]) {
-  const int lane = lane_id();
-  uint32_t mine = 0;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    codes[q] = 0u;
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const int j = 4 * q + h;
-      const uint32_t e = int8_block_code(__reduce_max_sync(0xffffffffu, abs_bits(u, j)));
-      if (lane == j) mine = e;
-      codes[q] |= int8_block_byte(u, j, e) << (8 * h);
-    }
-  }
-  return mine;
-}
-
 template <typename T, int ACT, bool ALIGNED>
 __global__ void __launch_bounds__(256) act_encode_kernel(EncodeParams p) {
   constexpr bool FP16 = std::is_same_v<T, __half>;
@@ -117,47 +98,35 @@ __global__ void __launch_bounds__(256) act_encode_kernel(EncodeParams p) {
   const T* xr = static_cast<const T*>(p.x) + row * p.ld;
   uint16_t* ar = static_cast<uint16_t*>(p.a) + row * p.lda;
   for (int first = threadIdx.x - lane; first * 16 < row_bytes; first += blockDim.x) {
-    const int col = ALIGNED ? (first + lane) * 16 : first * 16;
+    const int col = (first + lane) * 16;
     Unit<T> v[H];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       if constexpr (ALIGNED) v[h] = load_unit<T, true>(xr + h * p.F, col, p.F);
-      else v[h] = load_spread<T>(xr + h * p.F, col, p.F);
+      else v[h] = load_unit_anywhere<T>(xr + h * p.F, col, p.F);
     }
-    uint32_t o[8];
+    if (col < p.F) {  // (a's rows are padded to whole units)
+      uint32_t o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 a = f2_split(unit_pair(v[0], i)), b = f2_split(unit_pair(v[H - 1], i));
-      o[i] = pack16<FP16>(act_value<ACT>(a.x, b.x), act_value<ACT>(a.y, b.y));
-    }
-    if constexpr (ALIGNED) {
-      if (col < p.F) st256(ar + col, o);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (col + 32 * j + lane < p.F) ar[col + 32 * j + lane] = (uint16_t)(o[j >> 1] >> (16 * (j & 1)));
+      for (int i = 0; i < 8; ++i) {
+        const float2 a = f2_split(unit_pair(v[0], i)), b = f2_split(unit_pair(v[H - 1], i));
+        if constexpr (ACT == kActNone) o[i] = v[0].w[i];
+        else o[i] = pack16<FP16>(act_value<ACT>(a.x, b.x), act_value<ACT>(a.y, b.y));
+      }
+      st256(ar + col, o);
     }
     if (p.kept.data == nullptr) continue;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      int8_t* dr = p.kept.data + (row * H + h) * row_bytes;
-      uint8_t* er = p.kept.exponents + (row * H + h) * nb;
+      uint32_t amax = absmax_bits(v[h]);  // a block is two lanes' units
+      amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      const uint32_t e = int8_block_code(amax);
       uint32_t codes[4];
-      if constexpr (ALIGNED) {  // a block is two lanes' units
-        uint32_t amax = absmax_bits(v[h]);
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        const uint32_t e = int8_block_code(amax);
-        int8_encode_block(v[h], e, codes);
-        if (col < row_bytes) {
-          *reinterpret_cast<uint4*>(dr + col) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-          if ((lane & 1) == 0) er[col / kInt8Block] = (uint8_t)e;
-        }
-      } else {
-        const uint32_t e = encode_spread(v[h], codes);
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (col + 32 * j < row_bytes) dr[col + 32 * j + lane] = (int8_t)(codes[j >> 2] >> (8 * (j & 3)));
-        if (lane < 16 && col / kInt8Block + lane < nb) er[col / kInt8Block + lane] = (uint8_t)e;
+      int8_encode_block(v[h], e, codes);
+      if (col < row_bytes) {
+        const int64_t r = row * H + h;
+        *reinterpret_cast<uint4*>(p.kept.data + r * row_bytes + col) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+        if ((lane & 1) == 0) p.kept.exponents[r * nb + col / kInt8Block] = (uint8_t)e;
       }
     }
   }
@@ -474,10 +443,47 @@ at::Tensor column_sum(const at::Tensor& g, at::ScalarType type, cudaStream_t str
 }
 
 // ---------------------------------------------------------------- products
-// Rows that TMA can read: contiguous columns, rows on 16 bytes; copied where t is laid out otherwise.
-at::Tensor tma_rows(const at::Tensor& t) {
-  if (t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)
-    return t;
+int halves(int64_t act) { return act == kActSwiglu ? 2 : 1; }
+
+Kept kept_of(const at::Tensor& data, const at::Tensor& exponents) {
+  return Kept{reinterpret_cast<int8_t*>(data.data_ptr()), exponents.data_ptr<uint8_t>()};
+}
+
+// act(x) [R, F] (no activation: a copy of x) with rows on 32 bytes, and the codes of x where they are kept.
+at::Tensor encode(const at::Tensor& x2, int64_t F, int64_t act, const Kept& kept, cudaStream_t stream) {
+  const int64_t R = x2.size(0), lda = (F + 15) / 16 * 16;
+  at::Tensor a = at::empty({R, lda}, x2.options().requires_grad(false));
+  if (R > 0) {
+    const EncodeParams p{x2.data_ptr(), x2.stride(0), (int)R, (int)F, a.data_ptr(), lda, kept};
+    const bool aligned = F % 16 == 0 && x2.stride(0) % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 32 == 0;
+    const dim3 block = row_block(int8_row_bytes(F) / 16);
+    const unsigned grid = (unsigned)((R + block.y - 1) / block.y);
+    auto go = [&](auto tag, auto which) {
+      using T = decltype(tag);
+      constexpr int ACT = decltype(which)::value;
+      if (aligned) act_encode_kernel<T, ACT, true><<<grid, block, 0, stream>>>(p);
+      else act_encode_kernel<T, ACT, false><<<grid, block, 0, stream>>>(p);
+    };
+    auto typed = [&](auto tag) {
+      if (act == kActNone) go(tag, std::integral_constant<int, kActNone>{});
+      else if (act == kActGelu) go(tag, std::integral_constant<int, kActGelu>{});
+      else go(tag, std::integral_constant<int, kActSwiglu>{});
+    };
+    if (x2.scalar_type() == at::kHalf) typed(__half{});
+    else typed(__nv_bfloat16{});
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  return a.narrow(1, 0, F);
+}
+
+// Whether TMA can read t's rows: contiguous columns, rows on 16 bytes.
+bool tma_readable(const at::Tensor& t) {
+  return t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+// Such rows: t, or a copy where it is laid out otherwise.
+at::Tensor tma_rows(const at::Tensor& t, cudaStream_t stream) {
+  if (tma_readable(t)) return t;
+  if (t.stride(1) == 1) return encode(t, t.size(1), kActNone, Kept{nullptr, nullptr}, stream);
   at::Tensor p = at::empty({t.size(0), (t.size(1) + 7) / 8 * 8}, t.options().requires_grad(false)).narrow(1, 0, t.size(1));
   p.copy_(t);
   return p;
@@ -541,38 +547,6 @@ void product(const Operand& A, const Operand& B, const Result& r, cudaStream_t s
 }
 
 
-int halves(int64_t act) { return act == kActSwiglu ? 2 : 1; }
-
-Kept kept_of(const at::Tensor& data, const at::Tensor& exponents) {
-  return Kept{reinterpret_cast<int8_t*>(data.data_ptr()), exponents.data_ptr<uint8_t>()};
-}
-
-// act(x) [R, F] with rows on 32 bytes, and the codes of x.
-at::Tensor encode(const at::Tensor& x2, int64_t F, int64_t act, const Kept& kept, cudaStream_t stream) {
-  const int64_t R = x2.size(0), lda = (F + 15) / 16 * 16;
-  at::Tensor a = at::empty({R, lda}, x2.options().requires_grad(false));
-  if (R > 0) {
-    const EncodeParams p{x2.data_ptr(), x2.stride(0), (int)R, (int)F, a.data_ptr(), lda, kept};
-    const bool aligned = F % 16 == 0 && x2.stride(0) % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 32 == 0;
-    const dim3 block = row_block(int8_row_bytes(F) / 16);
-    const unsigned grid = (unsigned)((R + block.y - 1) / block.y);
-    auto go = [&](auto tag, auto which) {
-      using T = decltype(tag);
-      constexpr int ACT = decltype(which)::value;
-      if (aligned) act_encode_kernel<T, ACT, true><<<grid, block, 0, stream>>>(p);
-      else act_encode_kernel<T, ACT, false><<<grid, block, 0, stream>>>(p);
-    };
-    auto typed = [&](auto tag) {
-      if (act == kActGelu) go(tag, std::integral_constant<int, kActGelu>{});
-      else go(tag, std::integral_constant<int, kActSwiglu>{});
-    };
-    if (x2.scalar_type() == at::kHalf) typed(__half{});
-    else typed(__nv_bfloat16{});
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-  }
-  return a.narrow(1, 0, F);
-}
-
 // act(x') [R, F] of the codes.
 at::Tensor decode(const Kept& kept, int64_t R, int64_t F, int64_t act, const at::TensorOptions& options, cudaStream_t stream) {
   const int64_t lda = (F + 15) / 16 * 16;
@@ -630,11 +604,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_forward(const at::Tensor& x,
   }
   // copies before the pass over x, so that the product may overlap that pass without reading anything younger
   const bool some = R > 0 && N > 0;
-  const at::Tensor wt = some ? tma_rows(w) : w;
+  const at::Tensor wt = some ? tma_rows(w, stream) : w;
   at::Tensor a;
+  bool copied = act != kActNone;
   if (act == kActNone) {
-    if (some) a = tma_rows(x2);
-    if (keep) int8_quantize_launch(x2, Int8Matrix{kept.data, nullptr, kept.exponents, R, F}, stream);
+    if (some && !tma_readable(x2)) {
+      a = encode(x2, F, act, kept, stream);  // a copy and the codes in one pass
+      copied = true;
+    } else {
+      a = x2;
+      if (keep) int8_quantize_launch(x2, Int8Matrix{kept.data, nullptr, kept.exponents, R, F}, stream);
+    }
   } else {
     a = encode(x2, F, act, kept, stream);
   }
@@ -645,7 +625,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_forward(const at::Tensor& x,
     Result r;
     r.out[0] = out_rows(y.data_ptr(), N, R, N);
     r.bias = float_row(b);
-    r.early = act != kActNone ? 1 : keep ? 2 : 0;
+    r.early = copied ? 1 : keep ? 2 : 0;
     product(Operand{a, false}, Operand{wt, false}, r, stream);
   }
   return {y, data, exponents};
@@ -669,8 +649,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_backward(const at::Tensor& g
   }
   // Copies, then the passes that only read them and the codes, then the products, each overlapping the end of the kernel
   // before it: the first one reads nothing that those passes write (early 2) or, for want_w, what the one before did.
-  const at::Tensor gt = tma_rows(g.dim() == 2 ? g : g.reshape({R, N}));
-  const at::Tensor wt = want_x ? tma_rows(w) : w;
+  const at::Tensor gt = tma_rows(g.dim() == 2 ? g : g.reshape({R, N}), stream);
+  const at::Tensor wt = want_x ? tma_rows(w, stream) : w;
   const Kept kept = data.defined() ? kept_of(data, exponents) : Kept{nullptr, nullptr};
   at::Tensor a;  // act(x')
   if (want_b) db = column_sum(gt, bias_type, stream);

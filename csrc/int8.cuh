@@ -127,43 +127,4 @@ __device__ __forceinline__ void int8_encode_row(const Unit<T>& u, float s, float
   }
 }
 
-// Elements of a unit of rows that do not start on 32 bytes: every 32nd column from c0 + lane on, so that a warp's loads are
-// runs of its 32 lanes.
-template <typename T>
-__device__ __forceinline__ Unit<T> load_spread(const T* __restrict__ row, int c0, int K) {
-  Unit<T> u;
-  const int c = c0 + lane_id();
-  if constexpr (sizeof(T) == 4) {
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(row);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) u.w[i] = c + 32 * i < K ? __ldg(p + c + 32 * i) : 0u;
-  } else {
-    const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t lo = c + 64 * i < K ? __ldg(p + c + 64 * i) : 0u;
-      const uint32_t hi = c + 64 * i + 32 < K ? __ldg(p + c + 64 * i + 32) : 0u;
-      u.w[i] = lo | (hi << 16);
-    }
-  }
-  return u;
-}
-
-// |x| of element i of a unit as the bits of an fp32 number.
-template <typename T>
-__device__ __forceinline__ uint32_t abs_bits(const Unit<T>& u, int i) {
-  if constexpr (sizeof(T) == 4) return u.w[i] & 0x7fffffffu;
-  const float2 v = f2_split(unit_pair(u, i >> 1));
-  return __float_as_uint(i & 1 ? v.y : v.x) & 0x7fffffffu;
-}
-
-// Element i of a unit in a block with the scale byte e, as a byte.
-template <typename T>
-__device__ __forceinline__ uint32_t int8_block_byte(const Unit<T>& u, int i, uint32_t e) {
-  const float2 x = f2_split(unit_pair(u, i >> 1));
-  const float m = __uint_as_float((254u - min(e, 254u)) << 23);
-  const float t = clamp127((i & 1 ? x.y : x.x) * m) + kRoundMagic;
-  return e == 0xffu ? 0u : __float_as_uint(t) & 0xffu;
-}
-
 }  // namespace dmad

@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kVectorThreads, kVectorBlocks) int8_vector_ker
     for (int i = 0; i < kVectorUnits; ++i) {
       const int unit = threadIdx.x + i * kVectorThreads;
       if constexpr (ALIGNED) u[i] = load_unit<T, true>(x, unit * 16, p.K);
-      else u[i] = load_spread<T>(x, (unit - lane) * 16, p.K);
+      else u[i] = load_unit_anywhere<T>(x, unit * 16, p.K);
       top = max(top, absmax_bits(u[i]));
     }
     top = __reduce_max_sync(0xffffffffu, top);
@@ -223,16 +223,11 @@ __global__ void __launch_bounds__(kVectorThreads, kVectorBlocks) int8_vector_ker
     ra = int8_row_scale(top, inv);
 #pragma unroll
     for (int i = 0; i < kVectorUnits; ++i) {
-      const int unit = threadIdx.x + i * kVectorThreads, col = ALIGNED ? unit * 16 : (unit - lane) * 16;
+      const int col = (int)(threadIdx.x + i * kVectorThreads) * 16;
       if (col >= pieces * 512) break;  // (units past the columns are zeros)
       uint32_t q[4] = {0u, 0u, 0u, 0u};
       if (top < kInfBits) int8_encode_row(u[i], ra, inv, q);
-      if constexpr (ALIGNED) {
-        *reinterpret_cast<uint4*>(codes + col) = make_uint4(q[0], q[1], q[2], q[3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) codes[col + 32 * j + lane] = (int8_t)(q[j >> 2] >> (8 * (j & 3)));
-      }
+      *reinterpret_cast<uint4*>(codes + col) = make_uint4(q[0], q[1], q[2], q[3]);
     }
   }
   __syncthreads();

@@ -3,8 +3,7 @@
 // The kernels read each element once and are bound by HBM.  A thread takes units of 16 columns (one 32-byte load of 16-bit
 // elements, one 16-byte store of codes); a row with one scale is held by one block in registers between its maximum and the
 // encoding (up to 32768 columns of 16 bits, 16384 of 32; longer rows are read twice).  Rows that do not start on 32
-// bytes are read and written by runs of a warp's lanes instead, every 32nd column a lane, so that a block of 32 columns is one
-// load of the warp and its maximum one reduction.
+// bytes are read, and written back, in the aligned pieces around a unit (row_units.cuh).
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -40,27 +39,16 @@ __global__ void __launch_bounds__(512, sizeof(T) == 4 || UPT > 2 ? 1 : 2) int8_q
   int8_t* out = p.data + row * row_bytes;
   const int chunks = (row_bytes / 16 + TX * UPT - 1) / (TX * UPT);
   Unit<T> v[UPT];
-  // first column of unit i: of its 16 columns, or of the warp's 512
-  auto column = [&](int c, int i) {
-    const int u = threadIdx.x + (c * UPT + i) * TX;
-    return ALIGNED ? u * 16 : (u - lane) * 16;
-  };
+  auto column = [&](int c, int i) { return (int)(threadIdx.x + (c * UPT + i) * TX) * 16; };  // first one of unit i
   auto load = [&](int c) {
 #pragma unroll
     for (int i = 0; i < UPT; ++i) {
       if constexpr (ALIGNED) v[i] = load_unit<T, true>(xr, column(c, i), K);
-      else v[i] = load_spread<T>(xr, column(c, i), K);
+      else v[i] = load_unit_anywhere<T>(xr, column(c, i), K);
     }
   };
   auto store = [&](int col, const uint32_t (&codes)[4]) {
-    if (!live) return;
-    if constexpr (ALIGNED) {
-      if (col < row_bytes) *reinterpret_cast<uint4*>(out + col) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (col + 32 * j < row_bytes) out[col + 32 * j + lane] = (int8_t)(codes[j >> 2] >> (8 * (j & 3)));
-    }
+    if (live && col < row_bytes) *reinterpret_cast<uint4*>(out + col) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
   };
   if constexpr (BLOCKS) {
     const int nb = row_bytes / kInt8Block;
@@ -71,27 +59,11 @@ __global__ void __launch_bounds__(512, sizeof(T) == 4 || UPT > 2 ? 1 : 2) int8_q
       for (int i = 0; i < UPT; ++i) {
         const int col = column(c, i);
         uint32_t codes[4];
-        if constexpr (ALIGNED) {  // a block is two lanes' units
-          uint32_t amax = absmax_bits(v[i]);
-          amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-          const uint32_t e = int8_block_code(amax);
-          int8_encode_block(v[i], e, codes);
-          if (live && (lane & 1) == 0 && col < row_bytes) er[col / kInt8Block] = (uint8_t)e;
-        } else {  // a block is element j of all lanes
-          uint32_t mine = 0;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            codes[q] = 0u;
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              const int j = 4 * q + h;
-              const uint32_t e = int8_block_code(__reduce_max_sync(0xffffffffu, abs_bits(v[i], j)));
-              if (lane == j) mine = e;
-              codes[q] |= int8_block_byte(v[i], j, e) << (8 * h);
-            }
-          }
-          if (live && lane < 16 && col / kInt8Block + lane < nb) er[col / kInt8Block + lane] = (uint8_t)mine;
-        }
+        uint32_t amax = absmax_bits(v[i]);  // a block is two lanes' units
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        const uint32_t e = int8_block_code(amax);
+        int8_encode_block(v[i], e, codes);
+        if (live && (lane & 1) == 0 && col < row_bytes) er[col / kInt8Block] = (uint8_t)e;
         store(col, codes);
       }
     }
@@ -163,57 +135,67 @@ template <typename O, bool BLOCKS, bool ALIGNED>
 __global__ void __launch_bounds__(256) int8_dequant_kernel(const int8_t* __restrict__ data, const float* __restrict__ row_scale,
                                                            const uint8_t* __restrict__ exponents, O* __restrict__ out, int64_t ld,
                                                            int R, int K) {
+  __shared__ uint32_t turn[!ALIGNED && sizeof(O) == 4 ? 8 : 1][!ALIGNED && sizeof(O) == 4 ? 32 * 17 : 1];
   launch_dependents();
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= R) return;
+  if (row >= R) return;  // whole warps
   const int row_bytes = (int)int8_row_bytes(K), nb = row_bytes / kInt8Block;
   const int8_t* dr = data + row * row_bytes;
   O* orow = out + row * ld;
-  float s = BLOCKS ? 0.f : row_scale[row];
-  if constexpr (ALIGNED) {  // K is a multiple of 16
-    for (int c = threadIdx.x * 16; c < K; c += blockDim.x * 16) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(dr + c));
+  float s = BLOCKS ? 1.f : row_scale[row];
+  const int lane = threadIdx.x & 31;
+  // whole warps stay together
+  for (int first = (threadIdx.x - lane) * 16; first < K; first += blockDim.x * 16) {
+    const int c = first + lane * 16;
+    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+    if (c < K) {
+      w = __ldg(reinterpret_cast<const uint4*>(dr + c));
       if constexpr (BLOCKS) s = int8_block_scale(__ldg(exponents + row * nb + c / kInt8Block));
-      const uint64_t s2 = f2(s, s);
-      const uint32_t q[4] = {w.x, w.y, w.z, w.w};
-      if constexpr (sizeof(O) == 4) {
-        uint32_t o[16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint64_t lo, hi;
-          bytes_to_float(q[i], lo, hi);
-          const float2 a = f2_split(f2_mul(lo, s2)), b = f2_split(f2_mul(hi, s2));
-          o[4 * i] = __float_as_uint(a.x);
-          o[4 * i + 1] = __float_as_uint(a.y);
-          o[4 * i + 2] = __float_as_uint(b.x);
-          o[4 * i + 3] = __float_as_uint(b.y);
-        }
-        st256(orow + c, o);
-        st256(orow + c + 8, o + 8);
-      } else {
-        uint32_t o[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint64_t lo, hi;
-          bytes_to_float(q[i], lo, hi);
-          o[2 * i] = pack_pair<O>(f2_mul(lo, s2));
-          o[2 * i + 1] = pack_pair<O>(f2_mul(hi, s2));
-        }
-        st256(orow + c, o);
-      }
     }
-  } else {
-    const int lane = threadIdx.x & 31;
-    for (int c0 = (threadIdx.x - lane) * 16; c0 < K; c0 += blockDim.x * 16) {
+    const uint64_t s2 = f2(s, s);
+    const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (sizeof(O) == 4) {
+      uint32_t o[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int c = c0 + 32 * j + lane;
-        if (c >= K) break;
-        if constexpr (BLOCKS) s = int8_block_scale(__ldg(exponents + row * nb + c / kInt8Block));
-        const float v = (float)__ldg(dr + c) * s;
-        if constexpr (sizeof(O) == 4) orow[c] = v;
-        else if constexpr (std::is_same_v<O, __nv_bfloat16>) orow[c] = __float2bfloat16_rn(v);
-        else orow[c] = __float2half_rn(v);
+      for (int i = 0; i < 4; ++i) {
+        uint64_t lo, hi;
+        bytes_to_float(q[i], lo, hi);
+        const float2 a = f2_split(f2_mul(lo, s2)), b = f2_split(f2_mul(hi, s2));
+        o[4 * i] = __float_as_uint(a.x);
+        o[4 * i + 1] = __float_as_uint(a.y);
+        o[4 * i + 2] = __float_as_uint(b.x);
+        o[4 * i + 3] = __float_as_uint(b.y);
+      }
+      if constexpr (ALIGNED) {  // K is a multiple of 16
+        if (c < K) {
+          st256(orow + c, o);
+          st256(orow + c + 8, o + 8);
+        }
+      } else {  // through shared memory, in runs of the warp's lanes
+        uint32_t* t = turn[threadIdx.y * (blockDim.x >> 5) + (threadIdx.x >> 5)];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t[lane * 17 + i] = o[i];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int e = i * 32 + lane;
+          if (first + e < K) reinterpret_cast<uint32_t*>(orow)[first + e] = t[(e >> 4) * 17 + (e & 15)];
+        }
+      }
+    } else {
+      uint32_t o[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint64_t lo, hi;
+        bytes_to_float(q[i], lo, hi);
+        o[2 * i] = pack_pair<O>(f2_mul(lo, s2));
+        o[2 * i + 1] = pack_pair<O>(f2_mul(hi, s2));
+      }
+      if constexpr (ALIGNED) {
+        if (c < K) st256(orow + c, o);
+      } else {
+        store_unit_anywhere(reinterpret_cast<uint16_t*>(orow), c, K, o);
       }
     }
   }

@@ -245,3 +245,22 @@ def test_refusals():
             bad()
     with pytest.raises(RuntimeError, match="forward only"):
         ops.int8_linear(x.requires_grad_(True), w)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("K", [1, 15, 17, 31, 500, 513, 529, 1039, 4111])
+def test_rows_that_start_anywhere(K, dtype):
+    """Every offset of a row's start, read and written back, and nothing written beside the rows."""
+    ops = _ops()
+    for start in range(0, 18):
+        wide = _matrix(7, K + 40, dtype, K + start)
+        x, xg = wide[:, start:start + K], wide.to(dev)[:, start:start + K]
+        for block in (0, 32):
+            q, ref = ops.quantize_int8(xg, block), ops.quantize_int8(x.contiguous(), block)
+            _same(q, ref)
+            assert torch.equal(ops.dequantize_int8(q, dtype).cpu(), ops.dequantize_int8(ref, dtype))
+    w = ops.quantize_int8(torch.randn(40, K, device=dev))
+    line = torch.randn(K + 40, device=dev).to(torch.bfloat16)
+    for start in range(0, 18):  # one row: coded within the product
+        x = line[start:start + K]
+        assert torch.equal(ops.int8_linear(x, w), ops.int8_linear(ops.quantize_int8(x), w, None, torch.bfloat16))
