@@ -506,6 +506,7 @@ struct Result {
   OutRows value{};
   bool want_value = false;
   int early = 0;
+  bool b_old = false;
 };
 
 template <bool FP16, int ACT>
@@ -514,6 +515,7 @@ void product_typed(const Operand& A, const Operand& B, const Result& r, int devi
   const int64_t M = A.rows(), N = B.rows(), K = A.K();
   PairGemm p = pair_gemm(M, N, K, 2, A.mn, B.mn, device);
   p.early = r.early;
+  p.b_old = r.b_old ? 1 : 0;
   const at::Tensor parts = part_memory(p, A.t.options());
   const CUtensorMap ma = A.map(), mb = B.map();
   auto map_of = [&](const OutRows& o) { return o.tma && o.d != nullptr ? out_rows_map(o) : ma; };
@@ -626,6 +628,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> act8_forward(const at::Tensor& x,
     r.out[0] = out_rows(y.data_ptr(), N, R, N);
     r.bias = float_row(b);
     r.early = copied ? 1 : keep ? 2 : 0;
+    r.b_old = true;
     product(Operand{a, false}, Operand{wt, false}, r, stream);
   }
   return {y, data, exponents};

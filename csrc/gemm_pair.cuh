@@ -68,6 +68,7 @@ struct PairGemm {
   int tiles_m, tiles_n, items;  // work items: `whole` tiles, then `split` of each other tile
   int whole, split, per_split;  // per_split: K steps of a part
   int a_mn, b_mn;         // 1: stored [K, rows]
+  int b_old;              // (early 1) B is older than the kernel before: its first stages are loaded before the wait
   int early;              // launched to overlap the kernel before it: 1 reads what that writes, 2 does not (operands and
                           // epilogue's inputs older); either way results are stored after its end
   int* status;
@@ -187,14 +188,25 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = sm.tmem_base;
-  if (p.early == 1 ? warp != 1 : p.early == 2 && warp > 1) wait_for_previous_grid();
+  if (p.early != 0 && warp > 1) wait_for_previous_grid();
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (elect_one()) {
-      int it = 0, s = 0;
+      int it = 0, s = 0, b_loaded = 0;  // stages whose part of B has been loaded
       uint32_t ph = 0;
       bool ok = true;
+      if (p.early == 1 && p.b_old && pair < p.items) {
+        int tm, tn, k0, k1;
+        p.tile(pair, tm, tn);
+        p.steps(pair, k0, k1);
+        b_loaded = min(kStages, k1 - k0);
+        for (int j = 0; j < b_loaded; ++j) {
+          if (rank == 0) mbar_arrive_expect_tx(&sm.full[j], 4 * kPairTileBytes);
+          load_pair_operand(sm.b[j], &tm_b, cluster_map(&sm.full[j], 0), k0 + j, tn * kPairN + (int)rank * kPairHalf, kStep, p.b_mn);
+        }
+      }
+      if (p.early == 1) wait_for_previous_grid();
       for (int t = pair; ok && t < p.items; t += pairs) {
         int tm, tn, k0, k1;
         p.tile(t, tm, tn);
@@ -203,10 +215,12 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
         for (int k = k0; k < k1; ++k, ++it) {
           if (!(ok = mbar_wait(&sm.empty[s], ph ^ 1, kStatusTimeoutEmpty, abort_flag, p.status))) break;
           // boxes are written, and counted, whole: zeros past the operands
-          if (rank == 0) mbar_arrive_expect_tx(&sm.full[s], 4 * kPairTileBytes);
           const uint32_t full = cluster_map(&sm.full[s], 0);
+          if (it >= b_loaded) {
+            if (rank == 0) mbar_arrive_expect_tx(&sm.full[s], 4 * kPairTileBytes);
+            load_pair_operand(sm.b[s], &tm_b, full, k, rb, kStep, p.b_mn);
+          }
           load_pair_operand(sm.a[s], &tm_a, full, k, ra, kStep, p.a_mn);
-          load_pair_operand(sm.b[s], &tm_b, full, k, rb, kStep, p.b_mn);
           if (++s == kStages) s = 0, ph ^= 1;
         }
       }
@@ -486,7 +500,7 @@ inline PairGemm pair_gemm(int64_t M, int64_t N, int64_t K, int bytes, bool a_mn,
   p.items = p.whole + (int)(tiles - p.whole) * p.split;
   p.a_mn = a_mn ? 1 : 0;
   p.b_mn = b_mn ? 1 : 0;
-  p.early = 0;
+  p.early = p.b_old = 0;
   p.status = device_status_ptr(device);
   return p;
 }

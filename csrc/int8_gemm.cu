@@ -535,6 +535,7 @@ void launch_pair(const Int8Matrix& a, const Int8Matrix& b, const Factors& f, at:
   const int64_t M = a.rows, N = b.rows;
   PairGemm p = pair_gemm(M, N, a.cols, 1, false, false, device);
   p.early = early ? 1 : 0;
+  p.b_old = 1;
   const CUtensorMap ma = code_map(a, kPairHalf), mb = code_map(b, kPairHalf);
   const OutRows out = out_rows(d.data_ptr(), N, M, N);
   const typename ScaleEpilogue<FP16>::Args args{out.tma ? out_rows_map(out) : ma, out, f};
