@@ -36,38 +36,55 @@ __device__ __forceinline__ float rcp_fast(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
-// 1 / (1 + 2^z): 2^z of 2^128 and more is infinity, and the quotient 0
-__device__ __forceinline__ float logistic2(float z) { return rcp_fast(1.f + ex2_approx(z)); }
+// 1 / (1 + 2^z) of two numbers: 2^z of 2^128 and more is infinity, and the quotient 0.
+__device__ __forceinline__ uint64_t logistic2(uint64_t z) {
+  const float2 v = f2_split(z);
+  const float2 d = f2_split(f2_add(f2(ex2_approx(v.x), ex2_approx(v.y)), f2(1.f, 1.f)));
+  return f2(rcp_fast(d.x), rcp_fast(d.y));
+}
+__device__ __forceinline__ uint64_t both(float v) { return f2(v, v); }
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kGeluA = -2.f * 0.7978845608028654f * kLog2e, kGeluB = 0.044715f;
+constexpr float kGeluC = 2.f * 0.7978845608028654f, kGeluA = -kGeluC * kLog2e, kGeluB = 0.044715f;
 
+// Two elements at a time, in packed arithmetic: act(v), or act(v, u) of value and gate.
 template <int ACT>
-__device__ __forceinline__ float act_value(float v, float u) {
-  if constexpr (ACT == kActGelu) return v * logistic2(kGeluA * v * fmaf(kGeluB * v, v, 1.f));
-  else if constexpr (ACT == kActSwiglu) return v * u * logistic2(-kLog2e * u);
-  else return v;
+__device__ __forceinline__ uint64_t act_value(uint64_t v, uint64_t u) {
+  if constexpr (ACT == kActGelu) {
+    const uint64_t z = f2_mul(v, f2_fma(f2_mul(v, v), both(kGeluA * kGeluB), both(kGeluA)));  // -2 u log2(e)
+    return f2_mul(v, logistic2(z));
+  } else if constexpr (ACT == kActSwiglu) {
+    return f2_mul(v, f2_mul(u, logistic2(f2_mul(u, both(-kLog2e)))));
+  } else {
+    return v;
+  }
 }
 
 // act(x') and da act'(x'): dv, and for a SwiGLU du.
 template <int ACT>
-__device__ __forceinline__ void act_backward(float da, float v, float u, float& a, float& dv, float& du) {
+__device__ __forceinline__ void act_backward(uint64_t da, uint64_t v, uint64_t u, uint64_t& a, uint64_t& dv, uint64_t& du) {
   if constexpr (ACT == kActGelu) {
-    const float w = kGeluB * v * v, p = logistic2(kGeluA * v * (1.f + w));
-    a = v * p;
-    // 2 u' = -kGeluA / log2(e) (1 + 3 w)
-    dv = da * fmaf(a * (1.f - p), (-kGeluA / kLog2e) * fmaf(3.f, w, 1.f), p);
-    du = 0.f;
+    const uint64_t s = f2_mul(v, v), p = logistic2(f2_mul(v, f2_fma(s, both(kGeluA * kGeluB), both(kGeluA))));
+    a = f2_mul(v, p);
+    const uint64_t rest = f2_sub(a, f2_mul(a, p)), slope = f2_fma(s, both(3.f * kGeluB * kGeluC), both(kGeluC));  // v p (1 - p), 2 u'
+    dv = f2_mul(da, f2_fma(rest, slope, p));
+    du = 0;
   } else if constexpr (ACT == kActSwiglu) {
-    const float p = logistic2(-kLog2e * u), up = u * p;
-    a = v * up;
-    dv = da * up;
-    du = da * v * fmaf(up, 1.f - p, p);
+    const uint64_t p = logistic2(f2_mul(u, both(-kLog2e))), up = f2_mul(u, p);
+    a = f2_mul(v, up);
+    dv = f2_mul(da, up);
+    du = f2_mul(f2_mul(da, v), f2_add(f2_sub(up, f2_mul(up, p)), p));
   } else {
     a = v;
     dv = da;
-    du = 0.f;
+    du = 0;
   }
+}
+
+template <bool FP16>
+__device__ __forceinline__ uint32_t pack16x2(uint64_t v) {
+  const float2 f = f2_split(v);
+  return pack16<FP16>(f.x, f.y);
 }
 
 // Kept input: H = 2 for a SwiGLU (row r's halves are rows 2 r and 2 r + 1 of the codes), else 1.
@@ -109,9 +126,8 @@ __global__ void __launch_bounds__(256) act_encode_kernel(EncodeParams p) {
       uint32_t o[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float2 a = f2_split(unit_pair(v[0], i)), b = f2_split(unit_pair(v[H - 1], i));
         if constexpr (ACT == kActNone) o[i] = v[0].w[i];
-        else o[i] = pack16<FP16>(act_value<ACT>(a.x, b.x), act_value<ACT>(a.y, b.y));
+        else o[i] = pack16x2<FP16>(act_value<ACT>(unit_pair(v[0], i), unit_pair(v[H - 1], i)));
       }
       st256(ar + col, o);
     }
@@ -141,20 +157,19 @@ __global__ void __launch_bounds__(256) act_decode_kernel(Kept kept, uint16_t* a,
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= R) return;
   for (int c = threadIdx.x * 4; c < F; c += blockDim.x * 4) {
-    float2 v[H][2];
+    uint64_t v[H][2];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       const int64_t r = row * H + h;
       const float s = int8_block_scale(__ldg(kept.exponents + r * nb + c / kInt8Block));
       uint64_t lo, hi;
       bytes_to_float(__ldg(reinterpret_cast<const uint32_t*>(kept.data + r * row_bytes + c)), lo, hi);
-      v[h][0] = f2_split(f2_mul(lo, f2(s, s)));
-      v[h][1] = f2_split(f2_mul(hi, f2(s, s)));
+      v[h][0] = f2_mul(lo, both(s));
+      v[h][1] = f2_mul(hi, both(s));
     }
     uint32_t o[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      o[i] = pack16<FP16>(act_value<ACT>(v[0][i].x, v[H - 1][i].x), act_value<ACT>(v[0][i].y, v[H - 1][i].y));
+    for (int i = 0; i < 2; ++i) o[i] = pack16x2<FP16>(act_value<ACT>(v[0][i], v[H - 1][i]));
     *reinterpret_cast<uint2*>(a + row * lda + c) = make_uint2(o[0], o[1]);
   }
 }
@@ -279,24 +294,23 @@ struct ActGradEpilogue {
     }
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      float2 x[H][2];
+      uint64_t x[H][2];
 #pragma unroll
       for (int h = 0; h < H; ++h) {
         const uint32_t bytes = w == 0 ? k[h].lo.x : w == 1 ? k[h].lo.y : w == 2 ? k[h].lo.z : w == 3 ? k[h].lo.w
                                : w == 4 ? k[h].hi.x : w == 5 ? k[h].hi.y : w == 6 ? k[h].hi.z : k[h].hi.w;
         uint64_t lo, hi;
         bytes_to_float(bytes, lo, hi);
-        x[h][0] = f2_split(f2_mul(lo, s[h]));
-        x[h][1] = f2_split(f2_mul(hi, s[h]));
+        x[h][0] = f2_mul(lo, s[h]);
+        x[h][1] = f2_mul(hi, s[h]);
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float a0, v0, u0, a1, v1, u1;
-        act_backward<ACT>(__uint_as_float(v[4 * w + 2 * j]), x[0][j].x, x[H - 1][j].x, a0, v0, u0);
-        act_backward<ACT>(__uint_as_float(v[4 * w + 2 * j + 1]), x[0][j].y, x[H - 1][j].y, a1, v1, u1);
-        oa[2 * w + j] = pack16<FP16>(a0, a1);
-        od[0][2 * w + j] = pack16<FP16>(v0, v1);
-        if constexpr (H == 2) od[1][2 * w + j] = pack16<FP16>(u0, u1);
+        uint64_t act, dv, du;
+        act_backward<ACT>(f2(__uint_as_float(v[4 * w + 2 * j]), __uint_as_float(v[4 * w + 2 * j + 1])), x[0][j], x[H - 1][j], act, dv, du);
+        oa[2 * w + j] = pack16x2<FP16>(act);
+        od[0][2 * w + j] = pack16x2<FP16>(dv);
+        if constexpr (H == 2) od[1][2 * w + j] = pack16x2<FP16>(du);
       }
     }
     auto store = [&](const OutRows& out, const CUtensorMap* map, const uint32_t (&o)[16]) {
@@ -345,19 +359,26 @@ __global__ void __launch_bounds__(kPartThreads) part_sum_kernel(const __grid_con
     store4<FP16>(p.out[0], m, n, v);
   } else {
     const int row_bytes = (int)int8_row_bytes(p.g.N), nb = row_bytes / kInt8Block;
-    float x[H][4];
+    uint64_t x[H][2];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       const int64_t r = (int64_t)m * H + h;
       const float s = int8_block_scale(__ldg(p.kept.exponents + r * nb + n / kInt8Block));
       uint64_t lo, hi;
       bytes_to_float(__ldg(reinterpret_cast<const uint32_t*>(p.kept.data + r * row_bytes + n)), lo, hi);
-      const float2 a = f2_split(f2_mul(lo, f2(s, s))), b = f2_split(f2_mul(hi, f2(s, s)));
-      x[h][0] = a.x, x[h][1] = a.y, x[h][2] = b.x, x[h][3] = b.y;
+      x[h][0] = f2_mul(lo, both(s));
+      x[h][1] = f2_mul(hi, both(s));
     }
     float act[4], dv[4], du[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) act_backward<ACT>(v[i], x[0][i], x[H - 1][i], act[i], dv[i], du[i]);
+    for (int j = 0; j < 2; ++j) {
+      uint64_t a2, v2, u2;
+      act_backward<ACT>(f2(v[2 * j], v[2 * j + 1]), x[0][j], x[H - 1][j], a2, v2, u2);
+      const float2 fa = f2_split(a2), fv = f2_split(v2), fu = f2_split(u2);
+      act[2 * j] = fa.x, act[2 * j + 1] = fa.y;
+      dv[2 * j] = fv.x, dv[2 * j + 1] = fv.y;
+      du[2 * j] = fu.x, du[2 * j + 1] = fu.y;
+    }
     store4<FP16>(p.out[0], m, n, dv);
     if constexpr (H == 2) store4<FP16>(p.out[1], m, n, du);
     if (p.want_act) store4<FP16>(p.act, m, n, act);
