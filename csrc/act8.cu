@@ -235,7 +235,7 @@ struct BiasEpilogue {
 template <bool FP16, int ACT>
 struct ActGradEpilogue {
   static constexpr int H = ACT == kActSwiglu ? 2 : 1;
-  static constexpr int kStages = 5, kWarps = 16, kOutBytes = 2048;
+  static constexpr int kStages = 6, kWarps = 16, kOutBytes = 2048;
   static constexpr bool kShared = false, kAhead = false;
   struct Args {
     CUtensorMap map_dx[H], map_a;

@@ -96,12 +96,12 @@ struct EpiPlace {
   uint32_t rank;
 };
 
-template <int STAGES, int WARPS, int OUT_BYTES>
+template <int STAGES, int WARPS, int OUT_BYTES, bool SHARED>
 struct PairGemmSmem {
   uint8_t a[STAGES][kPairTileBytes];
   uint8_t b[STAGES][kPairTileBytes];
   uint8_t out[WARPS][OUT_BYTES];
-  float2 col[2][kPairN];
+  float2 col[2][SHARED ? kPairN : 1];
   uint64_t full[STAGES], empty[STAGES];
   uint64_t acc_full[2], acc_free[2];
   uint64_t drain;
@@ -152,7 +152,7 @@ pair_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant
                  const PairGemm p) {
   constexpr int kStages = Epi::kStages, kWarps = Epi::kWarps, kGroups = kWarps / 4, kChunks = kPairN / 32 / kGroups;
   static_assert(!Epi::kShared || 32 * kWarps == kPairN, "a column a thread");
-  using Smem = PairGemmSmem<kStages, kWarps, Epi::kOutBytes>;
+  using Smem = PairGemmSmem<kStages, kWarps, Epi::kOutBytes, Epi::kShared>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   volatile int* abort_flag = &sm.abort_flag;
@@ -540,7 +540,7 @@ inline at::Tensor part_memory(const PairGemm& p, const at::TensorOptions& option
 template <Mma KIND, class Epi>
 void launch_pair_gemm(const CUtensorMap& a, const CUtensorMap& b, const at::Tensor& parts, const typename Epi::Args& args,
                       const PairGemm& p, int device, cudaStream_t stream) {
-  constexpr int smem = (int)sizeof(PairGemmSmem<Epi::kStages, Epi::kWarps, Epi::kOutBytes>) + 1024;
+  constexpr int smem = (int)sizeof(PairGemmSmem<Epi::kStages, Epi::kWarps, Epi::kOutBytes, Epi::kShared>) + 1024;
   static_assert(smem <= 232448 && Epi::kOutBytes >= 2048, "shared memory of an SM, of a part's rows");
   CUtensorMap mp = a;
   if (parts.defined()) {
