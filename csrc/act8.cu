@@ -282,7 +282,6 @@ struct ActGradEpilogue {
     n0 = tn * kPairN;
     load(at.group);
   }
-  __device__ __forceinline__ void met(int) {}
   __device__ __forceinline__ void chunk(int c, const uint32_t (&v)[32]) {
     const int nc = n0 + c * 32;
     Codes k[H];

@@ -51,9 +51,9 @@ __device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_
                "tcgen05.mma.cta_group::" GROUP ".kind::" TYPE " [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc),   \
                "l"(b_desc), "r"(idesc), "r"(accumulate)                                                                  \
                : "memory")
-  if constexpr (KIND == Mma::kI8 && CG == 1) DMAD_MMA("1", "i8");
+  static_assert(CG == 2 || KIND == Mma::kI8, "one CTA's MMAs: 8-bit integers (the few-rows product)");
+  if constexpr (CG == 1) DMAD_MMA("1", "i8");
   else if constexpr (KIND == Mma::kI8) DMAD_MMA("2", "i8");
-  else if constexpr (CG == 1) DMAD_MMA("1", "f16");
   else DMAD_MMA("2", "f16");
 #undef DMAD_MMA
 }
@@ -126,7 +126,7 @@ __device__ __forceinline__ void load_pair_operand(uint8_t* dst, const CUtensorMa
 //   Epi(args, gemm, place)
 //   first(item)                 before the first tile
 //   begin(item, next, parity)   before the tile's accumulator is waited for; next: the item after it, or -1
-//   met(next)                   behind the warps' barrier (kShared)
+//   met(next)                   behind the warps' barrier (kShared only)
 //   chunk(c, v)                 the accumulator's columns 32 c .. 32 c + 31 of the lane's row
 // (of a part only the calls that the barrier's warps share are made)
 // Columns 32 c .. of the lane's row of a part, through 2 KB of shared memory: twice 16 columns of 32 rows (64-byte swizzle).

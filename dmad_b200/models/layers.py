@@ -607,7 +607,7 @@ def quantize_int8_(module: nn.Module) -> int:
 def enable_act8(module: nn.Module, on: bool = True) -> int:
     """Makes every ``SegLinear`` of ``module`` keep its input in 8 bits for the backward pass (``SegLinear.act8``), or the
     16 bits that it was given; returns how many.  For blocks that are not recomputed: one under activation checkpointing
-    keeps nothing anyway."""
+    keeps nothing anyway.  On CUDA the layers are bf16 or fp16."""
     n = 0
     for m in module.modules():
         if isinstance(m, SegLinear):

@@ -37,7 +37,7 @@ _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 class Int8Tensor:
     """A matrix [R, K] in 8 bits (leading dimensions of ``shape`` are flattened into R).
 
-    ``data`` int8 [R, ceil(K / 32) * 32], zeros past K.  ``scale``: fp32 [R] (``block`` 0), or uint8 [R, ceil(K / 32)],
+    ``data`` int8 [R, ceil(K / 32) * 32], from -127 to 127 (what is stored past K is not used).  ``scale``: fp32 [R] (``block`` 0), or uint8 [R, ceil(K / 32)],
     the exponent plus 127 of each block's power of two, 255 for NaN (``block`` 32)."""
 
     data: torch.Tensor

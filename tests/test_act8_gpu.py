@@ -269,3 +269,36 @@ def test_differentiable_once_and_refusals():
     dx, = torch.autograd.grad(ops.linear_act8(x, w).float().square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once"):
         dx.sum().backward()
+
+
+def test_steps_one_behind_the_other():
+    """Steps whose kernels overlap, over memory that the steps before have just freed: the results of steps that are waited
+    for."""
+    ops = _ops()
+    cases = []
+    for i, (R, N, F, act) in enumerate([(300, 1280, 2048, None), (1001, 777, 1543, "gelu_tanh"), (64, 96, 200, "swiglu"), (2500, 2600, 1300, None),
+                                        (3000, 512, 4104, "gelu_tanh"), (1500, 1000, 3001, "swiglu")]):
+        x, w, b, g = _inputs(R, N, F, act, torch.bfloat16, torch.float32, i)
+        torch.cuda.synchronize()
+        out = _run(ops, x, w, b, g, act)
+        torch.cuda.synchronize()
+        cases.append(((x, w, b, g, act), [t.detach() for t in out]))
+    wrong = torch.zeros((), device=dev, dtype=torch.int64)
+    for i in torch.randint(0, len(cases), (150,), generator=torch.Generator().manual_seed(2)).tolist():
+        args, want = cases[i]
+        for t, ref in zip(_run(ops, *args), want):
+            wrong += (t.detach() != ref).sum()
+    assert int(wrong) == 0
+    ops.check_device_status()
+
+
+def test_frozen_weight_and_shared_leaves():
+    ops = _ops()
+    x, w, b, g = _inputs(200, 64, 96, None, torch.bfloat16, torch.float32, 4)
+    full = _run(ops, x, w, b, g, None)
+    frozen = ops.linear_act8(x, w.detach())
+    assert torch.equal(torch.autograd.grad(frozen, x, g)[0], full[1])
+    # one input through two layers of one weight: the gradients add up
+    y = ops.linear_act8(x, w, b) + ops.linear_act8(x, w, b)
+    got = torch.autograd.grad(y, (x, w, b), g)
+    assert all(torch.equal(p, 2 * q) for p, q in zip(got, full[1:]))

@@ -264,3 +264,51 @@ def test_rows_that_start_anywhere(K, dtype):
     for start in range(0, 18):  # one row: coded within the product
         x = line[start:start + K]
         assert torch.equal(ops.int8_linear(x, w), ops.int8_linear(ops.quantize_int8(x), w, None, torch.bfloat16))
+
+
+def test_offsets_past_32_bits():
+    ops = _ops()
+    R, K = 70000, 32768  # 2.3e9 elements
+    x = torch.zeros(R, K, dtype=torch.bfloat16, device=dev)
+    rows = [0, 1, 65535, 65536, 65537, R - 1]
+    part = torch.randn(len(rows), K, device=dev).to(torch.bfloat16)
+    x[rows] = part
+    for block in (0, 32):
+        q = ops.quantize_int8(x, block)
+        ref = ops.quantize_int8(part, block)
+        assert torch.equal(q.data[rows], ref.data) and torch.equal(q.scale[rows], ref.scale)
+        assert torch.equal(ops.dequantize_int8(q)[rows], ops.dequantize_int8(ref))
+        del q
+    del x
+    torch.cuda.empty_cache()
+    w = ops.quantize_int8(torch.randn(K, 64, device=dev))
+    x = torch.randn(R, 64, device=dev, dtype=torch.bfloat16)
+    y = ops.int8_linear(x, w)  # 2.3e9 outputs
+    for r in (0, 65535, 65536, R - 200):
+        assert torch.equal(y[r:r + 200], ops.int8_linear(x[r:r + 200].contiguous(), w))
+    del y
+    torch.cuda.empty_cache()
+
+
+def test_calls_one_behind_the_other():
+    """Calls whose kernels overlap, over memory that the calls before have just freed: the results of calls that are waited for."""
+    ops = _ops()
+    g = torch.Generator().manual_seed(9)
+    shapes = [(1, 700, 500), (40, 1000, 4000), (200, 300, 5000), (300, 2500, 1001), (1200, 5200, 640), (2600, 2600, 2600)]
+    args = [(torch.randn(M, K, generator=g).to(torch.bfloat16).to(dev), ops.quantize_int8(torch.randn(N, K, generator=g).to(dev)),
+             torch.randn(N, generator=g).to(dev)) for M, N, K in shapes]
+    want = []
+    for x, w, b in args:
+        torch.cuda.synchronize()
+        want.append((ops.int8_linear(x, w, b), ops.dequantize_int8(ops.quantize_int8(x, 32))))
+    torch.cuda.synchronize()
+    order = torch.randint(0, len(shapes), (300,), generator=g).tolist()
+    wrong = torch.zeros((), device=dev, dtype=torch.int64)
+    for i in order:
+        x, w, b = args[i]
+        y, z = ops.int8_linear(x, w, b), ops.dequantize_int8(ops.quantize_int8(x, 32))
+        wrong += (y != want[i][0]).sum() + (z != want[i][1]).sum()
+        del y, z
+    assert int(wrong) == 0
+    kept = [(i, ops.int8_linear(*args[i])) for i in order[:100]]
+    assert all(torch.equal(y, want[i][0]) for i, y in kept)
