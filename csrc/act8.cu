@@ -311,7 +311,8 @@ struct ActGradEpilogue {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         uint64_t act, dv, du;
-        act_backward<ACT>(f2(__uint_as_float(v[4 * w + 2 * j]), __uint_as_float(v[4 * w + 2 * j + 1])), x[0][j], x[H - 1][j], act, dv, du);
+        const uint64_t da = f2(__uint_as_float(v[4 * w + 2 * j]), __uint_as_float(v[4 * w + 2 * j + 1]));
+        act_backward<ACT>(da, x[0][j], x[H - 1][j], act, dv, du);
         oa[2 * w + j] = pack16x2<FP16>(act);
         od[0][2 * w + j] = pack16x2<FP16>(dv);
         if constexpr (H == 2) od[1][2 * w + j] = pack16x2<FP16>(du);
@@ -568,9 +569,14 @@ void product_typed(const Operand& A, const Operand& B, const Result& r, int devi
 void product(const Operand& A, const Operand& B, const Result& r, cudaStream_t stream) {
   const bool fp16 = A.t.scalar_type() == at::kHalf;
   const int device = A.t.get_device();
-  if (r.act == kActGelu) fp16 ? product_typed<true, kActGelu>(A, B, r, device, stream) : product_typed<false, kActGelu>(A, B, r, device, stream);
-  else if (r.act == kActSwiglu) fp16 ? product_typed<true, kActSwiglu>(A, B, r, device, stream) : product_typed<false, kActSwiglu>(A, B, r, device, stream);
-  else fp16 ? product_typed<true, kActNone>(A, B, r, device, stream) : product_typed<false, kActNone>(A, B, r, device, stream);
+  auto typed = [&](auto act) {
+    constexpr int ACT = decltype(act)::value;
+    if (fp16) product_typed<true, ACT>(A, B, r, device, stream);
+    else product_typed<false, ACT>(A, B, r, device, stream);
+  };
+  if (r.act == kActGelu) typed(std::integral_constant<int, kActGelu>{});
+  else if (r.act == kActSwiglu) typed(std::integral_constant<int, kActSwiglu>{});
+  else typed(std::integral_constant<int, kActNone>{});
 }
 
 

@@ -60,7 +60,8 @@ struct LinearAct8 : torch::autograd::Function<LinearAct8> {
 at::Tensor linear_act8(const at::Tensor& x, const at::Tensor& w, OptTensor bias, int64_t act) {
   act8_check(x, w, bias, act);
   const bool db = bias.has_value() && bias->defined() && bias->requires_grad();
-  if (!at::GradMode::is_enabled() || !(x.requires_grad() || w.requires_grad() || db)) return std::get<0>(act8_forward(x, w, bias, act, false));
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || w.requires_grad() || db))
+    return std::get<0>(act8_forward(x, w, bias, act, false));
   // the input is kept for the weight's gradient, and for the activation's derivative
   return LinearAct8::apply(x, w, bias, act, w.requires_grad() || (act != kActNone && x.requires_grad()));
 }

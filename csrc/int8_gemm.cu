@@ -575,9 +575,14 @@ void launch_vector(const void* x, at::ScalarType type, const float* x_scale, con
                  (int)b.rows, (int)b.cols};
   const bool aligned = b.cols % 16 == 0 && reinterpret_cast<uintptr_t>(x) % 32 == 0;
   const int device = d.get_device();
+  auto typed = [&](auto tag) {
+    using T = decltype(tag);
+    if (aligned) launch_vector_as<T, true>(p, device, stream);
+    else launch_vector_as<T, false>(p, device, stream);
+  };
   if (type == at::kChar) launch_vector_as<int8_t, true>(p, device, stream);
-  else if (type == at::kHalf) aligned ? launch_vector_as<__half, true>(p, device, stream) : launch_vector_as<__half, false>(p, device, stream);
-  else aligned ? launch_vector_as<__nv_bfloat16, true>(p, device, stream) : launch_vector_as<__nv_bfloat16, false>(p, device, stream);
+  else if (type == at::kHalf) typed(__half{});
+  else typed(__nv_bfloat16{});
 }
 
 // d [a.rows, b.rows] (bf16 or fp16, contiguous) = a b^T + bias, on the current device and stream.  early: the kernel before
