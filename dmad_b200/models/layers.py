@@ -32,6 +32,7 @@ import torch.nn.functional as F
 from .. import ops
 from ..ops import attention as attn_ops
 from ..ops import norm as norm_ops
+from .sac import inside_checkpoint
 
 
 # ----------------------------------------------------------------------------- spectral norm helpers
@@ -370,8 +371,10 @@ class SegLinear(nn.Module):
         return F.linear(x, w, b)
 
     def _keeps_act8(self):
-        """Whether ``forward`` keeps its input in 8 bits: not under ``torch.no_grad``, with an adapter or coded weights."""
-        return self.act8 and not self.lora_rank and self.weight is not None and torch.is_grad_enabled()
+        """Whether ``forward`` keeps its input in 8 bits: not under ``torch.no_grad``, with an adapter or coded weights, or in
+        a block that is computed again for the backward pass."""
+        return (self.act8 and not self.lora_rank and self.weight is not None and torch.is_grad_enabled()
+                and not inside_checkpoint())
 
     # ------------------------------------------------------------------ state dict (per-segment keys)
     def _split_prefix(self, prefix):
@@ -606,8 +609,8 @@ def quantize_int8_(module: nn.Module) -> int:
 
 def enable_act8(module: nn.Module, on: bool = True) -> int:
     """Makes every ``SegLinear`` of ``module`` keep its input in 8 bits for the backward pass (``SegLinear.act8``), or the
-    16 bits that it was given; returns how many.  For blocks that are not recomputed: one under activation checkpointing
-    keeps nothing anyway.  On CUDA the layers are bf16 or fp16."""
+    16 bits that it was given; returns how many.  For blocks that are not recomputed: those under ``checkpoint_block`` keep
+    nothing, and run as without it.  On CUDA the layers are bf16 or fp16."""
     n = 0
     for m in module.modules():
         if isinstance(m, SegLinear):

@@ -12,10 +12,14 @@ Parity: train/wan/rcm/utils/selective_activation_checkpoint.py:26-74.
 * ``"block_int8"`` (not in the reference): as ``"block_wise"``, with the block's first input, its hidden states, kept in
   8-bit integers of which 32 columns share a power of two (``ops.quantize_int8(x, 32)``): half the memory, and gradients at
   the decoded input.  The forward pass is not changed.
+
+Layers that keep their inputs in 8 bits (``SegLinear.act8``) run as plain ones inside of a block under any of the policies, in
+its forward pass and in its recomputation: what they would keep is thrown away, and ``mm_only`` keeps library products only.
 """
 from __future__ import annotations
 
 import functools
+import threading
 
 import torch
 from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
@@ -65,8 +69,28 @@ def _checkpoint_int8(fn, x, *args):
     return y
 
 
+_inside = threading.local()  # (a backward pass recomputes in threads of its own)
+
+
+def inside_checkpoint() -> bool:
+    """Whether the calling thread is in a block that ``checkpoint_block`` runs, the first time or again."""
+    return getattr(_inside, "depth", 0) > 0
+
+
+def _marked(fn):
+    def run(*args):
+        _inside.depth = getattr(_inside, "depth", 0) + 1
+        try:
+            return fn(*args)
+        finally:  # a recomputation ends in an exception, once it has what the backward pass wants
+            _inside.depth -= 1
+
+    return run
+
+
 def checkpoint_block(fn, *args, policy: str = "block_wise"):
     """``fn(*args)`` under activation checkpointing with the given policy (non-reentrant)."""
+    fn = _marked(fn)
     if policy == "mm_only":
         return checkpoint(fn, *args, use_reentrant=False, context_fn=mm_only_context)
     if policy == "block_int8":
