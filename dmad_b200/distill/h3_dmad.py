@@ -284,7 +284,9 @@ class H3DMAD:
         sig = (shift_sigma(base, self.cfg.video_shift), shift_sigma(base, self.cfg.audio_shift))
         xg = self.add_noise(G, (torch.randn_like(G[0]), torch.randn_like(G[1])), sig)
         self._freeze_critic(True)
-        self.fake.eval()
+        # sharded blocks are checkpointed here too: autograd would keep views of a gathered copy that the weights of a later
+        # block overwrite
+        self.fake.train(self.cfg.shard_weights)
         try:
             d_r, d_t = self.critic_logits(xg, sig, cond)
             w, E_w = self.gap.weights(torch.tensor([self.sigma_band(sig[0])]))
