@@ -32,6 +32,7 @@ from ..algorithms import CriticHeads, GapRouter, PowerEMA, critic_bce_loss, gene
 from ..algorithms.dmad import NUM_GAP_BANDS
 from ..inference.h3 import H3Geometry, build_packed_sequence, build_row_timesteps, latent_shape_of, shift_sigma
 from ..models.h3 import H3Config, H3Model
+from ..models.layers import warn_without_act8_layers
 from ..ops.optim import FusedAdamW
 from ..parallel.dist import broadcast_module, get_world_size
 from ..parallel.dp import GradSync
@@ -64,7 +65,10 @@ class H3DMADConfig:
     head_wd: float = 0.01
     gradient_checkpointing: bool = True
     checkpoint_policy: str = "block_wise"  # "mm_only": keep matmul / attention outputs; "block_int8": block inputs in 8 bits
-    act8: bool = False                # without checkpointing: linear layers without LoRA keep their inputs in 8 bits
+    # the blocks' linear layers keep their inputs in 8 bits: those without LoRA, in blocks that are not checkpointed.  That is
+    # a critic with fake_train_type "full", with gradient_checkpointing in the student's stage only (a warning where no
+    # layer is left)
+    act8: bool = False
     fused_qk_norm: bool = False       # q / k norms and RoPE as one kernel, forward and backward
     text_tokens: int = 256
     model_dir: str | None = None      # H3 release folder: transformer/config.json sets ``model``, shards load
@@ -143,6 +147,9 @@ class H3DMAD:
         if cfg.gradient_checkpointing:
             self.student.checkpoint_blocks = len(self.student.transformer_blocks)
             self.fake.checkpoint_blocks = len(self.fake.transformer_blocks)
+        if cfg.act8:  # (the student's stage checkpoints no block of the critic, unless they are sharded)
+            warn_without_act8_layers((self.student.transformer_blocks, self.student.checkpoint_blocks),
+                                     (self.fake.transformer_blocks, self.fake.checkpoint_blocks if cfg.shard_weights else 0))
         self.heads = CriticHeads(cfg.model.dim, rms_input=True).to(self.device, torch.float32)
         for m in (self.student, self.fake, self.heads):
             broadcast_module(m)

@@ -33,6 +33,7 @@ from ..algorithms import (CriticHeads, GapRouter, TrigFlowScaling, UniformShift,
                           ema_exp_coefficient, generator_linear_loss, rf_to_trig_time, trig_to_rf_time)
 from ..algorithms.dmad import band_of_cdf, critic_accuracies
 from ..algorithms.spectral import apply_spectral_norm
+from ..models.layers import warn_without_act8_layers
 from ..models.wan import WanConfig, WanModel, WAN_1P3B
 from ..ops.optim import FusedAdamW
 from ..parallel.dist import broadcast_module
@@ -74,7 +75,8 @@ class WanDMADConfig:
     # "mm_only": keep matmul / attention outputs; "block_int8": block inputs in 8 bits
     checkpoint_student_policy: str = "block_wise"
     checkpoint_critic_policy: str = "block_wise"
-    # linear layers of the blocks that are not checkpointed keep their inputs in 8 bits (those with LoRA: as they are)
+    # linear layers of the blocks that are not checkpointed keep their inputs in 8 bits (those with LoRA: as they are; a
+    # warning where no layer is left)
     act8: bool = False
     rectified_flow_t_scaling_factor: float = 1000.0
     # rCM consistency term (0 = pure DMAD, as the reference's DMAD experiments; > 0 adds the sCM /
@@ -192,6 +194,10 @@ class WanDMAD(nn.Module):
                 cfg.checkpoint_student_blocks = nl
                 self.net.checkpoint_blocks = nl
                 self.fsdp["student"] = ShardedTrainableBlocks(self.net.blocks, lr=cfg.lr, ema=cfg.ema_enabled, **kw_b)
+        if cfg.act8:
+            phases = (cfg.checkpoint_critic_blocks, cfg.checkpoint_critic_blocks_student_phase)
+            warn_without_act8_layers((self.net.blocks, self.net.checkpoint_blocks),
+                                     (self.net_fake_score.blocks, min(n for n in phases if n is not None)))
         self.gap = GapRouter("allreduce", tau=cfg.gap_tau, beta=cfg.gap_ema_beta, enabled=cfg.gap_route).to(device)
         self.scaling = TrigFlowScaling(1.0, cfg.rectified_flow_t_scaling_factor)
         self.p_D = LogNormal(*cfg.p_D_lognormal) if cfg.p_D_lognormal else UniformShift(cfg.p_D_shift)

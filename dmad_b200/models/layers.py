@@ -23,6 +23,7 @@
 from __future__ import annotations
 
 import math
+import warnings
 from typing import Sequence
 
 import torch
@@ -617,6 +618,19 @@ def enable_act8(module: nn.Module, on: bool = True) -> int:
             m.act8 = bool(on)
             n += 1
     return n
+
+
+def act8_layers(blocks, checkpointed: int = 0) -> int:
+    """How many layers of ``blocks`` keep their inputs in 8 bits while the first ``checkpointed`` blocks are computed again
+    for the backward pass."""
+    return sum(m.act8 and not m.lora_rank for b in list(blocks)[checkpointed:] for m in b.modules() if isinstance(m, SegLinear))
+
+
+def warn_without_act8_layers(*nets):
+    """Warns where none of the ``(blocks, checkpointed)`` has such a layer: ``act8`` was asked for and does nothing."""
+    if not any(act8_layers(*n) for n in nets):
+        warnings.warn("act8 reaches no layer: every block is activation-checkpointed or has LoRA adapters on its layers",
+                      stacklevel=3)
 
 
 class _CrossAttnCore(torch.autograd.Function):
