@@ -68,7 +68,10 @@ __device__ __forceinline__ uint64_t act_value(uint64_t v, uint64_t u) {
 template <int ACT>
 __device__ __forceinline__ void act_backward(uint64_t da, uint64_t v, uint64_t u, uint64_t& a, uint64_t& dv, uint64_t& du) {
   if constexpr (ACT == kActGelu) {
-    const uint64_t s = f2_mul(v, v), p = logistic2(f2_mul(v, f2_fma(s, both(kGeluA * kGeluB), both(kGeluA))));
+    // v v is bounded, so that slope stays finite where rest is 0: for |v| above 11, p is 0 or 1
+    const float2 vv = f2_split(f2_mul(v, v));
+    const uint64_t s = f2(fminf(vv.x, 1024.f), fminf(vv.y, 1024.f));
+    const uint64_t p = logistic2(f2_mul(v, f2_fma(s, both(kGeluA * kGeluB), both(kGeluA))));
     a = f2_mul(v, p);
     const uint64_t rest = f2_sub(a, f2_mul(a, p)), slope = f2_fma(s, both(3.f * kGeluB * kGeluC), both(kGeluC));  // v p (1 - p), 2 u'
     dv = f2_mul(da, f2_fma(rest, slope, p));

@@ -13,6 +13,8 @@ checkpoint policy keeps whole blocks' inputs in the same code.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -32,6 +34,14 @@ def _act(h: torch.Tensor, act):
         v, u = h.chunk(2, dim=-1)
         return v * F.silu(u)
     return h
+
+
+def _gelu_slope(v: torch.Tensor):
+    """The derivative of gelu_tanh, 1 or 0 for far values of either sign (the library's is NaN where v v overflows)."""
+    s = (v * v).clamp(max=1024.0)  # above, p (1 - p) is 0
+    u = (2 / math.pi) ** 0.5 * v * (1 + 0.044715 * s)
+    p = torch.sigmoid(2 * u)
+    return p + p * (1 - p) * v * (2 * (2 / math.pi) ** 0.5) * (1 + 3 * 0.044715 * s)
 
 
 def _kept(x2: torch.Tensor, act):
@@ -64,7 +74,9 @@ class _LinearAct8Reference(torch.autograd.Function):
             v = dequantize_int8_reference(Int8Tensor(data, scale, 32, (data.shape[0], w.shape[1]))).reshape(g2.shape[0], shape[-1])
         if ctx.needs_input_grad[0]:
             da = g2 @ w.float()
-            if act is not None:
+            if act == "gelu_tanh":
+                da = da * _gelu_slope(v)
+            elif act is not None:
                 with torch.enable_grad():
                     at = v.detach().requires_grad_(True)
                     da, = torch.autograd.grad(_act(at, act), at, da)
