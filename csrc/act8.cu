@@ -80,7 +80,7 @@ __device__ __forceinline__ void act_backward(uint64_t da, uint64_t v, uint64_t u
     const uint64_t p = logistic2(f2_mul(u, both(-kLog2e))), up = f2_mul(u, p);
     a = f2_mul(v, up);
     dv = f2_mul(da, up);
-    du = f2_mul(f2_mul(da, v), f2_add(f2_sub(up, f2_mul(up, p)), p));
+    du = f2_mul(f2_mul(da, f2_add(f2_sub(up, f2_mul(up, p)), p)), v);  // (da v may be larger than fp32 where the slope is 0)
   } else {
     a = v;
     dv = da;

@@ -44,6 +44,14 @@ def _gelu_slope(v: torch.Tensor):
     return p + p * (1 - p) * v * (2 * (2 / math.pi) ** 0.5) * (1 + 3 * 0.044715 * s)
 
 
+def _swiglu_backward(da: torch.Tensor, h: torch.Tensor):
+    """da times the derivatives of value * silu(gate), for far values too: da value is not formed, which may overflow where
+    the gate's slope is 0."""
+    v, u = h.chunk(2, dim=-1)
+    p = torch.sigmoid(u)
+    return torch.cat([da * (u * p), da * (p + u * p * (1 - p)) * v], dim=-1)
+
+
 def _kept(x2: torch.Tensor, act):
     """Codes of rows x2, a SwiGLU's halves as rows of their own."""
     rows = x2.reshape(-1, x2.shape[1] // 2) if act == "swiglu" else x2
@@ -76,10 +84,8 @@ class _LinearAct8Reference(torch.autograd.Function):
             da = g2 @ w.float()
             if act == "gelu_tanh":
                 da = da * _gelu_slope(v)
-            elif act is not None:
-                with torch.enable_grad():
-                    at = v.detach().requires_grad_(True)
-                    da, = torch.autograd.grad(_act(at, act), at, da)
+            elif act == "swiglu":
+                da = _swiglu_backward(da, v)
             dx = da.to(g.dtype).reshape(shape)
         if ctx.needs_input_grad[1]:
             dw = (g2.t() @ _act(v, act)).to(w.dtype)
