@@ -76,7 +76,7 @@ class _LinearAct8Reference(torch.autograd.Function):
     def backward(ctx, g):
         w, data, scale = ctx.saved_tensors
         act, shape, bias_type = ctx.cfg
-        g2 = g.reshape(-1, w.shape[0]).float()
+        g2 = g.reshape(g.shape[:-1].numel(), w.shape[0]).float()
         dx = dw = db = None
         if data is not None:
             v = dequantize_int8_reference(Int8Tensor(data, scale, 32, (data.shape[0], w.shape[1]))).reshape(g2.shape[0], shape[-1])
