@@ -270,9 +270,9 @@ __global__ void __launch_bounds__(kVectorThreads, kVectorBlocks) int8_vector_ker
 }
 
 // ---------------------------------------------------------------- few rows
-// For few rows of x, D^T = B A^T: 128 rows of the weight B are the MMA's 128 rows and a tile of x's rows its N, so one
-// token costs a tile of 32 columns, and the K loop of a tile is split over a cluster of up to six CTAs.  Each leaves its
-// int32 part in its shared memory, [column of x's tile][128 rows], and adds a share of the columns over all parts (exactly,
+// For few rows of x, D^T = B A^T: 128 rows of the weight B are the MMA's 128 rows and x's rows its N, so up to 32
+// tokens cost a tile of 32 columns, and the K loop of a tile is split over a cluster of up to six CTAs.  Each leaves its
+// int32 part in its shared memory, [row of x][128 rows], and adds a share of the columns over all parts (exactly,
 // whatever the order), applies factors and bias and stores runs of the output row.
 //   warp 0      producer (a ring of as many stages as fit); with `early` the grid was launched to overlap the quantiser of
 //               x: the weight's part of the first stages is loaded before waiting for it
@@ -299,9 +299,8 @@ struct SmallParams {
   bool rows8;        // D's rows start on 8 bytes
   int M, N;          // rows of x, rows of the weight
   int ksteps, k_last;
-  int bn;            // rows of x of a tile: a multiple of 32 up to 128, and 128 where there are several tiles
+  int bn;            // rows of x, up to a multiple of 32
   int stages, stage_bytes;
-  int tiles_x;       // tiles along x
   int split, per_split;  // CTAs of a cluster, K steps of each
   int early;
   int* status;
@@ -315,10 +314,8 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_co
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   volatile int* abort_flag = &sm.abort_flag;
   const int warp = warp_id(), lane = lane_id();
-  const int tile = blockIdx.x / p.split, rank = blockIdx.x % p.split;  // rank = rank in the cluster
-  const int tw = tile / p.tiles_x, tx = tile % p.tiles_x;
+  const int tw = blockIdx.x / p.split, rank = blockIdx.x % p.split;  // tile of the weight's rows, rank in the cluster
   const int k0 = rank * p.per_split, steps = max(0, min(p.ksteps, k0 + p.per_split) - k0);
-  const int x0 = tx * p.bn;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSmallStages; ++s) {
@@ -350,7 +347,7 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_co
         tma_load_2d(ring + s * p.stage_bytes, &tm_w, &sm.full[s], (k0 + i) * kBK, tw * kBM);
       };
       auto load_x = [&](int i, int s) {
-        tma_load_2d(ring + s * p.stage_bytes + kABytes, &tm_x, &sm.full[s], (k0 + i) * kBK, x0);
+        tma_load_2d(ring + s * p.stage_bytes + kABytes, &tm_x, &sm.full[s], (k0 + i) * kBK, 0);
       };
       const int first = min(steps, p.stages);
       for (int i = 0; i < first; ++i) load_w(i, i);
@@ -425,7 +422,7 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_co
   }
   // this CTA's share of x's rows: a warp takes eight of them at a time (that many loads in flight), a lane four weight
   // rows of each
-  const int per = (p.bn + p.split - 1) / p.split, c_end = min(min(p.bn, p.M - x0), (rank + 1) * per);
+  const int per = (p.bn + p.split - 1) / p.split, c_end = min(p.M, (rank + 1) * per);
   constexpr int kWarps = kSmallThreads / 32, kRows = 8;
   const int n = tw * kBM + lane * 4;
   float2 cf[4];
@@ -455,7 +452,7 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_co
     for (int u = 0; u < kRows; ++u) {
       const int c = c0 + u * kWarps;
       if (c >= c_end || n >= p.N) continue;
-      const float ra = p.f.ra[x0 + c];
+      const float ra = p.f.ra[c];
       const bool far = far_out(ra);
       float y[4];
 #pragma unroll
@@ -463,7 +460,7 @@ int8_gemm_small_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_co
         const float s = __int2float_rn(v[u][q]);
         y[q] = far ? apply_factors_far(s, ra, cf[q].x, cf[q].y) : apply_factors(s, ra, cf[q].x, cf[q].y);
       }
-      uint16_t* d = static_cast<uint16_t*>(p.d) + (int64_t)(x0 + c) * p.ldd + n;
+      uint16_t* d = static_cast<uint16_t*>(p.d) + (int64_t)c * p.ldd + n;
       const uint32_t lo = p.out_fp16 ? pack16<true>(y[0], y[1]) : pack16<false>(y[0], y[1]);
       const uint32_t hi = p.out_fp16 ? pack16<true>(y[2], y[3]) : pack16<false>(y[2], y[3]);
       if (p.rows8) {
@@ -504,14 +501,13 @@ void launch_small(const Int8Matrix& a, const Int8Matrix& b, const Factors& f, at
   p.N = (int)b.rows;
   p.ksteps = (int)((a.cols + kBK - 1) / kBK);
   p.k_last = (int)((a.cols - (int64_t)(p.ksteps - 1) * kBK + 31) / 32);
-  p.tiles_x = (p.M + kSmallBN - 1) / kSmallBN;
-  p.bn = p.tiles_x > 1 ? kSmallBN : (p.M + 31) / 32 * 32;
+  p.bn = (p.M + 31) / 32 * 32;
   p.stage_bytes = kABytes + p.bn * 128;
   p.stages = std::min(kSmallStages, (kSmallSmem - 1024) / p.stage_bytes);
   // CTAs for up to four fifths of the places (two an SM): above that, and with clusters of more than six, they no longer
   // all run at once
-  const int tiles = ((p.N + kBM - 1) / kBM) * p.tiles_x;
-  p.split = std::max(1, std::min({6, sms * 2 * 4 / 5 / std::max(tiles, 1), p.ksteps}));
+  const int tiles = (p.N + kBM - 1) / kBM;
+  p.split = std::max(1, std::min({6, sms * 2 * 4 / 5 / tiles, p.ksteps}));
   p.per_split = (p.ksteps + p.split - 1) / p.split;
   p.early = early ? 1 : 0;
   p.status = device_status_ptr(device);
