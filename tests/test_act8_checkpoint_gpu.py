@@ -22,7 +22,7 @@ def test_checkpointed_blocks_keep_no_codes(policy, blocks, monkeypatch):
     ref.checkpoint_blocks, ref.checkpoint_policy = blocks, policy
     yr, gr = _step(ref)
     assert len(calls) == 7 * (2 - blocks)
-    if blocks == 2:  # the same kernels throughout; (the sums of attention's dQ take any order)
-        assert torch.equal(y, yr) and (g - gr).norm() <= 1e-3 * gr.norm()
+    if blocks == 2:  # the same kernels throughout (but attention's dQ is summed in any order, and then rounded: a step of bf16)
+        assert torch.equal(y, yr) and (g - gr).norm() <= 2.0 ** -7 * gr.norm()
     else:
         assert (y - yr).norm() <= 2e-2 * yr.norm() and 0 < (g - gr).norm() <= 5e-2 * gr.norm()
