@@ -16,9 +16,10 @@
 //               that product.
 // Few output tiles: the K steps of a tile are spread over several pairs, whose fp32 parts are added in order by a second
 // kernel, so that the sums are the same every time.
-// Measured, forward and backward in short runs: 32760 x 1536 -> 4608 1.03 ms (1.35 PFLOP/s), 32760 x 8960 -> 1536 with GELU 2.17
-// ms, 37966 x 15360 -> 5120 with SwiGLU 13.2 ms (1.36 PFLOP/s); bound by the tensor core (1.55 PFLOP/s in the plain products)
-// but for g W with few K steps, whose epilogue takes longer than its MMAs.  The coding pass: 32760 x 8960 GELU 230 us, 37966 x 15360
+// Measured, forward and backward in short runs on several cards: 32760 x 1536 -> 4608 1.03 to 1.09 ms (1.28 to 1.35 PFLOP/s),
+// 32760 x 8960 -> 1536 with GELU 2.17 to 2.30 ms, 37966 x 15360 -> 5120 with SwiGLU 13.2 to 15.9 ms (1.13 to 1.36 PFLOP/s); bound
+// by the tensor core (1.55 PFLOP/s in the plain products, less as the power limit takes the clock) but for g W with few K
+// steps, whose epilogue takes longer than its MMAs.  The coding pass: 32760 x 8960 GELU 230 us, 37966 x 15360
 // SwiGLU 690 us (6.7 TB/s).
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
@@ -238,8 +239,9 @@ struct BiasEpilogue {
 // dx = acc act'(x') and act(x'), from the accumulator (g W) and the kept codes.  Some thirty instructions an element, with
 // chains of dependent ones: sixteen warps, four a scheduler, and one copy of the code (eight warps with four unrolled
 // chunks: 32760 x 1536 -> 8960 GELU 826 us, stalled on results and on the instruction cache).  A lane reads its row's 32
-// codes of a chunk (one sector) while the chunk before is computed.  32760 x 1536 -> 8960: 745 us with the GELU's derivative, 920
-// us with the SwiGLU's, 610 us without any; 37966 x 5120 -> 15360 (four times as many K steps a tile) is bound by the MMAs.
+// codes of a chunk (one sector) while the chunk before is computed.  32760 x 1536 -> 8960: 740 to 762 us with the GELU's
+// derivative, 880 to 919 us with the SwiGLU's, 638 to 653 us without any (on two cards); 37966 x 5120 -> 15360 (four times as
+// many K steps a tile) is bound by the MMAs.
 template <bool FP16, int ACT>
 struct ActGradEpilogue {
   static constexpr int H = ACT == kActSwiglu ? 2 : 1;

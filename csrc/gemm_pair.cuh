@@ -472,8 +472,9 @@ inline CUtensorMap operand_map(const void* base, int64_t rows, int64_t K, int64_
   return bytes == 1 ? make_tmap_u8(base, 2, dims, strides, box) : make_tmap_bf16(base, 2, dims, strides, box);
 }
 
-// Parts of each tile of a round that fills no more than half of the pairs: as many as fill them, of four stages at least.
-// After whole rounds only where that saves twelve stages (some 3 us), for which the parts' kernel is paid.
+// Parts of each tile of a round that fills no more than half of the pairs: as many as fill them, of four stages on average at
+// least (all of one length but the last part, which may be shorter).  After whole rounds only where that saves twelve stages
+// (some 3 us), for which the parts' kernel is paid.
 inline int tile_split(int64_t tiles, int64_t stages, int pairs, bool only) {
   if (tiles == 0 || 2 * tiles > pairs) return 1;
   const int64_t split = std::max<int64_t>(1, std::min(pairs / tiles, stages / 4));

@@ -33,7 +33,8 @@ struct Factors {
 
 // ---------------------------------------------------------------- CTA pairs
 // Factors and bias on the accumulators of gemm_pair.cuh.  Bound by the tensor core (92 % busy at 8192 x 8192 x 8192): 3.2
-// POP/s there, 37966 x 30720 x 5120 3.9 ms in short runs and 4.4 ms over seconds, by the clock that the power limit leaves.
+// POP/s there, 37966 x 30720 x 5120 3.9 to 4.2 ms in short runs and 4.4 to 5.1 ms over seconds, by the card and the clock that
+// the power limit leaves.  N = 30719, whose rows of 16-bit results start off 16 bytes, 8 % more (4.48 against 4.16 ms).
 template <bool FP16>
 struct ScaleEpilogue {
   static constexpr int kStages = 6, kWarps = 8, kOutBytes = 2048;
@@ -144,9 +145,9 @@ __global__ void __launch_bounds__(kPartThreads) int8_part_sum_kernel(const __gri
 // products; no matrix instruction has to be fed, no second grid waits.  A row that two warps share is added up in shared
 // memory (whole numbers: the same in any order).  x is coded by every block for itself, from registers into shared memory (a
 // few KB from the L2), while the first loads of the weight are on their way.
-// 15360 x 5120: 13.9 us with the weight in the L2, 18 us without (the few-rows kernel behind a quantiser 15.2 and 20.5), some 6
-// us of it launch, coding and the last loads: 30720 rows take 11.7 us more (6.7 TB/s).  1536 x 1536 3.7 us (7.2).  Sixteen loads
-// in flight: 18.8 us; four blocks of 64 registers an SM, which spill: 24.3.
+// 15360 x 5120: 15.8 to 17.7 us with the weight in the L2, 17.6 us without (two rows, on the few-rows kernel behind a
+// quantiser: 15.4 and 18.8), some 6 us of it launch, coding and the last loads: 30720 rows take 11.9 us more (6.6 TB/s).  1536 x
+// 1536 3.7 us (two rows: 7.0).  Sixteen loads in flight: 18.8 us; four blocks of 64 registers an SM, which spill: 24.3.
 constexpr int kVectorThreads = 256, kVectorDepth = 8;
 constexpr int kVectorUnits = 4;                                            // units of 16 columns of x a thread
 constexpr int kVectorMaxK = kVectorThreads * kVectorUnits * 16;            // 16384
@@ -278,8 +279,8 @@ __global__ void __launch_bounds__(kVectorThreads, kVectorBlocks) int8_vector_ker
 //               x: the weight's part of the first stages is loaded before waiting for it
 //   warp 1      TMEM owner and MMAs
 //   warps 2..5  accumulator to shared memory; all warps add and store
-// Two CTAs fit an SM.  2 to 16 rows, 15360 x 5120: 15.2 to 16 us with the quantiser, the weight in the L2 (20.6 us without), bound by
-// the weight's bytes and the two kernels' latency; 128 x 5120 x 15360 24 us.
+// Two CTAs fit an SM.  2 to 16 rows, 15360 x 5120: 15.4 to 16.4 us with the quantiser, the weight in the L2 (18.8 to 19.3 us
+// without), bound by the weight's bytes and the two kernels' latency; 128 x 5120 x 15360 24.5 us (26.8).
 constexpr int kSmallThreads = 192, kSmallStages = 5;
 constexpr int kSmallBN = 128;
 

@@ -4,9 +4,10 @@
 // elements, one 16-byte store of codes); a row with one scale is held by one block in registers between its maximum and the
 // encoding (up to 32768 columns of 16 bits, 16384 of 32; longer rows are read twice).  Rows that do not start on 32
 // bytes are read, and written back, in the aligned pieces around a unit (row_units.cuh).
-// Measured at 37966 x 5120 bf16 (583 MB coded, 583 MB read back): blocks 88 us (6.6 TB/s), rows 137 us (4.25 TB/s: six rows
-// share an SM, each some 3 us from its first load over its maximum to its last store), inverse 88 us (6.6 TB/s); fp32 blocks
-// 138 us, rows 151 us (6.4 TB/s), inverse 146 us.  37966 x 5121 bf16: blocks 142 us, rows 194 us, inverse 142 to 152 us.
+// Measured at 37966 x 5120 bf16 (583 MB coded, 583 MB read back): blocks 88 to 91 us (6.4 to 6.6 TB/s), rows 137 to 140 us (4.2
+// TB/s: six rows share an SM, each some 3 us from its first load over its maximum to its last store), inverse 88 to 91 us;
+// fp32 blocks 138 to 140 us, rows 151 to 154 us (6.4 TB/s), inverse 146 to 148 us.  37966 x 5121: bf16 blocks 142 to 144 us,
+// rows 194 to 197 us, inverse 142 to 155 us; fp32 183, 251, 161 to 179 us.
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -109,7 +110,7 @@ void launch_quant(const QuantParams& p, cudaStream_t stream) {
     int8_quant_kernel<T, BLOCKS, ALIGNED, U><<<(unsigned)(((int64_t)p.R + ty - 1) / ty), dim3(tx, ty), 0, stream>>>(p);
   };
   // Two units a thread keep the rows of up to 16384 columns in one block of 512 threads.  (37966 x 5120 bf16, one scale a
-  // row: 137 us; one unit a thread in 42 registers 217 us, four in 64, which spill, 168 us.)
+  // row: 137 to 140 us; one unit a thread in 42 registers 217 us, four in 64, which spill, 168 us.)
   if constexpr (BLOCKS || UPT == 2) {
     go(std::integral_constant<int, 2>{});
   } else {

@@ -319,7 +319,7 @@ class H3Model(nn.Module):
 
     def enable_act8(self, on: bool = True) -> int:
         """The blocks' projections keep their inputs (the SwiGLU's: its value and gate) in 8 bits for the backward pass;
-        those with a LoRA adapter keep them as they are."""
+        those with a LoRA adapter, and blocks under activation checkpointing, run as without it."""
         return enable_act8(self.transformer_blocks, on)
 
     def lora_linears(self, targets=("to_q", "to_k", "to_v", "to_out.0", "ff.net.0.proj", "ff.net.2")):

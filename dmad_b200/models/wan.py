@@ -377,7 +377,7 @@ class WanModel(nn.Module):
 
     def enable_act8(self, on: bool = True) -> int:
         """The blocks' linear layers keep their inputs (the feed-forward's: what the GELU reads) in 8 bits for the backward
-        pass; those with a LoRA adapter keep them as they are."""
+        pass; those with a LoRA adapter, and blocks under activation checkpointing, run as without it."""
         return enable_act8(self.blocks, on)
 
     # --------------------------------------------------------------- utilities
